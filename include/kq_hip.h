@@ -675,6 +675,187 @@ kq_status kq_hip_moe_block_f32(kq_hip_context *context, const kq_hip_gr_dimensio
                                kq_diagnostic *diagnostic);
 
 /* ------------------------------------------------------------------ */
+/* Sequences: rows of token arrays cut into sequences, each with a state in
+ * a slot of a state array. What a GDN layer keeps of a sequence between
+ * calls is its convolution's last inputs and its attention's state; the two
+ * entry points below read such a state, run over the sequence's rows and
+ * write the state behind its last row.
+ *
+ * offsets: device [sequence_count + 1], not decreasing and at most
+ * token_count: sequence s has rows offsets[s] .. offsets[s + 1] - 1. A
+ * sequence may have no row (its state is passed on). NULL: one row a
+ * sequence (token_count == sequence_count), the form for decoding.
+ * slots: device [sequence_count], sequence s's state in the state arrays
+ * [slot_count][...]; NULL: slot s. KQ_HIP_NO_SLOT takes the sequence out of
+ * the call (a padded batch). Two sequences may not share a slot.
+ * fresh: device [sequence_count], nonzero: the sequence starts from a state
+ * of zeros and the state array is not read; NULL: none does.
+ *
+ * Rows of no sequence, rows of a sequence taken out and slots that no
+ * sequence names keep what the outputs held. Offsets or slots that break
+ * these rules are found on the device: INVALID_ARGUMENT, outputs as after
+ * any failure. state_out may be the state array itself (not another overlap).
+ * A synchronous call that may have to restore its outputs copies the whole
+ * state_out array aside; a caller with a large pool calls asynchronously or
+ * switches the commit off. */
+#define KQ_HIP_NO_SLOT UINT32_MAX
+
+typedef struct kq_hip_sequences {
+    uint64_t token_count;    /* 1 .. 262,144 */
+    uint32_t sequence_count; /* 1 .. 65,535 */
+    uint32_t slot_count;
+    const uint32_t *offsets;
+    const uint32_t *slots;
+    const uint32_t *fresh;
+} kq_hip_sequences;
+
+typedef enum kq_hip_activation {
+    KQ_HIP_ACTIVATION_NONE = 0,
+    KQ_HIP_ACTIVATION_SIGMOID,
+    KQ_HIP_ACTIVATION_SILU
+} kq_hip_activation;
+
+/* Causal depthwise convolution (the GDN layer's ssm_conv1d between attn_qkv
+ * and the attention), for each channel c of a sequence's rows x_0, x_1, ...:
+ *   y_t[c] = activation(bias[c] + sum_j weight[c][j] x_(t - (taps-1) + j)[c])
+ * where x_-1 .. x_-(taps-1) are the state: [slots][taps-1][channels], oldest
+ * first. state_out gets the last taps-1 inputs. weight [channels][taps] (the
+ * GGUF tensor's order), bias [channels] or NULL; 2 .. 8 taps. Strides count
+ * floats between rows, at least `channels`; every buffer 4-byte aligned
+ * (16-byte aligned ones with channels and strides in fours are faster).
+ * No entry point of the reference corresponds at this boundary: its GDN
+ * operator holds the step (src/kq_gdn_qwen38.c). */
+typedef struct kq_hip_causal_conv {
+    uint32_t channels;
+    uint32_t taps;
+    const float *weight;
+    const float *bias;
+    uint32_t activation; /* KQ_HIP_ACTIVATION_NONE or _SILU */
+} kq_hip_causal_conv;
+
+kq_status kq_hip_causal_conv_f32(kq_hip_context *context, const kq_hip_causal_conv *conv,
+                                 const kq_hip_sequences *sequences, const float *device_input,
+                                 uint64_t input_stride, const float *device_state,
+                                 float *device_state_out, float *device_output,
+                                 uint64_t output_stride, kq_diagnostic *diagnostic);
+
+/* Linear attention with a decay for each head, with or without the delta
+ * correction (the core of the GDN layer). Value head h reads key head
+ * h / (value_heads / key_heads) and holds a state S [key_width][value_width];
+ * for each row of a sequence:
+ *   g = rate[h] softplus(alpha[h] + bias[h])     (alpha NULL: g = rate[h])
+ *   q = scale query / n(query), k = key / n(key)  n(x) = sqrt(sum x^2 +
+ *                         epsilon) with normalize, else 1
+ *   S = e^g S
+ *   d = sigmoid(beta[h]) (value - S^T k)          (beta NULL: d = value)
+ *   S = S + k d^T,  output = S^T q
+ * Rates are at most 0. bias NULL: zeros. state arrays [slots][value_heads]
+ * [key_width][value_width], output rows [value_heads][value_width]. Widths 64
+ * or 128; 1 .. 256 value heads, a multiple of the key heads. Strides count
+ * floats between rows; query, key, value, output, the states and the
+ * scratch 16-byte aligned, and the strides of the four in fours.
+ * Long sequences run in chunks of 64 rows on the matrix cores, single
+ * rows and short sequences in the recurrent form.
+ * Non-finite inputs and results and rates above 0 give NUMERIC_DOMAIN. */
+typedef struct kq_hip_linear_attention {
+    uint32_t key_heads;
+    uint32_t value_heads;
+    uint32_t key_width;
+    uint32_t value_width;
+    float scale;
+    uint32_t normalize; /* 0 or 1 */
+    float epsilon;      /* with normalize: at least 1e-20 */
+    const float *rate;  /* device [value_heads] */
+    const float *bias;  /* device [value_heads] or NULL */
+} kq_hip_linear_attention;
+
+typedef struct kq_hip_linear_attention_inputs {
+    const float *query; /* [tokens][key_heads][key_width] */
+    uint64_t query_stride;
+    const float *key;
+    uint64_t key_stride;
+    const float *value; /* [tokens][value_heads][value_width] */
+    uint64_t value_stride;
+    const float *alpha; /* [tokens][value_heads] or NULL */
+    uint64_t alpha_stride;
+    const float *beta;  /* [tokens][value_heads] or NULL */
+    uint64_t beta_stride;
+} kq_hip_linear_attention_inputs;
+
+/* Device scratch of a call with these sizes (only the counts and whether
+ * offsets is NULL are looked at); 0 for a call that needs none, and for
+ * arguments that the call refuses. */
+uint64_t kq_hip_linear_attention_scratch_bytes(const kq_hip_linear_attention *attention,
+                                               const kq_hip_sequences *sequences);
+kq_status kq_hip_linear_attention_f32(kq_hip_context *context,
+                                      const kq_hip_linear_attention *attention,
+                                      const kq_hip_sequences *sequences,
+                                      const kq_hip_linear_attention_inputs *inputs,
+                                      const float *device_state, float *device_state_out,
+                                      float *device_output, uint64_t output_stride,
+                                      void *device_scratch, uint64_t scratch_bytes,
+                                      kq_diagnostic *diagnostic);
+
+/* ------------------------------------------------------------------ */
+/* Norms around a block, with its gate and its residual. rms(x) below is
+ * x / sqrt(mean(x^2) + epsilon). */
+
+/* RMS norm of each group of a row, times its weight and its gate (the GDN
+ * heads behind the attention; without a gate, the norm before a block):
+ *   y[t][g][i] = rms(x[t][g])[i] (weight_offset + weight[i]) act(gate[t][g][i])
+ * weight [width], or [groups][width] with weight_per_group; NULL: ones. With
+ * KQ_HIP_ACTIVATION_NONE there is no gate (its argument is not looked at).
+ * width 1 .. 16,384; strides count floats between rows, at least groups *
+ * width; 4-byte alignment (16 bytes, with width and strides in fours, is
+ * faster). The output may be the input, or the gate, with its stride. */
+typedef struct kq_hip_gated_norm {
+    uint32_t groups;
+    uint32_t width;
+    float epsilon;
+    float weight_offset;
+    const float *weight;
+    uint32_t weight_per_group;
+    uint32_t gate_activation;
+} kq_hip_gated_norm;
+
+kq_status kq_hip_gated_norm_f32(kq_hip_context *context, const kq_hip_gated_norm *norm,
+                                uint64_t token_count, const float *device_input,
+                                uint64_t input_stride, const float *device_gate,
+                                uint64_t gate_stride, float *device_output,
+                                uint64_t output_stride, kq_diagnostic *diagnostic);
+
+/* The end of a block and the norm before the next one:
+ *   y[t]    = block_output[t], normed if post_weight is given:
+ *             rms(block_output[t]) (post_offset + post_weight),
+ *             times act(gate[t]) with a gate activation
+ *   r[t][b] = residual[t][b] + (residual_scale * branch_gate[t][b]) y[t]
+ *   n[t][b] = rms(r[t][b]) (pre_offset + pre_weight[b])
+ * for the branches b of a token (1: an ordinary residual; the gated
+ * residual's branches and write gates: kq_hip_gr_write_f32). block_output and
+ * gate [tokens][hidden], residual, residual_out and normalized
+ * [tokens][branches][hidden], branch_gate [tokens][branches] (NULL: ones).
+ * pre_weight [branches][hidden] and normalized go together: both or neither.
+ * residual_out may be the residual. hidden 1 .. 16,384, 1 .. 64 branches;
+ * 4-byte alignment (16 bytes, with hidden in fours, is faster). */
+typedef struct kq_hip_block_join {
+    uint32_t branch_count;
+    uint32_t hidden_size;
+    float epsilon;
+    const float *post_weight;
+    float post_offset;
+    uint32_t gate_activation;
+    float residual_scale;
+    const float *pre_weight;
+    float pre_offset;
+} kq_hip_block_join;
+
+kq_status kq_hip_block_join_f32(kq_hip_context *context, const kq_hip_block_join *join,
+                                uint64_t token_count, const float *device_block_output,
+                                const float *device_gate, const float *device_residual,
+                                const float *device_branch_gate, float *device_residual_out,
+                                float *device_normalized, kq_diagnostic *diagnostic);
+
+/* ------------------------------------------------------------------ */
 /* Elementwise binary32 expf with the bits of the libm expf the reference
  * calls (src/kq_numeric.c:628-638, :776-813). No reference entry point of
  * its own; it exposes the device expf that the softmax uses so callers can

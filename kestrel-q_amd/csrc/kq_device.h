@@ -18,6 +18,7 @@
 #define KQ_DEV_INPUT 4u      /* non-finite input (checked first by the
                                 reference) -> NUMERIC_DOMAIN */
 #define KQ_DEV_RANGE 8u      /* an index input out of range -> INVALID_ARGUMENT */
+#define KQ_DEV_SEQUENCE 16u  /* a sequence's rows or slot -> INVALID_ARGUMENT */
 
 #define KQ_WAVE 64
 

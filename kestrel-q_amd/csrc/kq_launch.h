@@ -362,6 +362,68 @@ int kq_launch_sample_fast(uint32_t count, uint32_t top_k, float top_p);
 /* the full sort and the tail on the prep already in the scratch */
 hipError_t kq_launch_sample_full(const kq_launch_sample_args *args, hipStream_t s);
 
+/* sequences of rows with a state each (kq_seq.h; include/kq_hip.h) */
+typedef struct kq_launch_seqs {
+    uint64_t tokens;
+    uint32_t count, slot_count;
+    const uint32_t *offsets, *slots, *fresh;
+} kq_launch_seqs;
+
+/* causal depthwise convolution (kq_conv.hip); strides in floats */
+typedef struct kq_launch_conv {
+    uint32_t channels, taps;
+    const float *weight, *bias;
+    uint32_t silu;
+} kq_launch_conv;
+hipError_t kq_launch_causal_conv(const kq_launch_conv *conv, const kq_launch_seqs *seqs,
+                                 const float *x, uint64_t x_stride, const float *state,
+                                 float *state_out, float *y, uint64_t y_stride,
+                                 uint32_t *status, hipStream_t stream);
+
+/* linear attention with a decay for each head (kq_linattn.hip: checks of the
+ * sequences, the recurrent form; kq_linattn_chunk.hip: chunks of 64 rows) */
+typedef struct kq_launch_linattn {
+    uint32_t key_heads, value_heads, key_width, value_width;
+    float scale;
+    uint32_t normalize;
+    float epsilon;
+    const float *rate, *bias;
+    const float *q, *k, *v, *alpha, *beta;
+    uint64_t qs, ks, vs, as, bs;
+    const float *state;
+    float *state_out, *y;
+    uint64_t ys;
+} kq_launch_linattn;
+/* bytes of the chunked form's scratch (0: these sizes run without) */
+uint64_t kq_launch_linattn_scratch(const kq_launch_linattn *a, uint64_t tokens, uint32_t count);
+hipError_t kq_launch_linattn_run(const kq_launch_linattn *a, const kq_launch_seqs *seqs,
+                                 void *scratch, uint32_t *status, hipStream_t stream);
+
+/* norms around a block (kq_norm.hip) */
+typedef struct kq_launch_norm {
+    uint32_t groups, width;
+    float epsilon, offset;
+    const float *weight;
+    uint32_t per_group, gate;
+} kq_launch_norm;
+hipError_t kq_launch_gated_norm(const kq_launch_norm *norm, uint64_t tokens, const float *x,
+                                uint64_t xs, const float *gate, uint64_t gs, float *y,
+                                uint64_t ys, uint32_t *status, hipStream_t stream);
+typedef struct kq_launch_join {
+    uint32_t branches, hidden;
+    float epsilon;
+    const float *post;
+    float post_offset;
+    uint32_t gate_kind;
+    float scale;
+    const float *pre;
+    float pre_offset;
+    const float *block, *gate, *residual, *branch_gate;
+    float *residual_out, *normalized;
+} kq_launch_join;
+hipError_t kq_launch_block_join(const kq_launch_join *join, uint64_t tokens, uint32_t *status,
+                                hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,194 @@
+/*
+ * kq_linattn.hip — linear attention with a decay for each head on gfx950,
+ * the recurrent form (include/kq_hip.h, kq_hip_linear_attention_f32): single
+ * rows and short sequences.
+ *
+ * For a row with query q, key k, value v, log decay g and beta b, the state
+ * S [dk][dv] of a value head becomes
+ *   S' = e^g S + k d^T,  d = b (v - e^g S^T k),  o = S'^T q = e^g S^T q + (q.k) d,
+ * so S^T k and S^T q are formed in one pass over S, which stays in registers
+ * from the first row to the last.
+ *
+ * A wave holds 4 CG columns of one head's state: lane = rg CG + cg has rows
+ * rg R .. rg R + R - 1 of columns 4 cg .. 4 cg + 3, and every sum over the rows
+ * is finished by lane exchanges, without LDS or a barrier. For one row a
+ * sequence the state's read and write are the bound: 131,072 bytes a head of
+ * 128 x 128, against 100 KFLOP.
+ */
+#include "kq_device.h"
+#include "kq_launch.h"
+#include "kq_linattn.h"
+#include "kq_seq.h"
+
+namespace {
+
+/* one row of a lane: its part of q and k, its columns of v, the head's gates */
+template <int R>
+struct Row {
+    float q[R], k[R], v[4], alpha, beta;
+    __device__ __forceinline__ void load(const kq_launch_linattn &a, uint64_t t, uint32_t qk,
+                                         uint32_t vc, uint32_t h) {
+        const float4 *qp = (const float4 *)(a.q + t * a.qs + qk);
+        const float4 *kp = (const float4 *)(a.k + t * a.ks + qk);
+#pragma unroll
+        for (int i = 0; i < R / 4; ++i) {
+            const float4 x = qp[i], y = kp[i];
+            q[4 * i] = x.x; q[4 * i + 1] = x.y; q[4 * i + 2] = x.z; q[4 * i + 3] = x.w;
+            k[4 * i] = y.x; k[4 * i + 1] = y.y; k[4 * i + 2] = y.z; k[4 * i + 3] = y.w;
+        }
+        const float4 x = *(const float4 *)(a.v + t * a.vs + vc);
+        v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
+        alpha = a.alpha != nullptr ? a.alpha[t * a.as + h] : 0.0f;
+        beta = a.beta != nullptr ? a.beta[t * a.bs + h] : 0.0f;
+    }
+};
+
+/* 1 / n(x) for a lane's part of x, where SUM are the bits of the lanes that
+ * hold the rest. Squares past the type's range are formed of x 2^-96. */
+template <int R, int SUM>
+__device__ __forceinline__ float inverse_norm(const float (&x)[R], float eps) {
+    float s = 0.0f;
+#pragma unroll
+    for (int i = 0; i < R; ++i) s = fmaf(x[i], x[i], s);
+    s = kq::lanes_sum<SUM>(s);
+    if (s < 3.0e38f) return 1.0f / sqrtf(s + eps); /* the same way in every lane */
+    s = 0.0f;
+#pragma unroll
+    for (int i = 0; i < R; ++i) s = fmaf(x[i] * 0x1p-96f, x[i] * 0x1p-96f, s);
+    return 0x1p-96f / sqrtf(kq::lanes_sum<SUM>(s));
+}
+
+/* grid (waves of columns of all heads / waves a workgroup, sequences): the
+ * sequences of at most max_rows rows */
+template <int DK, int CG>
+__global__ __launch_bounds__(256) void linattn_rows(kq_launch_linattn a, kq_launch_seqs q,
+                                                    uint32_t max_rows, uint32_t *status) {
+    constexpr int RG = 64 / CG, R = DK / RG, SUM = 63 & ~(CG - 1);
+    const uint32_t lane = threadIdx.x & 63u;
+    const uint32_t s = blockIdx.y;
+    bool badseq = false;
+    const kq::SeqSpan sp = kq::seq_span(q, s, badseq);
+    if (blockIdx.x == 0u) {
+        if (sp.live && q.slots != nullptr)
+            for (uint32_t j = threadIdx.x; j < s; j += blockDim.x) badseq |= q.slots[j] == sp.slot;
+        if (badseq) kq_flag(status, KQ_DEV_SEQUENCE);
+    }
+    if (!sp.live || sp.rows > max_rows) return;
+    const uint32_t tiles = a.value_width / (4u * CG);
+    const uint32_t w = __builtin_amdgcn_readfirstlane(blockIdx.x * (blockDim.x >> 6) +
+                                                      (threadIdx.x >> 6));
+    const uint32_t h = w / tiles;
+    if (h >= a.value_heads) return;
+    const uint32_t col = (w % tiles) * (4u * CG) + (lane % CG) * 4u;
+    const uint32_t row0 = (lane / CG) * R;
+    const uint32_t qk = h / (a.value_heads / a.key_heads) * DK + row0;
+    const uint32_t vc = h * a.value_width + col;
+    const size_t at = (((size_t)sp.slot * a.value_heads + h) * DK + row0) * a.value_width + col;
+
+    float S[R][4];
+    if (!sp.fresh) {
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            const float4 x = *(const float4 *)(a.state + at + (size_t)i * a.value_width);
+            S[i][0] = x.x; S[i][1] = x.y; S[i][2] = x.z; S[i][3] = x.w;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < R; ++i) S[i][0] = S[i][1] = S[i][2] = S[i][3] = 0.0f;
+    }
+    const float rate = a.rate[h], bias = a.bias != nullptr ? a.bias[h] : 0.0f;
+    bool badin = !kq_isfinite(rate) || rate > 0.0f || !kq_isfinite(bias), bad = false;
+    Row<R> next;
+    if (sp.rows != 0u) next.load(a, sp.begin, qk, vc, h);
+    for (uint32_t n = 0; n < sp.rows; ++n) {
+        Row<R> r = next;
+        const uint64_t t = (uint64_t)sp.begin + n;
+        if (n + 1u < sp.rows) next.load(a, t + 1u, qk, vc, h);
+        badin |= !kq_isfinite(r.alpha) || !kq_isfinite(r.beta);
+        float g = rate;
+        if (a.alpha != nullptr) g = rate * kq::softplus(r.alpha + bias);
+        const float e = kq::exp_neg(g);
+        float nq = a.scale, nk = 1.0f;
+        if (a.normalize != 0u) {
+            nq *= inverse_norm<R, SUM>(r.q, a.epsilon);
+            nk = inverse_norm<R, SUM>(r.k, a.epsilon);
+        }
+        float qkv = 0.0f, sk[4], sq[4];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) sk[c] = sq[c] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            badin |= !kq_isfinite(r.q[i]) || !kq_isfinite(r.k[i]);
+            r.q[i] *= nq;
+            r.k[i] *= nk;
+            qkv = fmaf(r.q[i], r.k[i], qkv);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                sk[c] = fmaf(r.k[i], S[i][c], sk[c]);
+                sq[c] = fmaf(r.q[i], S[i][c], sq[c]);
+            }
+        }
+        qkv = kq::lanes_sum<SUM>(qkv);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            sk[c] = kq::lanes_sum<SUM>(sk[c]);
+            sq[c] = kq::lanes_sum<SUM>(sq[c]);
+        }
+        const float b = a.beta != nullptr ? kq::sigmoid(r.beta) : 1.0f;
+        float d[4], o[4];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            badin |= !kq_isfinite(r.v[c]);
+            d[c] = r.v[c];
+            if (a.beta != nullptr) d[c] = b * (r.v[c] - e * sk[c]);
+            o[c] = fmaf(qkv, d[c], e * sq[c]);
+            bad |= !kq_isfinite(o[c]);
+        }
+#pragma unroll
+        for (int i = 0; i < R; ++i)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) S[i][c] = fmaf(r.k[i], d[c], e * S[i][c]);
+        if (lane < CG)
+            *(float4 *)(a.y + t * a.ys + vc) = make_float4(o[0], o[1], o[2], o[3]);
+    }
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+        *(float4 *)(a.state_out + at + (size_t)i * a.value_width) =
+            make_float4(S[i][0], S[i][1], S[i][2], S[i][3]);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) bad |= !kq_isfinite(S[i][c]);
+    }
+    if (badin) kq_flag(status, KQ_DEV_INPUT);
+    if (bad) kq_flag(status, KQ_DEV_NUMERIC);
+}
+
+}  // namespace
+
+hipError_t kq_linattn_recurrent(const kq_launch_linattn &a, const kq_launch_seqs &q,
+                                uint32_t max_rows, uint32_t *status, hipStream_t s) {
+    const uint32_t waves = a.value_heads * a.value_width / 32u;
+    /* few waves: one a workgroup, so that they spread over the device */
+    const uint32_t per = (uint64_t)waves * q.count <= 1024u ? 1u : 4u;
+    const dim3 grid((waves + per - 1u) / per, q.count), block(64u * per);
+    if (a.key_width == 128u)
+        hipLaunchKernelGGL(HIP_KERNEL_NAME(linattn_rows<128, 8>), grid, block, 0, s, a, q, max_rows,
+                           status);
+    else
+        hipLaunchKernelGGL(HIP_KERNEL_NAME(linattn_rows<64, 8>), grid, block, 0, s, a, q, max_rows,
+                           status);
+    return hipGetLastError();
+}
+
+extern "C" uint64_t kq_launch_linattn_scratch(const kq_launch_linattn *a, uint64_t tokens,
+                                              uint32_t count) {
+    (void)a;
+    (void)tokens;
+    (void)count;
+    return 0u;
+}
+
+extern "C" hipError_t kq_launch_linattn_run(const kq_launch_linattn *a, const kq_launch_seqs *q,
+                                            void *scratch, uint32_t *status, hipStream_t s) {
+    (void)scratch;
+    return kq_linattn_recurrent(*a, *q, 0xffffffffu, status, s);
+}

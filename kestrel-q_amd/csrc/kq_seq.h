@@ -1,0 +1,112 @@
+/*
+ * kq_seq.h — sequences on the device: where a sequence's rows and its state
+ * lie, checked before anything is indexed with them (include/kq_hip.h,
+ * "Sequences").
+ */
+#ifndef KQ_SEQ_H
+#define KQ_SEQ_H
+
+#include "kq_device.h"
+#include "kq_launch.h"
+
+#define KQ_NO_SLOT 0xffffffffu
+
+namespace kq {
+
+struct SeqSpan {
+    uint32_t begin, rows, slot;
+    bool fresh;
+    bool live; /* false: taken out of the call, or refused */
+};
+
+/* Sequence s of the call. A span or slot that breaks the rules is not live
+ * and sets `bad`, so nothing is read or written through it. */
+__device__ __forceinline__ SeqSpan seq_span(const kq_launch_seqs &q, uint32_t s, bool &bad) {
+    SeqSpan r;
+    r.begin = s;
+    r.rows = 1u;
+    r.slot = q.slots != nullptr ? q.slots[s] : s;
+    r.live = r.slot != KQ_NO_SLOT;
+    if (q.offsets != nullptr) {
+        const uint32_t a = q.offsets[s], b = q.offsets[s + 1u];
+        r.begin = a;
+        r.rows = b - a;
+        if (a > b || b > q.tokens) {
+            bad = true;
+            r.live = false;
+        }
+    }
+    if (r.live && r.slot >= q.slot_count) {
+        bad = true;
+        r.live = false;
+    }
+    r.fresh = q.fresh != nullptr && q.fresh[s] != 0u;
+    return r;
+}
+
+/* Whether a sequence before s names s's slot too. All NT threads of a
+ * workgroup look at a part; each returns its own finding. */
+template <int NT>
+__device__ __forceinline__ bool seq_slot_taken(const kq_launch_seqs &q, uint32_t s,
+                                               uint32_t slot) {
+    bool taken = false;
+    if (q.slots != nullptr && slot != KQ_NO_SLOT)
+        for (uint32_t j = threadIdx.x; j < s; j += NT) taken |= q.slots[j] == slot;
+    return taken;
+}
+
+/* e^x, x <= 0, to about one unit in the last place: x log2(e) as a rounded
+ * product t and its error r, 2^t of the hardware, and 1 + r ln 2. Below
+ * -150 it is 0 in 32 bits. */
+__device__ __forceinline__ float exp_neg(float x) {
+    x = fmaxf(x, -150.0f);
+    const float t = x * 0x1.715476p+0f;
+    const float r = fmaf(x, 0x1.4ae0cp-26f, fmaf(x, 0x1.715476p+0f, -t));
+    const float e = __builtin_amdgcn_exp2f(t);
+    return fmaf(e, r * 0x1.62e43p-1f, e);
+}
+
+/* e^x, x <= 0 in 64 bits (a difference of sums of log decays): rounding the
+ * base-2 exponent to 32 bits costs at most |x| 2^-24 of a value e^x, 0.37
+ * 2^-24 of 1 */
+__device__ __forceinline__ float exp_of(double x) {
+    return __builtin_amdgcn_exp2f((float)(x * 1.4426950408889634));
+}
+
+/* 1 / d, d in [1, 2]: the hardware's reciprocal and one Newton step */
+__device__ __forceinline__ float inverse_of(float d) {
+    const float r = __builtin_amdgcn_rcpf(d);
+    return fmaf(fmaf(-d, r, 1.0f), r, r);
+}
+
+/* ln(1 + e^x) of a finite sum x that may have left the range */
+__device__ __forceinline__ float softplus(float x) {
+    x = fminf(x, 0x1.fffffep127f);
+    return fmaxf(x, 0.0f) + log1pf(exp_neg(-fabsf(x)));
+}
+
+__device__ __forceinline__ float sigmoid(float x) {
+    const float e = exp_neg(-fabsf(x));
+    const float r = inverse_of(1.0f + e);
+    return x >= 0.0f ? r : e * r;
+}
+
+/* sum over the lanes that differ in the bits of MASK */
+template <int MASK>
+__device__ __forceinline__ float lanes_sum(float v) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1)
+        if (MASK & o) v += __shfl_xor(v, o, KQ_WAVE);
+    return v;
+}
+template <int MASK>
+__device__ __forceinline__ float lanes_max(float v) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1)
+        if (MASK & o) v = fmaxf(v, __shfl_xor(v, o, KQ_WAVE));
+    return v;
+}
+
+}  // namespace kq
+
+#endif

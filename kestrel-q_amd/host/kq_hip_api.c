@@ -27,6 +27,7 @@
 #define KQ_DEV_NUMERIC 2u
 #define KQ_DEV_INPUT 4u
 #define KQ_DEV_RANGE 8u
+#define KQ_DEV_SEQUENCE 16u
 /* output ranges one call can restore */
 #define KQ_SNAP_RANGES 4u
 
@@ -81,6 +82,10 @@ static kq_status set_device(kq_hip_context *c, kq_diagnostic *diag) {
 static kq_status device_flags(uint32_t flags, kq_diagnostic *diag) {
     if (flags & KQ_DEV_RANGE)
         return kq_fail(diag, KQ_STATUS_INVALID_ARGUMENT, "an expert id is out of range");
+    if (flags & KQ_DEV_SEQUENCE)
+        return kq_fail(diag, KQ_STATUS_INVALID_ARGUMENT,
+                       "a sequence's rows decrease or pass the tokens, or its slot is out of "
+                       "range or taken twice");
     if (flags & KQ_DEV_INPUT)
         return kq_fail(diag, KQ_STATUS_NUMERIC_DOMAIN, "non-finite input on the device path");
     if (flags & KQ_DEV_MALFORMED)
@@ -305,6 +310,18 @@ kq_status kqi_context_begin(kq_hip_context *c, kq_diagnostic *diag) {
 void *kqi_context_stream_ptr(const kq_hip_context *c) { return (void *)c->stream; }
 
 kq_status kqi_context_drain(kq_hip_context *c, kq_diagnostic *diag) { return drain(c, diag); }
+
+uint32_t *kqi_context_status_word(const kq_hip_context *c) { return c->d_status; }
+
+kq_status kqi_context_snapshot(kq_hip_context *c, uint32_t n, void *const *p, const uint64_t *len,
+                               kq_diagnostic *diag) {
+    return snapshot(c, n, p, len, diag);
+}
+
+kq_status kqi_context_finish(kq_hip_context *c, int launch, const char *what,
+                             kq_diagnostic *diag) {
+    return finish(c, (hipError_t)launch, what, diag);
+}
 
 kq_status kqi_hip_fail(kq_diagnostic *diag, int e, const char *what) {
     return hip_fail(diag, (hipError_t)e, what);

@@ -68,6 +68,47 @@ class GrWeights(C.Structure):
                 ("up_type", C.c_uint32), ("up", C.c_void_p), ("inject", C.c_void_p)]
 
 
+class Sequences(C.Structure):
+    _fields_ = [("token_count", C.c_uint64), ("sequence_count", C.c_uint32),
+                ("slot_count", C.c_uint32), ("offsets", C.c_void_p), ("slots", C.c_void_p),
+                ("fresh", C.c_void_p)]
+
+
+class CausalConv(C.Structure):
+    _fields_ = [("channels", C.c_uint32), ("taps", C.c_uint32), ("weight", C.c_void_p),
+                ("bias", C.c_void_p), ("activation", C.c_uint32)]
+
+
+class LinearAttention(C.Structure):
+    _fields_ = [("key_heads", C.c_uint32), ("value_heads", C.c_uint32),
+                ("key_width", C.c_uint32), ("value_width", C.c_uint32), ("scale", C.c_float),
+                ("normalize", C.c_uint32), ("epsilon", C.c_float), ("rate", C.c_void_p),
+                ("bias", C.c_void_p)]
+
+
+class LinearAttentionInputs(C.Structure):
+    _fields_ = [f for n in ("query", "key", "value", "alpha", "beta")
+                for f in ((n, C.c_void_p), (n + "_stride", C.c_uint64))]
+
+
+class GatedNorm(C.Structure):
+    _fields_ = [("groups", C.c_uint32), ("width", C.c_uint32), ("epsilon", C.c_float),
+                ("weight_offset", C.c_float), ("weight", C.c_void_p),
+                ("weight_per_group", C.c_uint32), ("gate_activation", C.c_uint32)]
+
+
+class BlockJoin(C.Structure):
+    _fields_ = [("branch_count", C.c_uint32), ("hidden_size", C.c_uint32),
+                ("epsilon", C.c_float), ("post_weight", C.c_void_p),
+                ("post_offset", C.c_float), ("gate_activation", C.c_uint32),
+                ("residual_scale", C.c_float), ("pre_weight", C.c_void_p),
+                ("pre_offset", C.c_float)]
+
+
+NO_SLOT = 0xFFFFFFFF
+ACTIVATIONS = {"none": 0, "sigmoid": 1, "silu": 2}
+
+
 class MoeWeights(C.Structure):
     _fields_ = [("router", C.c_void_p),
                 ("routed_gate_type", C.c_uint32), ("routed_gate", C.c_void_p),
@@ -338,6 +379,14 @@ SIGNATURES = {
     "kq_hip_moe_block_f32": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p,
                                        C.c_void_p, C.c_void_p, C.c_uint64, C.c_void_p,
                                        C.c_void_p, C.c_void_p, C.c_uint64, C.c_void_p]),
+    "kq_hip_causal_conv_f32": (C.c_int, [_P, _P, _P, _P, C.c_uint64, _P, _P, _P, C.c_uint64,
+                                         _P]),
+    "kq_hip_linear_attention_scratch_bytes": (C.c_uint64, [_P, _P]),
+    "kq_hip_linear_attention_f32": (C.c_int, [_P, _P, _P, _P, _P, _P, _P, C.c_uint64, _P,
+                                              C.c_uint64, _P]),
+    "kq_hip_gated_norm_f32": (C.c_int, [_P, _P, C.c_uint64, _P, C.c_uint64, _P, C.c_uint64, _P,
+                                        C.c_uint64, _P]),
+    "kq_hip_block_join_f32": (C.c_int, [_P, _P, C.c_uint64, _P, _P, _P, _P, _P, _P, _P]),
 }
 
 _lib = None
@@ -408,6 +457,55 @@ def expert_member_span(type_id, rows, cols, experts, expert_id) -> tuple[int, in
     check(lib().kq_hip_expert_member_span(type_id, rows, cols, experts, expert_id,
                                           C.byref(off), C.byref(cnt), C.byref(d)), d)
     return off.value, cnt.value
+
+
+def _ptr(x):
+    """The device address of a DeviceBuffer or of an int; None stays None."""
+    return C.c_void_p(x.ptr if hasattr(x, "ptr") else x)
+
+
+def sequences(tokens: int, count: int, slot_count: int, offsets=None, slots=None,
+              fresh=None) -> Sequences:
+    """Device arrays: offsets [count + 1] (None: one token each), slots
+    [count] (None: slot s), fresh [count] (None: every sequence goes on)."""
+    return Sequences(tokens, count, slot_count, _ptr(offsets), _ptr(slots), _ptr(fresh))
+
+
+def causal_conv(channels: int, taps: int, weight, bias=None,
+                activation: str = "silu") -> CausalConv:
+    return CausalConv(channels, taps, _ptr(weight), _ptr(bias), ACTIVATIONS[activation])
+
+
+def linear_attention(key_heads: int, value_heads: int, key_width: int, value_width: int,
+                     scale: float, rate, bias=None, normalize: bool = True,
+                     epsilon: float = 1.0e-6) -> LinearAttention:
+    return LinearAttention(key_heads, value_heads, key_width, value_width, scale,
+                           int(normalize), epsilon, _ptr(rate), _ptr(bias))
+
+
+def linear_attention_inputs(query, query_stride: int, key, key_stride: int, value,
+                            value_stride: int, alpha=None, alpha_stride: int = 0, beta=None,
+                            beta_stride: int = 0) -> LinearAttentionInputs:
+    return LinearAttentionInputs(_ptr(query), query_stride, _ptr(key), key_stride, _ptr(value),
+                                 value_stride, _ptr(alpha), alpha_stride, _ptr(beta),
+                                 beta_stride)
+
+
+def linear_attention_scratch_bytes(attention: LinearAttention, seqs: Sequences) -> int:
+    return lib().kq_hip_linear_attention_scratch_bytes(C.byref(attention), C.byref(seqs))
+
+
+def gated_norm(groups: int, width: int, epsilon: float, weight=None, weight_offset: float = 0.0,
+               per_group: bool = False, gate: str = "none") -> GatedNorm:
+    return GatedNorm(groups, width, epsilon, weight_offset, _ptr(weight), int(per_group),
+                     ACTIVATIONS[gate])
+
+
+def block_join(branches: int, hidden: int, epsilon: float, post=None, post_offset: float = 0.0,
+               gate: str = "none", scale: float = 1.0, pre=None,
+               pre_offset: float = 0.0) -> BlockJoin:
+    return BlockJoin(branches, hidden, epsilon, _ptr(post), post_offset, ACTIVATIONS[gate], scale,
+                     _ptr(pre), pre_offset)
 
 
 class DeviceBuffer:
@@ -754,6 +852,36 @@ class Context:
         check(lib().kq_hip_gr_write_f32(self._h, C.byref(dims), self._p(x),
                                         self._p(block_output), self._p(write_gate), tokens,
                                         self._p(out), C.byref(d)), d)
+
+    def causal_conv(self, conv: CausalConv, seqs: Sequences, x, x_stride: int, state, state_out,
+                    y, y_stride: int) -> None:
+        d = Diagnostic()
+        check(lib().kq_hip_causal_conv_f32(self._h, C.byref(conv), C.byref(seqs), _ptr(x),
+                                           x_stride, _ptr(state), _ptr(state_out), _ptr(y),
+                                           y_stride, C.byref(d)), d)
+
+    def linear_attention(self, attention: LinearAttention, seqs: Sequences,
+                         inputs: LinearAttentionInputs, state, state_out, y, y_stride: int,
+                         scratch=None, scratch_bytes: int = 0) -> None:
+        d = Diagnostic()
+        check(lib().kq_hip_linear_attention_f32(self._h, C.byref(attention), C.byref(seqs),
+                                                C.byref(inputs), _ptr(state), _ptr(state_out),
+                                                _ptr(y), y_stride, _ptr(scratch), scratch_bytes,
+                                                C.byref(d)), d)
+
+    def gated_norm(self, norm: GatedNorm, tokens: int, x, x_stride: int, gate, gate_stride: int,
+                   y, y_stride: int) -> None:
+        d = Diagnostic()
+        check(lib().kq_hip_gated_norm_f32(self._h, C.byref(norm), tokens, _ptr(x), x_stride,
+                                          _ptr(gate), gate_stride, _ptr(y), y_stride,
+                                          C.byref(d)), d)
+
+    def block_join(self, join: BlockJoin, tokens: int, block_output, gate, residual, branch_gate,
+                   residual_out, normalized=None) -> None:
+        d = Diagnostic()
+        check(lib().kq_hip_block_join_f32(self._h, C.byref(join), tokens, _ptr(block_output),
+                                          _ptr(gate), _ptr(residual), _ptr(branch_gate),
+                                          _ptr(residual_out), _ptr(normalized), C.byref(d)), d)
 
     def moe_block(self, dims: GrDims, gr: GrWeights, cfg: MoeConfig, moe: MoeWeights, x,
                   tokens: int, out, ids, scratch, scratch_bytes: int) -> None:
