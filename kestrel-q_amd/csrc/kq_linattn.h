@@ -5,11 +5,48 @@
 #ifndef KQ_LINATTN_H
 #define KQ_LINATTN_H
 
+#include "kq_device.h"
 #include "kq_launch.h"
+#include "kq_seq.h"
+
+namespace kq {
+
+/* a row's log decay g <= 0 of a head */
+__device__ __forceinline__ float log_decay(const kq_launch_linattn &a, uint64_t t, uint32_t h,
+                                           float rate, float bias, bool &badin) {
+    float g = rate;
+    if (a.alpha != nullptr) {
+        const float x = a.alpha[t * a.as + h];
+        badin |= !kq_isfinite(x);
+        g = rate * softplus(x + bias);
+    }
+    return fmaxf(g, -1.0e30f);
+}
+
+/* S e^g as c0 S + c1 S. A decay near 1 that is rounded to 32 bits is off by
+ * up to 2^-25 in the same direction row after row, which a memory of many
+ * rows adds up; e^g - 1 has its own 24 bits. Where much of S is lost the
+ * sum would cancel, and e^g itself is exact enough. */
+struct Decay {
+    float c0, c1;
+};
+__device__ __forceinline__ Decay decay_of(float g) {
+    Decay d;
+    d.c0 = g > -0.5f ? 1.0f : 0.0f;
+    d.c1 = g > -0.5f ? expm1f(g) : exp_neg(g);
+    return d;
+}
+
+}  // namespace kq
 
 /* the recurrent form over the sequences of at most max_rows rows; checks all
  * sequences */
 hipError_t kq_linattn_recurrent(const kq_launch_linattn &a, const kq_launch_seqs &q,
                                 uint32_t max_rows, uint32_t *status, hipStream_t s);
+/* the chunked form over the sequences of more rows */
+uint64_t kq_linattn_chunked_scratch(const kq_launch_linattn &a, uint64_t tokens, uint32_t count,
+                                    uint32_t max_rows);
+hipError_t kq_linattn_chunked(const kq_launch_linattn &a, const kq_launch_seqs &q,
+                              uint32_t max_rows, void *scratch, uint32_t *status, hipStream_t s);
 
 #endif

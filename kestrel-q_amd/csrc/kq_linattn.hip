@@ -15,19 +15,18 @@
  * sequence the state's read and write are the bound: 131,072 bytes a head of
  * 128 x 128, against 100 KFLOP.
  */
-#include "kq_device.h"
-#include "kq_launch.h"
 #include "kq_linattn.h"
-#include "kq_seq.h"
 
 namespace {
 
 /* one row of a lane: its part of q and k, its columns of v, the head's gates */
 template <int R>
 struct Row {
-    float q[R], k[R], v[4], alpha, beta;
+    float q[R], k[R], v[4], beta;
+    kq::Decay e;
     __device__ __forceinline__ void load(const kq_launch_linattn &a, uint64_t t, uint32_t qk,
-                                         uint32_t vc, uint32_t h) {
+                                         uint32_t vc, uint32_t h, float rate, float bias,
+                                         bool &badin) {
         const float4 *qp = (const float4 *)(a.q + t * a.qs + qk);
         const float4 *kp = (const float4 *)(a.k + t * a.ks + qk);
 #pragma unroll
@@ -38,8 +37,9 @@ struct Row {
         }
         const float4 x = *(const float4 *)(a.v + t * a.vs + vc);
         v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
-        alpha = a.alpha != nullptr ? a.alpha[t * a.as + h] : 0.0f;
         beta = a.beta != nullptr ? a.beta[t * a.bs + h] : 0.0f;
+        badin |= !kq_isfinite(beta);
+        e = kq::decay_of(kq::log_decay(a, t, h, rate, bias, badin));
     }
 };
 
@@ -99,15 +99,12 @@ __global__ __launch_bounds__(256) void linattn_rows(kq_launch_linattn a, kq_laun
     const float rate = a.rate[h], bias = a.bias != nullptr ? a.bias[h] : 0.0f;
     bool badin = !kq_isfinite(rate) || rate > 0.0f || !kq_isfinite(bias), bad = false;
     Row<R> next;
-    if (sp.rows != 0u) next.load(a, sp.begin, qk, vc, h);
+    if (sp.rows != 0u) next.load(a, sp.begin, qk, vc, h, rate, bias, badin);
     for (uint32_t n = 0; n < sp.rows; ++n) {
         Row<R> r = next;
         const uint64_t t = (uint64_t)sp.begin + n;
-        if (n + 1u < sp.rows) next.load(a, t + 1u, qk, vc, h);
-        badin |= !kq_isfinite(r.alpha) || !kq_isfinite(r.beta);
-        float g = rate;
-        if (a.alpha != nullptr) g = rate * kq::softplus(r.alpha + bias);
-        const float e = kq::exp_neg(g);
+        if (n + 1u < sp.rows) next.load(a, t + 1u, qk, vc, h, rate, bias, badin);
+        const float c0 = r.e.c0, c1 = r.e.c1;
         float nq = a.scale, nk = 1.0f;
         if (a.normalize != 0u) {
             nq *= inverse_norm<R, SUM>(r.q, a.epsilon);
@@ -140,14 +137,14 @@ __global__ __launch_bounds__(256) void linattn_rows(kq_launch_linattn a, kq_laun
         for (int c = 0; c < 4; ++c) {
             badin |= !kq_isfinite(r.v[c]);
             d[c] = r.v[c];
-            if (a.beta != nullptr) d[c] = b * (r.v[c] - e * sk[c]);
-            o[c] = fmaf(qkv, d[c], e * sq[c]);
+            if (a.beta != nullptr) d[c] = b * (r.v[c] - fmaf(c1, sk[c], c0 * sk[c]));
+            o[c] = fmaf(qkv, d[c], fmaf(c1, sq[c], c0 * sq[c]));
             bad |= !kq_isfinite(o[c]);
         }
 #pragma unroll
         for (int i = 0; i < R; ++i)
 #pragma unroll
-            for (int c = 0; c < 4; ++c) S[i][c] = fmaf(r.k[i], d[c], e * S[i][c]);
+            for (int c = 0; c < 4; ++c) S[i][c] = fmaf(r.k[i], d[c], fmaf(c1, S[i][c], c0 * S[i][c]));
         if (lane < CG)
             *(float4 *)(a.y + t * a.ys + vc) = make_float4(o[0], o[1], o[2], o[3]);
     }
@@ -179,16 +176,18 @@ hipError_t kq_linattn_recurrent(const kq_launch_linattn &a, const kq_launch_seqs
     return hipGetLastError();
 }
 
+/* sequences up to this long run in the recurrent form */
+constexpr uint32_t kShort = 16u;
+
 extern "C" uint64_t kq_launch_linattn_scratch(const kq_launch_linattn *a, uint64_t tokens,
                                               uint32_t count) {
-    (void)a;
-    (void)tokens;
-    (void)count;
-    return 0u;
+    return tokens <= kShort ? 0u : kq_linattn_chunked_scratch(*a, tokens, count, kShort);
 }
 
 extern "C" hipError_t kq_launch_linattn_run(const kq_launch_linattn *a, const kq_launch_seqs *q,
                                             void *scratch, uint32_t *status, hipStream_t s) {
-    (void)scratch;
-    return kq_linattn_recurrent(*a, *q, 0xffffffffu, status, s);
+    if (q->offsets == nullptr || q->tokens <= kShort)
+        return kq_linattn_recurrent(*a, *q, kShort, status, s);
+    const hipError_t e = kq_linattn_chunked(*a, *q, kShort, scratch, status, s);
+    return e == hipSuccess ? kq_linattn_recurrent(*a, *q, kShort, status, s) : e;
 }
