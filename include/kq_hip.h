@@ -721,7 +721,7 @@ typedef enum kq_hip_activation {
  * where x_-1 .. x_-(taps-1) are the state: [slots][taps-1][channels], oldest
  * first. state_out gets the last taps-1 inputs. weight [channels][taps] (the
  * GGUF tensor's order), bias [channels] or NULL; 2 .. 8 taps. Strides count
- * floats between rows, at least `channels`; every buffer 4-byte aligned
+ * floats between rows, `channels` .. 2^22; every buffer 4-byte aligned
  * (16-byte aligned ones with channels and strides in fours are faster).
  * No entry point of the reference corresponds at this boundary: its GDN
  * operator holds the step (src/kq_gdn_qwen38.c). */
@@ -752,7 +752,7 @@ kq_status kq_hip_causal_conv_f32(kq_hip_context *context, const kq_hip_causal_co
  * Rates are at most 0. bias NULL: zeros. state arrays [slots][value_heads]
  * [key_width][value_width], output rows [value_heads][value_width]. Widths 64
  * or 128; 1 .. 256 value heads, a multiple of the key heads. Strides count
- * floats between rows; query, key, value, output, the states and the
+ * floats between rows, up to 2^22; query, key, value, output, the states and the
  * scratch 16-byte aligned, and the strides of the four in fours.
  * Long sequences run in chunks of 64 rows on the matrix cores, single
  * rows and short sequences in the recurrent form.
@@ -805,8 +805,8 @@ kq_status kq_hip_linear_attention_f32(kq_hip_context *context,
  *   y[t][g][i] = rms(x[t][g])[i] (weight_offset + weight[i]) act(gate[t][g][i])
  * weight [width], or [groups][width] with weight_per_group; NULL: ones. With
  * KQ_HIP_ACTIVATION_NONE there is no gate (its argument is not looked at).
- * width 1 .. 16,384; strides count floats between rows, at least groups *
- * width; 4-byte alignment (16 bytes, with width and strides in fours, is
+ * width 1 .. 16,384; strides count floats between rows, groups * width ..
+ * 2^22; 4-byte alignment (16 bytes, with width and strides in fours, is
  * faster). The output may be the input, or the gate, with its stride. */
 typedef struct kq_hip_gated_norm {
     uint32_t groups;

@@ -3,11 +3,13 @@
  * gfx950, the chunked form (include/kq_hip.h, kq_hip_linear_attention_f32).
  *
  * For the 64 rows of a chunk that starts from the state S, with log decays
- * summed from its start G_i (inclusive), rows of k, q, v as matrices, and
- * K~ = diag(e^G) K, the d of the recurrent form solve
- *   (1 + L) D = diag(b) (V - K~ S),   L_ij = b_i e^(G_i - G_j) k_i.k_j  (j < i)
- *   O = diag(e^G) Q S + M D,          M_ij = e^(G_i - G_j) q_i.k_j      (j <= i)
- *   S' = e^(G_64) S + sum_j e^(G_64 - G_j) k_j d_j^T
+ * summed from its start G_i (inclusive), rows of k, q, v as matrices, norms
+ * taken out of the rows of k = n k', the e_i = n_i d_i of the recurrent form
+ * solve
+ *   (1 + L) E = diag(b) (diag(n) V - diag(n^2 e^G) K' S),
+ *                                     L_ij = b_i n_i^2 e^(G_i - G_j) k'_i.k'_j  (j < i)
+ *   O = diag(e^G) Q S + M E,          M_ij = e^(G_i - G_j) q_i.k'_j      (j <= i)
+ *   S' = e^(G_64) S + sum_j e^(G_64 - G_j) k'_j e_j^T
  * so that everything but three products with S is independent of it, and a
  * chunk costs seven matrix products instead of 64 dependent steps.
  *
@@ -19,16 +21,14 @@
  *                 A = (1 + L)^-1 diag(b) and M
  *   linattn_scan  a workgroup for each sequence, head and 32 columns of v:
  *                 S in registers from the first chunk to the last,
- *                 D = A (V - K~ S), O, S'
+ *                 E = A (the right-hand side), O, S'
  *
  * Operands are two fp16 numbers hi + lo (22 bits) in three products
  * hi hi + hi lo + lo hi with binary32 sums: off by at most 2^-22 of a
  * product, 5 times the rate of binary32 products on these cores. The ranges
  * that fp16 lacks are kept outside: a row of k or q is scaled by a power of
- * two to below 1 and its norm becomes a factor of the row, A, the right-hand
- * sides, D and S carry a power of two for each workgroup (its largest value
- * at 2^14 .. 2^15: values down to 2^-17 of it keep all 22 bits, the rest an
- * error of 2^-40 of it). Log decays are summed in 64 bits, since their
+ * two to below 1 and its norm becomes a factor of the row; A, the right-hand
+ * sides, E and S carry a power of two for each workgroup. Log decays are summed in 64 bits, since their
  * differences are what counts.
  */
 #include "kq_linattn.h"
@@ -306,9 +306,9 @@ __global__ __launch_bounds__(256) void linattn_prep(kq_launch_linattn a, Work w,
             const float from = kq::exp_of(G), to = kq::exp_of(end - G);
             float *f = (float *)(w.data + (uint64_t)c * w.chunk_bytes + w.value_at +
                                  (uint64_t)h * w.value_bytes + kMat);
-            f[lane] = from * nks[lane];
+            f[lane] = from * nks[lane] * nks[lane];
             f[kC + lane] = nks[lane];
-            f[2 * kC + lane] = to * nks[lane];
+            f[2 * kC + lane] = to;
             f[3 * kC + lane] = nqs[lane];
             f[4 * kC + lane] = from * nqs[lane];
             const kq::Decay d = kq::decay_of((float)end);
@@ -329,14 +329,13 @@ __global__ __launch_bounds__(256) void linattn_prep(kq_launch_linattn a, Work w,
                 if (jt > (int)wave) continue;
                 const uint32_t j = 16u * jt + r16;
                 const double gj = sum[hh][j];
-                const float nkj = nks[j];
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     const uint32_t i = 16u * wave + 4u * g4 + r;
                     const float fall = j <= i ? kq::exp_of(gi[r] - gj) : 0.0f;
                     mixbuf[wave][4u * g4 + r][j] = qk[jt][r] * fall * (kMixUnit / kUnit / kUnit);
                     if (DELTA && j < i)
-                        solve[hh][i][j] = beta[hh][i] * nks[i] * nkj * fall *
+                        solve[hh][i][j] = beta[hh][i] * nks[i] * nks[i] * fall *
                                           (kk[jt][r] * (1.0f / kUnit / kUnit));
                 }
             }
@@ -413,262 +412,296 @@ __global__ __launch_bounds__(256) void linattn_prep(kq_launch_linattn a, Work w,
 /* ------------------------------------------------------------------ */
 
 constexpr uint32_t kTile = 32; /* columns of v that a workgroup holds */
+constexpr int kScanWaves = 8;
 
-/* a lane's part of an operand, hi and lo, N pieces 1024 bytes apart */
+/* a lane's part of an operand, hi and lo, N pieces 2048 bytes apart */
 template <int N>
 struct Frag {
     h8 hi[N], lo[N];
-    __device__ __forceinline__ void load(const char *p) {
+    __device__ __forceinline__ void load(KqBuf b, uint32_t lane16, uint32_t at) {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            hi[i] = *(const h8 *)(p + i * 2048);
-            lo[i] = *(const h8 *)(p + i * 2048 + 1024);
+            hi[i] = __builtin_bit_cast(h8, kq_ld128(b, lane16, at + i * 2048u));
+            lo[i] = __builtin_bit_cast(h8, kq_ld128(b, lane16, at + i * 2048u + 1024u));
+        }
+    }
+    __device__ __forceinline__ void read(const char *p, int step) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            hi[i] = *(const h8 *)(p + i * step);
+            lo[i] = *(const h8 *)(p + i * step + 1024);
         }
     }
 };
 
 /* Four values of consecutive rows (of which `row` is the first, in fours) of
- * column r16 of column tile ct, as part of the right operand at p */
+ * column r16 of column tile ct, times s, as part of the right operand at p */
 __device__ __forceinline__ void put(char *p, uint32_t row, uint32_t ct, uint32_t r16, const f4 &x,
                                     float s) {
-    float y[4];
-#pragma unroll
-    for (int r = 0; r < 4; ++r) y[r] = x[r] * s;
     h4 hi, lo;
-    split<4>(y, hi, lo);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) hi[r] = (_Float16)(x[r] * s);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) lo[r] = (_Float16)fmaf(x[r], s, -(float)hi[r]);
     char *to = p + (((row >> 5) * 2u + ct) * 2u) * 1024u + (((row & 31u) >> 3) * 16u + r16) * 16u +
                (row & 7u) * 2u;
     *(h4 *)to = hi;
     *(h4 *)(to + 1024u) = lo;
 }
 
-__device__ __forceinline__ float largest(float m, const f4 &x) {
-#pragma unroll
-    for (int r = 0; r < 4; ++r) m = fmaxf(m, fabsf(x[r]));
-    return m;
+__device__ __forceinline__ float largest(const f4 &x) {
+    return fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3])));
+}
+
+/* The scale of an operand that the workgroup's waves share, from one chunk
+ * to the next: a power of two under which the largest value lay at 2^13 when
+ * it was set. It holds while that value stays within 2^10 .. 2^15: values
+ * down to 2^-13 of the largest keep 22 bits, the others an error of 2^-35 of
+ * it. */
+struct Scale {
+    float s, inv;
+    __device__ __forceinline__ void set(float m) {
+        const int e = scale_exp(m) - 2;
+        s = pow2(e);
+        inv = pow2(-e);
+    }
+    __device__ __forceinline__ bool holds(float m) const {
+        const float y = m * s;
+        return y < 32768.0f && (y >= 1024.0f || m == 0.0f);
+    }
+};
+
+__device__ __forceinline__ float top_of(const float *p) {
+    const f4 a = *(const f4 *)p, b = *(const f4 *)(p + 4);
+    return fmaxf(fmaxf(fmaxf(a[0], a[1]), fmaxf(a[2], a[3])),
+                 fmaxf(fmaxf(b[0], b[1]), fmaxf(b[2], b[3])));
 }
 
 template <int DK, bool DELTA>
-__global__ __launch_bounds__(256) void linattn_scan(kq_launch_linattn a, kq_launch_seqs q, Work w,
-                                                    uint32_t *status) {
+__global__ __launch_bounds__(64 * kScanWaves) void linattn_scan(kq_launch_linattn a,
+                                                                kq_launch_seqs q, Work w,
+                                                                uint32_t *status) {
     constexpr int KS = DK / 32, RT = DK / 64;
+    constexpr uint32_t kKeyImage = 256u * DK;
     __shared__ __attribute__((aligned(16))) char sbuf[KS * 4096], rbuf[8192], ebuf[8192],
         fbuf[8192];
-    __shared__ float top[4][4]; /* largest values: of S, the right-hand sides, E, F by wave */
+    /* largest values by wave: of S, the right-hand sides, E, F */
+    __shared__ __attribute__((aligned(16))) float top[4][kScanWaves];
     const uint32_t s = blockIdx.y;
     const uint2 mine = w.seq[s];
     if (mine.y == 0u) return;
     bool badseq = false, bad = false, badin = false;
     const kq::SeqSpan sp = kq::seq_span(q, s, badseq);
     if (!sp.live) return;
-    const uint32_t lane = threadIdx.x & 63u, r16 = lane & 15u, g4 = lane >> 4;
+    const uint32_t lane = threadIdx.x & 63u, r16 = lane & 15u, g4 = lane >> 4, lane16 = lane * 16u;
+    /* a wave has 16 rows of a chunk, or RT x 16 rows of S, of 16 columns */
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t rt0 = wave >> 1, ct = wave & 1u, fr = 16u * rt0 + 4u * g4;
     /* workgroups go round the 8 XCDs: those of a head, which read the same
      * operands, to one of them */
     uint32_t b = blockIdx.x;
     if (gridDim.x % 8u == 0u) b = (b % 8u) * (gridDim.x / 8u) + b / 8u;
     const uint32_t tiles = a.value_width / kTile;
-    const uint32_t h = b / tiles, col = (b % tiles) * kTile + r16;
+    const uint32_t h = b / tiles, col = (b % tiles) * kTile + 16u * ct + r16;
     const uint32_t kh = h / (a.value_heads / a.key_heads);
     const size_t sat = ((size_t)sp.slot * a.value_heads + h) * DK * a.value_width + col;
 
-    f4 S[RT][2];
+    f4 S[RT];
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
-        for (int ct = 0; ct < 2; ++ct)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const uint32_t d = (wave * RT + rt) * 16u + 4u * g4 + r;
-                S[rt][ct][r] = sp.fresh ? 0.0f
-                                        : a.state[sat + (size_t)d * a.value_width + 16u * ct];
-            }
+        for (int r = 0; r < 4; ++r) {
+            const uint32_t d = (rt0 * RT + rt) * 16u + 4u * g4 + r;
+            S[rt][r] = sp.fresh ? 0.0f : a.state[sat + (size_t)d * a.value_width];
+        }
 
-    const char *kb = w.data + (uint64_t)mine.x * w.chunk_bytes + (uint64_t)kh * w.key_bytes;
-    const char *vb = w.data + (uint64_t)mine.x * w.chunk_bytes + w.value_at +
-                     (uint64_t)h * w.value_bytes;
-    constexpr uint32_t kKeyImage = 256u * DK;
+    const char *data = w.data + (uint64_t)mine.x * w.chunk_bytes;
+    const uint32_t kat = kh * w.key_bytes, vat = w.value_at + h * w.value_bytes;
+    const uint32_t aat = vat + kMat + kRowF * 4u;
+    uint32_t vo[4], yo[4]; /* the wave's rows of v and of the output, in bytes */
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+        vo[r] = ((fr + r) * (uint32_t)a.vs + col) * 4u;
+        yo[r] = ((fr + r) * (uint32_t)a.ys + col) * 4u;
+    }
     Frag<KS> K, Q;
     Frag<2> A, M, T[RT];
-    f4 V[2];
-    auto load_kq = [&](uint32_t n) {
-        const char *p = kb + (uint64_t)n * w.chunk_bytes + wave * KS * 2048u + lane * 16u;
-        if (DELTA) K.load(p);
-        Q.load(p + kKeyImage);
+    f4 V, nk, ne, nf, nq, np; /* rows of v and the rows' factors */
+    float n0, n1, na = 0.0f;
+    auto chunk = [&](uint32_t n) {
+        return kq_buf(data + (uint64_t)n * w.chunk_bytes, (uint32_t)w.chunk_bytes);
     };
-    auto load_v = [&](uint32_t n) {
+    auto load_kq = [&](KqBuf c) {
+        if (DELTA) K.load(c, lane16, kat + rt0 * KS * 2048u);
+        Q.load(c, lane16, kat + kKeyImage + rt0 * KS * 2048u);
+    };
+    auto load_v = [&](KqBuf c, uint32_t n) {
+        auto f = [&](uint32_t i) {
+            return __builtin_bit_cast(f4, kq_ld128(c, fr * 4u, vat + kMat + i * kC * 4u));
+        };
+        nk = f(0u);
+        ne = f(1u);
+        nf = f(2u);
+        nq = f(3u);
+        np = f(4u);
+        n0 = __uint_as_float(kq_ld32(c, 0u, vat + kMat + 5u * kC * 4u));
+        n1 = __uint_as_float(kq_ld32(c, 4u, vat + kMat + 5u * kC * 4u));
+        if (DELTA) na = __uint_as_float(kq_ld32(c, 8u, vat + kMat + 5u * kC * 4u));
+        const uint32_t left = sp.rows - n * kC; /* rows past it read as zeros */
+        const KqBuf v = kq_buf(a.v + ((uint64_t)sp.begin + n * kC) * a.vs + h * a.value_width,
+                               (left < kC ? left : kC) * (uint32_t)a.vs * 4u);
 #pragma unroll
-        for (int ct = 0; ct < 2; ++ct)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const uint32_t i = n * kC + 16u * wave + 4u * g4 + r;
-                V[ct][r] = i < sp.rows ? a.v[((uint64_t)sp.begin + i) * a.vs +
-                                             h * a.value_width + col + 16u * ct]
-                                       : 0.0f;
-            }
+        for (int r = 0; r < 4; ++r) V[r] = __uint_as_float(kq_ld32(v, vo[r], 0u));
     };
-    auto load_a = [&](uint32_t n) {
-        A.load(vb + (uint64_t)n * w.chunk_bytes + kMat + kRowF * 4u + wave * 4096u + lane * 16u);
-    };
-    auto load_mt = [&](uint32_t n) {
-        M.load(vb + (uint64_t)n * w.chunk_bytes + wave * 4096u + lane * 16u);
+    auto load_mt = [&](KqBuf c) {
+        M.load(c, lane16, vat + rt0 * 4096u);
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt)
-            T[rt].load(kb + (uint64_t)n * w.chunk_bytes + 2u * kKeyImage +
-                       (wave * RT + rt) * 4096u + lane * 16u);
+            T[rt].load(c, lane16, kat + 2u * kKeyImage + (rt0 * RT + rt) * 4096u);
     };
-    load_kq(0u);
-    load_v(0u);
-    if (DELTA) load_a(0u);
-    load_mt(0u);
+    {
+        const KqBuf c = chunk(0u);
+        load_kq(c);
+        load_v(c, 0u);
+        if (DELTA) A.load(c, lane16, aat + rt0 * 4096u);
+        load_mt(c);
+    }
+    /* S as an operand */
+    Scale ss, sr, se, sf;
+    ss.s = ss.inv = sr.s = sr.inv = se.s = se.inv = sf.s = sf.inv = 1.0f;
+    auto put_s = [&]() {
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt)
+            put(sbuf, (rt0 * RT + rt) * 16u + 4u * g4, ct, r16, S[rt], ss.s);
+    };
+    auto share_s = [&]() {
+        float m = largest(S[0]);
+#pragma unroll
+        for (int rt = 1; rt < RT; ++rt) m = fmaxf(m, largest(S[rt]));
+        m = kq::lanes_max<63>(m);
+        if (lane == 0u) top[0][wave] = m;
+        put_s();
+        kq_lds_barrier();
+        const float t = top_of(top[0]);
+        if (!ss.holds(t)) { /* the same in all waves, none of which has read on */
+            ss.set(t);
+            put_s();
+            kq_lds_barrier();
+        }
+    };
+    share_s();
 
     for (uint32_t n = 0; n < mine.y; ++n) {
         const uint32_t more = n + 1u < mine.y ? n + 1u : n; /* the last loads again */
-        const float *f = (const float *)(vb + (uint64_t)n * w.chunk_bytes + kMat);
-        const uint32_t fr = 16u * wave + 4u * g4;
-        const f4 fk = *(const f4 *)(f + fr), fe = *(const f4 *)(f + kC + fr),
-                 ff = *(const f4 *)(f + 2 * kC + fr), fq = *(const f4 *)(f + 3 * kC + fr),
-                 fp = *(const f4 *)(f + 4 * kC + fr);
-        const float c0 = f[5 * kC], c1 = f[5 * kC + 1], ia = DELTA ? f[5 * kC + 2] : 0.0f;
-
-        /* S as an operand */
-        float m = 0.0f;
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-            for (int ct = 0; ct < 2; ++ct) m = largest(m, S[rt][ct]);
-        m = kq::lanes_max<63>(m);
-        if (lane == 0u) top[0][wave] = m;
-        kq_lds_barrier();
-        const int es = scale_exp(fmaxf(fmaxf(top[0][0], top[0][1]), fmaxf(top[0][2], top[0][3])));
-        const float ss = pow2(es), is = ldexpf(1.0f / kUnit, -es);
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-            for (int ct = 0; ct < 2; ++ct)
-                put(sbuf, (wave * RT + rt) * 16u + 4u * g4, ct, r16, S[rt][ct], ss);
-        kq_lds_barrier();
+        const KqBuf next = chunk(more);
+        const f4 fk = nk, fe = ne, ff = nf, fq = nq, fp = np;
+        const float c0 = n0, c1 = n1, ia = na;
 
         /* K S and Q S for the wave's 16 rows */
-        f4 X[2], P[2];
+        f4 X = f4{0.0f, 0.0f, 0.0f, 0.0f}, P = X;
+        {
+            Frag<KS> B;
+            B.read(sbuf + ct * 2048u + lane16, 4096);
 #pragma unroll
-        for (int ct = 0; ct < 2; ++ct) X[ct] = P[ct] = f4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks)
-#pragma unroll
-            for (int ct = 0; ct < 2; ++ct) {
-                const char *p = sbuf + ((ks * 2 + ct) * 2) * 1024 + lane * 16u;
-                const h8 bh = *(const h8 *)p, bl = *(const h8 *)(p + 1024);
-                if (DELTA) X[ct] = mfma3(K.hi[ks], K.lo[ks], bh, bl, X[ct]);
-                P[ct] = mfma3(Q.hi[ks], Q.lo[ks], bh, bl, P[ct]);
+            for (int ks = 0; ks < KS; ++ks) {
+                if (DELTA) X = mfma3(K.hi[ks], K.lo[ks], B.hi[ks], B.lo[ks], X);
+                P = mfma3(Q.hi[ks], Q.lo[ks], B.hi[ks], B.lo[ks], P);
             }
-        load_kq(more);
-
-        f4 D[2];
+        }
+        load_kq(next);
+        const float is = ss.inv * (1.0f / kUnit);
+        f4 E;
 #pragma unroll
-        for (int ct = 0; ct < 2; ++ct)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                badin |= !kq_isfinite(V[ct][r]);
-                D[ct][r] = DELTA ? V[ct][r] - fk[r] * (X[ct][r] * is) : V[ct][r];
-            }
-        load_v(more);
+        for (int r = 0; r < 4; ++r) {
+            badin |= !kq_isfinite(V[r]);
+            E[r] = fe[r] * V[r];
+            if (DELTA) E[r] -= fk[r] * (X[r] * is);
+        }
+        load_v(next, more);
         if (DELTA) {
-            /* D = A (V - K~ S) */
-            m = kq::lanes_max<63>(largest(largest(0.0f, D[0]), D[1]));
+            /* E = A E */
+            const float m = kq::lanes_max<63>(largest(E));
             if (lane == 0u) top[1][wave] = m;
+            put(rbuf, fr, ct, r16, E, sr.s);
             kq_lds_barrier();
-            const int er =
-                scale_exp(fmaxf(fmaxf(top[1][0], top[1][1]), fmaxf(top[1][2], top[1][3])));
-            const float sr = pow2(er);
-#pragma unroll
-            for (int ct = 0; ct < 2; ++ct) put(rbuf, fr, ct, r16, D[ct], sr);
-            kq_lds_barrier();
-            const float ir = ia * pow2(-er);
-#pragma unroll
-            for (int ct = 0; ct < 2; ++ct) {
-                f4 x = f4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                for (int ks = 0; ks < 2; ++ks) {
-                    const char *p = rbuf + ((ks * 2 + ct) * 2) * 1024 + lane * 16u;
-                    x = mfma3(A.hi[ks], A.lo[ks], *(const h8 *)p, *(const h8 *)(p + 1024), x);
-                }
-                D[ct] = x * ir;
+            const float t = top_of(top[1]);
+            if (!sr.holds(t)) {
+                sr.set(t);
+                put(rbuf, fr, ct, r16, E, sr.s);
+                kq_lds_barrier();
             }
-            load_a(more);
-        }
-        /* E: rows of D times the norm of k; F: and the decay to the chunk's end */
-        f4 E[2], F[2];
-        float me = 0.0f, mf = 0.0f;
+            Frag<2> B;
+            B.read(rbuf + ct * 2048u + lane16, 4096);
+            f4 x = f4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int ct = 0; ct < 2; ++ct) {
-            E[ct] = D[ct] * fe;
-            F[ct] = D[ct] * ff;
-            me = largest(me, E[ct]);
-            mf = largest(mf, F[ct]);
+            for (int ks = 0; ks < 2; ++ks)
+                x = mfma3(A.hi[ks], A.lo[ks], B.hi[ks], B.lo[ks], x);
+            E = x * (ia * sr.inv);
+            A.load(next, lane16, aat + rt0 * 4096u);
         }
-        me = kq::lanes_max<63>(me);
-        mf = kq::lanes_max<63>(mf);
-        if (lane == 0u) {
-            top[2][wave] = me;
-            top[3][wave] = mf;
+        /* and with the decay to the chunk's end */
+        const f4 F = E * ff;
+        {
+            const float me = kq::lanes_max<63>(largest(E)), mf = kq::lanes_max<63>(largest(F));
+            if (lane == 0u) {
+                top[2][wave] = me;
+                top[3][wave] = mf;
+            }
+            put(ebuf, fr, ct, r16, E, se.s);
+            put(fbuf, fr, ct, r16, F, sf.s);
+            kq_lds_barrier();
+            const float te = top_of(top[2]), tf = top_of(top[3]);
+            if (!se.holds(te) || !sf.holds(tf)) {
+                se.set(te);
+                sf.set(tf);
+                put(ebuf, fr, ct, r16, E, se.s);
+                put(fbuf, fr, ct, r16, F, sf.s);
+                kq_lds_barrier();
+            }
         }
-        kq_lds_barrier();
-        const int ee = scale_exp(fmaxf(fmaxf(top[2][0], top[2][1]), fmaxf(top[2][2], top[2][3])));
-        const int ef = scale_exp(fmaxf(fmaxf(top[3][0], top[3][1]), fmaxf(top[3][2], top[3][3])));
-        const float se = pow2(ee), sf = pow2(ef);
+        /* S' = e^G S + K^T F, and O = Q~ S + M E */
+        f4 O = f4{0.0f, 0.0f, 0.0f, 0.0f}, x[RT];
+        {
+            Frag<2> BE, BF;
+            BF.read(fbuf + ct * 2048u + lane16, 4096);
+            BE.read(ebuf + ct * 2048u + lane16, 4096);
 #pragma unroll
-        for (int ct = 0; ct < 2; ++ct) {
-            put(ebuf, fr, ct, r16, E[ct], se);
-            put(fbuf, fr, ct, r16, F[ct], sf);
-        }
-        kq_lds_barrier();
-        const float ie = ldexpf(1.0f / kMixUnit, -ee), jf = ldexpf(1.0f / kUnit, -ef);
-        /* O = Q~ S + M E and S' = e^G S + K^T F */
-        f4 O[2];
-#pragma unroll
-        for (int ct = 0; ct < 2; ++ct) {
-            O[ct] = f4{0.0f, 0.0f, 0.0f, 0.0f};
-            f4 x[RT];
-#pragma unroll
-            for (int rt = 0; rt < RT; ++rt) x[rt] = O[ct];
+            for (int rt = 0; rt < RT; ++rt) x[rt] = O;
 #pragma unroll
             for (int ks = 0; ks < 2; ++ks) {
-                const uint32_t at = ((ks * 2 + ct) * 2) * 1024 + lane * 16u;
-                const h8 eh = *(const h8 *)(ebuf + at), el = *(const h8 *)(ebuf + at + 1024);
-                const h8 fh = *(const h8 *)(fbuf + at), fl = *(const h8 *)(fbuf + at + 1024);
-                O[ct] = mfma3(M.hi[ks], M.lo[ks], eh, el, O[ct]);
 #pragma unroll
-                for (int rt = 0; rt < RT; ++rt) x[rt] = mfma3(T[rt].hi[ks], T[rt].lo[ks], fh, fl, x[rt]);
+                for (int rt = 0; rt < RT; ++rt)
+                    x[rt] = mfma3(T[rt].hi[ks], T[rt].lo[ks], BF.hi[ks], BF.lo[ks], x[rt]);
+                O = mfma3(M.hi[ks], M.lo[ks], BE.hi[ks], BE.lo[ks], O);
             }
-#pragma unroll
-            for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-                for (int r = 0; r < 4; ++r)
-                    S[rt][ct][r] = fmaf(x[rt][r], jf, fmaf(c1, S[rt][ct][r], c0 * S[rt][ct][r]));
         }
-        load_mt(more);
+        load_mt(next);
+        const float jf = sf.inv * (1.0f / kUnit), ie = se.inv * (1.0f / kMixUnit);
 #pragma unroll
-        for (int ct = 0; ct < 2; ++ct)
+        for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const uint32_t i = n * kC + fr + r;
-                const float o = fmaf(fp[r], P[ct][r] * is, fq[r] * (O[ct][r] * ie));
-                bad |= !kq_isfinite(o);
-                if (i < sp.rows)
-                    a.y[((uint64_t)sp.begin + i) * a.ys + h * a.value_width + col + 16u * ct] = o;
-            }
+            for (int r = 0; r < 4; ++r)
+                S[rt][r] = fmaf(x[rt][r], jf, fmaf(c1, S[rt][r], c0 * S[rt][r]));
+        share_s();
+        const uint32_t left = sp.rows - n * kC;
+        const KqBuf y = kq_buf(a.y + ((uint64_t)sp.begin + n * kC) * a.ys + h * a.value_width,
+                               (left < kC ? left : kC) * (uint32_t)a.ys * 4u);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const float o = fmaf(fp[r], P[r] * is, fq[r] * (O[r] * ie));
+            bad |= !kq_isfinite(o);
+            /* rows past the sequence's last are past the buffer: not written */
+            __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(o), y.r, (int)yo[r], 0, 0);
+        }
     }
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
-        for (int ct = 0; ct < 2; ++ct)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const uint32_t d = (wave * RT + rt) * 16u + 4u * g4 + r;
-                bad |= !kq_isfinite(S[rt][ct][r]);
-                a.state_out[sat + (size_t)d * a.value_width + 16u * ct] = S[rt][ct][r];
-            }
+        for (int r = 0; r < 4; ++r) {
+            const uint32_t d = (rt0 * RT + rt) * 16u + 4u * g4 + r;
+            bad |= !kq_isfinite(S[rt][r]);
+            a.state_out[sat + (size_t)d * a.value_width] = S[rt][r];
+        }
     if (badin) kq_flag(status, KQ_DEV_INPUT);
     if (bad) kq_flag(status, KQ_DEV_NUMERIC);
 }
@@ -709,8 +742,8 @@ hipError_t run(const kq_launch_linattn &a, const kq_launch_seqs &q, const Work &
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     hipLaunchKernelGGL(HIP_KERNEL_NAME(linattn_scan<DK, DELTA>),
-                       dim3(a.value_heads * (a.value_width / kTile), q.count), dim3(256), 0, s, a,
-                       q, w, status);
+                       dim3(a.value_heads * (a.value_width / kTile), q.count),
+                       dim3(64 * kScanWaves), 0, s, a, q, w, status);
     return hipGetLastError();
 }
 

@@ -91,20 +91,44 @@ __device__ __forceinline__ float sigmoid(float x) {
     return x >= 0.0f ? r : e * r;
 }
 
-/* sum over the lanes that differ in the bits of MASK */
+/* x of lane l ^ BIT, bits below 16: DPP controls, for bit 4 the half-row
+ * mirror where the lanes of a quad hold the same already (QUAD) */
+template <int BIT, bool QUAD>
+__device__ __forceinline__ float lane_xor(float x) {
+    if constexpr (BIT == 4 && !QUAD) return __shfl_xor(x, 4, KQ_WAVE);
+    constexpr int ctrl = BIT == 1 ? 0xB1 : BIT == 2 ? 0x4E : BIT == 4 ? 0x141 : 0x128;
+    return __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(x), ctrl,
+                                                                 0xf, 0xf, false));
+}
+
+/* v over the lanes that differ in the bits of MASK, by an operation that does
+ * not look at the order of its two operands; rows of 16 lanes are swapped
+ * (bits 16 and 32), so that nothing goes through LDS */
+template <int MASK, int BIT = 1, typename Op>
+__device__ __forceinline__ float lanes_all(float v, Op op) {
+    if constexpr (BIT < 64) {
+        if constexpr ((MASK & BIT) != 0) {
+            if constexpr (BIT == 16 || BIT == 32) {
+                const uint32_t u = __float_as_uint(v);
+                auto r = BIT == 16 ? __builtin_amdgcn_permlane16_swap(u, u, false, false)
+                                   : __builtin_amdgcn_permlane32_swap(u, u, false, false);
+                v = op(__uint_as_float(r[0]), __uint_as_float(r[1]));
+            } else {
+                v = op(v, lane_xor<BIT, (MASK & 3) == 3>(v));
+            }
+        }
+        return lanes_all<MASK, BIT * 2>(v, op);
+    } else {
+        return v;
+    }
+}
 template <int MASK>
 __device__ __forceinline__ float lanes_sum(float v) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1)
-        if (MASK & o) v += __shfl_xor(v, o, KQ_WAVE);
-    return v;
+    return lanes_all<MASK>(v, [](float a, float b) { return a + b; });
 }
 template <int MASK>
 __device__ __forceinline__ float lanes_max(float v) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1)
-        if (MASK & o) v = fmaxf(v, __shfl_xor(v, o, KQ_WAVE));
-    return v;
+    return lanes_all<MASK>(v, [](float a, float b) { return fmaxf(a, b); });
 }
 
 }  // namespace kq

@@ -55,9 +55,9 @@ static int aliased(const span *outs, uint32_t n, const span *ins, uint32_t m,
     return 0;
 }
 
-/* a row stride in floats: at least the row, and far from a 64-bit overflow */
+/* a row stride in floats: at least the row; 64 rows within 32-bit offsets */
 static int stride_ok(uint64_t stride, uint64_t width) {
-    return stride >= width && stride <= (UINT64_C(1) << 32);
+    return stride >= width && stride <= (UINT64_C(1) << 22);
 }
 
 static kq_status sequences_ok(const kq_hip_sequences *q, kq_diagnostic *diag) {
@@ -110,7 +110,7 @@ kq_status kq_hip_causal_conv_f32(kq_hip_context *c, const kq_hip_causal_conv *v,
     st = sequences_ok(q, diag);
     if (st != KQ_STATUS_OK) return st;
     if (!stride_ok(xs, v->channels) || !stride_ok(ys, v->channels))
-        return kq_fail(diag, KQ_STATUS_DIMENSION_MISMATCH, "row strides hold the channels at least");
+        return kq_fail(diag, KQ_STATUS_DIMENSION_MISMATCH, "row strides hold the channels and at most 2^22 floats");
     if (!on(x, 4u) || !on(y, 4u) || !on(state, 4u) || !on(state_out, 4u) || !on(v->weight, 4u) ||
         !on(v->bias, 4u))
         return kq_fail(diag, KQ_STATUS_INVALID_ALIGNMENT, "convolution buffers need 4-byte alignment");
@@ -218,7 +218,7 @@ kq_status kq_hip_linear_attention_f32(kq_hip_context *c, const kq_hip_linear_att
         !stride_ok(in->value_stride, vw) || !stride_ok(ys, vw) ||
         (in->alpha != NULL && !stride_ok(in->alpha_stride, a->value_heads)) ||
         (in->beta != NULL && !stride_ok(in->beta_stride, a->value_heads)))
-        return kq_fail(diag, KQ_STATUS_DIMENSION_MISMATCH, "row strides hold the heads at least");
+        return kq_fail(diag, KQ_STATUS_DIMENSION_MISMATCH, "row strides hold the heads and at most 2^22 floats");
     need = kq_hip_linear_attention_scratch_bytes(a, q);
     if (need != 0u && scratch == NULL)
         return kq_fail(diag, KQ_STATUS_INVALID_ARGUMENT, "linear attention scratch is required");
@@ -304,13 +304,13 @@ kq_status kq_hip_gated_norm_f32(kq_hip_context *c, const kq_hip_gated_norm *v, u
     if (!isfinite(v->epsilon) || !(v->epsilon > 0.0f) || !isfinite(v->weight_offset))
         return kq_fail(diag, KQ_STATUS_INVALID_ARGUMENT,
                        "the norm needs a positive epsilon and a finite weight offset");
-    if (v->width > KQ_MAX_WIDTH || v->groups > (1u << 20) || tokens > KQ_MAX_TOKENS)
+    if (v->width > KQ_MAX_WIDTH || (uint64_t)v->groups * v->width > (1u << 22) || tokens > KQ_MAX_TOKENS)
         return kq_fail(diag, KQ_STATUS_LIMIT_EXCEEDED,
-                       "norm: groups of at most %u, 2^20 groups, %u tokens", KQ_MAX_WIDTH,
+                       "norm: groups of at most %u, rows of 2^22, %u tokens", KQ_MAX_WIDTH,
                        KQ_MAX_TOKENS);
     w = (uint64_t)v->groups * v->width;
     if (!stride_ok(xs, w) || !stride_ok(ys, w) || (gated && !stride_ok(gs, w)))
-        return kq_fail(diag, KQ_STATUS_DIMENSION_MISMATCH, "row strides hold the groups at least");
+        return kq_fail(diag, KQ_STATUS_DIMENSION_MISMATCH, "row strides hold the groups and at most 2^22 floats");
     if (!on(x, 4u) || !on(y, 4u) || (gated && !on(gate, 4u)) || !on(v->weight, 4u))
         return kq_fail(diag, KQ_STATUS_INVALID_ALIGNMENT, "norm buffers need 4-byte alignment");
     {
