@@ -472,21 +472,28 @@ struct Scale {
 };
 
 __device__ __forceinline__ float top_of(const float *p) {
-    const f4 a = *(const f4 *)p, b = *(const f4 *)(p + 4);
-    return fmaxf(fmaxf(fmaxf(a[0], a[1]), fmaxf(a[2], a[3])),
-                 fmaxf(fmaxf(b[0], b[1]), fmaxf(b[2], b[3])));
+    const f4 a = *(const f4 *)p;
+    return fmaxf(fmaxf(a[0], a[1]), fmaxf(a[2], a[3]));
 }
 
+/*
+ * Eight waves. Waves 0 .. 3 (the solvers) form K' S for 16 rows of the chunk
+ * each, the right-hand sides and E; waves 4 .. 7 (the writers) Q S for 16 rows
+ * each, the chunk's output, one phase behind, and its stores; every wave
+ * holds 16 rows of S and forms their K'^T F. So an operand is loaded by one
+ * wave, for both column tiles, and what no other step waits for runs beside
+ * the chain S -> E -> S'. Three phases a chunk, with a barrier each.
+ */
 template <int DK, bool DELTA>
 __global__ __launch_bounds__(64 * kScanWaves) void linattn_scan(kq_launch_linattn a,
                                                                 kq_launch_seqs q, Work w,
                                                                 uint32_t *status) {
-    constexpr int KS = DK / 32, RT = DK / 64;
+    constexpr int KS = DK / 32, NU = DK / 64; /* steps over S's rows; tiles of S a wave holds */
     constexpr uint32_t kKeyImage = 256u * DK;
-    __shared__ __attribute__((aligned(16))) char sbuf[KS * 4096], rbuf[8192], ebuf[8192],
+    __shared__ __attribute__((aligned(16))) char sbuf[KS * 4096], rbuf[8192], ebuf[2][8192],
         fbuf[8192];
     /* largest values by wave: of S, the right-hand sides, E, F */
-    __shared__ __attribute__((aligned(16))) float top[4][kScanWaves];
+    __shared__ __attribute__((aligned(16))) float top_s[8], top_r[4], top_e[4], top_f[4];
     const uint32_t s = blockIdx.y;
     const uint2 mine = w.seq[s];
     if (mine.y == 0u) return;
@@ -494,213 +501,299 @@ __global__ __launch_bounds__(64 * kScanWaves) void linattn_scan(kq_launch_linatt
     const kq::SeqSpan sp = kq::seq_span(q, s, badseq);
     if (!sp.live) return;
     const uint32_t lane = threadIdx.x & 63u, r16 = lane & 15u, g4 = lane >> 4, lane16 = lane * 16u;
-    /* a wave has 16 rows of a chunk, or RT x 16 rows of S, of 16 columns */
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const uint32_t rt0 = wave >> 1, ct = wave & 1u, fr = 16u * rt0 + 4u * g4;
+    const bool solver = wave < 4u;
+    const uint32_t rt = wave & 3u, fr = 16u * rt + 4u * g4; /* rows of the chunk */
+    const uint32_t srt = DK == 128 ? wave : wave >> 1, sct = DK == 128 ? 0u : wave & 1u;
+    const uint32_t srow = 16u * srt + 4u * g4; /* rows of S, from column tile sct on */
     /* workgroups go round the 8 XCDs: those of a head, which read the same
      * operands, to one of them */
     uint32_t b = blockIdx.x;
     if (gridDim.x % 8u == 0u) b = (b % 8u) * (gridDim.x / 8u) + b / 8u;
     const uint32_t tiles = a.value_width / kTile;
-    const uint32_t h = b / tiles, col = (b % tiles) * kTile + 16u * ct + r16;
+    const uint32_t h = b / tiles, col = (b % tiles) * kTile + r16;
     const uint32_t kh = h / (a.value_heads / a.key_heads);
-    const size_t sat = ((size_t)sp.slot * a.value_heads + h) * DK * a.value_width + col;
+    const size_t sat = (((size_t)sp.slot * a.value_heads + h) * DK + srow) * a.value_width + col +
+                       16u * sct;
 
-    f4 S[RT];
+    f4 S[NU];
 #pragma unroll
-    for (int rt = 0; rt < RT; ++rt)
+    for (int u = 0; u < NU; ++u)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const uint32_t d = (rt0 * RT + rt) * 16u + 4u * g4 + r;
-            S[rt][r] = sp.fresh ? 0.0f : a.state[sat + (size_t)d * a.value_width];
-        }
+        for (int r = 0; r < 4; ++r)
+            S[u][r] = sp.fresh ? 0.0f : a.state[sat + (size_t)r * a.value_width + 16u * u];
 
     const char *data = w.data + (uint64_t)mine.x * w.chunk_bytes;
     const uint32_t kat = kh * w.key_bytes, vat = w.value_at + h * w.value_bytes;
-    const uint32_t aat = vat + kMat + kRowF * 4u;
-    uint32_t vo[4], yo[4]; /* the wave's rows of v and of the output, in bytes */
+    const uint32_t fat = vat + kMat;                              /* the rows' factors */
+    const uint32_t at1 = kat + (solver ? 0u : kKeyImage) + rt * KS * 2048u; /* K' or Q */
+    const uint32_t at2 = vat + (solver ? kMat + kRowF * 4u : 0u) + rt * 4096u; /* A or M */
+    const uint32_t at3 = kat + 2u * kKeyImage + srt * 4096u;      /* K'^T */
+    uint32_t io[4]; /* the wave's rows of v or of the output, in bytes */
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-        vo[r] = ((fr + r) * (uint32_t)a.vs + col) * 4u;
-        yo[r] = ((fr + r) * (uint32_t)a.ys + col) * 4u;
-    }
-    Frag<KS> K, Q;
-    Frag<2> A, M, T[RT];
-    f4 V, nk, ne, nf, nq, np; /* rows of v and the rows' factors */
-    float n0, n1, na = 0.0f;
+    for (int r = 0; r < 4; ++r)
+        io[r] = ((fr + r) * (uint32_t)(solver ? a.vs : a.ys) + col) * 4u;
+    Frag<KS> W1;
+    Frag<2> W2, T;
+    float n0, n1;
     auto chunk = [&](uint32_t n) {
         return kq_buf(data + (uint64_t)n * w.chunk_bytes, (uint32_t)w.chunk_bytes);
     };
-    auto load_kq = [&](KqBuf c) {
-        if (DELTA) K.load(c, lane16, kat + rt0 * KS * 2048u);
-        Q.load(c, lane16, kat + kKeyImage + rt0 * KS * 2048u);
+    auto factors = [&](KqBuf c, uint32_t i) {
+        return __builtin_bit_cast(f4, kq_ld128(c, fr * 4u, fat + i * kC * 4u));
     };
-    auto load_v = [&](KqBuf c, uint32_t n) {
-        auto f = [&](uint32_t i) {
-            return __builtin_bit_cast(f4, kq_ld128(c, fr * 4u, vat + kMat + i * kC * 4u));
-        };
-        nk = f(0u);
-        ne = f(1u);
-        nf = f(2u);
-        nq = f(3u);
-        np = f(4u);
-        n0 = __uint_as_float(kq_ld32(c, 0u, vat + kMat + 5u * kC * 4u));
-        n1 = __uint_as_float(kq_ld32(c, 4u, vat + kMat + 5u * kC * 4u));
-        if (DELTA) na = __uint_as_float(kq_ld32(c, 8u, vat + kMat + 5u * kC * 4u));
-        const uint32_t left = sp.rows - n * kC; /* rows past it read as zeros */
-        const KqBuf v = kq_buf(a.v + ((uint64_t)sp.begin + n * kC) * a.vs + h * a.value_width,
-                               (left < kC ? left : kC) * (uint32_t)a.vs * 4u);
-#pragma unroll
-        for (int r = 0; r < 4; ++r) V[r] = __uint_as_float(kq_ld32(v, vo[r], 0u));
+    auto scalar = [&](KqBuf c, uint32_t i) {
+        return __uint_as_float(kq_ld32(c, i * 4u, fat + 5u * kC * 4u));
     };
-    auto load_mt = [&](KqBuf c) {
-        M.load(c, lane16, vat + rt0 * 4096u);
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt)
-            T[rt].load(c, lane16, kat + 2u * kKeyImage + (rt0 * RT + rt) * 4096u);
+    auto load_end = [&](KqBuf c) {
+        T.load(c, lane16, at3);
+        n0 = scalar(c, 0u);
+        n1 = scalar(c, 1u);
     };
-    {
-        const KqBuf c = chunk(0u);
-        load_kq(c);
-        load_v(c, 0u);
-        if (DELTA) A.load(c, lane16, aat + rt0 * 4096u);
-        load_mt(c);
-    }
     /* S as an operand */
     Scale ss, sr, se, sf;
     ss.s = ss.inv = sr.s = sr.inv = se.s = se.inv = sf.s = sf.inv = 1.0f;
     auto put_s = [&]() {
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt)
-            put(sbuf, (rt0 * RT + rt) * 16u + 4u * g4, ct, r16, S[rt], ss.s);
+        for (int u = 0; u < NU; ++u) put(sbuf, srow, sct + u, r16, S[u], ss.s);
     };
     auto share_s = [&]() {
         float m = largest(S[0]);
 #pragma unroll
-        for (int rt = 1; rt < RT; ++rt) m = fmaxf(m, largest(S[rt]));
+        for (int u = 1; u < NU; ++u) m = fmaxf(m, largest(S[u]));
         m = kq::lanes_max<63>(m);
-        if (lane == 0u) top[0][wave] = m;
+        if (lane == 0u) top_s[wave] = m;
         put_s();
         kq_lds_barrier();
-        const float t = top_of(top[0]);
+        const float t = fmaxf(top_of(top_s), top_of(top_s + 4));
         if (!ss.holds(t)) { /* the same in all waves, none of which has read on */
             ss.set(t);
             put_s();
             kq_lds_barrier();
         }
     };
-    share_s();
-
-    for (uint32_t n = 0; n < mine.y; ++n) {
-        const uint32_t more = n + 1u < mine.y ? n + 1u : n; /* the last loads again */
-        const KqBuf next = chunk(more);
-        const f4 fk = nk, fe = ne, ff = nf, fq = nq, fp = np;
-        const float c0 = n0, c1 = n1, ia = na;
-
-        /* K S and Q S for the wave's 16 rows */
-        f4 X = f4{0.0f, 0.0f, 0.0f, 0.0f}, P = X;
-        {
-            Frag<KS> B;
-            B.read(sbuf + ct * 2048u + lane16, 4096);
+    /* the wave's 16 rows of W1 times S */
+    auto times_s = [&](f4(&x)[2]) {
+        Frag<KS> B[2];
 #pragma unroll
-            for (int ks = 0; ks < KS; ++ks) {
-                if (DELTA) X = mfma3(K.hi[ks], K.lo[ks], B.hi[ks], B.lo[ks], X);
-                P = mfma3(Q.hi[ks], Q.lo[ks], B.hi[ks], B.lo[ks], P);
-            }
+        for (int ct = 0; ct < 2; ++ct) {
+            B[ct].read(sbuf + ct * 2048u + lane16, 4096);
+            x[ct] = f4{0.0f, 0.0f, 0.0f, 0.0f};
         }
-        load_kq(next);
-        const float is = ss.inv * (1.0f / kUnit);
-        f4 E;
+        __builtin_amdgcn_sched_barrier(0); /* all reads in flight, then the products */
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            badin |= !kq_isfinite(V[r]);
-            E[r] = fe[r] * V[r];
-            if (DELTA) E[r] -= fk[r] * (X[r] * is);
+        for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+            for (int ct = 0; ct < 2; ++ct)
+                x[ct] = mfma3(W1.hi[ks], W1.lo[ks], B[ct].hi[ks], B[ct].lo[ks], x[ct]);
+    };
+    /* its 16 rows of W2 times the operand at p */
+    auto times = [&](const char *p, f4(&x)[2]) {
+        Frag<2> B[2];
+#pragma unroll
+        for (int ct = 0; ct < 2; ++ct) {
+            B[ct].read(p + ct * 2048u + lane16, 4096);
+            x[ct] = f4{0.0f, 0.0f, 0.0f, 0.0f};
         }
-        load_v(next, more);
-        if (DELTA) {
-            /* E = A E */
-            const float m = kq::lanes_max<63>(largest(E));
-            if (lane == 0u) top[1][wave] = m;
-            put(rbuf, fr, ct, r16, E, sr.s);
-            kq_lds_barrier();
-            const float t = top_of(top[1]);
-            if (!sr.holds(t)) {
-                sr.set(t);
-                put(rbuf, fr, ct, r16, E, sr.s);
-                kq_lds_barrier();
-            }
-            Frag<2> B;
-            B.read(rbuf + ct * 2048u + lane16, 4096);
-            f4 x = f4{0.0f, 0.0f, 0.0f, 0.0f};
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int ks = 0; ks < 2; ++ks)
-                x = mfma3(A.hi[ks], A.lo[ks], B.hi[ks], B.lo[ks], x);
-            E = x * (ia * sr.inv);
-            A.load(next, lane16, aat + rt0 * 4096u);
+        for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+            for (int ct = 0; ct < 2; ++ct)
+                x[ct] = mfma3(W2.hi[ks], W2.lo[ks], B[ct].hi[ks], B[ct].lo[ks], x[ct]);
+    };
+    /* phase 3 of both: S' = e^G S + K'^T F */
+    auto next_s = [&](KqBuf next) {
+        Frag<2> B[NU];
+        f4 x[NU];
+#pragma unroll
+        for (int u = 0; u < NU; ++u) {
+            B[u].read(fbuf + (sct + u) * 2048u + lane16, 4096);
+            x[u] = f4{0.0f, 0.0f, 0.0f, 0.0f};
         }
-        /* and with the decay to the chunk's end */
-        const f4 F = E * ff;
-        {
-            const float me = kq::lanes_max<63>(largest(E)), mf = kq::lanes_max<63>(largest(F));
-            if (lane == 0u) {
-                top[2][wave] = me;
-                top[3][wave] = mf;
-            }
-            put(ebuf, fr, ct, r16, E, se.s);
-            put(fbuf, fr, ct, r16, F, sf.s);
-            kq_lds_barrier();
-            const float te = top_of(top[2]), tf = top_of(top[3]);
-            if (!se.holds(te) || !sf.holds(tf)) {
-                se.set(te);
-                sf.set(tf);
-                put(ebuf, fr, ct, r16, E, se.s);
-                put(fbuf, fr, ct, r16, F, sf.s);
-                kq_lds_barrier();
-            }
-        }
-        /* S' = e^G S + K^T F, and O = Q~ S + M E */
-        f4 O = f4{0.0f, 0.0f, 0.0f, 0.0f}, x[RT];
-        {
-            Frag<2> BE, BF;
-            BF.read(fbuf + ct * 2048u + lane16, 4096);
-            BE.read(ebuf + ct * 2048u + lane16, 4096);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int rt = 0; rt < RT; ++rt) x[rt] = O;
+        for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
-            for (int ks = 0; ks < 2; ++ks) {
+            for (int u = 0; u < NU; ++u)
+                x[u] = mfma3(T.hi[ks], T.lo[ks], B[u].hi[ks], B[u].lo[ks], x[u]);
+        const float jf = sf.inv * (1.0f / kUnit);
 #pragma unroll
-                for (int rt = 0; rt < RT; ++rt)
-                    x[rt] = mfma3(T[rt].hi[ks], T[rt].lo[ks], BF.hi[ks], BF.lo[ks], x[rt]);
-                O = mfma3(M.hi[ks], M.lo[ks], BE.hi[ks], BE.lo[ks], O);
-            }
-        }
-        load_mt(next);
-        const float jf = sf.inv * (1.0f / kUnit), ie = se.inv * (1.0f / kMixUnit);
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt)
+        for (int u = 0; u < NU; ++u)
 #pragma unroll
             for (int r = 0; r < 4; ++r)
-                S[rt][r] = fmaf(x[rt][r], jf, fmaf(c1, S[rt][r], c0 * S[rt][r]));
+                S[u][r] = fmaf(x[u][r], jf, fmaf(n1, S[u][r], n0 * S[u][r]));
+        load_end(next);
         share_s();
-        const uint32_t left = sp.rows - n * kC;
-        const KqBuf y = kq_buf(a.y + ((uint64_t)sp.begin + n * kC) * a.ys + h * a.value_width,
-                               (left < kC ? left : kC) * (uint32_t)a.ys * 4u);
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const float o = fmaf(fp[r], P[r] * is, fq[r] * (O[r] * ie));
-            bad |= !kq_isfinite(o);
-            /* rows past the sequence's last are past the buffer: not written */
-            __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(o), y.r, (int)yo[r], 0, 0);
+    };
+    /* whether the scales of a barrier held; the same in all waves */
+    auto held_r = [&]() {
+        const float t = top_of(top_r);
+        const bool ok = sr.holds(t);
+        if (!ok) sr.set(t);
+        return ok;
+    };
+    auto held_ef = [&]() {
+        const float te = top_of(top_e), tf = top_of(top_f);
+        const bool ok = se.holds(te) && sf.holds(tf);
+        if (!ok) {
+            se.set(te);
+            sf.set(tf);
         }
+        return ok;
+    };
+    const uint32_t last = mine.y - 1u;
+
+    if (solver) {
+        f4 V[2], f0, f1, f2; /* n^2 e^G, n, e^(G_64 - G) */
+        float na = 0.0f;
+        auto load_v = [&](KqBuf c, uint32_t n) {
+            f1 = factors(c, 1u);
+            if (DELTA) f0 = factors(c, 0u);
+            const uint32_t left = sp.rows - n * kC; /* rows past it read as zeros */
+            const KqBuf v = kq_buf(a.v + ((uint64_t)sp.begin + n * kC) * a.vs + h * a.value_width,
+                                   (left < kC ? left : kC) * (uint32_t)a.vs * 4u);
+#pragma unroll
+            for (int ct = 0; ct < 2; ++ct)
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    V[ct][r] = __uint_as_float(kq_ld32(v, io[r], 64u * ct));
+        };
+        auto load_a = [&](KqBuf c) {
+            f2 = factors(c, 2u);
+            if (DELTA) {
+                na = scalar(c, 2u);
+                W2.load(c, lane16, at2);
+            }
+        };
+        const KqBuf first = chunk(0u);
+        if (DELTA) W1.load(first, lane16, at1);
+        load_v(first, 0u);
+        load_a(first);
+        load_end(first);
+        share_s();
+        for (uint32_t n = 0; n <= last; ++n) {
+            const uint32_t more = n < last ? n + 1u : n; /* the last loads again */
+            const KqBuf next = chunk(more);
+            char *eb = ebuf[n & 1u];
+            /* 1: the right-hand sides */
+            f4 E[2], F[2];
+            if (DELTA) {
+                times_s(E);
+                W1.load(next, lane16, at1);
+            }
+            const float is = ss.inv * (1.0f / kUnit);
+#pragma unroll
+            for (int ct = 0; ct < 2; ++ct)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    badin |= !kq_isfinite(V[ct][r]);
+                    const float x = f1[r] * V[ct][r];
+                    E[ct][r] = DELTA ? fmaf(-f0[r], E[ct][r] * is, x) : x;
+                }
+            load_v(next, more);
+            if (DELTA) {
+                const float m = kq::lanes_max<63>(fmaxf(largest(E[0]), largest(E[1])));
+                if (lane == 0u) top_r[wave] = m;
+                auto put_r = [&]() {
+#pragma unroll
+                    for (int ct = 0; ct < 2; ++ct) put(rbuf, fr, ct, r16, E[ct], sr.s);
+                };
+                put_r();
+                kq_lds_barrier();
+                if (!held_r()) {
+                    put_r();
+                    kq_lds_barrier();
+                }
+                /* 2: E, and F with the decay to the chunk's end */
+                times(rbuf, E);
+                const float ir = na * sr.inv;
+#pragma unroll
+                for (int ct = 0; ct < 2; ++ct) E[ct] *= ir;
+            }
+#pragma unroll
+            for (int ct = 0; ct < 2; ++ct) F[ct] = E[ct] * f2;
+            load_a(next);
+            const float me = kq::lanes_max<63>(fmaxf(largest(E[0]), largest(E[1])));
+            const float mf = kq::lanes_max<63>(fmaxf(largest(F[0]), largest(F[1])));
+            if (lane == 0u) {
+                top_e[wave] = me;
+                top_f[wave] = mf;
+            }
+            auto put_ef = [&]() {
+#pragma unroll
+                for (int ct = 0; ct < 2; ++ct) {
+                    put(fbuf, fr, ct, r16, F[ct], sf.s);
+                    put(eb, fr, ct, r16, E[ct], se.s);
+                }
+            };
+            put_ef();
+            kq_lds_barrier();
+            if (!held_ef()) {
+                put_ef();
+                kq_lds_barrier();
+            }
+            next_s(next);
+        }
+    } else {
+        f4 P[2], f0, f1; /* Q S; the factors of q, and with e^G */
+        float ps = 0.0f;
+        P[0] = P[1] = f0 = f1 = f4{0.0f, 0.0f, 0.0f, 0.0f};
+        auto write = [&](uint32_t n) {
+            f4 O[2];
+            times(ebuf[n & 1u], O);
+            const float pe = se.inv * (1.0f / kMixUnit);
+            const uint32_t left = sp.rows - n * kC;
+            const KqBuf y = kq_buf(a.y + ((uint64_t)sp.begin + n * kC) * a.ys + h * a.value_width,
+                                   (left < kC ? left : kC) * (uint32_t)a.ys * 4u);
+#pragma unroll
+            for (int ct = 0; ct < 2; ++ct)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const float o = fmaf(f1[r], P[ct][r] * ps, f0[r] * (O[ct][r] * pe));
+                    bad |= !kq_isfinite(o);
+                    /* rows past the sequence's last are past the buffer: not written */
+                    __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(o), y.r, (int)io[r],
+                                                          64 * ct, 0);
+                }
+        };
+        auto load_m = [&](KqBuf c) {
+            W2.load(c, lane16, at2);
+            f0 = factors(c, 3u);
+            f1 = factors(c, 4u);
+        };
+        const KqBuf first = chunk(0u);
+        W1.load(first, lane16, at1);
+        load_m(first);
+        load_end(first);
+        share_s();
+        for (uint32_t n = 0; n <= last; ++n) {
+            const KqBuf next = chunk(n < last ? n + 1u : n);
+            /* 1: the last chunk's output */
+            if (n != 0u) {
+                write(n - 1u);
+                load_m(chunk(n));
+            }
+            if (DELTA) {
+                kq_lds_barrier();
+                if (!held_r()) kq_lds_barrier();
+            }
+            /* 2: Q S */
+            times_s(P);
+            ps = ss.inv * (1.0f / kUnit);
+            W1.load(next, lane16, at1);
+            kq_lds_barrier();
+            if (!held_ef()) kq_lds_barrier();
+            next_s(next);
+        }
+        write(last);
     }
 #pragma unroll
-    for (int rt = 0; rt < RT; ++rt)
+    for (int u = 0; u < NU; ++u)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            const uint32_t d = (rt0 * RT + rt) * 16u + 4u * g4 + r;
-            bad |= !kq_isfinite(S[rt][r]);
-            a.state_out[sat + (size_t)d * a.value_width] = S[rt][r];
+            bad |= !kq_isfinite(S[u][r]);
+            a.state_out[sat + (size_t)r * a.value_width + 16u * u] = S[u][r];
         }
     if (badin) kq_flag(status, KQ_DEV_INPUT);
     if (bad) kq_flag(status, KQ_DEV_NUMERIC);
