@@ -8,27 +8,27 @@
  * solve
  *   (1 + L) E = diag(b) (diag(n) V - diag(n^2 e^G) K' S),
  *                                     L_ij = b_i n_i^2 e^(G_i - G_j) k'_i.k'_j  (j < i)
+ * so that with T = (1 + L)^-1 diag(b), U = T diag(n) V, W = T diag(n^2 e^G) K'
+ *   E = U - W S
  *   O = diag(e^G) Q S + M E,          M_ij = e^(G_i - G_j) q_i.k'_j      (j <= i)
  *   S' = e^(G_64) S + sum_j e^(G_64 - G_j) k'_j e_j^T
- * so that everything but three products with S is independent of it, and a
- * chunk costs seven matrix products instead of 64 dependent steps.
+ * and what hangs on the chunk before is four products with S and E.
+ * Without the delta correction E = diag(n) V.
  *
  * Three launches:
  *   linattn_plan  cuts the sequences into chunks (on the device: the lengths
  *                 are there)
- *   linattn_prep  a workgroup for each chunk and key head: K, Q as operands
- *                 of the matrix cores, and for each of its value heads
- *                 A = (1 + L)^-1 diag(b) and M
+ *   linattn_prep  a workgroup for each chunk and key head: Q, K'^T as operands
+ *                 of the matrix cores, and for each of its value heads M, W, U
  *   linattn_scan  a workgroup for each sequence, head and 32 columns of v:
- *                 S in registers from the first chunk to the last,
- *                 E = A (the right-hand side), O, S'
+ *                 S in registers from the first chunk to the last
  *
  * Operands are two fp16 numbers hi + lo (22 bits) in three products
  * hi hi + hi lo + lo hi with binary32 sums: off by at most 2^-22 of a
  * product, 5 times the rate of binary32 products on these cores. The ranges
  * that fp16 lacks are kept outside: a row of k or q is scaled by a power of
- * two to below 1 and its norm becomes a factor of the row; A, the right-hand
- * sides, E and S carry a power of two for each workgroup. Log decays are summed in 64 bits, since their
+ * two to below 1 and its norm becomes a factor of the row; T, W, V, E and S
+ * carry powers of two. Log decays are summed in 64 bits, since their
  * differences are what counts.
  */
 #include "kq_linattn.h"
@@ -42,10 +42,13 @@ typedef float f4 __attribute__((ext_vector_type(4)));
 constexpr uint32_t kC = 64;       /* rows of a chunk */
 constexpr uint32_t kHeads = 3;    /* value heads that linattn_prep takes at a time */
 constexpr uint32_t kPitch = 68;   /* floats of an LDS row of 64 */
+constexpr uint32_t kBlk = 20;     /* and of a row of a 16 x 16 block */
 constexpr uint32_t kMat = 16384;  /* bytes of a 64 x 64 operand, hi and lo */
-constexpr uint32_t kRowF = 6 * kC; /* floats of a value head's row factors */
+constexpr uint32_t kRowF = 5 * kC; /* floats of a value head's factors */
 
 constexpr float kUnit = 0x1p10f;   /* of the rows of k and q */
+/* W from its product T K' with T at 2^14 .. 2^15: |W| <= 64 x 2 max |T| */
+constexpr int kWDown = 7;
 constexpr float kMixUnit = 0x1p6f; /* of M: |q.k| <= 512 of such rows (128 values, below 2) */
 
 /* where the parts of the scratch lie */
@@ -169,31 +172,99 @@ __device__ __forceinline__ float unit_row(float (&x)[KS][8], uint32_t normalize,
             s = fmaf(x[i][e], x[i][e], s);
         }
     s = kq::lanes_sum<48>(s);
+    if (m == 0.0f) return 0.0f; /* 1 / sqrt(eps) would make the others' share of a scale small */
     if (normalize == 0u) return pow2(p);
     /* 2^p / sqrt(2^2p s + eps) */
     return (float)(1.0 / sqrt((double)s + ldexp((double)eps, -2 * p)));
 }
 
+/* the lower blocks of a 64 x 64 matrix, 16 x 16 each, in LDS */
+typedef float Lower[10][16][kBlk];
+__device__ __forceinline__ constexpr int blk(int i, int j) { return i * (i + 1) / 2 + j; }
+
+/* C + A B in binary32, where a lane has A[r16][4 g4 ..] and B[4 g4 ..][r16],
+ * the layout of C itself */
+__device__ __forceinline__ f4 mfma_f32(f4 a, f4 b, f4 c) {
+#pragma unroll
+    for (int s = 0; s < 4; ++s) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[s], b[s], c, 0, 0, 0);
+    return c;
+}
+
+/* The inverse of 1 + L by one wave, L's lower blocks (below the diagonal) in
+ * `m`, into x (a lane: rows 4 g4 .., column r16 of each block). The diagonal
+ * blocks by forward substitution, a lane for each column of each; the others
+ * from X_ij = -X_ii sum_k L_ik X_kj. */
+__device__ __forceinline__ void invert(Lower &m, uint32_t lane, f4 (&x)[10]) {
+    const uint32_t r16 = lane & 15u, g4 = lane >> 4;
+    {
+        const int d[4] = {blk(0, 0), blk(1, 1), blk(2, 2), blk(3, 3)};
+        const float(*l)[kBlk] = m[g4 == 0u ? d[0] : g4 == 1u ? d[1] : g4 == 2u ? d[2] : d[3]];
+        float t[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            float s0 = (int)r16 == i ? 1.0f : 0.0f, s1 = 0.0f;
+#pragma unroll
+            for (int j = 0; j < i; ++j) {
+                if (j & 1)
+                    s1 = fmaf(-l[i][j], t[j], s1);
+                else
+                    s0 = fmaf(-l[i][j], t[j], s0);
+            }
+            t[i] = s0 + s1;
+        }
+        __builtin_amdgcn_wave_barrier();
+        float(*o)[kBlk] = m[g4 == 0u ? d[0] : g4 == 1u ? d[1] : g4 == 2u ? d[2] : d[3]];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[i][r16] = t[i];
+        __builtin_amdgcn_wave_barrier();
+    }
+    f4 diag[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        diag[i] = *(const f4 *)&m[blk(i, i)][r16][4u * g4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) x[blk(i, i)][r] = m[blk(i, i)][4u * g4 + r][r16];
+    }
+#pragma unroll
+    for (int d = 1; d < 4; ++d)
+#pragma unroll
+        for (int j = 0; j + d < 4; ++j) {
+            const int i = j + d;
+            f4 p = f4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int k = j; k < i; ++k)
+                p = mfma_f32(*(const f4 *)&m[blk(i, k)][r16][4u * g4], x[blk(k, j)], p);
+            x[blk(i, j)] = -mfma_f32(diag[i], p, f4{0.0f, 0.0f, 0.0f, 0.0f});
+        }
+}
+
 template <int DK, bool DELTA>
-__global__ __launch_bounds__(256) void linattn_prep(kq_launch_linattn a, Work w,
+__global__ __launch_bounds__(256, 2) void linattn_prep(kq_launch_linattn a, Work w,
                                                     uint32_t *status) {
-    constexpr int KS = DK / 32;
-    constexpr uint32_t kKeyImage = 256u * DK, kSolve = DELTA ? kHeads * kC * kPitch * 4u : 0u;
+    constexpr int KS = DK / 32, NT = DK / 64; /* dk tiles of a wave */
+    constexpr uint32_t kKeyImage = 256u * DK, kSolve = DELTA ? kHeads * sizeof(Lower) : 0u;
+    constexpr uint32_t kMixBuf = 4u * 16u * kPitch * 4u, kTri = DELTA ? 24576u : 0u;
+    /* K' as an operand, then the triangles of the heads */
     __shared__ __attribute__((aligned(16))) char pool[kKeyImage > kSolve ? kKeyImage : kSolve];
-    __shared__ __attribute__((aligned(16))) float mixbuf[4][16][kPitch];
+    /* M, then T with its two column factors as operands */
+    __shared__ __attribute__((aligned(16))) char tri[kTri > kMixBuf ? kTri : kMixBuf];
+    __shared__ __attribute__((aligned(16))) float turn[4][16][36];
     __shared__ double sum[kHeads][kC];
-    __shared__ float beta[kHeads][kC], nks[kC], nqs[kC];
+    __shared__ float bet[kHeads][kC], cw[kHeads][kC], cu[kHeads][kC], nks[kC], nqs[kC];
+    __shared__ int pw[kHeads], pu[kHeads];
     const uint32_t c = blockIdx.x, kh = blockIdx.y;
     if (c >= *w.total) return;
     const uint4 ch = w.chunk[c];
     const uint32_t lane = threadIdx.x & 63u, r16 = lane & 15u, g4 = lane >> 4;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    char *kb = w.data + (uint64_t)c * w.chunk_bytes + (uint64_t)kh * w.key_bytes;
+    char *cb = w.data + (uint64_t)c * w.chunk_bytes;
+    char *kb = cb + (uint64_t)kh * w.key_bytes;
     bool badin = false;
 
     /* rows 16 wave + r16 of k and q as operands */
-    h8 kh8[KS], kl8[KS], qh8[KS], ql8[KS];
+    f4 kk[4], qk[4];
     {
+        h8 kh8[KS], kl8[KS], qh8[KS], ql8[KS];
         const uint32_t i = 16u * wave + r16;
         float x[KS][8], y[KS][8];
 #pragma unroll
@@ -233,58 +304,52 @@ __global__ __launch_bounds__(256) void linattn_prep(kq_launch_linattn a, Work w,
             const uint32_t at = ((wave * KS + ks) * 2u) * 1024u + lane * 16u;
             *(h8 *)(pool + at) = kh8[ks];
             *(h8 *)(pool + at + 1024u) = kl8[ks];
-            if (DELTA) {
-                *(h8 *)(kb + at) = kh8[ks];
-                *(h8 *)(kb + at + 1024u) = kl8[ks];
-            }
-            *(h8 *)(kb + kKeyImage + at) = qh8[ks];
-            *(h8 *)(kb + kKeyImage + at + 1024u) = ql8[ks];
+            *(h8 *)(kb + at) = qh8[ks];
+            *(h8 *)(kb + at + 1024u) = ql8[ks];
+        }
+        __syncthreads();
+        /* k_i.k_j and q_i.k_j, times kUnit^2: row 16 wave + 4 g4 + r, column 16 jt + r16 */
+#pragma unroll
+        for (int jt = 0; jt < 4; ++jt) {
+            kk[jt] = qk[jt] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+            if (jt <= (int)wave)
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks) {
+                    const uint32_t at = ((jt * KS + ks) * 2u) * 1024u + lane * 16u;
+                    const h8 bh = *(const h8 *)(pool + at), bl = *(const h8 *)(pool + at + 1024u);
+                    if (DELTA) kk[jt] = mfma3(kh8[ks], kl8[ks], bh, bl, kk[jt]);
+                    qk[jt] = mfma3(qh8[ks], ql8[ks], bh, bl, qk[jt]);
+                }
         }
     }
-    __syncthreads();
-
-    /* k_i.k_j and q_i.k_j, times kUnit^2: row 16 wave + 4 g4 + r, column 16 jt + r16 */
-    f4 kk[4], qk[4];
+    /* K'^T: row 16 (NT wave + t) + r16 of DK, 8 of the 64 columns */
+    h8 kth[NT][2], ktl[NT][2];
 #pragma unroll
-    for (int jt = 0; jt < 4; ++jt) {
-        kk[jt] = qk[jt] = f4{0.0f, 0.0f, 0.0f, 0.0f};
-        if (jt <= (int)wave)
-#pragma unroll
-            for (int ks = 0; ks < KS; ++ks) {
-                const uint32_t at = ((jt * KS + ks) * 2u) * 1024u + lane * 16u;
-                const h8 bh = *(const h8 *)(pool + at), bl = *(const h8 *)(pool + at + 1024u);
-                if (DELTA) kk[jt] = mfma3(kh8[ks], kl8[ks], bh, bl, kk[jt]);
-                qk[jt] = mfma3(qh8[ks], ql8[ks], bh, bl, qk[jt]);
-            }
-    }
-    /* k transposed: row 16 rt + r16 of DK, 8 of the 64 columns */
-    for (uint32_t rt = wave; rt < DK / 16u; rt += 4u) {
-        const uint32_t d = 16u * rt + r16;
+    for (int t = 0; t < NT; ++t) {
+        const uint32_t d = 16u * (NT * wave + t) + r16;
         const uint32_t from = (d >> 5) * 2048u + ((d & 31u) >> 3) * 256u + (d & 7u) * 2u;
 #pragma unroll
-        for (uint32_t ks = 0; ks < 2u; ++ks)
+        for (uint32_t ks = 0; ks < 2u; ++ks) {
 #pragma unroll
-            for (uint32_t plane = 0; plane < 2u; ++plane) {
-                h8 v;
-#pragma unroll
-                for (uint32_t e = 0; e < 8u; ++e) {
-                    const uint32_t t = 32u * ks + 8u * g4 + e;
-                    v[e] = *(const _Float16 *)(pool + from + plane * 1024u +
-                                               (t >> 4) * (KS * 2048u) + (t & 15u) * 16u);
-                }
-                *(h8 *)(kb + 2u * kKeyImage + ((rt * 2u + ks) * 2u + plane) * 1024u +
-                        lane * 16u) = v;
+            for (uint32_t e = 0; e < 8u; ++e) {
+                const uint32_t j = 32u * ks + 8u * g4 + e;
+                const uint32_t at = from + (j >> 4) * (KS * 2048u) + (j & 15u) * 16u;
+                kth[t][ks][e] = *(const _Float16 *)(pool + at);
+                ktl[t][ks][e] = *(const _Float16 *)(pool + at + 1024u);
             }
+            char *to = kb + kKeyImage + (((NT * wave + t) * 2u + ks) * 2u) * 1024u + lane * 16u;
+            *(h8 *)to = kth[t][ks];
+            *(h8 *)(to + 1024u) = ktl[t][ks];
+        }
     }
-    /* columns of M that no tile below writes */
-#pragma unroll
-    for (int k = 0; k < 16; ++k) mixbuf[wave][k][lane] = 0.0f;
     __syncthreads(); /* the image of k is free */
 
-    float(*solve)[kC][kPitch] = (float(*)[kC][kPitch])pool;
+    Lower *solve = (Lower *)pool;
+    float(*mix)[kPitch] = (float(*)[kPitch])(tri + wave * (16u * kPitch * 4u));
     const uint32_t per = a.value_heads / a.key_heads;
     for (uint32_t h0 = 0; h0 < per; h0 += kHeads) {
         const uint32_t nh = per - h0 < kHeads ? per - h0 : kHeads;
+        char *vb0 = cb + w.value_at + (uint64_t)(kh * per + h0) * w.value_bytes;
         if (wave < nh) { /* a wave for each head, a lane for each row */
             const uint32_t h = kh * per + h0 + wave;
             const float rate = a.rate[h], bias = a.bias != nullptr ? a.bias[h] : 0.0f;
@@ -301,26 +366,28 @@ __global__ __launch_bounds__(256) void linattn_prep(kq_launch_linattn a, Work w,
             }
             const double G = kq_wave_scan_f64((double)g);
             const double end = kq_readlane_f64(G, 63);
+            const float from = kq::exp_of(G), n = nks[lane];
             sum[wave][lane] = G;
-            beta[wave][lane] = b;
-            const float from = kq::exp_of(G), to = kq::exp_of(end - G);
-            float *f = (float *)(w.data + (uint64_t)c * w.chunk_bytes + w.value_at +
-                                 (uint64_t)h * w.value_bytes + kMat);
-            f[lane] = from * nks[lane] * nks[lane];
-            f[kC + lane] = nks[lane];
-            f[2 * kC + lane] = to;
-            f[3 * kC + lane] = nqs[lane];
-            f[4 * kC + lane] = from * nqs[lane];
+            bet[wave][lane] = b * n * n;
+            cw[wave][lane] = b * n * n * from;
+            cu[wave][lane] = b * n;
+            float *f = (float *)(vb0 + wave * w.value_bytes + kMat);
+            f[lane] = n;
+            f[kC + lane] = kq::exp_of(end - G);
+            f[2 * kC + lane] = nqs[lane];
+            f[3 * kC + lane] = from * nqs[lane];
             const kq::Decay d = kq::decay_of((float)end);
             if (lane == 0u) {
-                f[5 * kC] = d.c0;
-                f[5 * kC + 1] = d.c1;
+                f[4 * kC] = d.c0;
+                f[4 * kC + 1] = d.c1;
             }
         }
+        /* columns of M that no tile below writes */
+#pragma unroll
+        for (int k = 0; k < 16; ++k) mix[k][lane] = 0.0f;
         __syncthreads();
         for (uint32_t hh = 0; hh < nh; ++hh) {
-            char *vb = w.data + (uint64_t)c * w.chunk_bytes + w.value_at +
-                       (uint64_t)(kh * per + h0 + hh) * w.value_bytes;
+            char *vb = vb0 + hh * w.value_bytes;
             double gi[4];
 #pragma unroll
             for (int r = 0; r < 4; ++r) gi[r] = sum[hh][16u * wave + 4u * g4 + r];
@@ -333,20 +400,18 @@ __global__ __launch_bounds__(256) void linattn_prep(kq_launch_linattn a, Work w,
                 for (int r = 0; r < 4; ++r) {
                     const uint32_t i = 16u * wave + 4u * g4 + r;
                     const float fall = j <= i ? kq::exp_of(gi[r] - gj) : 0.0f;
-                    mixbuf[wave][4u * g4 + r][j] = qk[jt][r] * fall * (kMixUnit / kUnit / kUnit);
-                    if (DELTA && j < i)
-                        solve[hh][i][j] = beta[hh][i] * nks[i] * nks[i] * fall *
-                                          (kk[jt][r] * (1.0f / kUnit / kUnit));
+                    mix[4u * g4 + r][j] = qk[jt][r] * fall * (kMixUnit / kUnit / kUnit);
+                    if (DELTA)
+                        solve[hh][blk((int)wave, jt)][4u * g4 + r][r16] =
+                            bet[hh][i] * fall * (kk[jt][r] * (1.0f / kUnit / kUnit));
                 }
             }
-            /* the wave's own rows: its LDS operations complete in order */
-            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront", "local");
-            __builtin_amdgcn_wave_barrier();
+            __builtin_amdgcn_wave_barrier(); /* the wave's own rows of M, in order */
 #pragma unroll
             for (int ks = 0; ks < 2; ++ks) {
                 float x[8];
 #pragma unroll
-                for (int e = 0; e < 8; ++e) x[e] = mixbuf[wave][r16][32u * ks + 8u * g4 + e];
+                for (int e = 0; e < 8; ++e) x[e] = mix[r16][32u * ks + 8u * g4 + e];
                 h8 hi, lo;
                 split<8>(x, hi, lo);
                 char *to = vb + ((wave * 2u + ks) * 2u) * 1024u + lane * 16u;
@@ -355,56 +420,154 @@ __global__ __launch_bounds__(256) void linattn_prep(kq_launch_linattn a, Work w,
             }
             __builtin_amdgcn_wave_barrier();
         }
-        if constexpr (!DELTA) {
-            __syncthreads();
-            continue;
+        __syncthreads();
+        if constexpr (!DELTA) continue;
+        if (wave < nh) {
+            f4 x[10];
+            invert(solve[wave], lane, x);
+            float mw = 0.0f, mu = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int j = 0; j <= i; ++j) {
+                    const float fw = cw[wave][16 * j + r16], fu = cu[wave][16 * j + r16];
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const float t = x[blk(i, j)][r];
+                        mw = fmaxf(mw, fabsf(t * fw));
+                        mu = fmaxf(mu, fabsf(t * fu));
+                        if (i != j) solve[wave][blk(i, j)][4u * g4 + r][r16] = t;
+                    }
+                }
+            mw = kq::lanes_max<63>(mw);
+            mu = kq::lanes_max<63>(mu);
+            if (lane == 0u) {
+                const int p = scale_exp(mw);
+                pw[wave] = p;
+                pu[wave] = scale_exp(mu);
+                *(float *)(vb0 + wave * w.value_bytes + kMat + (4 * kC + 2) * 4u) =
+                    pow2(kWDown - p);
+            }
         }
         __syncthreads();
-        if (wave < nh) {
-            /* column `lane` of (1 + L)^-1, row after row */
-            float t[kC];
+        for (uint32_t hh = 0; hh < nh; ++hh) {
+            char *vb = vb0 + hh * w.value_bytes + kMat + kRowF * 4u;
+            const uint32_t h = kh * per + h0 + hh;
+            /* the wave's columns of V, 16 (nt wave + t) + r16, rows 32 ks + 8 g4 + e */
+            const uint32_t nt = a.value_width / 64u;
+            float v[2][2][8];
+            {
+                const KqBuf vr = kq_buf(a.v + (uint64_t)ch.x * a.vs + h * a.value_width,
+                                        ch.y * (uint32_t)a.vs * 4u); /* zeros past the rows */
 #pragma unroll
-            for (uint32_t i = 0; i < kC; ++i) {
-                float s[4] = {lane == i ? 1.0f : 0.0f, 0.0f, 0.0f, 0.0f};
+                for (uint32_t t = 0; t < 2u; ++t)
 #pragma unroll
-                for (uint32_t j = 0; j < i; ++j)
-                    s[j & 3u] = fmaf(-solve[wave][i][j], t[j], s[j & 3u]);
-                t[i] = (s[0] + s[1]) + (s[2] + s[3]);
+                    for (uint32_t ks = 0; ks < 2u; ++ks)
+#pragma unroll
+                        for (uint32_t e = 0; e < 8u; ++e)
+                            v[t][ks][e] =
+                                t < nt ? __uint_as_float(kq_ld32(
+                                             vr, ((32u * ks + 8u * g4 + e) * (uint32_t)a.vs +
+                                                  16u * (nt * wave + t) + r16) * 4u, 0u))
+                                       : 0.0f;
             }
-            const float b = beta[wave][lane];
-            float m = 0.0f;
+            /* T's rows 16 wave + r16 with the factors of its columns, as operands */
+            const float sw = pow2(pw[hh]), su = pow2(pu[hh]);
 #pragma unroll
-            for (uint32_t i = 0; i < kC; ++i) {
-                t[i] *= b;
-                m = fmaxf(m, fabsf(t[i]));
+            for (uint32_t ks = 0; ks < 2u; ++ks) {
+                if (ks > wave >> 1) continue;
+                const uint32_t jb = 2u * ks + (g4 >> 1), j0 = 32u * ks + 8u * g4;
+                const float *row = &solve[hh][blk((int)wave, 0) + (jb <= wave ? jb : 0u)][r16]
+                                         [8u * (g4 & 1u)];
+                float xw[8], xu[8];
+#pragma unroll
+                for (uint32_t e = 0; e < 8u; ++e) {
+                    const float t = jb <= wave ? row[e] : 0.0f;
+                    xw[e] = t * cw[hh][j0 + e] * sw;
+                    xu[e] = t * cu[hh][j0 + e] * su;
+                }
+                h8 hi, lo;
+                char *to = tri + (wave < 2u ? wave : 2u * wave - 2u + ks) * 2048u + lane * 16u;
+                split<8>(xw, hi, lo);
+                *(h8 *)to = hi;
+                *(h8 *)(to + 1024u) = lo;
+                split<8>(xu, hi, lo);
+                *(h8 *)(to + 12288u) = hi;
+                *(h8 *)(to + 12288u + 1024u) = lo;
             }
-            m = kq::lanes_max<63>(m);
-            const int p = scale_exp(m);
-            char *vb = w.data + (uint64_t)c * w.chunk_bytes + w.value_at +
-                       (uint64_t)(kh * per + h0 + wave) * w.value_bytes;
-            if (lane == 0u) *(float *)(vb + kMat + (5 * kC + 2) * 4u) = pow2(-p);
-            __builtin_amdgcn_wave_barrier(); /* the rows of L have been read */
+            __syncthreads();
+            /* W's columns 16 (NT wave + t) + r16 */
 #pragma unroll
-            for (uint32_t i = 0; i < kC; ++i) solve[wave][i][lane] = ldexpf(t[i], p);
-            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront", "local");
-            __builtin_amdgcn_wave_barrier();
-            vb += kMat + kRowF * 4u;
+            for (int rt = 0; rt < 4; ++rt) {
+                f4 x[NT];
 #pragma unroll
-            for (uint32_t rt = 0; rt < 4u; ++rt)
+                for (int t = 0; t < NT; ++t) x[t] = f4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                for (uint32_t ks = 0; ks < 2u; ++ks) {
-                    float x[8];
+                for (int ks = 0; ks <= rt >> 1; ++ks) {
+                    const char *p = tri + (rt < 2 ? rt : 2 * rt - 2 + ks) * 2048 + lane * 16u;
+                    const h8 ah = *(const h8 *)p, al = *(const h8 *)(p + 1024);
+#pragma unroll
+                    for (int t = 0; t < NT; ++t)
+                        x[t] = mfma3(ah, al, kth[t][ks], ktl[t][ks], x[t]);
+                }
+#pragma unroll
+                for (int t = 0; t < NT; ++t)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        turn[wave][4u * g4 + r][16 * t + r16] =
+                            x[t][r] * (1.0f / kUnit / (1 << kWDown));
+                __builtin_amdgcn_wave_barrier();
+                /* as an operand: row r16, 8 columns in a row */
+                if (NT == 2 || (g4 >> 1) == (wave & 1u)) {
+                    float y[8];
 #pragma unroll
                     for (uint32_t e = 0; e < 8u; ++e)
-                        x[e] = solve[wave][16u * rt + r16][32u * ks + 8u * g4 + e];
+                        y[e] = turn[wave][r16][8u * (NT == 2 ? g4 : g4 & 1u) + e];
                     h8 hi, lo;
-                    split<8>(x, hi, lo);
-                    char *to = vb + ((rt * 2u + ks) * 2u) * 1024u + lane * 16u;
+                    split<8>(y, hi, lo);
+                    const uint32_t ks = NT == 2 ? wave : wave >> 1;
+                    char *to = vb + ((rt * KS + ks) * 2u) * 1024u + lane * 16u;
                     *(h8 *)to = hi;
                     *(h8 *)(to + 1024u) = lo;
                 }
+                __builtin_amdgcn_wave_barrier();
+            }
+            /* U's columns: each with its own power of two */
+#pragma unroll
+            for (uint32_t t = 0; t < 2u; ++t) {
+                if (t >= nt) continue;
+                float m = 0.0f;
+#pragma unroll
+                for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        badin |= !kq_isfinite(v[t][ks][e]);
+                        m = fmaxf(m, fabsf(v[t][ks][e]));
+                    }
+                const int p = scale_exp(kq::lanes_max<48>(m));
+                const float sv = pow2(p), iv = ldexpf(pow2(-pu[hh]), -p);
+                h8 bh[2], bl[2];
+#pragma unroll
+                for (int ks = 0; ks < 2; ++ks) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) v[t][ks][e] *= sv;
+                    split<8>(v[t][ks], bh[ks], bl[ks]);
+                }
+#pragma unroll
+                for (int rt = 0; rt < 4; ++rt) {
+                    f4 x = f4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                    for (int ks = 0; ks <= rt >> 1; ++ks) {
+                        const char *q = tri + 12288 + (rt < 2 ? rt : 2 * rt - 2 + ks) * 2048 +
+                                        lane * 16u;
+                        x = mfma3(*(const h8 *)q, *(const h8 *)(q + 1024), bh[ks], bl[ks], x);
+                    }
+                    *(f4 *)(vb + kKeyImage + ((nt * wave + t) * 4u + rt) * 1024u + lane * 16u) =
+                        x * iv;
+                }
+            }
+            __syncthreads();
         }
-        __syncthreads();
     }
     if (badin) kq_flag(status, KQ_DEV_INPUT);
 }
@@ -477,12 +640,12 @@ __device__ __forceinline__ float top_of(const float *p) {
 }
 
 /*
- * Eight waves. Waves 0 .. 3 (the solvers) form K' S for 16 rows of the chunk
- * each, the right-hand sides and E; waves 4 .. 7 (the writers) Q S for 16 rows
- * each, the chunk's output, one phase behind, and its stores; every wave
- * holds 16 rows of S and forms their K'^T F. So an operand is loaded by one
- * wave, for both column tiles, and what no other step waits for runs beside
- * the chain S -> E -> S'. Three phases a chunk, with a barrier each.
+ * Eight waves. Waves 0 .. 3 (the solvers) form W S and E for 16 rows of the
+ * chunk each; waves 4 .. 7 (the writers) the output of 16 rows of the chunk
+ * before and their Q S; every wave holds 16 rows of S (of one column tile
+ * with width 64) and forms their K'^T F. So an operand is loaded by one wave,
+ * and what no other step waits for runs beside the chain S -> E -> S'. Two
+ * phases a chunk, with a barrier each.
  */
 template <int DK, bool DELTA>
 __global__ __launch_bounds__(64 * kScanWaves) void linattn_scan(kq_launch_linattn a,
@@ -490,10 +653,9 @@ __global__ __launch_bounds__(64 * kScanWaves) void linattn_scan(kq_launch_linatt
                                                                 uint32_t *status) {
     constexpr int KS = DK / 32, NU = DK / 64; /* steps over S's rows; tiles of S a wave holds */
     constexpr uint32_t kKeyImage = 256u * DK;
-    __shared__ __attribute__((aligned(16))) char sbuf[KS * 4096], rbuf[8192], ebuf[2][8192],
-        fbuf[8192];
-    /* largest values by wave: of S, the right-hand sides, E, F */
-    __shared__ __attribute__((aligned(16))) float top_s[8], top_r[4], top_e[4], top_f[4];
+    __shared__ __attribute__((aligned(16))) char sbuf[KS * 4096], ebuf[2][8192], fbuf[8192];
+    /* largest values by wave: of S, E, F */
+    __shared__ __attribute__((aligned(16))) float top_s[8], top_e[4], top_f[4];
     const uint32_t s = blockIdx.y;
     const uint2 mine = w.seq[s];
     if (mine.y == 0u) return;
@@ -511,7 +673,7 @@ __global__ __launch_bounds__(64 * kScanWaves) void linattn_scan(kq_launch_linatt
     uint32_t b = blockIdx.x;
     if (gridDim.x % 8u == 0u) b = (b % 8u) * (gridDim.x / 8u) + b / 8u;
     const uint32_t tiles = a.value_width / kTile;
-    const uint32_t h = b / tiles, col = (b % tiles) * kTile + r16;
+    const uint32_t h = b / tiles, tile = b % tiles, col = tile * kTile + r16;
     const uint32_t kh = h / (a.value_heads / a.key_heads);
     const size_t sat = (((size_t)sp.slot * a.value_heads + h) * DK + srow) * a.value_width + col +
                        16u * sct;
@@ -526,9 +688,10 @@ __global__ __launch_bounds__(64 * kScanWaves) void linattn_scan(kq_launch_linatt
     const char *data = w.data + (uint64_t)mine.x * w.chunk_bytes;
     const uint32_t kat = kh * w.key_bytes, vat = w.value_at + h * w.value_bytes;
     const uint32_t fat = vat + kMat;                              /* the rows' factors */
-    const uint32_t at1 = kat + (solver ? 0u : kKeyImage) + rt * KS * 2048u; /* K' or Q */
-    const uint32_t at2 = vat + (solver ? kMat + kRowF * 4u : 0u) + rt * 4096u; /* A or M */
-    const uint32_t at3 = kat + 2u * kKeyImage + srt * 4096u;      /* K'^T */
+    const uint32_t wat = fat + kRowF * 4u;                        /* W, then U */
+    const uint32_t at1 = (solver ? wat : kat) + rt * KS * 2048u;  /* W or Q */
+    const uint32_t at2 = vat + rt * 4096u;                        /* M */
+    const uint32_t at3 = kat + kKeyImage + srt * 4096u;           /* K'^T */
     uint32_t io[4]; /* the wave's rows of v or of the output, in bytes */
 #pragma unroll
     for (int r = 0; r < 4; ++r)
@@ -543,7 +706,7 @@ __global__ __launch_bounds__(64 * kScanWaves) void linattn_scan(kq_launch_linatt
         return __builtin_bit_cast(f4, kq_ld128(c, fr * 4u, fat + i * kC * 4u));
     };
     auto scalar = [&](KqBuf c, uint32_t i) {
-        return __uint_as_float(kq_ld32(c, i * 4u, fat + 5u * kC * 4u));
+        return __uint_as_float(kq_ld32(c, i * 4u, fat + 4u * kC * 4u));
     };
     auto load_end = [&](KqBuf c) {
         T.load(c, lane16, at3);
@@ -551,8 +714,8 @@ __global__ __launch_bounds__(64 * kScanWaves) void linattn_scan(kq_launch_linatt
         n1 = scalar(c, 1u);
     };
     /* S as an operand */
-    Scale ss, sr, se, sf;
-    ss.s = ss.inv = sr.s = sr.inv = se.s = se.inv = sf.s = sf.inv = 1.0f;
+    Scale ss, se, sf;
+    ss.s = ss.inv = se.s = se.inv = sf.s = sf.inv = 1.0f;
     auto put_s = [&]() {
 #pragma unroll
         for (int u = 0; u < NU; ++u) put(sbuf, srow, sct + u, r16, S[u], ss.s);
@@ -602,7 +765,7 @@ __global__ __launch_bounds__(64 * kScanWaves) void linattn_scan(kq_launch_linatt
             for (int ct = 0; ct < 2; ++ct)
                 x[ct] = mfma3(W2.hi[ks], W2.lo[ks], B[ct].hi[ks], B[ct].lo[ks], x[ct]);
     };
-    /* phase 3 of both: S' = e^G S + K'^T F */
+    /* phase 2 of both: S' = e^G S + K'^T F */
     auto next_s = [&](KqBuf next) {
         Frag<2> B[NU];
         f4 x[NU];
@@ -626,13 +789,7 @@ __global__ __launch_bounds__(64 * kScanWaves) void linattn_scan(kq_launch_linatt
         load_end(next);
         share_s();
     };
-    /* whether the scales of a barrier held; the same in all waves */
-    auto held_r = [&]() {
-        const float t = top_of(top_r);
-        const bool ok = sr.holds(t);
-        if (!ok) sr.set(t);
-        return ok;
-    };
+    /* whether the scales of E and F held; the same in all waves */
     auto held_ef = [&]() {
         const float te = top_of(top_e), tf = top_of(top_f);
         const bool ok = se.holds(te) && sf.holds(tf);
@@ -645,75 +802,56 @@ __global__ __launch_bounds__(64 * kScanWaves) void linattn_scan(kq_launch_linatt
     const uint32_t last = mine.y - 1u;
 
     if (solver) {
-        f4 V[2], f0, f1, f2; /* n^2 e^G, n, e^(G_64 - G) */
-        float na = 0.0f;
+        f4 V[2], f0, f1; /* U, or V with the factors n; e^(G_64 - G) */
+        float iw = 0.0f;
         auto load_v = [&](KqBuf c, uint32_t n) {
-            f1 = factors(c, 1u);
-            if (DELTA) f0 = factors(c, 0u);
-            const uint32_t left = sp.rows - n * kC; /* rows past it read as zeros */
-            const KqBuf v = kq_buf(a.v + ((uint64_t)sp.begin + n * kC) * a.vs + h * a.value_width,
-                                   (left < kC ? left : kC) * (uint32_t)a.vs * 4u);
-#pragma unroll
-            for (int ct = 0; ct < 2; ++ct)
-#pragma unroll
-                for (int r = 0; r < 4; ++r)
-                    V[ct][r] = __uint_as_float(kq_ld32(v, io[r], 64u * ct));
-        };
-        auto load_a = [&](KqBuf c) {
-            f2 = factors(c, 2u);
             if (DELTA) {
-                na = scalar(c, 2u);
-                W2.load(c, lane16, at2);
+#pragma unroll
+                for (int ct = 0; ct < 2; ++ct)
+                    V[ct] = __builtin_bit_cast(
+                        f4, kq_ld128(c, lane16, wat + kKeyImage +
+                                                    ((2u * tile + ct) * 4u + rt) * 1024u));
+                iw = scalar(c, 2u);
+            } else {
+                f0 = factors(c, 0u);
+                const uint32_t left = sp.rows - n * kC; /* rows past it read as zeros */
+                const KqBuf v =
+                    kq_buf(a.v + ((uint64_t)sp.begin + n * kC) * a.vs + h * a.value_width,
+                           (left < kC ? left : kC) * (uint32_t)a.vs * 4u);
+#pragma unroll
+                for (int ct = 0; ct < 2; ++ct)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        V[ct][r] = __uint_as_float(kq_ld32(v, io[r], 64u * ct));
             }
         };
         const KqBuf first = chunk(0u);
         if (DELTA) W1.load(first, lane16, at1);
         load_v(first, 0u);
-        load_a(first);
+        f1 = factors(first, 1u);
         load_end(first);
         share_s();
         for (uint32_t n = 0; n <= last; ++n) {
             const uint32_t more = n < last ? n + 1u : n; /* the last loads again */
             const KqBuf next = chunk(more);
             char *eb = ebuf[n & 1u];
-            /* 1: the right-hand sides */
+            /* 1: E, and F with the decay to the chunk's end */
             f4 E[2], F[2];
             if (DELTA) {
                 times_s(E);
                 W1.load(next, lane16, at1);
             }
-            const float is = ss.inv * (1.0f / kUnit);
+            const float is = ss.inv * iw;
 #pragma unroll
             for (int ct = 0; ct < 2; ++ct)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    badin |= !kq_isfinite(V[ct][r]);
-                    const float x = f1[r] * V[ct][r];
-                    E[ct][r] = DELTA ? fmaf(-f0[r], E[ct][r] * is, x) : x;
+                    if (!DELTA) badin |= !kq_isfinite(V[ct][r]);
+                    E[ct][r] = DELTA ? fmaf(-is, E[ct][r], V[ct][r]) : f0[r] * V[ct][r];
+                    F[ct][r] = E[ct][r] * f1[r];
                 }
             load_v(next, more);
-            if (DELTA) {
-                const float m = kq::lanes_max<63>(fmaxf(largest(E[0]), largest(E[1])));
-                if (lane == 0u) top_r[wave] = m;
-                auto put_r = [&]() {
-#pragma unroll
-                    for (int ct = 0; ct < 2; ++ct) put(rbuf, fr, ct, r16, E[ct], sr.s);
-                };
-                put_r();
-                kq_lds_barrier();
-                if (!held_r()) {
-                    put_r();
-                    kq_lds_barrier();
-                }
-                /* 2: E, and F with the decay to the chunk's end */
-                times(rbuf, E);
-                const float ir = na * sr.inv;
-#pragma unroll
-                for (int ct = 0; ct < 2; ++ct) E[ct] *= ir;
-            }
-#pragma unroll
-            for (int ct = 0; ct < 2; ++ct) F[ct] = E[ct] * f2;
-            load_a(next);
+            f1 = factors(next, 1u);
             const float me = kq::lanes_max<63>(fmaxf(largest(E[0]), largest(E[1])));
             const float mf = kq::lanes_max<63>(fmaxf(largest(F[0]), largest(F[1])));
             if (lane == 0u) {
@@ -759,8 +897,8 @@ __global__ __launch_bounds__(64 * kScanWaves) void linattn_scan(kq_launch_linatt
         };
         auto load_m = [&](KqBuf c) {
             W2.load(c, lane16, at2);
-            f0 = factors(c, 3u);
-            f1 = factors(c, 4u);
+            f0 = factors(c, 2u);
+            f1 = factors(c, 3u);
         };
         const KqBuf first = chunk(0u);
         W1.load(first, lane16, at1);
@@ -774,11 +912,7 @@ __global__ __launch_bounds__(64 * kScanWaves) void linattn_scan(kq_launch_linatt
                 write(n - 1u);
                 load_m(chunk(n));
             }
-            if (DELTA) {
-                kq_lds_barrier();
-                if (!held_r()) kq_lds_barrier();
-            }
-            /* 2: Q S */
+            /* and Q S */
             times_s(P);
             ps = ss.inv * (1.0f / kUnit);
             W1.load(next, lane16, at1);
@@ -817,13 +951,15 @@ Work carve(const kq_launch_linattn &a, uint64_t tokens, uint32_t count, uint32_t
     w.seq = (uint2 *)(p + 256u);
     w.chunk = (uint4 *)((char *)w.seq + up256(8u * (uint64_t)count));
     w.data = (char *)w.chunk + up256(16u * n);
-    w.key_bytes = 768u * a.key_width;
+    w.key_bytes = 512u * a.key_width;
     w.value_at = w.key_bytes * a.key_heads;
-    w.value_bytes = kMat * (delta ? 2u : 1u) + kRowF * 4u;
+    const uint32_t least = kMat + kRowF * 4u;
+    const uint32_t solved = least + 256u * (a.key_width + a.value_width);
+    w.value_bytes = delta ? solved : least;
     w.chunk_bytes = w.value_at + (uint64_t)w.value_bytes * a.value_heads;
     /* room for the delta form, which the sizes alone do not tell */
     *bytes = 512u + up256(8u * (uint64_t)count) + up256(16u * n) +
-             n * (w.value_at + (uint64_t)(2u * kMat + kRowF * 4u) * a.value_heads);
+             n * (w.value_at + (uint64_t)solved * a.value_heads);
     return w;
 }
 
