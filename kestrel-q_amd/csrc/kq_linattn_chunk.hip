@@ -612,15 +612,16 @@ __device__ __forceinline__ void put(char *p, uint32_t row, uint32_t ct, uint32_t
     *(h4 *)(to + 1024u) = lo;
 }
 
-__device__ __forceinline__ float largest(const f4 &x) {
-    return fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3])));
+__device__ __forceinline__ float largest(float m, const f4 &x) {
+    return fmaxf(fmaxf(m, fmaxf(fabsf(x[0]), fabsf(x[1]))), fmaxf(fabsf(x[2]), fabsf(x[3])));
 }
 
 /* The scale of an operand that the workgroup's waves share, from one chunk
  * to the next: a power of two under which the largest value lay at 2^13 when
  * it was set. It holds while that value stays within 2^10 .. 2^15: values
  * down to 2^-13 of the largest keep 22 bits, the others an error of 2^-35 of
- * it. */
+ * it. A wave tells of its part only whether it has values past the range,
+ * values at its upper end, values at all. */
 struct Scale {
     float s, inv;
     __device__ __forceinline__ void set(float m) {
@@ -628,9 +629,13 @@ struct Scale {
         s = pow2(e);
         inv = pow2(-e);
     }
-    __device__ __forceinline__ bool holds(float m) const {
+    __device__ __forceinline__ uint32_t tell(float m) const {
         const float y = m * s;
-        return y < 32768.0f && (y >= 1024.0f || m == 0.0f);
+        return (__ballot(!(y < 32768.0f)) != 0ull ? 1u : 0u) |
+               (__ballot(y >= 1024.0f) != 0ull ? 2u : 0u) | (__ballot(m > 0.0f) != 0ull ? 4u : 0u);
+    }
+    static __device__ __forceinline__ bool holds(uint32_t told) {
+        return (told & 1u) == 0u && (told & 6u) != 4u;
     }
 };
 
@@ -639,23 +644,31 @@ __device__ __forceinline__ float top_of(const float *p) {
     return fmaxf(fmaxf(a[0], a[1]), fmaxf(a[2], a[3]));
 }
 
+__device__ __forceinline__ uint32_t told_of(const uint32_t *p) {
+    const uint4 a = *(const uint4 *)p;
+    return (uint32_t)__builtin_amdgcn_readfirstlane((int)(a.x | a.y | a.z | a.w));
+}
+
 /*
- * Eight waves. Waves 0 .. 3 (the solvers) form W S and E for 16 rows of the
- * chunk each; waves 4 .. 7 (the writers) the output of 16 rows of the chunk
- * before and their Q S; every wave holds 16 rows of S (of one column tile
- * with width 64) and forms their K'^T F. So an operand is loaded by one wave,
- * and what no other step waits for runs beside the chain S -> E -> S'. Two
- * phases a chunk, with a barrier each.
+ * Eight waves. Waves 0 .. 3 (the solvers) run the chain S -> E -> S': W S and
+ * E for 16 rows of the chunk each, then K'^T F for a fourth of S's rows, which
+ * they hold. Waves 4 .. 7 (the writers) form Q S and M E for 16 rows each and
+ * store the output. So an operand is loaded by one wave, for both column
+ * tiles, and what no other step waits for runs beside the chain. Two phases a
+ * chunk with a barrier each:
+ *   1  S's operand is there: W S, E, F | Q S
+ *   2  E's and F's are there: S' | M E, the output
  */
 template <int DK, bool DELTA>
 __global__ __launch_bounds__(64 * kScanWaves) void linattn_scan(kq_launch_linattn a,
                                                                 kq_launch_seqs q, Work w,
                                                                 uint32_t *status) {
-    constexpr int KS = DK / 32, NU = DK / 64; /* steps over S's rows; tiles of S a wave holds */
+    constexpr int KS = DK / 32, NR = DK / 64; /* steps over S's rows; row tiles of a solver */
     constexpr uint32_t kKeyImage = 256u * DK;
-    __shared__ __attribute__((aligned(16))) char sbuf[KS * 4096], ebuf[2][8192], fbuf[8192];
-    /* largest values by wave: of S, E, F */
-    __shared__ __attribute__((aligned(16))) float top_s[8], top_e[4], top_f[4];
+    __shared__ __attribute__((aligned(16))) char sbuf[KS * 4096], ebuf[8192], fbuf[8192];
+    /* what the solvers tell of S, of E and F; their largest values, of S, E, F */
+    __shared__ __attribute__((aligned(16))) uint32_t told_s[4], told_ef[4];
+    __shared__ __attribute__((aligned(16))) float top_s[4], top_e[4], top_f[4];
     const uint32_t s = blockIdx.y;
     const uint2 mine = w.seq[s];
     if (mine.y == 0u) return;
@@ -664,10 +677,7 @@ __global__ __launch_bounds__(64 * kScanWaves) void linattn_scan(kq_launch_linatt
     if (!sp.live) return;
     const uint32_t lane = threadIdx.x & 63u, r16 = lane & 15u, g4 = lane >> 4, lane16 = lane * 16u;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const bool solver = wave < 4u;
     const uint32_t rt = wave & 3u, fr = 16u * rt + 4u * g4; /* rows of the chunk */
-    const uint32_t srt = DK == 128 ? wave : wave >> 1, sct = DK == 128 ? 0u : wave & 1u;
-    const uint32_t srow = 16u * srt + 4u * g4; /* rows of S, from column tile sct on */
     /* workgroups go round the 8 XCDs: those of a head, which read the same
      * operands, to one of them */
     uint32_t b = blockIdx.x;
@@ -675,30 +685,11 @@ __global__ __launch_bounds__(64 * kScanWaves) void linattn_scan(kq_launch_linatt
     const uint32_t tiles = a.value_width / kTile;
     const uint32_t h = b / tiles, tile = b % tiles, col = tile * kTile + r16;
     const uint32_t kh = h / (a.value_heads / a.key_heads);
-    const size_t sat = (((size_t)sp.slot * a.value_heads + h) * DK + srow) * a.value_width + col +
-                       16u * sct;
-
-    f4 S[NU];
-#pragma unroll
-    for (int u = 0; u < NU; ++u)
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-            S[u][r] = sp.fresh ? 0.0f : a.state[sat + (size_t)r * a.value_width + 16u * u];
 
     const char *data = w.data + (uint64_t)mine.x * w.chunk_bytes;
-    const uint32_t kat = kh * w.key_bytes, vat = w.value_at + h * w.value_bytes;
-    const uint32_t fat = vat + kMat;                              /* the rows' factors */
-    const uint32_t wat = fat + kRowF * 4u;                        /* W, then U */
-    const uint32_t at1 = (solver ? wat : kat) + rt * KS * 2048u;  /* W or Q */
-    const uint32_t at2 = vat + rt * 4096u;                        /* M */
-    const uint32_t at3 = kat + kKeyImage + srt * 4096u;           /* K'^T */
-    uint32_t io[4]; /* the wave's rows of v or of the output, in bytes */
-#pragma unroll
-    for (int r = 0; r < 4; ++r)
-        io[r] = ((fr + r) * (uint32_t)(solver ? a.vs : a.ys) + col) * 4u;
-    Frag<KS> W1;
-    Frag<2> W2, T;
-    float n0, n1;
+    const uint32_t kat = kh * w.key_bytes, vat = w.value_at + h * w.value_bytes; /* Q; M */
+    const uint32_t fat = vat + kMat;           /* the rows' factors */
+    const uint32_t wat = fat + kRowF * 4u;     /* W, then U */
     auto chunk = [&](uint32_t n) {
         return kq_buf(data + (uint64_t)n * w.chunk_bytes, (uint32_t)w.chunk_bytes);
     };
@@ -708,138 +699,116 @@ __global__ __launch_bounds__(64 * kScanWaves) void linattn_scan(kq_launch_linatt
     auto scalar = [&](KqBuf c, uint32_t i) {
         return __uint_as_float(kq_ld32(c, i * 4u, fat + 4u * kC * 4u));
     };
-    auto load_end = [&](KqBuf c) {
-        T.load(c, lane16, at3);
-        n0 = scalar(c, 0u);
-        n1 = scalar(c, 1u);
+    auto zero = [](f4(&x)[2]) { x[0] = x[1] = f4{0.0f, 0.0f, 0.0f, 0.0f}; };
+    /* rows of v or of the output of chunk n, the call's column tile */
+    auto rows_at = [&](const float *p, uint64_t stride, uint32_t n) {
+        const uint32_t left = sp.rows - n * kC; /* rows past it are past the buffer */
+        return kq_buf(p + ((uint64_t)sp.begin + n * kC) * stride + h * a.value_width,
+                      (left < kC ? left : kC) * (uint32_t)stride * 4u);
     };
-    /* S as an operand */
     Scale ss, se, sf;
     ss.s = ss.inv = se.s = se.inv = sf.s = sf.inv = 1.0f;
-    auto put_s = [&]() {
-#pragma unroll
-        for (int u = 0; u < NU; ++u) put(sbuf, srow, sct + u, r16, S[u], ss.s);
-    };
-    auto share_s = [&]() {
-        float m = largest(S[0]);
-#pragma unroll
-        for (int u = 1; u < NU; ++u) m = fmaxf(m, largest(S[u]));
-        m = kq::lanes_max<63>(m);
-        if (lane == 0u) top_s[wave] = m;
-        put_s();
-        kq_lds_barrier();
-        const float t = fmaxf(top_of(top_s), top_of(top_s + 4));
-        if (!ss.holds(t)) { /* the same in all waves, none of which has read on */
-            ss.set(t);
-            put_s();
-            kq_lds_barrier();
-        }
-    };
-    /* the wave's 16 rows of W1 times S */
-    auto times_s = [&](f4(&x)[2]) {
-        Frag<KS> B[2];
-#pragma unroll
-        for (int ct = 0; ct < 2; ++ct) {
-            B[ct].read(sbuf + ct * 2048u + lane16, 4096);
-            x[ct] = f4{0.0f, 0.0f, 0.0f, 0.0f};
-        }
-        __builtin_amdgcn_sched_barrier(0); /* all reads in flight, then the products */
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks)
-#pragma unroll
-            for (int ct = 0; ct < 2; ++ct)
-                x[ct] = mfma3(W1.hi[ks], W1.lo[ks], B[ct].hi[ks], B[ct].lo[ks], x[ct]);
-    };
-    /* its 16 rows of W2 times the operand at p */
-    auto times = [&](const char *p, f4(&x)[2]) {
-        Frag<2> B[2];
-#pragma unroll
-        for (int ct = 0; ct < 2; ++ct) {
-            B[ct].read(p + ct * 2048u + lane16, 4096);
-            x[ct] = f4{0.0f, 0.0f, 0.0f, 0.0f};
-        }
-        __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int ks = 0; ks < 2; ++ks)
-#pragma unroll
-            for (int ct = 0; ct < 2; ++ct)
-                x[ct] = mfma3(W2.hi[ks], W2.lo[ks], B[ct].hi[ks], B[ct].lo[ks], x[ct]);
-    };
-    /* phase 2 of both: S' = e^G S + K'^T F */
-    auto next_s = [&](KqBuf next) {
-        Frag<2> B[NU];
-        f4 x[NU];
-#pragma unroll
-        for (int u = 0; u < NU; ++u) {
-            B[u].read(fbuf + (sct + u) * 2048u + lane16, 4096);
-            x[u] = f4{0.0f, 0.0f, 0.0f, 0.0f};
-        }
-        __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int ks = 0; ks < 2; ++ks)
-#pragma unroll
-            for (int u = 0; u < NU; ++u)
-                x[u] = mfma3(T.hi[ks], T.lo[ks], B[u].hi[ks], B[u].lo[ks], x[u]);
-        const float jf = sf.inv * (1.0f / kUnit);
-#pragma unroll
-        for (int u = 0; u < NU; ++u)
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-                S[u][r] = fmaf(x[u][r], jf, fmaf(n1, S[u][r], n0 * S[u][r]));
-        load_end(next);
-        share_s();
-    };
-    /* whether the scales of E and F held; the same in all waves */
-    auto held_ef = [&]() {
-        const float te = top_of(top_e), tf = top_of(top_f);
-        const bool ok = se.holds(te) && sf.holds(tf);
-        if (!ok) {
-            se.set(te);
-            sf.set(tf);
-        }
-        return ok;
-    };
     const uint32_t last = mine.y - 1u;
 
-    if (solver) {
+    if (wave < 4u) {
+        __builtin_amdgcn_s_setprio(3); /* the chain first */
+        const uint32_t srow = 16u * NR * rt + 4u * g4;
+        const size_t sat = (((size_t)sp.slot * a.value_heads + h) * DK + srow) * a.value_width + col;
+        f4 S[NR][2];
+#pragma unroll
+        for (int t = 0; t < NR; ++t)
+#pragma unroll
+            for (int ct = 0; ct < 2; ++ct)
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    S[t][ct][r] = sp.fresh ? 0.0f
+                                           : a.state[sat + (size_t)(16 * t + r) * a.value_width +
+                                                     16u * ct];
+        Frag<KS> W;
+        Frag<2> T[NR];
         f4 V[2], f0, f1; /* U, or V with the factors n; e^(G_64 - G) */
-        float iw = 0.0f;
+        float iw = 0.0f, c0, c1;
+        uint32_t io[4]; /* the wave's rows of v, in bytes */
+        if (!DELTA)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) io[r] = ((fr + r) * (uint32_t)a.vs + col) * 4u;
+        auto load_w = [&](KqBuf c) {
+            if (DELTA) W.load(c, lane16, wat + rt * KS * 2048u);
+        };
         auto load_v = [&](KqBuf c, uint32_t n) {
             if (DELTA) {
 #pragma unroll
                 for (int ct = 0; ct < 2; ++ct)
                     V[ct] = __builtin_bit_cast(
-                        f4, kq_ld128(c, lane16, wat + kKeyImage +
-                                                    ((2u * tile + ct) * 4u + rt) * 1024u));
+                        f4, kq_ld128(c, lane16,
+                                     wat + kKeyImage + ((2u * tile + ct) * 4u + rt) * 1024u));
                 iw = scalar(c, 2u);
             } else {
                 f0 = factors(c, 0u);
-                const uint32_t left = sp.rows - n * kC; /* rows past it read as zeros */
-                const KqBuf v =
-                    kq_buf(a.v + ((uint64_t)sp.begin + n * kC) * a.vs + h * a.value_width,
-                           (left < kC ? left : kC) * (uint32_t)a.vs * 4u);
+                const KqBuf v = rows_at(a.v, a.vs, n);
 #pragma unroll
                 for (int ct = 0; ct < 2; ++ct)
 #pragma unroll
                     for (int r = 0; r < 4; ++r)
                         V[ct][r] = __uint_as_float(kq_ld32(v, io[r], 64u * ct));
             }
+            f1 = factors(c, 1u);
+        };
+        auto load_t = [&](KqBuf c) {
+#pragma unroll
+            for (int t = 0; t < NR; ++t)
+                T[t].load(c, lane16, kat + kKeyImage + (NR * rt + t) * 4096u);
+            c0 = scalar(c, 0u);
+            c1 = scalar(c, 1u);
+        };
+        /* S as an operand */
+        auto put_s = [&]() {
+#pragma unroll
+            for (int t = 0; t < NR; ++t)
+#pragma unroll
+                for (int ct = 0; ct < 2; ++ct) put(sbuf, srow + 16u * t, ct, r16, S[t][ct], ss.s);
+        };
+        float ms = 0.0f;
+        auto share_s = [&]() {
+            ms = 0.0f;
+#pragma unroll
+            for (int t = 0; t < NR; ++t)
+#pragma unroll
+                for (int ct = 0; ct < 2; ++ct) ms = largest(ms, S[t][ct]);
+            const uint32_t told = ss.tell(ms);
+            if (lane == 0u) told_s[rt] = told;
+            put_s();
         };
         const KqBuf first = chunk(0u);
-        if (DELTA) W1.load(first, lane16, at1);
+        load_w(first);
         load_v(first, 0u);
-        f1 = factors(first, 1u);
-        load_end(first);
+        load_t(first);
         share_s();
         for (uint32_t n = 0; n <= last; ++n) {
             const uint32_t more = n < last ? n + 1u : n; /* the last loads again */
             const KqBuf next = chunk(more);
-            char *eb = ebuf[n & 1u];
+            kq_lds_barrier();
             /* 1: E, and F with the decay to the chunk's end */
             f4 E[2], F[2];
+            zero(E);
+            if (!Scale::holds(told_of(told_s))) { /* the same in all waves */
+                const float m = kq::lanes_max<63>(ms);
+                if (lane == 0u) top_s[rt] = m;
+                kq_lds_barrier();
+                ss.set(top_of(top_s));
+                put_s();
+                kq_lds_barrier();
+            }
             if (DELTA) {
-                times_s(E);
-                W1.load(next, lane16, at1);
+                Frag<KS> B[2];
+#pragma unroll
+                for (int ct = 0; ct < 2; ++ct) B[ct].read(sbuf + ct * 2048u + lane16, 4096);
+                __builtin_amdgcn_sched_barrier(0); /* all in flight, then the products */
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+                    for (int ct = 0; ct < 2; ++ct)
+                        E[ct] = mfma3(W.hi[ks], W.lo[ks], B[ct].hi[ks], B[ct].lo[ks], E[ct]);
             }
             const float is = ss.inv * iw;
 #pragma unroll
@@ -850,85 +819,149 @@ __global__ __launch_bounds__(64 * kScanWaves) void linattn_scan(kq_launch_linatt
                     E[ct][r] = DELTA ? fmaf(-is, E[ct][r], V[ct][r]) : f0[r] * V[ct][r];
                     F[ct][r] = E[ct][r] * f1[r];
                 }
-            load_v(next, more);
-            f1 = factors(next, 1u);
-            const float me = kq::lanes_max<63>(fmaxf(largest(E[0]), largest(E[1])));
-            const float mf = kq::lanes_max<63>(fmaxf(largest(F[0]), largest(F[1])));
-            if (lane == 0u) {
-                top_e[wave] = me;
-                top_f[wave] = mf;
-            }
+            const float me = largest(largest(0.0f, E[0]), E[1]);
+            const float mf = largest(largest(0.0f, F[0]), F[1]);
+            const uint32_t told = se.tell(me) | sf.tell(mf) << 8;
+            if (lane == 0u) told_ef[rt] = told;
             auto put_ef = [&]() {
 #pragma unroll
                 for (int ct = 0; ct < 2; ++ct) {
                     put(fbuf, fr, ct, r16, F[ct], sf.s);
-                    put(eb, fr, ct, r16, E[ct], se.s);
+                    put(ebuf, fr, ct, r16, E[ct], se.s);
                 }
             };
             put_ef();
+            load_w(next);
+            load_v(next, more);
             kq_lds_barrier();
-            if (!held_ef()) {
-                put_ef();
-                kq_lds_barrier();
+            /* 2: S' = e^G S + K'^T F */
+            f4 x[NR][2];
+            {
+                const uint32_t all = told_of(told_ef);
+                if (!Scale::holds(all) || !Scale::holds(all >> 8)) {
+                    const float m0 = kq::lanes_max<63>(me), m1 = kq::lanes_max<63>(mf);
+                    if (lane == 0u) {
+                        top_e[rt] = m0;
+                        top_f[rt] = m1;
+                    }
+                    kq_lds_barrier();
+                    se.set(top_of(top_e));
+                    sf.set(top_of(top_f));
+                    put_ef();
+                    kq_lds_barrier();
+                }
+                Frag<2> B[2];
+#pragma unroll
+                for (int ct = 0; ct < 2; ++ct) B[ct].read(fbuf + ct * 2048u + lane16, 4096);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int t = 0; t < NR; ++t) zero(x[t]);
+#pragma unroll
+                for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+                    for (int t = 0; t < NR; ++t)
+#pragma unroll
+                        for (int ct = 0; ct < 2; ++ct)
+                            x[t][ct] = mfma3(T[t].hi[ks], T[t].lo[ks], B[ct].hi[ks], B[ct].lo[ks],
+                                             x[t][ct]);
             }
-            next_s(next);
+            const float jf = sf.inv * (1.0f / kUnit);
+#pragma unroll
+            for (int t = 0; t < NR; ++t)
+#pragma unroll
+                for (int ct = 0; ct < 2; ++ct)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        S[t][ct][r] =
+                            fmaf(x[t][ct][r], jf, fmaf(c1, S[t][ct][r], c0 * S[t][ct][r]));
+            share_s();
+            load_t(next);
         }
+#pragma unroll
+        for (int t = 0; t < NR; ++t)
+#pragma unroll
+            for (int ct = 0; ct < 2; ++ct)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    bad |= !kq_isfinite(S[t][ct][r]);
+                    a.state_out[sat + (size_t)(16 * t + r) * a.value_width + 16u * ct] =
+                        S[t][ct][r];
+                }
     } else {
-        f4 P[2], f0, f1; /* Q S; the factors of q, and with e^G */
-        float ps = 0.0f;
-        P[0] = P[1] = f0 = f1 = f4{0.0f, 0.0f, 0.0f, 0.0f};
-        auto write = [&](uint32_t n) {
-            f4 O[2];
-            times(ebuf[n & 1u], O);
+        Frag<KS> Q;
+        Frag<2> M;
+        f4 f0, f1; /* the factors of q, and with e^G */
+        uint32_t io[4]; /* the wave's rows of the output, in bytes */
+#pragma unroll
+        for (int r = 0; r < 4; ++r) io[r] = ((fr + r) * (uint32_t)a.ys + col) * 4u;
+        auto load_q = [&](KqBuf c) { Q.load(c, lane16, kat + rt * KS * 2048u); };
+        auto load_m = [&](KqBuf c) {
+            M.load(c, lane16, vat + rt * 4096u);
+            f0 = factors(c, 2u);
+            f1 = factors(c, 3u);
+        };
+        const KqBuf first = chunk(0u);
+        load_q(first);
+        load_m(first);
+        for (uint32_t n = 0; n <= last; ++n) {
+            const KqBuf next = chunk(n < last ? n + 1u : n);
+            kq_lds_barrier();
+            /* 1: Q S */
+            f4 P[2], O[2];
+            zero(P);
+            {
+                if (!Scale::holds(told_of(told_s))) {
+                    kq_lds_barrier();
+                    ss.set(top_of(top_s));
+                    kq_lds_barrier();
+                }
+                Frag<KS> B[2];
+#pragma unroll
+                for (int ct = 0; ct < 2; ++ct) B[ct].read(sbuf + ct * 2048u + lane16, 4096);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+                    for (int ct = 0; ct < 2; ++ct)
+                        P[ct] = mfma3(Q.hi[ks], Q.lo[ks], B[ct].hi[ks], B[ct].lo[ks], P[ct]);
+            }
+            const float ps = ss.inv * (1.0f / kUnit);
+            load_q(next);
+            kq_lds_barrier();
+            /* 2: M E, the output */
+            zero(O);
+            {
+                const uint32_t all = told_of(told_ef);
+                if (!Scale::holds(all) || !Scale::holds(all >> 8)) {
+                    kq_lds_barrier();
+                    se.set(top_of(top_e));
+                    sf.set(top_of(top_f));
+                    kq_lds_barrier();
+                }
+                Frag<2> B[2];
+#pragma unroll
+                for (int ct = 0; ct < 2; ++ct) B[ct].read(ebuf + ct * 2048u + lane16, 4096);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+                    for (int ct = 0; ct < 2; ++ct)
+                        O[ct] = mfma3(M.hi[ks], M.lo[ks], B[ct].hi[ks], B[ct].lo[ks], O[ct]);
+            }
             const float pe = se.inv * (1.0f / kMixUnit);
-            const uint32_t left = sp.rows - n * kC;
-            const KqBuf y = kq_buf(a.y + ((uint64_t)sp.begin + n * kC) * a.ys + h * a.value_width,
-                                   (left < kC ? left : kC) * (uint32_t)a.ys * 4u);
+            const KqBuf y = rows_at(a.y, a.ys, n);
 #pragma unroll
             for (int ct = 0; ct < 2; ++ct)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     const float o = fmaf(f1[r], P[ct][r] * ps, f0[r] * (O[ct][r] * pe));
                     bad |= !kq_isfinite(o);
-                    /* rows past the sequence's last are past the buffer: not written */
                     __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(o), y.r, (int)io[r],
                                                           64 * ct, 0);
                 }
-        };
-        auto load_m = [&](KqBuf c) {
-            W2.load(c, lane16, at2);
-            f0 = factors(c, 2u);
-            f1 = factors(c, 3u);
-        };
-        const KqBuf first = chunk(0u);
-        W1.load(first, lane16, at1);
-        load_m(first);
-        load_end(first);
-        share_s();
-        for (uint32_t n = 0; n <= last; ++n) {
-            const KqBuf next = chunk(n < last ? n + 1u : n);
-            /* 1: the last chunk's output */
-            if (n != 0u) {
-                write(n - 1u);
-                load_m(chunk(n));
-            }
-            /* and Q S */
-            times_s(P);
-            ps = ss.inv * (1.0f / kUnit);
-            W1.load(next, lane16, at1);
-            kq_lds_barrier();
-            if (!held_ef()) kq_lds_barrier();
-            next_s(next);
+            load_m(next);
         }
-        write(last);
     }
-#pragma unroll
-    for (int u = 0; u < NU; ++u)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            bad |= !kq_isfinite(S[u][r]);
-            a.state_out[sat + (size_t)r * a.value_width + 16u * u] = S[u][r];
-        }
     if (badin) kq_flag(status, KQ_DEV_INPUT);
     if (bad) kq_flag(status, KQ_DEV_NUMERIC);
 }
