@@ -35,8 +35,10 @@
 
 namespace {
 
+typedef _Float16 h2 __attribute__((ext_vector_type(2)));
 typedef _Float16 h4 __attribute__((ext_vector_type(4)));
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+typedef float f2 __attribute__((ext_vector_type(2)));
 typedef float f4 __attribute__((ext_vector_type(4)));
 
 constexpr uint32_t kC = 64;       /* rows of a chunk */
@@ -71,12 +73,16 @@ __device__ __forceinline__ f4 mfma3(h8 ah, h8 al, h8 bh, h8 bl, f4 c) {
     return mfma(ah, bh, c);
 }
 
+/* x s in two fp16 numbers: hi rounded from x s, lo from what is left */
 template <int N, typename H>
-__device__ __forceinline__ void split(const float *x, H &hi, H &lo) {
+__device__ __forceinline__ void split(const float *x, float s, H &hi, H &lo) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-        hi[i] = (_Float16)x[i];
-        lo[i] = (_Float16)(x[i] - (float)hi[i]);
+    for (int i = 0; i < N; i += 2) {
+        const h2 h = __builtin_convertvector(f2{x[i] * s, x[i + 1] * s}, h2);
+        hi[i] = h.x;
+        hi[i + 1] = h.y;
+        lo[i] = (_Float16)fmaf(x[i], s, -(float)h.x);
+        lo[i + 1] = (_Float16)fmaf(x[i + 1], s, -(float)h.y);
     }
 }
 
@@ -294,13 +300,8 @@ __global__ __launch_bounds__(256, 2) void linattn_prep(kq_launch_linattn a, Work
         }
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                x[ks][e] *= kUnit;
-                y[ks][e] *= kUnit;
-            }
-            split<8>(x[ks], kh8[ks], kl8[ks]);
-            split<8>(y[ks], qh8[ks], ql8[ks]);
+            split<8>(x[ks], kUnit, kh8[ks], kl8[ks]);
+            split<8>(y[ks], kUnit, qh8[ks], ql8[ks]);
             const uint32_t at = ((wave * KS + ks) * 2u) * 1024u + lane * 16u;
             *(h8 *)(pool + at) = kh8[ks];
             *(h8 *)(pool + at + 1024u) = kl8[ks];
@@ -376,11 +377,7 @@ __global__ __launch_bounds__(256, 2) void linattn_prep(kq_launch_linattn a, Work
             f[kC + lane] = kq::exp_of(end - G);
             f[2 * kC + lane] = nqs[lane];
             f[3 * kC + lane] = from * nqs[lane];
-            const kq::Decay d = kq::decay_of((float)end);
-            if (lane == 0u) {
-                f[4 * kC] = d.c0;
-                f[4 * kC + 1] = d.c1;
-            }
+            if (lane == 0u) f[4 * kC] = kq::exp_of(end);
         }
         /* columns of M that no tile below writes */
 #pragma unroll
@@ -400,7 +397,7 @@ __global__ __launch_bounds__(256, 2) void linattn_prep(kq_launch_linattn a, Work
                 for (int r = 0; r < 4; ++r) {
                     const uint32_t i = 16u * wave + 4u * g4 + r;
                     const float fall = j <= i ? kq::exp_of(gi[r] - gj) : 0.0f;
-                    mix[4u * g4 + r][j] = qk[jt][r] * fall * (kMixUnit / kUnit / kUnit);
+                    mix[4u * g4 + r][j] = qk[jt][r] * fall;
                     if (DELTA)
                         solve[hh][blk((int)wave, jt)][4u * g4 + r][r16] =
                             bet[hh][i] * fall * (kk[jt][r] * (1.0f / kUnit / kUnit));
@@ -413,7 +410,7 @@ __global__ __launch_bounds__(256, 2) void linattn_prep(kq_launch_linattn a, Work
 #pragma unroll
                 for (int e = 0; e < 8; ++e) x[e] = mix[r16][32u * ks + 8u * g4 + e];
                 h8 hi, lo;
-                split<8>(x, hi, lo);
+                split<8>(x, kMixUnit / kUnit / kUnit, hi, lo);
                 char *to = vb + ((wave * 2u + ks) * 2u) * 1024u + lane * 16u;
                 *(h8 *)to = hi;
                 *(h8 *)(to + 1024u) = lo;
@@ -445,7 +442,7 @@ __global__ __launch_bounds__(256, 2) void linattn_prep(kq_launch_linattn a, Work
                 const int p = scale_exp(mw);
                 pw[wave] = p;
                 pu[wave] = scale_exp(mu);
-                *(float *)(vb0 + wave * w.value_bytes + kMat + (4 * kC + 2) * 4u) =
+                *(float *)(vb0 + wave * w.value_bytes + kMat + (4 * kC + 1) * 4u) =
                     pow2(kWDown - p);
             }
         }
@@ -483,15 +480,15 @@ __global__ __launch_bounds__(256, 2) void linattn_prep(kq_launch_linattn a, Work
 #pragma unroll
                 for (uint32_t e = 0; e < 8u; ++e) {
                     const float t = jb <= wave ? row[e] : 0.0f;
-                    xw[e] = t * cw[hh][j0 + e] * sw;
-                    xu[e] = t * cu[hh][j0 + e] * su;
+                    xw[e] = t * cw[hh][j0 + e];
+                    xu[e] = t * cu[hh][j0 + e];
                 }
                 h8 hi, lo;
                 char *to = tri + (wave < 2u ? wave : 2u * wave - 2u + ks) * 2048u + lane * 16u;
-                split<8>(xw, hi, lo);
+                split<8>(xw, sw, hi, lo);
                 *(h8 *)to = hi;
                 *(h8 *)(to + 1024u) = lo;
-                split<8>(xu, hi, lo);
+                split<8>(xu, su, hi, lo);
                 *(h8 *)(to + 12288u) = hi;
                 *(h8 *)(to + 12288u + 1024u) = lo;
             }
@@ -514,8 +511,7 @@ __global__ __launch_bounds__(256, 2) void linattn_prep(kq_launch_linattn a, Work
                 for (int t = 0; t < NT; ++t)
 #pragma unroll
                     for (int r = 0; r < 4; ++r)
-                        turn[wave][4u * g4 + r][16 * t + r16] =
-                            x[t][r] * (1.0f / kUnit / (1 << kWDown));
+                        turn[wave][4u * g4 + r][16 * t + r16] = x[t][r];
                 __builtin_amdgcn_wave_barrier();
                 /* as an operand: row r16, 8 columns in a row */
                 if (NT == 2 || (g4 >> 1) == (wave & 1u)) {
@@ -524,7 +520,7 @@ __global__ __launch_bounds__(256, 2) void linattn_prep(kq_launch_linattn a, Work
                     for (uint32_t e = 0; e < 8u; ++e)
                         y[e] = turn[wave][r16][8u * (NT == 2 ? g4 : g4 & 1u) + e];
                     h8 hi, lo;
-                    split<8>(y, hi, lo);
+                    split<8>(y, 1.0f / kUnit / (1 << kWDown), hi, lo);
                     const uint32_t ks = NT == 2 ? wave : wave >> 1;
                     char *to = vb + ((rt * KS + ks) * 2u) * 1024u + lane * 16u;
                     *(h8 *)to = hi;
@@ -548,11 +544,7 @@ __global__ __launch_bounds__(256, 2) void linattn_prep(kq_launch_linattn a, Work
                 const float sv = pow2(p), iv = ldexpf(pow2(-pu[hh]), -p);
                 h8 bh[2], bl[2];
 #pragma unroll
-                for (int ks = 0; ks < 2; ++ks) {
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) v[t][ks][e] *= sv;
-                    split<8>(v[t][ks], bh[ks], bl[ks]);
-                }
+                for (int ks = 0; ks < 2; ++ks) split<8>(v[t][ks], sv, bh[ks], bl[ks]);
 #pragma unroll
                 for (int rt = 0; rt < 4; ++rt) {
                     f4 x = f4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -581,12 +573,13 @@ constexpr int kScanWaves = 8;
 template <int N>
 struct Frag {
     h8 hi[N], lo[N];
+    __device__ __forceinline__ void load1(KqBuf b, uint32_t lane16, uint32_t at, int i) {
+        hi[i] = __builtin_bit_cast(h8, kq_ld128(b, lane16, at + i * 2048u));
+        lo[i] = __builtin_bit_cast(h8, kq_ld128(b, lane16, at + i * 2048u + 1024u));
+    }
     __device__ __forceinline__ void load(KqBuf b, uint32_t lane16, uint32_t at) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            hi[i] = __builtin_bit_cast(h8, kq_ld128(b, lane16, at + i * 2048u));
-            lo[i] = __builtin_bit_cast(h8, kq_ld128(b, lane16, at + i * 2048u + 1024u));
-        }
+        for (int i = 0; i < N; ++i) load1(b, lane16, at, i);
     }
     __device__ __forceinline__ void read(const char *p, int step) {
 #pragma unroll
@@ -601,11 +594,9 @@ struct Frag {
  * column r16 of column tile ct, times s, as part of the right operand at p */
 __device__ __forceinline__ void put(char *p, uint32_t row, uint32_t ct, uint32_t r16, const f4 &x,
                                     float s) {
+    const float y[4] = {x[0], x[1], x[2], x[3]};
     h4 hi, lo;
-#pragma unroll
-    for (int r = 0; r < 4; ++r) hi[r] = (_Float16)(x[r] * s);
-#pragma unroll
-    for (int r = 0; r < 4; ++r) lo[r] = (_Float16)fmaf(x[r], s, -(float)hi[r]);
+    split<4>(y, s, hi, lo);
     char *to = p + (((row >> 5) * 2u + ct) * 2u) * 1024u + (((row & 31u) >> 3) * 16u + r16) * 16u +
                (row & 7u) * 2u;
     *(h4 *)to = hi;
@@ -656,8 +647,9 @@ __device__ __forceinline__ uint32_t told_of(const uint32_t *p) {
  * store the output. So an operand is loaded by one wave, for both column
  * tiles, and what no other step waits for runs beside the chain. Two phases a
  * chunk with a barrier each:
- *   1  S's operand is there: W S, E, F | Q S
- *   2  E's and F's are there: S' | M E, the output
+ *   1  S's operand is there: W S, E, F | M E of the chunk before, its output
+ *   2  E's and F's are there: S' | Q S
+ * (Q S beside W S would have both wait for the same LDS reads).
  */
 template <int DK, bool DELTA>
 __global__ __launch_bounds__(64 * kScanWaves) void linattn_scan(kq_launch_linattn a,
@@ -665,7 +657,7 @@ __global__ __launch_bounds__(64 * kScanWaves) void linattn_scan(kq_launch_linatt
                                                                 uint32_t *status) {
     constexpr int KS = DK / 32, NR = DK / 64; /* steps over S's rows; row tiles of a solver */
     constexpr uint32_t kKeyImage = 256u * DK;
-    __shared__ __attribute__((aligned(16))) char sbuf[KS * 4096], ebuf[8192], fbuf[8192];
+    __shared__ __attribute__((aligned(16))) char sbufs[2][KS * 4096], ebufs[2][8192], fbuf[8192];
     /* what the solvers tell of S, of E and F; their largest values, of S, E, F */
     __shared__ __attribute__((aligned(16))) uint32_t told_s[4], told_ef[4];
     __shared__ __attribute__((aligned(16))) float top_s[4], top_e[4], top_f[4];
@@ -727,7 +719,7 @@ __global__ __launch_bounds__(64 * kScanWaves) void linattn_scan(kq_launch_linatt
         Frag<KS> W;
         Frag<2> T[NR];
         f4 V[2], f0, f1; /* U, or V with the factors n; e^(G_64 - G) */
-        float iw = 0.0f, c0, c1;
+        float iw = 0.0f, c0;
         uint32_t io[4]; /* the wave's rows of v, in bytes */
         if (!DELTA)
 #pragma unroll
@@ -742,7 +734,7 @@ __global__ __launch_bounds__(64 * kScanWaves) void linattn_scan(kq_launch_linatt
                     V[ct] = __builtin_bit_cast(
                         f4, kq_ld128(c, lane16,
                                      wat + kKeyImage + ((2u * tile + ct) * 4u + rt) * 1024u));
-                iw = scalar(c, 2u);
+                iw = scalar(c, 1u);
             } else {
                 f0 = factors(c, 0u);
                 const KqBuf v = rows_at(a.v, a.vs, n);
@@ -759,9 +751,9 @@ __global__ __launch_bounds__(64 * kScanWaves) void linattn_scan(kq_launch_linatt
             for (int t = 0; t < NR; ++t)
                 T[t].load(c, lane16, kat + kKeyImage + (NR * rt + t) * 4096u);
             c0 = scalar(c, 0u);
-            c1 = scalar(c, 1u);
         };
         /* S as an operand */
+        char *sbuf = sbufs[0];
         auto put_s = [&]() {
 #pragma unroll
             for (int t = 0; t < NR; ++t)
@@ -787,6 +779,7 @@ __global__ __launch_bounds__(64 * kScanWaves) void linattn_scan(kq_launch_linatt
         for (uint32_t n = 0; n <= last; ++n) {
             const uint32_t more = n < last ? n + 1u : n; /* the last loads again */
             const KqBuf next = chunk(more);
+            char *ebuf = ebufs[n & 1u];
             kq_lds_barrier();
             /* 1: E, and F with the decay to the chunk's end */
             f4 E[2], F[2];
@@ -805,10 +798,13 @@ __global__ __launch_bounds__(64 * kScanWaves) void linattn_scan(kq_launch_linatt
                 for (int ct = 0; ct < 2; ++ct) B[ct].read(sbuf + ct * 2048u + lane16, 4096);
                 __builtin_amdgcn_sched_barrier(0); /* all in flight, then the products */
 #pragma unroll
-                for (int ks = 0; ks < KS; ++ks)
+                for (int ks = 0; ks < KS; ++ks) {
 #pragma unroll
                     for (int ct = 0; ct < 2; ++ct)
                         E[ct] = mfma3(W.hi[ks], W.lo[ks], B[ct].hi[ks], B[ct].lo[ks], E[ct]);
+                    W.load1(next, lane16, wat + rt * KS * 2048u, ks); /* of the next chunk */
+                    __builtin_amdgcn_sched_barrier(0);
+                }
             }
             const float is = ss.inv * iw;
 #pragma unroll
@@ -831,8 +827,6 @@ __global__ __launch_bounds__(64 * kScanWaves) void linattn_scan(kq_launch_linatt
                 }
             };
             put_ef();
-            load_w(next);
-            load_v(next, more);
             kq_lds_barrier();
             /* 2: S' = e^G S + K'^T F */
             f4 x[NR][2];
@@ -857,14 +851,20 @@ __global__ __launch_bounds__(64 * kScanWaves) void linattn_scan(kq_launch_linatt
 #pragma unroll
                 for (int t = 0; t < NR; ++t) zero(x[t]);
 #pragma unroll
-                for (int ks = 0; ks < 2; ++ks)
+                for (int ks = 0; ks < 2; ++ks) {
 #pragma unroll
                     for (int t = 0; t < NR; ++t)
 #pragma unroll
                         for (int ct = 0; ct < 2; ++ct)
                             x[t][ct] = mfma3(T[t].hi[ks], T[t].lo[ks], B[ct].hi[ks], B[ct].lo[ks],
                                              x[t][ct]);
+#pragma unroll
+                    for (int t = 0; t < NR; ++t)
+                        T[t].load1(next, lane16, kat + kKeyImage + (NR * rt + t) * 4096u, ks);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
             }
+            load_v(next, more);
             const float jf = sf.inv * (1.0f / kUnit);
 #pragma unroll
             for (int t = 0; t < NR; ++t)
@@ -872,11 +872,13 @@ __global__ __launch_bounds__(64 * kScanWaves) void linattn_scan(kq_launch_linatt
                 for (int ct = 0; ct < 2; ++ct)
 #pragma unroll
                     for (int r = 0; r < 4; ++r)
-                        S[t][ct][r] =
-                            fmaf(x[t][ct][r], jf, fmaf(c1, S[t][ct][r], c0 * S[t][ct][r]));
+                        S[t][ct][r] = fmaf(x[t][ct][r], jf, c0 * S[t][ct][r]);
+            __builtin_amdgcn_sched_barrier(0); /* c0 has been used: no copy that would wait */
+            c0 = scalar(next, 0u);
+            sbuf = sbufs[(n + 1u) & 1u];
             share_s();
-            load_t(next);
         }
+        kq_lds_barrier();
 #pragma unroll
         for (int t = 0; t < NR; ++t)
 #pragma unroll
@@ -894,59 +896,25 @@ __global__ __launch_bounds__(64 * kScanWaves) void linattn_scan(kq_launch_linatt
         uint32_t io[4]; /* the wave's rows of the output, in bytes */
 #pragma unroll
         for (int r = 0; r < 4; ++r) io[r] = ((fr + r) * (uint32_t)a.ys + col) * 4u;
-        auto load_q = [&](KqBuf c) { Q.load(c, lane16, kat + rt * KS * 2048u); };
-        auto load_m = [&](KqBuf c) {
-            M.load(c, lane16, vat + rt * 4096u);
-            f0 = factors(c, 2u);
-            f1 = factors(c, 3u);
-        };
-        const KqBuf first = chunk(0u);
-        load_q(first);
-        load_m(first);
-        for (uint32_t n = 0; n <= last; ++n) {
-            const KqBuf next = chunk(n < last ? n + 1u : n);
-            kq_lds_barrier();
-            /* 1: Q S */
-            f4 P[2], O[2];
-            zero(P);
-            {
-                if (!Scale::holds(told_of(told_s))) {
-                    kq_lds_barrier();
-                    ss.set(top_of(top_s));
-                    kq_lds_barrier();
-                }
-                Frag<KS> B[2];
-#pragma unroll
-                for (int ct = 0; ct < 2; ++ct) B[ct].read(sbuf + ct * 2048u + lane16, 4096);
-                __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-                for (int ks = 0; ks < KS; ++ks)
-#pragma unroll
-                    for (int ct = 0; ct < 2; ++ct)
-                        P[ct] = mfma3(Q.hi[ks], Q.lo[ks], B[ct].hi[ks], B[ct].lo[ks], P[ct]);
-            }
-            const float ps = ss.inv * (1.0f / kUnit);
-            load_q(next);
-            kq_lds_barrier();
-            /* 2: M E, the output */
+        f4 P[2];
+        float ps = 0.0f;
+        zero(P);
+        /* M E and the output of chunk n; the operands of chunk n + 1 */
+        auto write = [&](uint32_t n, KqBuf next) {
+            f4 O[2];
             zero(O);
-            {
-                const uint32_t all = told_of(told_ef);
-                if (!Scale::holds(all) || !Scale::holds(all >> 8)) {
-                    kq_lds_barrier();
-                    se.set(top_of(top_e));
-                    sf.set(top_of(top_f));
-                    kq_lds_barrier();
-                }
-                Frag<2> B[2];
+            Frag<2> B[2];
 #pragma unroll
-                for (int ct = 0; ct < 2; ++ct) B[ct].read(ebuf + ct * 2048u + lane16, 4096);
+            for (int ct = 0; ct < 2; ++ct)
+                B[ct].read(ebufs[n & 1u] + ct * 2048u + lane16, 4096);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int ks = 0; ks < 2; ++ks) {
+#pragma unroll
+                for (int ct = 0; ct < 2; ++ct)
+                    O[ct] = mfma3(M.hi[ks], M.lo[ks], B[ct].hi[ks], B[ct].lo[ks], O[ct]);
+                M.load1(next, lane16, vat + rt * 4096u, ks);
                 __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-                for (int ks = 0; ks < 2; ++ks)
-#pragma unroll
-                    for (int ct = 0; ct < 2; ++ct)
-                        O[ct] = mfma3(M.hi[ks], M.lo[ks], B[ct].hi[ks], B[ct].lo[ks], O[ct]);
             }
             const float pe = se.inv * (1.0f / kMixUnit);
             const KqBuf y = rows_at(a.y, a.ys, n);
@@ -959,8 +927,52 @@ __global__ __launch_bounds__(64 * kScanWaves) void linattn_scan(kq_launch_linatt
                     __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(o), y.r, (int)io[r],
                                                           64 * ct, 0);
                 }
-            load_m(next);
+            f0 = factors(next, 2u);
+            f1 = factors(next, 3u);
+        };
+        {
+            const KqBuf first = chunk(0u);
+            Q.load(first, lane16, kat + rt * KS * 2048u);
+            M.load(first, lane16, vat + rt * 4096u);
+            f0 = factors(first, 2u);
+            f1 = factors(first, 3u);
         }
+        for (uint32_t n = 0; n <= last; ++n) {
+            const KqBuf next = chunk(n < last ? n + 1u : n);
+            kq_lds_barrier();
+            /* 1 */
+            if (!Scale::holds(told_of(told_s))) {
+                kq_lds_barrier();
+                ss.set(top_of(top_s));
+                kq_lds_barrier();
+            }
+            if (n != 0u) write(n - 1u, chunk(n));
+            kq_lds_barrier();
+            /* 2: Q S */
+            const uint32_t all = told_of(told_ef);
+            if (!Scale::holds(all) || !Scale::holds(all >> 8)) {
+                kq_lds_barrier();
+                se.set(top_of(top_e));
+                sf.set(top_of(top_f));
+                kq_lds_barrier();
+            }
+            Frag<KS> B[2];
+#pragma unroll
+            for (int ct = 0; ct < 2; ++ct) B[ct].read(sbufs[n & 1u] + ct * 2048u + lane16, 4096);
+            zero(P);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+#pragma unroll
+                for (int ct = 0; ct < 2; ++ct)
+                    P[ct] = mfma3(Q.hi[ks], Q.lo[ks], B[ct].hi[ks], B[ct].lo[ks], P[ct]);
+                Q.load1(next, lane16, kat + rt * KS * 2048u, ks);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            ps = ss.inv * (1.0f / kUnit);
+        }
+        kq_lds_barrier();
+        write(last, chunk(last));
     }
     if (badin) kq_flag(status, KQ_DEV_INPUT);
     if (bad) kq_flag(status, KQ_DEV_NUMERIC);
