@@ -23,6 +23,11 @@
  *   linattn_scan  a workgroup for each sequence, head and 32 columns of v:
  *                 S in registers from the first chunk to the last
  *
+ * A lane's eight values of an operand's long axis are 4 g .. 4 g + 3 of one 16
+ * and the same four of the next (g = lane / 16), for both sides of a product:
+ * these are the rows that a lane holds of two results, so that S, E and F
+ * become operands, and M, W (formed transposed) too, without an exchange.
+ *
  * Operands are two fp16 numbers hi + lo (22 bits) in three products
  * hi hi + hi lo + lo hi with binary32 sums: off by at most 2^-22 of a
  * product, 5 times the rate of binary32 products on these cores. The ranges
@@ -43,8 +48,7 @@ typedef float f4 __attribute__((ext_vector_type(4)));
 
 constexpr uint32_t kC = 64;       /* rows of a chunk */
 constexpr uint32_t kHeads = 3;    /* value heads that linattn_prep takes at a time */
-constexpr uint32_t kPitch = 68;   /* floats of an LDS row of 64 */
-constexpr uint32_t kBlk = 20;     /* and of a row of a 16 x 16 block */
+constexpr uint32_t kBlk = 20;     /* floats of an LDS row of a 16 x 16 block */
 constexpr uint32_t kMat = 16384;  /* bytes of a 64 x 64 operand, hi and lo */
 constexpr uint32_t kRowF = 5 * kC; /* floats of a value head's factors */
 
@@ -57,8 +61,9 @@ constexpr float kMixUnit = 0x1p6f; /* of M: |q.k| <= 512 of such rows (128 value
 struct Work {
     uint32_t *total;  /* chunks */
     uint2 *seq;       /* of each sequence: its first chunk and their number */
-    uint4 *chunk;     /* first row, rows, sequence, 0 */
-    char *data;
+    uint4 *chunk;     /* first row, rows, sequence, number in it */
+    char *data;       /* operands of the chunks of a window */
+    uint32_t window;  /* chunks */
     uint64_t chunk_bytes;
     uint32_t key_bytes, value_at, value_bytes;
 };
@@ -141,7 +146,7 @@ __global__ __launch_bounds__(kPlanThreads) void linattn_plan(kq_launch_seqs q, u
             for (uint32_t k = lane; k < number[i]; k += 64u) {
                 const uint32_t left = rows[i] - k * kC;
                 w.chunk[first[i] + k] =
-                    make_uint4(begin[i] + k * kC, left < kC ? left : kC, base + i, 0u);
+                    make_uint4(begin[i] + k * kC, left < kC ? left : kC, base + i, k);
             }
         at = all;
         __syncthreads();
@@ -151,8 +156,8 @@ __global__ __launch_bounds__(kPlanThreads) void linattn_plan(kq_launch_seqs q, u
 
 /* ------------------------------------------------------------------ */
 
-/* A lane's part of a row x in the order of an operand, x[ks][8] the values
- * 32 ks + 8 (lane >> 4) ..; its four lanes differ in bits 4 and 5. Scales the
+/* A lane's part x[ks][8] of a row in the order of an operand; its four lanes
+ * differ in bits 4 and 5. Scales the
  * row to below 1 by a power of two and gives the factor that makes it the
  * row (over its norm) again. */
 template <int KS>
@@ -244,26 +249,26 @@ __device__ __forceinline__ void invert(Lower &m, uint32_t lane, f4 (&x)[10]) {
         }
 }
 
-template <int DK, bool DELTA>
+template <int DK, int DV, bool DELTA>
 __global__ __launch_bounds__(256, 2) void linattn_prep(kq_launch_linattn a, Work w,
-                                                    uint32_t *status) {
-    constexpr int KS = DK / 32, NT = DK / 64; /* dk tiles of a wave */
+                                                       uint32_t base, uint32_t *status) {
+    constexpr int KS = DK / 32, NT = DK / 64, NV = DV / 64; /* tiles of a wave */
     constexpr uint32_t kKeyImage = 256u * DK, kSolve = DELTA ? kHeads * sizeof(Lower) : 0u;
-    constexpr uint32_t kMixBuf = 4u * 16u * kPitch * 4u, kTri = DELTA ? 24576u : 0u;
     /* K' as an operand, then the triangles of the heads */
     __shared__ __attribute__((aligned(16))) char pool[kKeyImage > kSolve ? kKeyImage : kSolve];
-    /* M, then T with its two column factors as operands */
-    __shared__ __attribute__((aligned(16))) char tri[kTri > kMixBuf ? kTri : kMixBuf];
-    __shared__ __attribute__((aligned(16))) float turn[4][16][36];
-    __shared__ double sum[kHeads][kC];
-    __shared__ float bet[kHeads][kC], cw[kHeads][kC], cu[kHeads][kC], nks[kC], nqs[kC];
+    /* T with its two column factors as operands, the pieces below the diagonal */
+    __shared__ __attribute__((aligned(16))) char tri[DELTA ? 24576 : 16];
+    __shared__ __attribute__((aligned(16))) double sum[kHeads][kC];
+    __shared__ __attribute__((aligned(16))) float cw[kHeads][kC], cu[kHeads][kC];
+    __shared__ float bet[kHeads][kC], nks[kC], nqs[kC];
     __shared__ int pw[kHeads], pu[kHeads];
-    const uint32_t c = blockIdx.x, kh = blockIdx.y;
+    const uint32_t c = base + blockIdx.x, kh = blockIdx.y;
     if (c >= *w.total) return;
     const uint4 ch = w.chunk[c];
     const uint32_t lane = threadIdx.x & 63u, r16 = lane & 15u, g4 = lane >> 4;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    char *cb = w.data + (uint64_t)c * w.chunk_bytes;
+    const uint32_t per = a.value_heads / a.key_heads;
+    char *cb = w.data + (uint64_t)blockIdx.x * w.chunk_bytes;
     char *kb = cb + (uint64_t)kh * w.key_bytes;
     bool badin = false;
 
@@ -279,13 +284,13 @@ __global__ __launch_bounds__(256, 2) void linattn_prep(kq_launch_linattn a, Work
             for (int e = 0; e < 8; ++e) x[ks][e] = y[ks][e] = 0.0f;
         if (i < ch.y) {
             const uint64_t t = (uint64_t)ch.x + i;
-            const float4 *kp = (const float4 *)(a.k + t * a.ks + kh * DK + 8u * g4);
-            const float4 *qp = (const float4 *)(a.q + t * a.qs + kh * DK + 8u * g4);
+            const float4 *kp = (const float4 *)(a.k + t * a.ks + kh * DK + 4u * g4);
+            const float4 *qp = (const float4 *)(a.q + t * a.qs + kh * DK + 4u * g4);
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
                 for (int k = 0; k < 2; ++k) {
-                    const float4 u = kp[8 * ks + k], v = qp[8 * ks + k];
+                    const float4 u = kp[8 * ks + 4 * k], v = qp[8 * ks + 4 * k];
                     x[ks][4 * k] = u.x; x[ks][4 * k + 1] = u.y;
                     x[ks][4 * k + 2] = u.z; x[ks][4 * k + 3] = u.w;
                     y[ks][4 * k] = v.x; y[ks][4 * k + 1] = v.y;
@@ -309,7 +314,8 @@ __global__ __launch_bounds__(256, 2) void linattn_prep(kq_launch_linattn a, Work
             *(h8 *)(kb + at + 1024u) = ql8[ks];
         }
         __syncthreads();
-        /* k_i.k_j and q_i.k_j, times kUnit^2: row 16 wave + 4 g4 + r, column 16 jt + r16 */
+        /* k_j.k_i and k_j.q_i, times kUnit^2: row j = 16 jt + 4 g4 + r, column
+         * i = 16 wave + r16 */
 #pragma unroll
         for (int jt = 0; jt < 4; ++jt) {
             kk[jt] = qk[jt] = f4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -317,9 +323,9 @@ __global__ __launch_bounds__(256, 2) void linattn_prep(kq_launch_linattn a, Work
 #pragma unroll
                 for (int ks = 0; ks < KS; ++ks) {
                     const uint32_t at = ((jt * KS + ks) * 2u) * 1024u + lane * 16u;
-                    const h8 bh = *(const h8 *)(pool + at), bl = *(const h8 *)(pool + at + 1024u);
-                    if (DELTA) kk[jt] = mfma3(kh8[ks], kl8[ks], bh, bl, kk[jt]);
-                    qk[jt] = mfma3(qh8[ks], ql8[ks], bh, bl, qk[jt]);
+                    const h8 ah = *(const h8 *)(pool + at), al = *(const h8 *)(pool + at + 1024u);
+                    if (DELTA) kk[jt] = mfma3(ah, al, kh8[ks], kl8[ks], kk[jt]);
+                    qk[jt] = mfma3(ah, al, qh8[ks], ql8[ks], qk[jt]);
                 }
         }
     }
@@ -327,27 +333,43 @@ __global__ __launch_bounds__(256, 2) void linattn_prep(kq_launch_linattn a, Work
     h8 kth[NT][2], ktl[NT][2];
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-        const uint32_t d = 16u * (NT * wave + t) + r16;
-        const uint32_t from = (d >> 5) * 2048u + ((d & 31u) >> 3) * 256u + (d & 7u) * 2u;
+        const uint32_t tile = NT * wave + t;
+        const uint32_t from = (tile >> 1) * 2048u + (tile & 1u) * 8u + (r16 >> 2) * 256u +
+                              (r16 & 3u) * 2u + 4u * g4 * 16u;
 #pragma unroll
         for (uint32_t ks = 0; ks < 2u; ++ks) {
 #pragma unroll
-            for (uint32_t e = 0; e < 8u; ++e) {
-                const uint32_t j = 32u * ks + 8u * g4 + e;
-                const uint32_t at = from + (j >> 4) * (KS * 2048u) + (j & 15u) * 16u;
+            for (uint32_t e = 0; e < 8u; ++e) { /* row 32 ks + 16 (e / 4) + 4 g4 + e % 4 of K' */
+                const uint32_t at = from + (2u * ks + e / 4u) * (KS * 2048u) + (e & 3u) * 16u;
                 kth[t][ks][e] = *(const _Float16 *)(pool + at);
                 ktl[t][ks][e] = *(const _Float16 *)(pool + at + 1024u);
             }
-            char *to = kb + kKeyImage + (((NT * wave + t) * 2u + ks) * 2u) * 1024u + lane * 16u;
+            char *to = kb + kKeyImage + ((tile * 2u + ks) * 2u) * 1024u + lane * 16u;
             *(h8 *)to = kth[t][ks];
             *(h8 *)(to + 1024u) = ktl[t][ks];
         }
     }
+    /* The wave's columns of a head's V, 16 (NV wave + t) + r16: on their way
+     * while the head before is at work */
+    float v[NV][2][8];
+    auto load_v = [&](uint32_t h) {
+        const KqBuf vr = kq_buf(a.v + (uint64_t)ch.x * a.vs + h * DV,
+                                ch.y * (uint32_t)a.vs * 4u); /* zeros past the rows */
+        const uint32_t at = (4u * g4 * (uint32_t)a.vs + 16u * NV * wave + r16) * 4u;
+#pragma unroll
+        for (uint32_t t = 0; t < NV; ++t)
+#pragma unroll
+            for (uint32_t ks = 0; ks < 2u; ++ks)
+#pragma unroll
+                for (uint32_t e = 0; e < 8u; ++e)
+                    v[t][ks][e] = __uint_as_float(
+                        kq_ld32(vr, at + (32u * ks + 16u * (e / 4u) + e % 4u) * (uint32_t)a.vs * 4u,
+                                64u * t));
+    };
+    if (DELTA) load_v(kh * per);
     __syncthreads(); /* the image of k is free */
 
     Lower *solve = (Lower *)pool;
-    float(*mix)[kPitch] = (float(*)[kPitch])(tri + wave * (16u * kPitch * 4u));
-    const uint32_t per = a.value_heads / a.key_heads;
     for (uint32_t h0 = 0; h0 < per; h0 += kHeads) {
         const uint32_t nh = per - h0 < kHeads ? per - h0 : kHeads;
         char *vb0 = cb + w.value_at + (uint64_t)(kh * per + h0) * w.value_bytes;
@@ -379,43 +401,38 @@ __global__ __launch_bounds__(256, 2) void linattn_prep(kq_launch_linattn a, Work
             f[3 * kC + lane] = from * nqs[lane];
             if (lane == 0u) f[4 * kC] = kq::exp_of(end);
         }
-        /* columns of M that no tile below writes */
-#pragma unroll
-        for (int k = 0; k < 16; ++k) mix[k][lane] = 0.0f;
         __syncthreads();
         for (uint32_t hh = 0; hh < nh; ++hh) {
             char *vb = vb0 + hh * w.value_bytes;
-            double gi[4];
-#pragma unroll
-            for (int r = 0; r < 4; ++r) gi[r] = sum[hh][16u * wave + 4u * g4 + r];
-#pragma unroll
-            for (int jt = 0; jt < 4; ++jt) {
-                if (jt > (int)wave) continue;
-                const uint32_t j = 16u * jt + r16;
-                const double gj = sum[hh][j];
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const uint32_t i = 16u * wave + 4u * g4 + r;
-                    const float fall = j <= i ? kq::exp_of(gi[r] - gj) : 0.0f;
-                    mix[4u * g4 + r][j] = qk[jt][r] * fall;
-                    if (DELTA)
-                        solve[hh][blk((int)wave, jt)][4u * g4 + r][r16] =
-                            bet[hh][i] * fall * (kk[jt][r] * (1.0f / kUnit / kUnit));
-                }
-            }
-            __builtin_amdgcn_wave_barrier(); /* the wave's own rows of M, in order */
+            const double gi = sum[hh][16u * wave + r16];
+            const float bi = bet[hh][16u * wave + r16] * (1.0f / kUnit / kUnit);
 #pragma unroll
             for (int ks = 0; ks < 2; ++ks) {
                 float x[8];
 #pragma unroll
-                for (int e = 0; e < 8; ++e) x[e] = mix[r16][32u * ks + 8u * g4 + e];
+                for (int half = 0; half < 2; ++half) {
+                    const int jt = 2 * ks + half;
+                    f4 l;
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        x[4 * half + r] = l[r] = 0.0f;
+                        if (jt <= (int)wave) { /* rows of the diagonal tile above i: zeros */
+                            const bool above = jt == (int)wave && 4u * g4 + r > r16;
+                            const float fall =
+                                above ? 0.0f : kq::exp_of(gi - sum[hh][16 * jt + 4u * g4 + r]);
+                            x[4 * half + r] = qk[jt][r] * fall;
+                            l[r] = bi * fall * kk[jt][r];
+                        }
+                    }
+                    if (DELTA && jt <= (int)wave)
+                        *(f4 *)&solve[hh][blk((int)wave, 0) + jt][r16][4u * g4] = l;
+                }
                 h8 hi, lo;
                 split<8>(x, kMixUnit / kUnit / kUnit, hi, lo);
                 char *to = vb + ((wave * 2u + ks) * 2u) * 1024u + lane * 16u;
                 *(h8 *)to = hi;
                 *(h8 *)(to + 1024u) = lo;
             }
-            __builtin_amdgcn_wave_barrier();
         }
         __syncthreads();
         if constexpr (!DELTA) continue;
@@ -449,39 +466,24 @@ __global__ __launch_bounds__(256, 2) void linattn_prep(kq_launch_linattn a, Work
         __syncthreads();
         for (uint32_t hh = 0; hh < nh; ++hh) {
             char *vb = vb0 + hh * w.value_bytes + kMat + kRowF * 4u;
-            const uint32_t h = kh * per + h0 + hh;
-            /* the wave's columns of V, 16 (nt wave + t) + r16, rows 32 ks + 8 g4 + e */
-            const uint32_t nt = a.value_width / 64u;
-            float v[2][2][8];
-            {
-                const KqBuf vr = kq_buf(a.v + (uint64_t)ch.x * a.vs + h * a.value_width,
-                                        ch.y * (uint32_t)a.vs * 4u); /* zeros past the rows */
-#pragma unroll
-                for (uint32_t t = 0; t < 2u; ++t)
-#pragma unroll
-                    for (uint32_t ks = 0; ks < 2u; ++ks)
-#pragma unroll
-                        for (uint32_t e = 0; e < 8u; ++e)
-                            v[t][ks][e] =
-                                t < nt ? __uint_as_float(kq_ld32(
-                                             vr, ((32u * ks + 8u * g4 + e) * (uint32_t)a.vs +
-                                                  16u * (nt * wave + t) + r16) * 4u, 0u))
-                                       : 0.0f;
-            }
             /* T's rows 16 wave + r16 with the factors of its columns, as operands */
             const float sw = pow2(pw[hh]), su = pow2(pu[hh]);
 #pragma unroll
             for (uint32_t ks = 0; ks < 2u; ++ks) {
                 if (ks > wave >> 1) continue;
-                const uint32_t jb = 2u * ks + (g4 >> 1), j0 = 32u * ks + 8u * g4;
-                const float *row = &solve[hh][blk((int)wave, 0) + (jb <= wave ? jb : 0u)][r16]
-                                         [8u * (g4 & 1u)];
                 float xw[8], xu[8];
 #pragma unroll
-                for (uint32_t e = 0; e < 8u; ++e) {
-                    const float t = jb <= wave ? row[e] : 0.0f;
-                    xw[e] = t * cw[hh][j0 + e];
-                    xu[e] = t * cu[hh][j0 + e];
+                for (uint32_t half = 0; half < 2u; ++half) {
+                    const uint32_t jb = 2u * ks + half;
+                    f4 t = f4{0.0f, 0.0f, 0.0f, 0.0f};
+                    if (jb <= wave) t = *(const f4 *)&solve[hh][blk((int)wave, 0) + jb][r16][4u * g4];
+                    const f4 fw = *(const f4 *)&cw[hh][16u * jb + 4u * g4],
+                             fu = *(const f4 *)&cu[hh][16u * jb + 4u * g4];
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        xw[4 * half + r] = t[r] * fw[r];
+                        xu[4 * half + r] = t[r] * fu[r];
+                    }
                 }
                 h8 hi, lo;
                 char *to = tri + (wave < 2u ? wave : 2u * wave - 2u + ks) * 2048u + lane * 16u;
@@ -492,46 +494,11 @@ __global__ __launch_bounds__(256, 2) void linattn_prep(kq_launch_linattn a, Work
                 *(h8 *)(to + 12288u) = hi;
                 *(h8 *)(to + 12288u + 1024u) = lo;
             }
-            __syncthreads();
-            /* W's columns 16 (NT wave + t) + r16 */
+            /* the columns of V as operands, each with its own power of two */
+            h8 bh[NV][2], bl[NV][2];
+            float iv[NV];
 #pragma unroll
-            for (int rt = 0; rt < 4; ++rt) {
-                f4 x[NT];
-#pragma unroll
-                for (int t = 0; t < NT; ++t) x[t] = f4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                for (int ks = 0; ks <= rt >> 1; ++ks) {
-                    const char *p = tri + (rt < 2 ? rt : 2 * rt - 2 + ks) * 2048 + lane * 16u;
-                    const h8 ah = *(const h8 *)p, al = *(const h8 *)(p + 1024);
-#pragma unroll
-                    for (int t = 0; t < NT; ++t)
-                        x[t] = mfma3(ah, al, kth[t][ks], ktl[t][ks], x[t]);
-                }
-#pragma unroll
-                for (int t = 0; t < NT; ++t)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r)
-                        turn[wave][4u * g4 + r][16 * t + r16] = x[t][r];
-                __builtin_amdgcn_wave_barrier();
-                /* as an operand: row r16, 8 columns in a row */
-                if (NT == 2 || (g4 >> 1) == (wave & 1u)) {
-                    float y[8];
-#pragma unroll
-                    for (uint32_t e = 0; e < 8u; ++e)
-                        y[e] = turn[wave][r16][8u * (NT == 2 ? g4 : g4 & 1u) + e];
-                    h8 hi, lo;
-                    split<8>(y, 1.0f / kUnit / (1 << kWDown), hi, lo);
-                    const uint32_t ks = NT == 2 ? wave : wave >> 1;
-                    char *to = vb + ((rt * KS + ks) * 2u) * 1024u + lane * 16u;
-                    *(h8 *)to = hi;
-                    *(h8 *)(to + 1024u) = lo;
-                }
-                __builtin_amdgcn_wave_barrier();
-            }
-            /* U's columns: each with its own power of two */
-#pragma unroll
-            for (uint32_t t = 0; t < 2u; ++t) {
-                if (t >= nt) continue;
+            for (uint32_t t = 0; t < NV; ++t) {
                 float m = 0.0f;
 #pragma unroll
                 for (int ks = 0; ks < 2; ++ks)
@@ -541,24 +508,49 @@ __global__ __launch_bounds__(256, 2) void linattn_prep(kq_launch_linattn a, Work
                         m = fmaxf(m, fabsf(v[t][ks][e]));
                     }
                 const int p = scale_exp(kq::lanes_max<48>(m));
-                const float sv = pow2(p), iv = ldexpf(pow2(-pu[hh]), -p);
-                h8 bh[2], bl[2];
+                iv[t] = ldexpf(pow2(-pu[hh]), -p);
 #pragma unroll
-                for (int ks = 0; ks < 2; ++ks) split<8>(v[t][ks], sv, bh[ks], bl[ks]);
-#pragma unroll
-                for (int rt = 0; rt < 4; ++rt) {
-                    f4 x = f4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                    for (int ks = 0; ks <= rt >> 1; ++ks) {
-                        const char *q = tri + 12288 + (rt < 2 ? rt : 2 * rt - 2 + ks) * 2048 +
-                                        lane * 16u;
-                        x = mfma3(*(const h8 *)q, *(const h8 *)(q + 1024), bh[ks], bl[ks], x);
-                    }
-                    *(f4 *)(vb + kKeyImage + ((nt * wave + t) * 4u + rt) * 1024u + lane * 16u) =
-                        x * iv;
-                }
+                for (int ks = 0; ks < 2; ++ks) split<8>(v[t][ks], pow2(p), bh[t][ks], bl[t][ks]);
             }
-            __syncthreads();
+            if (h0 + hh + 1u < per) load_v(kh * per + h0 + hh + 1u);
+            kq_lds_barrier();
+#pragma unroll
+            for (int rt = 0; rt < 4; ++rt) {
+                /* W's rows 16 rt .., the wave's columns, transposed; U's, the wave's columns */
+                f4 x[NT], u[NV];
+#pragma unroll
+                for (int t = 0; t < NT; ++t) x[t] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int t = 0; t < NV; ++t) u[t] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int ks = 0; ks <= rt >> 1; ++ks) {
+                    const char *p = tri + (rt < 2 ? rt : 2 * rt - 2 + ks) * 2048 + lane * 16u;
+                    const h8 wh = *(const h8 *)p, wl = *(const h8 *)(p + 1024);
+                    const h8 uh = *(const h8 *)(p + 12288), ul = *(const h8 *)(p + 12288 + 1024);
+#pragma unroll
+                    for (int t = 0; t < NT; ++t)
+                        x[t] = mfma3(kth[t][ks], ktl[t][ks], wh, wl, x[t]);
+#pragma unroll
+                    for (int t = 0; t < NV; ++t) u[t] = mfma3(uh, ul, bh[t][ks], bl[t][ks], u[t]);
+                }
+                /* W as an operand: half of a lane's eight values from each tile */
+#pragma unroll
+                for (int t = 0; t < NT; ++t) {
+                    const uint32_t tile = NT * wave + t;
+                    const float y[4] = {x[t][0], x[t][1], x[t][2], x[t][3]};
+                    h4 hi, lo;
+                    split<4>(y, 1.0f / kUnit / (1 << kWDown), hi, lo);
+                    char *to = vb + ((rt * KS + (tile >> 1)) * 2u) * 1024u + lane * 16u +
+                               (tile & 1u) * 8u;
+                    *(h4 *)to = hi;
+                    *(h4 *)(to + 1024u) = lo;
+                }
+#pragma unroll
+                for (int t = 0; t < NV; ++t)
+                    *(f4 *)(vb + kKeyImage + ((NV * wave + t) * 4u + rt) * 1024u + lane * 16u) =
+                        u[t] * iv[t];
+            }
+            kq_lds_barrier();
         }
     }
     if (badin) kq_flag(status, KQ_DEV_INPUT);
@@ -590,15 +582,14 @@ struct Frag {
     }
 };
 
-/* Four values of consecutive rows (of which `row` is the first, in fours) of
- * column r16 of column tile ct, times s, as part of the right operand at p */
-__device__ __forceinline__ void put(char *p, uint32_t row, uint32_t ct, uint32_t r16, const f4 &x,
-                                    float s) {
+/* A lane's four rows of row tile `tile`, column tile ct of a result, times s,
+ * as part of the right operand at p */
+__device__ __forceinline__ void put(char *p, uint32_t tile, uint32_t ct, uint32_t lane16,
+                                    const f4 &x, float s) {
     const float y[4] = {x[0], x[1], x[2], x[3]};
     h4 hi, lo;
     split<4>(y, s, hi, lo);
-    char *to = p + (((row >> 5) * 2u + ct) * 2u) * 1024u + (((row & 31u) >> 3) * 16u + r16) * 16u +
-               (row & 7u) * 2u;
+    char *to = p + (((tile >> 1) * 2u + ct) * 2u) * 1024u + lane16 + (tile & 1u) * 8u;
     *(h4 *)to = hi;
     *(h4 *)(to + 1024u) = lo;
 }
@@ -654,6 +645,7 @@ __device__ __forceinline__ uint32_t told_of(const uint32_t *p) {
 template <int DK, bool DELTA>
 __global__ __launch_bounds__(64 * kScanWaves) void linattn_scan(kq_launch_linattn a,
                                                                 kq_launch_seqs q, Work w,
+                                                                uint32_t base,
                                                                 uint32_t *status) {
     constexpr int KS = DK / 32, NR = DK / 64; /* steps over S's rows; row tiles of a solver */
     constexpr uint32_t kKeyImage = 256u * DK;
@@ -661,12 +653,20 @@ __global__ __launch_bounds__(64 * kScanWaves) void linattn_scan(kq_launch_linatt
     /* what the solvers tell of S, of E and F; their largest values, of S, E, F */
     __shared__ __attribute__((aligned(16))) uint32_t told_s[4], told_ef[4];
     __shared__ __attribute__((aligned(16))) float top_s[4], top_e[4], top_f[4];
-    const uint32_t s = blockIdx.y;
-    const uint2 mine = w.seq[s];
-    if (mine.y == 0u) return;
+    /* the chunks of one sequence that lie in the window: from the window's
+     * first chunk, or the sequence's */
+    if (base + blockIdx.y >= *w.total) return;
+    const uint4 ch = w.chunk[base + blockIdx.y];
+    if (blockIdx.y != 0u && ch.w != 0u) return;
+    const uint2 mine = w.seq[ch.z];
+    const uint32_t left_here = w.window - blockIdx.y, left_seq = mine.y - ch.w;
+    const uint32_t last = (left_here < left_seq ? left_here : left_seq) - 1u;
     bool badseq = false, bad = false, badin = false;
-    const kq::SeqSpan sp = kq::seq_span(q, s, badseq);
+    const kq::SeqSpan sp = kq::seq_span(q, ch.z, badseq);
     if (!sp.live) return;
+    const uint32_t row0 = ch.w * kC, rows = sp.rows - row0; /* from the first chunk on */
+    const float *state = ch.w == 0u ? a.state : a.state_out; /* as the last window left it */
+    const bool fresh = sp.fresh && ch.w == 0u;
     const uint32_t lane = threadIdx.x & 63u, r16 = lane & 15u, g4 = lane >> 4, lane16 = lane * 16u;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t rt = wave & 3u, fr = 16u * rt + 4u * g4; /* rows of the chunk */
@@ -678,7 +678,7 @@ __global__ __launch_bounds__(64 * kScanWaves) void linattn_scan(kq_launch_linatt
     const uint32_t h = b / tiles, tile = b % tiles, col = tile * kTile + r16;
     const uint32_t kh = h / (a.value_heads / a.key_heads);
 
-    const char *data = w.data + (uint64_t)mine.x * w.chunk_bytes;
+    const char *data = w.data + (uint64_t)blockIdx.y * w.chunk_bytes;
     const uint32_t kat = kh * w.key_bytes, vat = w.value_at + h * w.value_bytes; /* Q; M */
     const uint32_t fat = vat + kMat;           /* the rows' factors */
     const uint32_t wat = fat + kRowF * 4u;     /* W, then U */
@@ -694,13 +694,12 @@ __global__ __launch_bounds__(64 * kScanWaves) void linattn_scan(kq_launch_linatt
     auto zero = [](f4(&x)[2]) { x[0] = x[1] = f4{0.0f, 0.0f, 0.0f, 0.0f}; };
     /* rows of v or of the output of chunk n, the call's column tile */
     auto rows_at = [&](const float *p, uint64_t stride, uint32_t n) {
-        const uint32_t left = sp.rows - n * kC; /* rows past it are past the buffer */
-        return kq_buf(p + ((uint64_t)sp.begin + n * kC) * stride + h * a.value_width,
+        const uint32_t left = rows - n * kC; /* rows past it are past the buffer */
+        return kq_buf(p + ((uint64_t)sp.begin + row0 + n * kC) * stride + h * a.value_width,
                       (left < kC ? left : kC) * (uint32_t)stride * 4u);
     };
     Scale ss, se, sf;
     ss.s = ss.inv = se.s = se.inv = sf.s = sf.inv = 1.0f;
-    const uint32_t last = mine.y - 1u;
 
     if (wave < 4u) {
         __builtin_amdgcn_s_setprio(3); /* the chain first */
@@ -713,9 +712,9 @@ __global__ __launch_bounds__(64 * kScanWaves) void linattn_scan(kq_launch_linatt
             for (int ct = 0; ct < 2; ++ct)
 #pragma unroll
                 for (int r = 0; r < 4; ++r)
-                    S[t][ct][r] = sp.fresh ? 0.0f
-                                           : a.state[sat + (size_t)(16 * t + r) * a.value_width +
-                                                     16u * ct];
+                    S[t][ct][r] =
+                        fresh ? 0.0f
+                              : state[sat + (size_t)(16 * t + r) * a.value_width + 16u * ct];
         Frag<KS> W;
         Frag<2> T[NR];
         f4 V[2], f0, f1; /* U, or V with the factors n; e^(G_64 - G) */
@@ -758,7 +757,7 @@ __global__ __launch_bounds__(64 * kScanWaves) void linattn_scan(kq_launch_linatt
 #pragma unroll
             for (int t = 0; t < NR; ++t)
 #pragma unroll
-                for (int ct = 0; ct < 2; ++ct) put(sbuf, srow + 16u * t, ct, r16, S[t][ct], ss.s);
+                for (int ct = 0; ct < 2; ++ct) put(sbuf, NR * rt + t, ct, lane16, S[t][ct], ss.s);
         };
         float ms = 0.0f;
         auto share_s = [&]() {
@@ -822,8 +821,8 @@ __global__ __launch_bounds__(64 * kScanWaves) void linattn_scan(kq_launch_linatt
             auto put_ef = [&]() {
 #pragma unroll
                 for (int ct = 0; ct < 2; ++ct) {
-                    put(fbuf, fr, ct, r16, F[ct], sf.s);
-                    put(ebuf, fr, ct, r16, E[ct], se.s);
+                    put(fbuf, rt, ct, lane16, F[ct], sf.s);
+                    put(ebuf, rt, ct, lane16, E[ct], se.s);
                 }
             };
             put_ef();
@@ -986,6 +985,11 @@ uint64_t most_chunks(uint64_t tokens, uint32_t count, uint32_t max_rows) {
     return (tokens + (kC - 1u) * (n < count ? n : count)) / kC;
 }
 
+/* The operands are made and used a window of chunks at a time, so that they
+ * stay in the memory-side cache between the two launches and are overwritten
+ * there. */
+constexpr uint64_t kWindowBytes = 160u << 20;
+
 Work carve(const kq_launch_linattn &a, uint64_t tokens, uint32_t count, uint32_t max_rows,
            void *scratch, uint64_t *bytes) {
     Work w;
@@ -1003,22 +1007,29 @@ Work carve(const kq_launch_linattn &a, uint64_t tokens, uint32_t count, uint32_t
     w.value_bytes = delta ? solved : least;
     w.chunk_bytes = w.value_at + (uint64_t)w.value_bytes * a.value_heads;
     /* room for the delta form, which the sizes alone do not tell */
+    const uint64_t most = w.value_at + (uint64_t)solved * a.value_heads;
+    const uint64_t fit = kWindowBytes / most < 8u ? 8u : kWindowBytes / most;
+    w.window = (uint32_t)(fit < n ? fit : n);
     *bytes = 512u + up256(8u * (uint64_t)count) + up256(16u * n) +
-             n * (w.value_at + (uint64_t)solved * a.value_heads);
+             w.window * most;
     return w;
 }
 
-template <int DK, bool DELTA>
+template <int DK, int DV, bool DELTA>
 hipError_t run(const kq_launch_linattn &a, const kq_launch_seqs &q, const Work &w, uint32_t chunks,
                uint32_t *status, hipStream_t s) {
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(linattn_prep<DK, DELTA>), dim3(chunks, a.key_heads),
-                       dim3(256), 0, s, a, w, status);
-    const hipError_t e = hipGetLastError();
-    if (e != hipSuccess) return e;
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(linattn_scan<DK, DELTA>),
-                       dim3(a.value_heads * (a.value_width / kTile), q.count),
-                       dim3(64 * kScanWaves), 0, s, a, q, w, status);
-    return hipGetLastError();
+    for (uint32_t base = 0u; base < chunks; base += w.window) {
+        hipLaunchKernelGGL(HIP_KERNEL_NAME(linattn_prep<DK, DV, DELTA>),
+                           dim3(w.window, a.key_heads), dim3(256), 0, s, a, w, base, status);
+        hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+        hipLaunchKernelGGL(HIP_KERNEL_NAME(linattn_scan<DK, DELTA>),
+                           dim3(a.value_heads * (a.value_width / kTile), w.window),
+                           dim3(64 * kScanWaves), 0, s, a, q, w, base, status);
+        e = hipGetLastError();
+        if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
 }
 
 }  // namespace
@@ -1039,9 +1050,13 @@ hipError_t kq_linattn_chunked(const kq_launch_linattn &a, const kq_launch_seqs &
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     const bool delta = a.beta != nullptr;
-    if (a.key_width == 128u)
-        return delta ? run<128, true>(a, q, w, chunks, status, s)
-                     : run<128, false>(a, q, w, chunks, status, s);
-    return delta ? run<64, true>(a, q, w, chunks, status, s)
-                 : run<64, false>(a, q, w, chunks, status, s);
+    const bool wide = a.key_width == 128u, wide_v = a.value_width == 128u;
+    if (!delta) /* v is not looked at before the scan */
+        return wide ? run<128, 64, false>(a, q, w, chunks, status, s)
+                    : run<64, 64, false>(a, q, w, chunks, status, s);
+    if (wide)
+        return wide_v ? run<128, 128, true>(a, q, w, chunks, status, s)
+                      : run<128, 64, true>(a, q, w, chunks, status, s);
+    return wide_v ? run<64, 128, true>(a, q, w, chunks, status, s)
+                  : run<64, 64, true>(a, q, w, chunks, status, s);
 }
