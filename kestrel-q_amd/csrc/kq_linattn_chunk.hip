@@ -8,8 +8,8 @@
  * solve
  *   (1 + L) E = diag(b) (diag(n) V - diag(n^2 e^G) K' S),
  *                                     L_ij = b_i n_i^2 e^(G_i - G_j) k'_i.k'_j  (j < i)
- * so that with T = (1 + L)^-1 diag(b), U = T diag(n) V, W = T diag(n^2 e^G) K'
- *   E = U - W S
+ * so that with T = (1 + L)^-1 diag(b), B = T diag(n), W = T diag(n^2 e^G) K'
+ *   E = B V - W S
  *   O = diag(e^G) Q S + M E,          M_ij = e^(G_i - G_j) q_i.k'_j      (j <= i)
  *   S' = e^(G_64) S + sum_j e^(G_64 - G_j) k'_j e_j^T
  * and what hangs on the chunk before is four products with S and E.
@@ -19,7 +19,7 @@
  *   linattn_plan  cuts the sequences into chunks (on the device: the lengths
  *                 are there)
  *   linattn_prep  a workgroup for each chunk and key head: Q, K'^T as operands
- *                 of the matrix cores, and for each of its value heads M, W, U
+ *                 of the matrix cores, and for each of its value heads M, W, B
  *   linattn_scan  a workgroup for each sequence, head and 32 columns of v:
  *                 S in registers from the first chunk to the last
  *
@@ -36,6 +36,8 @@
  * carry powers of two. Log decays are summed in 64 bits, since their
  * differences are what counts.
  */
+#include <type_traits>
+
 #include "kq_linattn.h"
 
 namespace {
@@ -49,7 +51,7 @@ typedef float f4 __attribute__((ext_vector_type(4)));
 constexpr uint32_t kC = 64;       /* rows of a chunk */
 constexpr uint32_t kHeads = 3;    /* value heads that linattn_prep takes at a time */
 constexpr uint32_t kBlk = 20;     /* floats of an LDS row of a 16 x 16 block */
-constexpr uint32_t kMat = 16384;  /* bytes of a 64 x 64 operand, hi and lo */
+constexpr uint32_t kMat = 12288;  /* bytes of a lower 64 x 64 operand, hi and lo */
 constexpr uint32_t kRowF = 5 * kC; /* floats of a value head's factors */
 
 constexpr float kUnit = 0x1p10f;   /* of the rows of k and q */
@@ -89,6 +91,12 @@ __device__ __forceinline__ void split(const float *x, float s, H &hi, H &lo) {
         lo[i] = (_Float16)fmaf(x[i], s, -(float)h.x);
         lo[i + 1] = (_Float16)fmaf(x[i + 1], s, -(float)h.y);
     }
+}
+
+/* Of a lower 64 x 64 operand the pieces (row tile rt, 32 columns from 32 ks)
+ * that are not zeros, 2048 bytes each: rt 0 and 1 have ks 0 only */
+__device__ __forceinline__ constexpr uint32_t piece(uint32_t rt, uint32_t ks) {
+    return (rt < 2u ? rt : 2u * rt - 2u + ks) * 2048u;
 }
 
 /* the power of two that brings m to 2^14 .. 2^15 */
@@ -211,18 +219,25 @@ __device__ __forceinline__ void invert(Lower &m, uint32_t lane, f4 (&x)[10]) {
         const int d[4] = {blk(0, 0), blk(1, 1), blk(2, 2), blk(3, 3)};
         const float(*l)[kBlk] = m[g4 == 0u ? d[0] : g4 == 1u ? d[1] : g4 == 2u ? d[2] : d[3]];
         float t[16];
+        t[0] = r16 == 0u ? 1.0f : 0.0f;
+        auto rows = [&](auto from, auto to) { /* all of their reads in flight at once */
+            f4 row[to - from][(to + 2) / 4];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            float s0 = (int)r16 == i ? 1.0f : 0.0f, s1 = 0.0f;
+            for (int i = from; i < to; ++i)
 #pragma unroll
-            for (int j = 0; j < i; ++j) {
-                if (j & 1)
-                    s1 = fmaf(-l[i][j], t[j], s1);
-                else
-                    s0 = fmaf(-l[i][j], t[j], s0);
+                for (int k = 0; 4 * k < i; ++k) row[i - from][k] = *(const f4 *)&l[i][4 * k];
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int i = from; i < to; ++i) {
+                float s[2] = {(int)r16 == i ? 1.0f : 0.0f, 0.0f};
+#pragma unroll
+                for (int j = 0; j < i; ++j)
+                    s[j & 1] = fmaf(-row[i - from][j / 4][j % 4], t[j], s[j & 1]);
+                t[i] = s[0] + s[1];
             }
-            t[i] = s0 + s1;
-        }
+        };
+        rows(std::integral_constant<int, 1>{}, std::integral_constant<int, 9>{});
+        rows(std::integral_constant<int, 9>{}, std::integral_constant<int, 16>{});
         __builtin_amdgcn_wave_barrier();
         float(*o)[kBlk] = m[g4 == 0u ? d[0] : g4 == 1u ? d[1] : g4 == 2u ? d[2] : d[3]];
 #pragma unroll
@@ -249,15 +264,15 @@ __device__ __forceinline__ void invert(Lower &m, uint32_t lane, f4 (&x)[10]) {
         }
 }
 
-template <int DK, int DV, bool DELTA>
+template <int DK, bool DELTA>
 __global__ __launch_bounds__(256, 2) void linattn_prep(kq_launch_linattn a, Work w,
                                                        uint32_t base, uint32_t *status) {
-    constexpr int KS = DK / 32, NT = DK / 64, NV = DV / 64; /* tiles of a wave */
+    constexpr int KS = DK / 32, NT = DK / 64; /* dk tiles of a wave */
     constexpr uint32_t kKeyImage = 256u * DK, kSolve = DELTA ? kHeads * sizeof(Lower) : 0u;
     /* K' as an operand, then the triangles of the heads */
     __shared__ __attribute__((aligned(16))) char pool[kKeyImage > kSolve ? kKeyImage : kSolve];
-    /* T with its two column factors as operands, the pieces below the diagonal */
-    __shared__ __attribute__((aligned(16))) char tri[DELTA ? 24576 : 16];
+    /* T diag(n^2 e^G) as an operand */
+    __shared__ __attribute__((aligned(16))) char tri[DELTA ? kMat : 16];
     __shared__ __attribute__((aligned(16))) double sum[kHeads][kC];
     __shared__ __attribute__((aligned(16))) float cw[kHeads][kC], cu[kHeads][kC];
     __shared__ float bet[kHeads][kC], nks[kC], nqs[kC];
@@ -271,6 +286,29 @@ __global__ __launch_bounds__(256, 2) void linattn_prep(kq_launch_linattn a, Work
     char *cb = w.data + (uint64_t)blockIdx.x * w.chunk_bytes;
     char *kb = cb + (uint64_t)kh * w.key_bytes;
     bool badin = false;
+
+    /* the gates of head h0 + wave, row `lane`: loaded first, formed while
+     * nothing else is under way that a wait for them would wait for too */
+    float g_rate = 0.0f, g_bias = 0.0f, g_alpha = 0.0f, g_beta = 0.0f, g_b = 0.0f;
+    double g_sum = 0.0, g_end = 0.0;
+    auto load_gates = [&](uint32_t h) {
+        const uint64_t t = (uint64_t)ch.x + (lane < ch.y ? lane : 0u);
+        g_rate = a.rate[h];
+        if (a.bias != nullptr) g_bias = a.bias[h];
+        if (a.alpha != nullptr) g_alpha = a.alpha[t * a.as + h];
+        if (DELTA) g_beta = a.beta[t * a.bs + h];
+    };
+    auto form_gates = [&]() {
+        badin |= !kq_isfinite(g_rate) || g_rate > 0.0f || !kq_isfinite(g_bias) ||
+                 !kq_isfinite(g_alpha) || !kq_isfinite(g_beta);
+        float g = g_rate;
+        if (a.alpha != nullptr) g *= kq::softplus(g_alpha + g_bias);
+        g = lane < ch.y ? fmaxf(g, -1.0e30f) : 0.0f;
+        if (DELTA) g_b = lane < ch.y ? kq::sigmoid(g_beta) : 0.0f;
+        g_sum = kq_wave_scan_f64((double)g);
+        g_end = kq_readlane_f64(g_sum, 63);
+    };
+    if (wave < kHeads && wave < per) load_gates(kh * per + wave);
 
     /* rows 16 wave + r16 of k and q as operands */
     f4 kk[4], qk[4];
@@ -297,6 +335,7 @@ __global__ __launch_bounds__(256, 2) void linattn_prep(kq_launch_linattn a, Work
                     y[ks][4 * k + 2] = v.z; y[ks][4 * k + 3] = v.w;
                 }
         }
+        if (wave < kHeads && wave < per) form_gates();
         const float nk = unit_row<KS>(x, a.normalize, a.epsilon, badin);
         const float nq = unit_row<KS>(y, a.normalize, a.epsilon, badin) * a.scale;
         if (g4 == 0u) {
@@ -349,24 +388,6 @@ __global__ __launch_bounds__(256, 2) void linattn_prep(kq_launch_linattn a, Work
             *(h8 *)(to + 1024u) = ktl[t][ks];
         }
     }
-    /* The wave's columns of a head's V, 16 (NV wave + t) + r16: on their way
-     * while the head before is at work */
-    float v[NV][2][8];
-    auto load_v = [&](uint32_t h) {
-        const KqBuf vr = kq_buf(a.v + (uint64_t)ch.x * a.vs + h * DV,
-                                ch.y * (uint32_t)a.vs * 4u); /* zeros past the rows */
-        const uint32_t at = (4u * g4 * (uint32_t)a.vs + 16u * NV * wave + r16) * 4u;
-#pragma unroll
-        for (uint32_t t = 0; t < NV; ++t)
-#pragma unroll
-            for (uint32_t ks = 0; ks < 2u; ++ks)
-#pragma unroll
-                for (uint32_t e = 0; e < 8u; ++e)
-                    v[t][ks][e] = __uint_as_float(
-                        kq_ld32(vr, at + (32u * ks + 16u * (e / 4u) + e % 4u) * (uint32_t)a.vs * 4u,
-                                64u * t));
-    };
-    if (DELTA) load_v(kh * per);
     __syncthreads(); /* the image of k is free */
 
     Lower *solve = (Lower *)pool;
@@ -374,22 +395,12 @@ __global__ __launch_bounds__(256, 2) void linattn_prep(kq_launch_linattn a, Work
         const uint32_t nh = per - h0 < kHeads ? per - h0 : kHeads;
         char *vb0 = cb + w.value_at + (uint64_t)(kh * per + h0) * w.value_bytes;
         if (wave < nh) { /* a wave for each head, a lane for each row */
-            const uint32_t h = kh * per + h0 + wave;
-            const float rate = a.rate[h], bias = a.bias != nullptr ? a.bias[h] : 0.0f;
-            badin |= !kq_isfinite(rate) || rate > 0.0f || !kq_isfinite(bias);
-            float g = 0.0f, b = 0.0f;
-            if (lane < ch.y) {
-                const uint64_t t = (uint64_t)ch.x + lane;
-                g = kq::log_decay(a, t, h, rate, bias, badin);
-                if (DELTA) {
-                    const float x = a.beta[t * a.bs + h];
-                    badin |= !kq_isfinite(x);
-                    b = kq::sigmoid(x);
-                }
+            if (h0 != 0u) {
+                load_gates(kh * per + h0 + wave);
+                form_gates();
             }
-            const double G = kq_wave_scan_f64((double)g);
-            const double end = kq_readlane_f64(G, 63);
-            const float from = kq::exp_of(G), n = nks[lane];
+            const double G = g_sum, end = g_end;
+            const float from = kq::exp_of(G), n = nks[lane], b = g_b;
             sum[wave][lane] = G;
             bet[wave][lane] = b * n * n;
             cw[wave][lane] = b * n * n * from;
@@ -412,14 +423,18 @@ __global__ __launch_bounds__(256, 2) void linattn_prep(kq_launch_linattn a, Work
 #pragma unroll
                 for (int half = 0; half < 2; ++half) {
                     const int jt = 2 * ks + half;
-                    f4 l;
+                    f4 l = f4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        x[4 * half + r] = l[r] = 0.0f;
-                        if (jt <= (int)wave) { /* rows of the diagonal tile above i: zeros */
-                            const bool above = jt == (int)wave && 4u * g4 + r > r16;
-                            const float fall =
-                                above ? 0.0f : kq::exp_of(gi - sum[hh][16 * jt + 4u * g4 + r]);
+                    for (int r = 0; r < 4; ++r) x[4 * half + r] = 0.0f;
+                    if (jt <= (int)wave) {
+                        double gj[4];
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) gj[r] = sum[hh][16 * jt + 4u * g4 + r];
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            float fall = kq::exp_of(gi - gj[r]);
+                            /* rows of the diagonal tile past column i: zeros */
+                            fall = jt == (int)wave && 4u * g4 + r > r16 ? 0.0f : fall;
                             x[4 * half + r] = qk[jt][r] * fall;
                             l[r] = bi * fall * kk[jt][r];
                         }
@@ -427,9 +442,10 @@ __global__ __launch_bounds__(256, 2) void linattn_prep(kq_launch_linattn a, Work
                     if (DELTA && jt <= (int)wave)
                         *(f4 *)&solve[hh][blk((int)wave, 0) + jt][r16][4u * g4] = l;
                 }
+                if (2 * ks > (int)wave) continue;
                 h8 hi, lo;
                 split<8>(x, kMixUnit / kUnit / kUnit, hi, lo);
-                char *to = vb + ((wave * 2u + ks) * 2u) * 1024u + lane * 16u;
+                char *to = vb + piece(wave, ks) + lane * 16u;
                 *(h8 *)to = hi;
                 *(h8 *)(to + 1024u) = lo;
             }
@@ -459,14 +475,15 @@ __global__ __launch_bounds__(256, 2) void linattn_prep(kq_launch_linattn a, Work
                 const int p = scale_exp(mw);
                 pw[wave] = p;
                 pu[wave] = scale_exp(mu);
-                *(float *)(vb0 + wave * w.value_bytes + kMat + (4 * kC + 1) * 4u) =
-                    pow2(kWDown - p);
+                float *f = (float *)(vb0 + wave * w.value_bytes + kMat) + 4 * kC;
+                f[1] = pow2(kWDown - p);
+                f[2] = pow2(-pu[wave]);
             }
         }
         __syncthreads();
         for (uint32_t hh = 0; hh < nh; ++hh) {
             char *vb = vb0 + hh * w.value_bytes + kMat + kRowF * 4u;
-            /* T's rows 16 wave + r16 with the factors of its columns, as operands */
+            /* T's rows 16 wave + r16 with the two factors of its columns, as operands */
             const float sw = pow2(pw[hh]), su = pow2(pu[hh]);
 #pragma unroll
             for (uint32_t ks = 0; ks < 2u; ++ks) {
@@ -486,69 +503,47 @@ __global__ __launch_bounds__(256, 2) void linattn_prep(kq_launch_linattn a, Work
                     }
                 }
                 h8 hi, lo;
-                char *to = tri + (wave < 2u ? wave : 2u * wave - 2u + ks) * 2048u + lane * 16u;
+                char *to = tri + piece(wave, ks) + lane * 16u;
                 split<8>(xw, sw, hi, lo);
                 *(h8 *)to = hi;
                 *(h8 *)(to + 1024u) = lo;
+                to = vb + kKeyImage + piece(wave, ks) + lane * 16u;
                 split<8>(xu, su, hi, lo);
-                *(h8 *)(to + 12288u) = hi;
-                *(h8 *)(to + 12288u + 1024u) = lo;
+                *(h8 *)to = hi;
+                *(h8 *)(to + 1024u) = lo;
             }
-            /* the columns of V as operands, each with its own power of two */
-            h8 bh[NV][2], bl[NV][2];
-            float iv[NV];
-#pragma unroll
-            for (uint32_t t = 0; t < NV; ++t) {
-                float m = 0.0f;
-#pragma unroll
-                for (int ks = 0; ks < 2; ++ks)
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        badin |= !kq_isfinite(v[t][ks][e]);
-                        m = fmaxf(m, fabsf(v[t][ks][e]));
-                    }
-                const int p = scale_exp(kq::lanes_max<48>(m));
-                iv[t] = ldexpf(pow2(-pu[hh]), -p);
-#pragma unroll
-                for (int ks = 0; ks < 2; ++ks) split<8>(v[t][ks], pow2(p), bh[t][ks], bl[t][ks]);
-            }
-            if (h0 + hh + 1u < per) load_v(kh * per + h0 + hh + 1u);
             kq_lds_barrier();
+            /* W's rows 16 rt .., the wave's columns, transposed */
 #pragma unroll
             for (int rt = 0; rt < 4; ++rt) {
-                /* W's rows 16 rt .., the wave's columns, transposed; U's, the wave's columns */
-                f4 x[NT], u[NV];
+                f4 x[NT];
 #pragma unroll
                 for (int t = 0; t < NT; ++t) x[t] = f4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                for (int t = 0; t < NV; ++t) u[t] = f4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
                 for (int ks = 0; ks <= rt >> 1; ++ks) {
-                    const char *p = tri + (rt < 2 ? rt : 2 * rt - 2 + ks) * 2048 + lane * 16u;
+                    const char *p = tri + piece(rt, ks) + lane * 16u;
                     const h8 wh = *(const h8 *)p, wl = *(const h8 *)(p + 1024);
-                    const h8 uh = *(const h8 *)(p + 12288), ul = *(const h8 *)(p + 12288 + 1024);
 #pragma unroll
                     for (int t = 0; t < NT; ++t)
                         x[t] = mfma3(kth[t][ks], ktl[t][ks], wh, wl, x[t]);
-#pragma unroll
-                    for (int t = 0; t < NV; ++t) u[t] = mfma3(uh, ul, bh[t][ks], bl[t][ks], u[t]);
                 }
-                /* W as an operand: half of a lane's eight values from each tile */
+                /* as an operand: half of a lane's eight values from each tile */
+                h8 hi, lo;
+                float y[4 * NT];
 #pragma unroll
-                for (int t = 0; t < NT; ++t) {
-                    const uint32_t tile = NT * wave + t;
-                    const float y[4] = {x[t][0], x[t][1], x[t][2], x[t][3]};
-                    h4 hi, lo;
-                    split<4>(y, 1.0f / kUnit / (1 << kWDown), hi, lo);
-                    char *to = vb + ((rt * KS + (tile >> 1)) * 2u) * 1024u + lane * 16u +
-                               (tile & 1u) * 8u;
-                    *(h4 *)to = hi;
-                    *(h4 *)(to + 1024u) = lo;
+                for (int k = 0; k < 4 * NT; ++k) y[k] = x[k / 4][k % 4];
+                const uint32_t tile = NT * wave;
+                char *to = vb + ((rt * KS + (tile >> 1)) * 2u) * 1024u + lane * 16u;
+                if constexpr (NT == 2) {
+                    split<8>(y, 1.0f / kUnit / (1 << kWDown), hi, lo);
+                    *(h8 *)to = hi;
+                    *(h8 *)(to + 1024u) = lo;
+                } else {
+                    h4 hi4, lo4;
+                    split<4>(y, 1.0f / kUnit / (1 << kWDown), hi4, lo4);
+                    *(h4 *)(to + (tile & 1u) * 8u) = hi4;
+                    *(h4 *)(to + (tile & 1u) * 8u + 1024u) = lo4;
                 }
-#pragma unroll
-                for (int t = 0; t < NV; ++t)
-                    *(f4 *)(vb + kKeyImage + ((NV * wave + t) * 4u + rt) * 1024u + lane * 16u) =
-                        u[t] * iv[t];
             }
             kq_lds_barrier();
         }
@@ -559,7 +554,6 @@ __global__ __launch_bounds__(256, 2) void linattn_prep(kq_launch_linattn a, Work
 /* ------------------------------------------------------------------ */
 
 constexpr uint32_t kTile = 32; /* columns of v that a workgroup holds */
-constexpr int kScanWaves = 8;
 
 /* a lane's part of an operand, hi and lo, N pieces 2048 bytes apart */
 template <int N>
@@ -572,6 +566,10 @@ struct Frag {
     __device__ __forceinline__ void load(KqBuf b, uint32_t lane16, uint32_t at) {
 #pragma unroll
         for (int i = 0; i < N; ++i) load1(b, lane16, at, i);
+    }
+    __device__ __forceinline__ void read1(const char *p, int i) {
+        hi[i] = *(const h8 *)p;
+        lo[i] = *(const h8 *)(p + 1024);
     }
     __device__ __forceinline__ void read(const char *p, int step) {
 #pragma unroll
@@ -632,27 +630,34 @@ __device__ __forceinline__ uint32_t told_of(const uint32_t *p) {
 }
 
 /*
- * Eight waves. Waves 0 .. 3 (the solvers) run the chain S -> E -> S': W S and
- * E for 16 rows of the chunk each, then K'^T F for a fourth of S's rows, which
- * they hold. Waves 4 .. 7 (the writers) form Q S and M E for 16 rows each and
- * store the output. So an operand is loaded by one wave, for both column
- * tiles, and what no other step waits for runs beside the chain. Two phases a
- * chunk with a barrier each:
- *   1  S's operand is there: W S, E, F | M E of the chunk before, its output
- *   2  E's and F's are there: S' | Q S
- * (Q S beside W S would have both wait for the same LDS reads).
+ * Waves 0 .. 3 (the solvers) run the chain S -> E -> S': W S and E for 16 rows
+ * of the chunk each, then K'^T F for a fourth of S's rows, which they hold.
+ * Waves 4 .. 7 (the writers) form Q S and M E for 16 rows each and store the
+ * output. Waves 8 .. 11, with the delta correction, split V and form B V. So
+ * an operand is loaded by one wave, for both column tiles, and what no other
+ * step waits for runs beside the chain. Two phases a chunk with a barrier each:
+ *   1  S's operand is there: W S, E, F | M E of the chunk before, its output |
+ *                            B V of the next
+ *   2  E's and F's are there: S' | Q S | V of the chunk after as an operand
+ * (Q S beside W S would have both wait for the same LDS reads). All loads of
+ * a role's loop are straight-line code: behind a branch the compiler could
+ * not tell how many are under way, and would wait for too many.
  */
+constexpr int scan_waves(bool delta) { return delta ? 12 : 8; }
+
 template <int DK, bool DELTA>
-__global__ __launch_bounds__(64 * kScanWaves) void linattn_scan(kq_launch_linattn a,
+__global__ __launch_bounds__(64 * scan_waves(DELTA)) void linattn_scan(kq_launch_linattn a,
                                                                 kq_launch_seqs q, Work w,
                                                                 uint32_t base,
                                                                 uint32_t *status) {
     constexpr int KS = DK / 32, NR = DK / 64; /* steps over S's rows; row tiles of a solver */
     constexpr uint32_t kKeyImage = 256u * DK;
-    __shared__ __attribute__((aligned(16))) char sbufs[2][KS * 4096], ebufs[2][8192], fbuf[8192];
+    __shared__ __attribute__((aligned(16))) char sbufs[2][KS * 4096], ebufs[2][8192], fbuf[8192],
+        vbuf[DELTA ? 8192 : 16], ubufs[2][DELTA ? 8192 : 16]; /* V; B V in 32 bits */
     /* what the solvers tell of S, of E and F; their largest values, of S, E, F */
     __shared__ __attribute__((aligned(16))) uint32_t told_s[4], told_ef[4];
     __shared__ __attribute__((aligned(16))) float top_s[4], top_e[4], top_f[4];
+    __shared__ float vscale[2][kTile]; /* of V's columns, by 32 rows */
     /* the chunks of one sequence that lie in the window: from the window's
      * first chunk, or the sequence's */
     if (base + blockIdx.y >= *w.total) return;
@@ -681,7 +686,7 @@ __global__ __launch_bounds__(64 * kScanWaves) void linattn_scan(kq_launch_linatt
     const char *data = w.data + (uint64_t)blockIdx.y * w.chunk_bytes;
     const uint32_t kat = kh * w.key_bytes, vat = w.value_at + h * w.value_bytes; /* Q; M */
     const uint32_t fat = vat + kMat;           /* the rows' factors */
-    const uint32_t wat = fat + kRowF * 4u;     /* W, then U */
+    const uint32_t wat = fat + kRowF * 4u;     /* W, then B */
     auto chunk = [&](uint32_t n) {
         return kq_buf(data + (uint64_t)n * w.chunk_bytes, (uint32_t)w.chunk_bytes);
     };
@@ -690,6 +695,14 @@ __global__ __launch_bounds__(64 * kScanWaves) void linattn_scan(kq_launch_linatt
     };
     auto scalar = [&](KqBuf c, uint32_t i) {
         return __uint_as_float(kq_ld32(c, i * 4u, fat + 4u * kC * 4u));
+    };
+    /* lower operands: the piece that rows 0 .. 31 lack lies past the buffer */
+    const uint32_t lane_k1 = rt < 2u ? 0x7fffff00u : lane16;
+    auto load_lower = [&](Frag<2> &x, KqBuf c, uint32_t at, int ks) {
+        x.hi[ks] = __builtin_bit_cast(
+            h8, kq_ld128(c, ks == 0 ? lane16 : lane_k1, at + piece(rt, rt < 2u ? 0u : ks)));
+        x.lo[ks] = __builtin_bit_cast(
+            h8, kq_ld128(c, ks == 0 ? lane16 : lane_k1, at + piece(rt, rt < 2u ? 0u : ks) + 1024u));
     };
     auto zero = [](f4(&x)[2]) { x[0] = x[1] = f4{0.0f, 0.0f, 0.0f, 0.0f}; };
     /* rows of v or of the output of chunk n, the call's column tile */
@@ -717,7 +730,7 @@ __global__ __launch_bounds__(64 * kScanWaves) void linattn_scan(kq_launch_linatt
                               : state[sat + (size_t)(16 * t + r) * a.value_width + 16u * ct];
         Frag<KS> W;
         Frag<2> T[NR];
-        f4 V[2], f0, f1; /* U, or V with the factors n; e^(G_64 - G) */
+        f4 V[2], f0, f1; /* B V, or V with the factors n; e^(G_64 - G) */
         float iw = 0.0f, c0;
         uint32_t io[4]; /* the wave's rows of v, in bytes */
         if (!DELTA)
@@ -728,11 +741,6 @@ __global__ __launch_bounds__(64 * kScanWaves) void linattn_scan(kq_launch_linatt
         };
         auto load_v = [&](KqBuf c, uint32_t n) {
             if (DELTA) {
-#pragma unroll
-                for (int ct = 0; ct < 2; ++ct)
-                    V[ct] = __builtin_bit_cast(
-                        f4, kq_ld128(c, lane16,
-                                     wat + kKeyImage + ((2u * tile + ct) * 4u + rt) * 1024u));
                 iw = scalar(c, 1u);
             } else {
                 f0 = factors(c, 0u);
@@ -775,6 +783,10 @@ __global__ __launch_bounds__(64 * kScanWaves) void linattn_scan(kq_launch_linatt
         load_v(first, 0u);
         load_t(first);
         share_s();
+        if (DELTA) { /* the writers' V and B V of the first chunk */
+            kq_lds_barrier();
+            kq_lds_barrier();
+        }
         for (uint32_t n = 0; n <= last; ++n) {
             const uint32_t more = n < last ? n + 1u : n; /* the last loads again */
             const KqBuf next = chunk(more);
@@ -792,15 +804,23 @@ __global__ __launch_bounds__(64 * kScanWaves) void linattn_scan(kq_launch_linatt
                 kq_lds_barrier();
             }
             if (DELTA) {
-                Frag<KS> B[2];
+                Frag<2> B[2]; /* two steps' at a time */
 #pragma unroll
                 for (int ct = 0; ct < 2; ++ct) B[ct].read(sbuf + ct * 2048u + lane16, 4096);
+#pragma unroll
+                for (int ct = 0; ct < 2; ++ct)
+                    V[ct] = *(const f4 *)(ubufs[n & 1u] + (ct * 4u + rt) * 1024u + lane16);
                 __builtin_amdgcn_sched_barrier(0); /* all in flight, then the products */
 #pragma unroll
                 for (int ks = 0; ks < KS; ++ks) {
 #pragma unroll
                     for (int ct = 0; ct < 2; ++ct)
-                        E[ct] = mfma3(W.hi[ks], W.lo[ks], B[ct].hi[ks], B[ct].lo[ks], E[ct]);
+                        E[ct] = mfma3(W.hi[ks], W.lo[ks], B[ct].hi[ks & 1], B[ct].lo[ks & 1],
+                                      E[ct]);
+                    if (ks + 2 < KS)
+#pragma unroll
+                        for (int ct = 0; ct < 2; ++ct)
+                            B[ct].read1(sbuf + ct * 2048u + lane16 + (ks + 2) * 4096, ks & 1);
                     W.load1(next, lane16, wat + rt * KS * 2048u, ks); /* of the next chunk */
                     __builtin_amdgcn_sched_barrier(0);
                 }
@@ -888,7 +908,7 @@ __global__ __launch_bounds__(64 * kScanWaves) void linattn_scan(kq_launch_linatt
                     a.state_out[sat + (size_t)(16 * t + r) * a.value_width + 16u * ct] =
                         S[t][ct][r];
                 }
-    } else {
+    } else if (wave < 8u) {
         Frag<KS> Q;
         Frag<2> M;
         f4 f0, f1; /* the factors of q, and with e^G */
@@ -912,7 +932,7 @@ __global__ __launch_bounds__(64 * kScanWaves) void linattn_scan(kq_launch_linatt
 #pragma unroll
                 for (int ct = 0; ct < 2; ++ct)
                     O[ct] = mfma3(M.hi[ks], M.lo[ks], B[ct].hi[ks], B[ct].lo[ks], O[ct]);
-                M.load1(next, lane16, vat + rt * 4096u, ks);
+                load_lower(M, next, vat, ks);
                 __builtin_amdgcn_sched_barrier(0);
             }
             const float pe = se.inv * (1.0f / kMixUnit);
@@ -932,22 +952,26 @@ __global__ __launch_bounds__(64 * kScanWaves) void linattn_scan(kq_launch_linatt
         {
             const KqBuf first = chunk(0u);
             Q.load(first, lane16, kat + rt * KS * 2048u);
-            M.load(first, lane16, vat + rt * 4096u);
+            load_lower(M, first, vat, 0);
+            load_lower(M, first, vat, 1);
             f0 = factors(first, 2u);
             f1 = factors(first, 3u);
         }
-        for (uint32_t n = 0; n <= last; ++n) {
-            const KqBuf next = chunk(n < last ? n + 1u : n);
+        if (DELTA) {
             kq_lds_barrier();
-            /* 1 */
+            kq_lds_barrier();
+        }
+        auto check_s = [&]() {
+            kq_lds_barrier();
             if (!Scale::holds(told_of(told_s))) {
                 kq_lds_barrier();
                 ss.set(top_of(top_s));
                 kq_lds_barrier();
             }
-            if (n != 0u) write(n - 1u, chunk(n));
+        };
+        /* 2: Q S */
+        auto second = [&](uint32_t n) {
             kq_lds_barrier();
-            /* 2: Q S */
             const uint32_t all = told_of(told_ef);
             if (!Scale::holds(all) || !Scale::holds(all >> 8)) {
                 kq_lds_barrier();
@@ -955,23 +979,126 @@ __global__ __launch_bounds__(64 * kScanWaves) void linattn_scan(kq_launch_linatt
                 sf.set(top_of(top_f));
                 kq_lds_barrier();
             }
-            Frag<KS> B[2];
+            const KqBuf next = chunk(n < last ? n + 1u : n);
+            const char *sb = sbufs[n & 1u] + lane16;
+            Frag<2> B[2];
 #pragma unroll
-            for (int ct = 0; ct < 2; ++ct) B[ct].read(sbufs[n & 1u] + ct * 2048u + lane16, 4096);
+            for (int ct = 0; ct < 2; ++ct) B[ct].read(sb + ct * 2048u, 4096);
             zero(P);
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
 #pragma unroll
                 for (int ct = 0; ct < 2; ++ct)
-                    P[ct] = mfma3(Q.hi[ks], Q.lo[ks], B[ct].hi[ks], B[ct].lo[ks], P[ct]);
+                    P[ct] = mfma3(Q.hi[ks], Q.lo[ks], B[ct].hi[ks & 1], B[ct].lo[ks & 1], P[ct]);
+                if (ks + 2 < KS)
+#pragma unroll
+                    for (int ct = 0; ct < 2; ++ct)
+                        B[ct].read1(sb + ct * 2048u + (ks + 2) * 4096, ks & 1);
                 Q.load1(next, lane16, kat + rt * KS * 2048u, ks);
                 __builtin_amdgcn_sched_barrier(0);
             }
             ps = ss.inv * (1.0f / kUnit);
+        };
+        check_s();
+        second(0u);
+        for (uint32_t n = 1; n <= last; ++n) {
+            check_s();
+            write(n - 1u, chunk(n));
+            second(n);
         }
         kq_lds_barrier();
         write(last, chunk(last));
+    } else if constexpr (DELTA) {
+        Frag<2> B2;
+        float ib;
+        /* V of a chunk: a wave has the 32 rows ks of column tile ct, in the
+         * order of an operand, a power of two for each column */
+        const uint32_t ct = rt & 1u, ks = rt >> 1;
+        float v[8];
+        auto load_v = [&](uint32_t n) {
+            const KqBuf vr = rows_at(a.v, a.vs, n < last ? n : last);
+            const uint32_t at = (4u * g4 * (uint32_t)a.vs + col) * 4u;
+#pragma unroll
+            for (uint32_t e = 0; e < 8u; ++e)
+                v[e] = __uint_as_float(
+                    kq_ld32(vr, at + (16u * (e / 4u) + e % 4u) * (uint32_t)a.vs * 4u,
+                            128u * ks * (uint32_t)a.vs + 64u * ct));
+        };
+        auto put_v = [&]() {
+            float m = 0.0f;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                badin |= !kq_isfinite(v[e]);
+                m = fmaxf(m, fabsf(v[e]));
+            }
+            const int p = scale_exp(kq::lanes_max<48>(m));
+            if (g4 == 0u) vscale[ks][16u * ct + r16] = pow2(-p);
+            h8 hi, lo;
+            split<8>(v, pow2(p), hi, lo);
+            char *to = vbuf + ((ks * 2u + ct) * 2u) * 1024u + lane16;
+            *(h8 *)to = hi;
+            *(h8 *)(to + 1024u) = lo;
+        };
+        /* B V of chunk n from vbuf; B of the chunk after */
+        auto times_v = [&](uint32_t n, KqBuf next) {
+            f4 U[2][2];
+            Frag<2> B[2];
+            float sc[2][2];
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                zero(U[t]);
+                B[t].read(vbuf + t * 2048u + lane16, 4096);
+                sc[t][0] = vscale[0][16 * t + r16] * ib;
+                sc[t][1] = vscale[1][16 * t + r16] * ib;
+            }
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+                    U[t][k] = mfma3(B2.hi[k], B2.lo[k], B[t].hi[k], B[t].lo[k], U[t][k]);
+                load_lower(B2, next, wat + kKeyImage, k);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+                *(f4 *)(ubufs[n & 1u] + (4u * t + rt) * 1024u + lane16) =
+                    U[t][0] * sc[t][0] + U[t][1] * sc[t][1];
+            __builtin_amdgcn_sched_barrier(0);
+            ib = scalar(next, 2u);
+        };
+        const KqBuf first = chunk(0u);
+        load_v(0u);
+        load_lower(B2, first, wat + kKeyImage, 0);
+        load_lower(B2, first, wat + kKeyImage, 1);
+        ib = scalar(first, 2u);
+        put_v();
+        load_v(1u);
+        kq_lds_barrier();
+        times_v(0u, chunk(last != 0u ? 1u : 0u));
+        kq_lds_barrier();
+        put_v();
+        load_v(2u);
+        for (uint32_t n = 0; n <= last; ++n) {
+            kq_lds_barrier();
+            if (!Scale::holds(told_of(told_s))) {
+                kq_lds_barrier();
+                kq_lds_barrier();
+            }
+            /* 1 (behind the last chunk, B V of it again) */
+            times_v(n + 1u, chunk(n + 2u < last ? n + 2u : last));
+            kq_lds_barrier();
+            const uint32_t all = told_of(told_ef);
+            if (!Scale::holds(all) || !Scale::holds(all >> 8)) {
+                kq_lds_barrier();
+                kq_lds_barrier();
+            }
+            /* 2 */
+            put_v();
+            load_v(n + 3u);
+        }
+        kq_lds_barrier();
     }
     if (badin) kq_flag(status, KQ_DEV_INPUT);
     if (bad) kq_flag(status, KQ_DEV_NUMERIC);
@@ -1003,7 +1130,7 @@ Work carve(const kq_launch_linattn &a, uint64_t tokens, uint32_t count, uint32_t
     w.key_bytes = 512u * a.key_width;
     w.value_at = w.key_bytes * a.key_heads;
     const uint32_t least = kMat + kRowF * 4u;
-    const uint32_t solved = least + 256u * (a.key_width + a.value_width);
+    const uint32_t solved = least + 256u * a.key_width + kMat;
     w.value_bytes = delta ? solved : least;
     w.chunk_bytes = w.value_at + (uint64_t)w.value_bytes * a.value_heads;
     /* room for the delta form, which the sizes alone do not tell */
@@ -1015,17 +1142,17 @@ Work carve(const kq_launch_linattn &a, uint64_t tokens, uint32_t count, uint32_t
     return w;
 }
 
-template <int DK, int DV, bool DELTA>
+template <int DK, bool DELTA>
 hipError_t run(const kq_launch_linattn &a, const kq_launch_seqs &q, const Work &w, uint32_t chunks,
                uint32_t *status, hipStream_t s) {
     for (uint32_t base = 0u; base < chunks; base += w.window) {
-        hipLaunchKernelGGL(HIP_KERNEL_NAME(linattn_prep<DK, DV, DELTA>),
+        hipLaunchKernelGGL(HIP_KERNEL_NAME(linattn_prep<DK, DELTA>),
                            dim3(w.window, a.key_heads), dim3(256), 0, s, a, w, base, status);
         hipError_t e = hipGetLastError();
         if (e != hipSuccess) return e;
         hipLaunchKernelGGL(HIP_KERNEL_NAME(linattn_scan<DK, DELTA>),
                            dim3(a.value_heads * (a.value_width / kTile), w.window),
-                           dim3(64 * kScanWaves), 0, s, a, q, w, base, status);
+                               dim3(64 * scan_waves(DELTA)), 0, s, a, q, w, base, status);
         e = hipGetLastError();
         if (e != hipSuccess) return e;
     }
@@ -1050,13 +1177,9 @@ hipError_t kq_linattn_chunked(const kq_launch_linattn &a, const kq_launch_seqs &
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     const bool delta = a.beta != nullptr;
-    const bool wide = a.key_width == 128u, wide_v = a.value_width == 128u;
-    if (!delta) /* v is not looked at before the scan */
-        return wide ? run<128, 64, false>(a, q, w, chunks, status, s)
-                    : run<64, 64, false>(a, q, w, chunks, status, s);
-    if (wide)
-        return wide_v ? run<128, 128, true>(a, q, w, chunks, status, s)
-                      : run<128, 64, true>(a, q, w, chunks, status, s);
-    return wide_v ? run<64, 128, true>(a, q, w, chunks, status, s)
-                  : run<64, 64, true>(a, q, w, chunks, status, s);
+    if (a.key_width == 128u)
+        return delta ? run<128, true>(a, q, w, chunks, status, s)
+                     : run<128, false>(a, q, w, chunks, status, s);
+    return delta ? run<64, true>(a, q, w, chunks, status, s)
+                 : run<64, false>(a, q, w, chunks, status, s);
 }
