@@ -1010,13 +1010,14 @@ __global__ __launch_bounds__(64 * scan_waves(DELTA)) void linattn_scan(kq_launch
         kq_lds_barrier();
         write(last, chunk(last));
     } else if constexpr (DELTA) {
-        Frag<2> B2;
-        float ib;
+        /* what a wait for a miss in every cache would hold up the chain for:
+         * two chunks on their way */
+        Frag<2> B2[2];
+        float ib[2], v[2][8];
         /* V of a chunk: a wave has the 32 rows ks of column tile ct, in the
          * order of an operand, a power of two for each column */
         const uint32_t ct = rt & 1u, ks = rt >> 1;
-        float v[8];
-        auto load_v = [&](uint32_t n) {
+        auto load_v = [&](float(&v)[8], uint32_t n) {
             const KqBuf vr = rows_at(a.v, a.vs, n < last ? n : last);
             const uint32_t at = (4u * g4 * (uint32_t)a.vs + col) * 4u;
 #pragma unroll
@@ -1025,7 +1026,7 @@ __global__ __launch_bounds__(64 * scan_waves(DELTA)) void linattn_scan(kq_launch
                     kq_ld32(vr, at + (16u * (e / 4u) + e % 4u) * (uint32_t)a.vs * 4u,
                             128u * ks * (uint32_t)a.vs + 64u * ct));
         };
-        auto put_v = [&]() {
+        auto put_v = [&](float(&v)[8]) {
             float m = 0.0f;
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
@@ -1040,8 +1041,14 @@ __global__ __launch_bounds__(64 * scan_waves(DELTA)) void linattn_scan(kq_launch
             *(h8 *)to = hi;
             *(h8 *)(to + 1024u) = lo;
         };
-        /* B V of chunk n from vbuf; B of the chunk after */
-        auto times_v = [&](uint32_t n, KqBuf next) {
+        auto load_b = [&](int i, uint32_t n) {
+            const KqBuf c = chunk(n < last ? n : last);
+            load_lower(B2[i], c, wat + kKeyImage, 0);
+            load_lower(B2[i], c, wat + kKeyImage, 1);
+            ib[i] = scalar(c, 2u);
+        };
+        /* B V of chunk n from vbuf; then B of chunk n + 2 */
+        auto times_v = [&](int i, uint32_t n) {
             f4 U[2][2];
             Frag<2> B[2];
             float sc[2][2];
@@ -1049,45 +1056,42 @@ __global__ __launch_bounds__(64 * scan_waves(DELTA)) void linattn_scan(kq_launch
             for (int t = 0; t < 2; ++t) {
                 zero(U[t]);
                 B[t].read(vbuf + t * 2048u + lane16, 4096);
-                sc[t][0] = vscale[0][16 * t + r16] * ib;
-                sc[t][1] = vscale[1][16 * t + r16] * ib;
+                sc[t][0] = vscale[0][16 * t + r16] * ib[i];
+                sc[t][1] = vscale[1][16 * t + r16] * ib[i];
             }
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {
+            for (int k = 0; k < 2; ++k)
 #pragma unroll
                 for (int t = 0; t < 2; ++t)
-                    U[t][k] = mfma3(B2.hi[k], B2.lo[k], B[t].hi[k], B[t].lo[k], U[t][k]);
-                load_lower(B2, next, wat + kKeyImage, k);
-                __builtin_amdgcn_sched_barrier(0);
-            }
+                    U[t][k] = mfma3(B2[i].hi[k], B2[i].lo[k], B[t].hi[k], B[t].lo[k], U[t][k]);
 #pragma unroll
             for (int t = 0; t < 2; ++t)
                 *(f4 *)(ubufs[n & 1u] + (4u * t + rt) * 1024u + lane16) =
                     U[t][0] * sc[t][0] + U[t][1] * sc[t][1];
             __builtin_amdgcn_sched_barrier(0);
-            ib = scalar(next, 2u);
+            load_b(i, n + 2u);
         };
-        const KqBuf first = chunk(0u);
-        load_v(0u);
-        load_lower(B2, first, wat + kKeyImage, 0);
-        load_lower(B2, first, wat + kKeyImage, 1);
-        ib = scalar(first, 2u);
-        put_v();
-        load_v(1u);
+        load_v(v[0], 0u);
+        load_v(v[1], 1u);
+        load_b(0, 0u);
+        load_b(1, 1u);
+        put_v(v[0]);
+        load_v(v[0], 2u);
         kq_lds_barrier();
-        times_v(0u, chunk(last != 0u ? 1u : 0u));
+        times_v(0, 0u);
         kq_lds_barrier();
-        put_v();
-        load_v(2u);
-        for (uint32_t n = 0; n <= last; ++n) {
+        put_v(v[1]);
+        load_v(v[1], 3u);
+        /* chunk n, with the registers of B of chunk n + 1 and of V of chunk n + 2 */
+        auto body = [&](int ib1, int iv, uint32_t n) {
             kq_lds_barrier();
             if (!Scale::holds(told_of(told_s))) {
                 kq_lds_barrier();
                 kq_lds_barrier();
             }
             /* 1 (behind the last chunk, B V of it again) */
-            times_v(n + 1u, chunk(n + 2u < last ? n + 2u : last));
+            times_v(ib1, n + 1u);
             kq_lds_barrier();
             const uint32_t all = told_of(told_ef);
             if (!Scale::holds(all) || !Scale::holds(all >> 8)) {
@@ -1095,8 +1099,13 @@ __global__ __launch_bounds__(64 * scan_waves(DELTA)) void linattn_scan(kq_launch
                 kq_lds_barrier();
             }
             /* 2 */
-            put_v();
-            load_v(n + 3u);
+            put_v(v[iv]);
+            load_v(v[iv], n + 4u);
+        };
+        for (uint32_t n = 0; n <= last; n += 2u) {
+            body(1, 0, n);
+            if (n == last) break;
+            body(0, 1, n + 1u);
         }
         kq_lds_barrier();
     }
@@ -1136,7 +1145,10 @@ Work carve(const kq_launch_linattn &a, uint64_t tokens, uint32_t count, uint32_t
     /* room for the delta form, which the sizes alone do not tell */
     const uint64_t most = w.value_at + (uint64_t)solved * a.value_heads;
     const uint64_t fit = kWindowBytes / most < 8u ? 8u : kWindowBytes / most;
-    w.window = (uint32_t)(fit < n ? fit : n);
+    /* whole rounds of linattn_prep's workgroups, two on each of 256 CUs */
+    const uint64_t round = a.key_heads < 512u ? 512u / a.key_heads : 1u;
+    const uint64_t whole = fit > round ? fit / round * round : fit;
+    w.window = (uint32_t)(whole < n ? whole : n);
     *bytes = 512u + up256(8u * (uint64_t)count) + up256(16u * n) +
              w.window * most;
     return w;
