@@ -5,14 +5,19 @@
  *   y_t[c] = act(bias[c] + sum_j w[c][j] x_(t - (K-1) + j)[c]),  K taps,
  *
  * the rows before a sequence's first from its state, oldest first. A thread
- * holds V neighbouring channels and walks kRows rows with the last K-1
+ * holds V neighbouring channels and walks a block of rows with the last K-1
  * inputs in registers, so that each input is read once (plus K-1 rows at a
- * walk's start). Bound by memory: 4 (K+1) operations a value of 8 bytes.
+ * walk's start, from a cache). Bound by memory: 2 K operations and a sigmoid
+ * for a value of 8 bytes moved. 4097 rows of 10,240 channels take 67 us, 5.0
+ * TB/s, what a large copy reaches; walks of 32 or 64 rows 72 us (fewer loads
+ * under way). One row a sequence, 32 x 10,240: 4.4 us, mostly the launch.
  *
- * The states are written by a second launch: a state that is updated in
- * place is read by the walk that holds the sequence's first row, which may
- * run behind the one that holds its last. With one row a sequence the same
- * thread reads and writes it, and one launch does both.
+ * A state may be written in place. Everything that reads it is therefore
+ * done by the workgroup that also writes it: those of a sequence take its
+ * first K-1 rows and write the state behind its last (inputs, or what is left
+ * of the old state). Those of a block of rows take all others, whatever
+ * sequences they belong to, and read inputs only. One launch has both, the
+ * sequences' first, so that many short sequences run side by side.
  */
 #include "kq_device.h"
 #include "kq_launch.h"
@@ -21,6 +26,11 @@
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int kBatch = 8; /* rows that a walk reads at a time */
+constexpr uint32_t kRows = 16; /* rows of a walk */
+constexpr uint32_t kParts = 1u << 15;
+
+typedef float f4 __attribute__((ext_vector_type(4)));
 
 template <int V>
 struct Vec {
@@ -45,6 +55,15 @@ __device__ __forceinline__ void store(float *p, const Vec<V> &r) {
         *(float4 *)p = make_float4(r.v[0], r.v[1], r.v[2], r.v[3]);
     else
         *p = r.v[0];
+}
+
+/* for outputs larger than the caches, read again by another launch */
+template <int V>
+__device__ __forceinline__ void store_nt(float *p, const Vec<V> &r) {
+    if constexpr (V == 4)
+        __builtin_nontemporal_store(__builtin_bit_cast(f4, r), (f4 *)p);
+    else
+        __builtin_nontemporal_store(r.v[0], p);
 }
 
 template <int V>
@@ -89,80 +108,143 @@ struct Taps {
     }
 };
 
-/* grid (channel groups, row blocks): rows [blockIdx.y * rows, + rows) of the
- * token array, whatever sequences they belong to */
+/* the state behind n rows from x on: entry n + j of [the old state, the rows] */
+template <int K, int V>
+__device__ __forceinline__ void write_state(const Vec<V> (&old)[K - 1], const float *x,
+                                            uint64_t xs, uint32_t n, float *to, uint32_t channels) {
+#pragma unroll
+    for (int j = 0; j < K - 1; ++j) {
+        Vec<V> v = old[j];
+        if (n + j >= (uint32_t)(K - 1)) {
+            v = load<V>(x + (size_t)(n + j - (K - 1)) * xs);
+        } else {
+#pragma unroll
+            for (int k = 0; k < K - 1; ++k)
+                if (n + j == (uint32_t)k) v = old[k];
+        }
+        store(to + (size_t)j * channels, v);
+    }
+}
+
+template <int K, int V>
+__device__ __forceinline__ void read_state(Vec<V> (&old)[K - 1], bool fresh, const float *from,
+                                           uint32_t channels) {
+#pragma unroll
+    for (int j = 0; j < K - 1; ++j) {
+        if (fresh) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) old[j].v[i] = 0.0f;
+        } else {
+            old[j] = load<V>(from + (size_t)j * channels);
+        }
+    }
+}
+
+/* the first K-1 rows of a sequence (or what it has), and its state */
+template <int K, int V>
+__device__ __forceinline__ void head_rows(const kq_launch_conv &c, const kq::SeqSpan &sp,
+                                          uint32_t ch, const float *x, uint64_t xs,
+                                          const float *state, float *state_out, float *y,
+                                          uint64_t ys, const Taps<K, V> &w, bool &badin,
+                                          bool &bad) {
+    const size_t at = (size_t)sp.slot * (K - 1) * c.channels + ch;
+    x += (size_t)sp.begin * xs + ch;
+    y += (size_t)sp.begin * ys + ch;
+    Vec<V> in[K - 1], hist[K - 1];
+    read_state<K, V>(hist, sp.fresh, state + at, c.channels);
+    if (sp.rows != 0u)
+#pragma unroll
+        for (int j = 0; j < K - 1; ++j) {
+            in[j] = load<V>(x + (j < (int)sp.rows ? (size_t)j * xs : 0u));
+            badin |= !finite(hist[j]);
+        }
+    write_state<K, V>(hist, x, xs, sp.rows, state_out + at, c.channels);
+#pragma unroll
+    for (int t = 0; t < K - 1; ++t) {
+        if (t >= (int)sp.rows) break;
+        badin |= !finite(in[t]);
+        const Vec<V> out = w.apply(hist, in[t], c.silu != 0u);
+        bad |= !finite(out);
+        store(y + (size_t)t * ys, out);
+#pragma unroll
+        for (int j = 0; j + 1 < K - 1; ++j) hist[j] = hist[j + 1];
+        hist[K - 2] = in[t];
+    }
+}
+
+/* grid: channel groups x (sequences, then blocks of kRows rows of the token
+ * array), the latter in y and z, kParts of them in y */
 template <int K, int V>
 __global__ __launch_bounds__(kThreads) void conv_rows(kq_launch_conv c, kq_launch_seqs q,
                                                       const float *__restrict__ x, uint64_t xs,
-                                                      const float *state, float *__restrict__ y,
-                                                      uint64_t ys, uint32_t rows,
+                                                      const float *state, float *state_out,
+                                                      float *__restrict__ y, uint64_t ys,
                                                       uint32_t *status) {
-    const uint32_t t0 = blockIdx.y * rows;
-    const uint32_t t1 = t0 + rows < (uint32_t)q.tokens ? t0 + rows : (uint32_t)q.tokens;
-    /* the last sequence that begins at or before t0: each wave counts */
-    uint32_t s = 0u;
-    {
+    const uint32_t part = blockIdx.z * kParts + blockIdx.y;
+    const uint32_t ch = (blockIdx.x * kThreads + threadIdx.x) * V;
+    const bool mine = ch < c.channels;
+    bool badin = false, bad = false, badseq = false;
+    Taps<K, V> w;
+    if (mine) badin |= !w.load(c, ch);
+    if (part < q.count) {
+        const kq::SeqSpan sp = kq::seq_span(q, part, badseq);
+        if (sp.live && blockIdx.x == 0u) badseq |= kq::seq_slot_taken<kThreads>(q, part, sp.slot);
+        if (sp.live && mine)
+            head_rows<K, V>(c, sp, ch, x, xs, state, state_out, y, ys, w, badin, bad);
+    } else {
+        const uint32_t tokens = (uint32_t)q.tokens, t0 = (part - q.count) * kRows; /* past the last row behind them all */
+        const uint32_t t1 = t0 + kRows < tokens ? t0 + kRows : tokens;
+        /* the last sequence that begins before t0: each wave counts them */
+        uint32_t s = 0u;
         const uint32_t lane = threadIdx.x & 63u;
         for (uint32_t base = 0u; base < q.count; base += 64u) {
-            const bool le = base + lane < q.count && q.offsets[base + lane] <= t0;
-            const uint64_t m = __ballot(le);
+            const uint64_t m = __ballot(base + lane < q.count && q.offsets[base + lane] < t0);
             s += (uint32_t)__popcll(m);
             if (m != ~0ull) break;
         }
-        if (s > 0u) s -= 1u;
-        s = __builtin_amdgcn_readfirstlane(s);
-    }
-    const uint32_t ch = (blockIdx.x * kThreads + threadIdx.x) * V;
-    if (ch >= c.channels) return;
-    Taps<K, V> w;
-    bool badin = !w.load(c, ch), bad = false, badseq = false;
-    Vec<V> hist[K - 1];
-    for (; s < q.count; ++s) {
-        if (q.offsets[s] >= t1) break;
-        const kq::SeqSpan sp = kq::seq_span(q, s, badseq);
-        if (!sp.live) continue;
-        const uint32_t end = sp.begin + sp.rows < t1 ? sp.begin + sp.rows : t1;
-        const uint32_t first = sp.begin > t0 ? sp.begin : t0;
-        if (first >= end) continue;
+        s = __builtin_amdgcn_readfirstlane(s > 0u ? s - 1u : 0u);
+        for (; mine && s < q.count && q.offsets[s] < t1; ++s) {
+            bool skip = false; /* its own workgroups say so */
+            const kq::SeqSpan sp = kq::seq_span(q, s, skip);
+            if (!sp.live || sp.rows < (uint32_t)K) continue;
+            const uint32_t from = sp.begin + (uint32_t)(K - 1), to = sp.begin + sp.rows;
+            const uint32_t first = from > t0 ? from : t0, end = to < t1 ? to : t1;
+            if (first >= end) continue;
+            Vec<V> hist[K - 1];
 #pragma unroll
-        for (int j = 0; j < K - 1; ++j) {
-            /* the sequence's row that tap j of row `first` reads */
-            const int32_t at = (int32_t)(first - sp.begin) - (K - 1) + j;
-            if (at >= 0) {
-                hist[j] = load<V>(x + (size_t)(sp.begin + at) * xs + ch);
-            } else if (sp.fresh) {
+            for (int j = 0; j < K - 1; ++j)
+                hist[j] = load<V>(x + (size_t)(first - (K - 1) + j) * xs + ch);
+            for (uint32_t t = first; t < end; t += kBatch) {
+                Vec<V> in[kBatch]; /* all under way before the first is used */
 #pragma unroll
-                for (int i = 0; i < V; ++i) hist[j].v[i] = 0.0f;
-            } else {
-                hist[j] = load<V>(state + ((size_t)sp.slot * (K - 1) + (size_t)(at + K - 1)) *
-                                              c.channels + ch);
-                badin |= !finite(hist[j]);
+                for (int i = 0; i < kBatch; ++i)
+                    in[i] = load<V>(x + (size_t)(t + i < end ? t + i : end - 1u) * xs + ch);
+#pragma unroll
+                for (int i = 0; i < kBatch; ++i) {
+                    if (t + i >= end) break;
+                    badin |= !finite(in[i]);
+                    const Vec<V> out = w.apply(hist, in[i], c.silu != 0u);
+                    bad |= !finite(out);
+                    store_nt(y + (size_t)(t + i) * ys + ch, out);
+#pragma unroll
+                    for (int j = 0; j + 1 < K - 1; ++j) hist[j] = hist[j + 1];
+                    hist[K - 2] = in[i];
+                }
             }
         }
-        for (uint32_t t = first; t < end; ++t) {
-            const Vec<V> in = load<V>(x + (size_t)t * xs + ch);
-            badin |= !finite(in);
-            const Vec<V> out = w.apply(hist, in, c.silu != 0u);
-            bad |= !finite(out);
-            store(y + (size_t)t * ys + ch, out);
-#pragma unroll
-            for (int j = 0; j + 1 < K - 1; ++j) hist[j] = hist[j + 1];
-            hist[K - 2] = in;
-        }
     }
+    if (badseq) kq_flag(status, KQ_DEV_SEQUENCE);
     if (badin) kq_flag(status, KQ_DEV_INPUT);
     if (bad) kq_flag(status, KQ_DEV_NUMERIC);
 }
 
-/* grid (channel groups, sequences). ROWS: one row a sequence, its output
- * formed here too; otherwise only the state behind the last row. Checks the
- * sequences of the call. */
-template <int K, int V, bool ROWS>
-__global__ __launch_bounds__(kThreads) void conv_states(kq_launch_conv c, kq_launch_seqs q,
-                                                        const float *__restrict__ x, uint64_t xs,
-                                                        const float *state, float *state_out,
-                                                        float *__restrict__ y, uint64_t ys,
-                                                        uint32_t *status) {
+/* grid (channel groups, sequences): one row a sequence */
+template <int K, int V>
+__global__ __launch_bounds__(kThreads) void conv_step(kq_launch_conv c, kq_launch_seqs q,
+                                                      const float *__restrict__ x, uint64_t xs,
+                                                      const float *state, float *state_out,
+                                                      float *__restrict__ y, uint64_t ys,
+                                                      uint32_t *status) {
     const uint32_t s = blockIdx.y;
     bool badseq = false, badin = false, bad = false;
     const kq::SeqSpan sp = kq::seq_span(q, s, badseq);
@@ -173,42 +255,21 @@ __global__ __launch_bounds__(kThreads) void conv_states(kq_launch_conv c, kq_lau
     const uint32_t ch = (blockIdx.x * kThreads + threadIdx.x) * V;
     if (ch >= c.channels || !sp.live) return;
     const size_t at = (size_t)sp.slot * (K - 1) * c.channels + ch;
+    const float *row = x + (size_t)sp.begin * xs + ch;
+    const Vec<V> in = load<V>(row);
     Vec<V> hist[K - 1];
+    read_state<K, V>(hist, sp.fresh, state + at, c.channels);
+    Taps<K, V> w;
+    badin |= !w.load(c, ch);
+    badin |= !finite(in);
 #pragma unroll
-    for (int j = 0; j < K - 1; ++j) {
-        if (sp.fresh) {
+    for (int j = 0; j < K - 1; ++j) badin |= !finite(hist[j]);
+    const Vec<V> out = w.apply(hist, in, c.silu != 0u);
+    bad |= !finite(out);
+    store(y + (size_t)sp.begin * ys + ch, out);
 #pragma unroll
-            for (int i = 0; i < V; ++i) hist[j].v[i] = 0.0f;
-        } else {
-            hist[j] = load<V>(state + at + (size_t)j * c.channels);
-        }
-    }
-    if constexpr (ROWS) {
-        Taps<K, V> w;
-        badin |= !w.load(c, ch);
-        const Vec<V> in = load<V>(x + (size_t)sp.begin * xs + ch);
-        badin |= !finite(in);
-#pragma unroll
-        for (int j = 0; j < K - 1; ++j) badin |= !finite(hist[j]);
-        const Vec<V> out = w.apply(hist, in, c.silu != 0u);
-        bad |= !finite(out);
-        store(y + (size_t)sp.begin * ys + ch, out);
-    }
-    const uint32_t n = sp.rows;
-#pragma unroll
-    for (int j = 0; j < K - 1; ++j) {
-        /* entry n + j of [the old state, the rows] */
-        Vec<V> v;
-        if (n + j >= (uint32_t)(K - 1)) {
-            v = load<V>(x + (size_t)(sp.begin + (n + j - (K - 1))) * xs + ch);
-        } else {
-            v = hist[j];
-#pragma unroll
-            for (int k = 0; k < K - 1; ++k)
-                if (n + j == (uint32_t)k) v = hist[k];
-        }
-        store(state_out + at + (size_t)j * c.channels, v);
-    }
+    for (int j = 0; j < K - 1; ++j)
+        store(state_out + at + (size_t)j * c.channels, j + 1 < K - 1 ? hist[j + 1] : in);
     if (badin) kq_flag(status, KQ_DEV_INPUT);
     if (bad) kq_flag(status, KQ_DEV_NUMERIC);
 }
@@ -219,18 +280,14 @@ hipError_t run(const kq_launch_conv &c, const kq_launch_seqs &q, const float *x,
                hipStream_t s) {
     const uint32_t groups = (c.channels / V + kThreads - 1) / kThreads;
     if (q.offsets == nullptr) {
-        hipLaunchKernelGGL(HIP_KERNEL_NAME(conv_states<K, V, true>), dim3(groups, q.count),
+        hipLaunchKernelGGL(HIP_KERNEL_NAME(conv_step<K, V>), dim3(groups, q.count),
                            dim3(kThreads), 0, s, c, q, x, xs, state, state_out, y, ys, status);
         return hipGetLastError();
     }
-    const uint32_t rows = 16u;
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(conv_rows<K, V>),
-                       dim3(groups, (uint32_t)((q.tokens + rows - 1) / rows)), dim3(kThreads), 0,
-                       s, c, q, x, xs, state, y, ys, rows, status);
-    hipError_t e = hipGetLastError();
-    if (e != hipSuccess) return e;
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(conv_states<K, V, false>), dim3(groups, q.count),
-                       dim3(kThreads), 0, s, c, q, x, xs, state, state_out, y, ys, status);
+    const uint32_t parts = q.count + (uint32_t)((q.tokens + kRows - 1) / kRows);
+    const dim3 grid(groups, parts < kParts ? parts : kParts, (parts + kParts - 1) / kParts);
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(conv_rows<K, V>), grid, dim3(kThreads), 0, s, c, q, x, xs,
+                       state, state_out, y, ys, status);
     return hipGetLastError();
 }
 
