@@ -285,6 +285,8 @@ extern "C" hipError_t kq_launch_block_join(const kq_launch_join *a, uint64_t tok
     } while (0)
     if (v4) {
         if (h <= 1024u) KQ_JOIN(256, 4, 1);
+        if (h <= 2048u) KQ_JOIN(256, 4, 2);
+        if (h <= 2560u) KQ_JOIN(320, 4, 2);
         if (h <= 4096u) KQ_JOIN(256, 4, 4);
         KQ_JOIN(1024, 4, 4);
     }
