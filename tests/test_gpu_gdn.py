@@ -256,6 +256,24 @@ def test_attention_long_prompt(ctx):
     check(a, a.got(ctx, off, None, [1], 1), spans, [0], [1])
 
 
+# many heads: the operands of 15 chunks (960 rows) fill a round of the work, so
+# that sequences go on from the state that an earlier round left
+@pytest.mark.parametrize("lengths", [[1100], [960, 30], [40, 700, 0, 500, 16, 17, 300]], ids=str)
+@pytest.mark.parametrize("delta", [True, False])
+def test_attention_rounds(ctx, lengths, delta):
+    say("rounds", lengths, delta)
+    off, spans, rows = table(lengths, lead=1, gap=1)
+    n = len(lengths)
+    a = Attention(11, 2, 256, 64, 64, rows, n + 1, delta=delta)
+    slots = [n - i for i in range(n)]
+    fresh = [i % 2 == 0 for i in range(n)]
+    if delta:
+        check(a, a.got(ctx, off, slots, fresh, n, in_place=True), spans, slots, fresh,
+              in_place=True)
+    else:
+        check(a, a.got(ctx, off, slots, fresh, n), spans, slots, fresh)
+
+
 def test_attention_split_prompt_is_one(ctx):
     # a prompt in two calls, its state carried on, against the prompt in one
     say("split prompt")
@@ -451,6 +469,21 @@ def test_conv(ctx, channels, taps):
     v.check(v.got(ctx, None, None, None, 7), one, list(range(7)), [0] * 7)
     v.check(v.got(ctx, None, [6, 0, NO, 1, 2, 3, 4], [0, 1, 0, 0, 1, 0, 0], 7, in_place=True),
             one, [6, 0, NO, 1, 2, 3, 4], [0, 1, 0, 0, 1, 0, 0], True)
+
+
+@pytest.mark.parametrize("taps", [2, 4, 8])
+def test_conv_many_sequences(ctx, taps):
+    # sequences shorter and longer than the taps, more of them than a wave
+    # counts, next to ones that fill several walks of rows
+    lengths = [(7 * i) % 12 for i in range(90)] + [1] * 70 + [100, 0, 33] + [0] * 5
+    off, spans, rows = table(lengths, lead=2, gap=3)
+    n = len(lengths)
+    c = Conv(taps, 36, taps, rows, n + 2)
+    slots = np.random.default_rng(taps).permutation(n + 2)[:n].tolist()
+    slots[91] = slots[4] = NO
+    fresh = [i % 3 == 0 for i in range(n)]
+    c.check(c.got(ctx, off, slots, fresh, n), spans, slots, fresh)
+    c.check(c.got(ctx, off, slots, fresh, n, in_place=True), spans, slots, fresh, True)
 
 
 def test_conv_layer(ctx):
