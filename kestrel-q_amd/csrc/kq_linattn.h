@@ -39,11 +39,20 @@ __device__ __forceinline__ Decay decay_of(float g) {
 
 }  // namespace kq
 
+/* the chunks of the sequences that the chunked form runs, in device memory */
+struct kq_linattn_plan {
+    uint32_t *total; /* their number; NULL for no plan */
+    uint2 *seq;      /* of each sequence: its first chunk and their number */
+    uint4 *chunk;    /* first row, rows, sequence, number in it */
+};
+constexpr uint32_t kChunkRows = 64;
+
 /* the recurrent form over the sequences of at most max_rows rows; checks all
- * sequences */
+ * sequences, and writes the plan of the others */
 hipError_t kq_linattn_recurrent(const kq_launch_linattn &a, const kq_launch_seqs &q,
-                                uint32_t max_rows, uint32_t *status, hipStream_t s);
-/* the chunked form over the sequences of more rows */
+                                uint32_t max_rows, const kq_linattn_plan &plan, uint32_t *status,
+                                hipStream_t s);
+/* both forms: the chunked one over the sequences of more rows */
 uint64_t kq_linattn_chunked_scratch(const kq_launch_linattn &a, uint64_t tokens, uint32_t count,
                                     uint32_t max_rows);
 hipError_t kq_linattn_chunked(const kq_launch_linattn &a, const kq_launch_seqs &q,

@@ -60,11 +60,73 @@ __device__ __forceinline__ float inverse_norm(const float (&x)[R], float eps) {
     return 0x1p-96f / sqrtf(kq::lanes_sum<SUM>(s));
 }
 
+/* the plan, by one workgroup of NT threads */
+template <int NT>
+__device__ __forceinline__ void cut(const kq_launch_seqs &q, uint32_t max_rows,
+                                    const kq_linattn_plan &w) {
+    __shared__ uint32_t first[NT], number[NT], begin[NT], rows[NT], sums[NT / 64];
+    __shared__ uint32_t refused;
+    const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6;
+    if (tid == 0u) refused = 0u;
+    __syncthreads();
+    bool bad = false;
+    for (uint32_t s = tid; s < q.count; s += NT) kq::seq_span(q, s, bad);
+    if (bad) refused = 1u; /* each sequence's own workgroups report it */
+    __syncthreads();
+    const bool none = refused != 0u;
+    uint32_t at = 0u;
+    for (uint32_t base = 0u; base < q.count; base += NT) {
+        const uint32_t s = base + tid;
+        uint32_t n = 0u;
+        if (s < q.count) {
+            const kq::SeqSpan sp = kq::seq_span(q, s, bad);
+            begin[tid] = sp.begin;
+            rows[tid] = sp.rows;
+            if (!none && sp.live && sp.rows > max_rows)
+                n = (sp.rows + kChunkRows - 1u) / kChunkRows;
+        }
+        uint32_t x = n; /* inclusive sum over the workgroup */
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const uint32_t y = __shfl_up(x, o, KQ_WAVE);
+            if (lane >= (uint32_t)o) x += y;
+        }
+        if (lane == 63u) sums[wave] = x;
+        __syncthreads();
+        uint32_t before = at, all = at;
+        for (uint32_t k = 0; k < NT / 64u; ++k) {
+            if (k < wave) before += sums[k];
+            all += sums[k];
+        }
+        first[tid] = before + x - n;
+        number[tid] = n;
+        if (s < q.count) w.seq[s] = make_uint2(before + x - n, n);
+        __syncthreads();
+        for (uint32_t i = wave; i < NT && base + i < q.count; i += NT / 64u)
+            for (uint32_t k = lane; k < number[i]; k += 64u) {
+                const uint32_t left = rows[i] - k * kChunkRows;
+                w.chunk[first[i] + k] =
+                    make_uint4(begin[i] + k * kChunkRows, left < kChunkRows ? left : kChunkRows,
+                               base + i, k);
+            }
+        at = all;
+        __syncthreads();
+    }
+    if (tid == 0u) *w.total = at;
+}
+
 /* grid (waves of columns of all heads / waves a workgroup, sequences): the
- * sequences of at most max_rows rows */
-template <int DK, int CG>
-__global__ __launch_bounds__(256) void linattn_rows(kq_launch_linattn a, kq_launch_seqs q,
-                                                    uint32_t max_rows, uint32_t *status) {
+ * sequences of at most max_rows rows. With a plan (CUT) one workgroup more in
+ * x, the first of which cuts the others into chunks: a launch of its own for
+ * that takes 5 us. */
+template <int DK, int CG, int NT, bool CUT>
+__global__ __launch_bounds__(NT) void linattn_rows(kq_launch_linattn a, kq_launch_seqs q,
+                                                   uint32_t max_rows, kq_linattn_plan plan,
+                                                   uint32_t *status) {
+    if (CUT && blockIdx.x == gridDim.x - 1u) {
+        if (blockIdx.y == 0u) cut<NT>(q, max_rows, plan);
+        return;
+    }
     constexpr int RG = 64 / CG, R = DK / RG, SUM = 63 & ~(CG - 1);
     const uint32_t lane = threadIdx.x & 63u;
     const uint32_t s = blockIdx.y;
@@ -72,12 +134,12 @@ __global__ __launch_bounds__(256) void linattn_rows(kq_launch_linattn a, kq_laun
     const kq::SeqSpan sp = kq::seq_span(q, s, badseq);
     if (blockIdx.x == 0u) {
         if (sp.live && q.slots != nullptr)
-            for (uint32_t j = threadIdx.x; j < s; j += blockDim.x) badseq |= q.slots[j] == sp.slot;
+            for (uint32_t j = threadIdx.x; j < s; j += NT) badseq |= q.slots[j] == sp.slot;
         if (badseq) kq_flag(status, KQ_DEV_SEQUENCE);
     }
     if (!sp.live || sp.rows > max_rows) return;
     const uint32_t tiles = a.value_width / (4u * CG);
-    const uint32_t w = __builtin_amdgcn_readfirstlane(blockIdx.x * (blockDim.x >> 6) +
+    const uint32_t w = __builtin_amdgcn_readfirstlane(blockIdx.x * (NT / 64) +
                                                       (threadIdx.x >> 6));
     const uint32_t h = w / tiles;
     if (h >= a.value_heads) return;
@@ -163,30 +225,35 @@ __global__ __launch_bounds__(256) void linattn_rows(kq_launch_linattn a, kq_laun
     if (bad) kq_flag(status, KQ_DEV_NUMERIC);
 }
 
-template <int DK, int CG>
+template <int DK, int CG, int NT, bool CUT>
 hipError_t launch(const kq_launch_linattn &a, const kq_launch_seqs &q, uint32_t max_rows,
-                  uint32_t *status, hipStream_t s) {
-    const uint32_t waves = a.value_heads * a.value_width / (4u * CG);
-    /* few waves: one a workgroup, so that they spread over the device */
-    const uint32_t per = (uint64_t)waves * q.count <= 1024u ? 1u : 4u;
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(linattn_rows<DK, CG>),
-                       dim3((waves + per - 1u) / per, q.count), dim3(64u * per), 0, s, a, q,
-                       max_rows, status);
+                  const kq_linattn_plan &plan, uint32_t *status, hipStream_t s) {
+    const uint32_t waves = a.value_heads * a.value_width / (4u * CG), per = NT / 64;
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(linattn_rows<DK, CG, NT, CUT>),
+                       dim3((waves + per - 1u) / per + (CUT ? 1u : 0u), q.count), dim3(NT), 0, s, a,
+                       q, max_rows, plan, status);
     return hipGetLastError();
+}
+
+/* Workgroups of four waves. Few waves (one sequence's row): half the columns
+ * each and one a workgroup, so that they spread over the device, which takes
+ * 48 heads of 128 x 128 from 6.4 to 5.6 us; 61 sequences 81 -> 83 us. */
+template <int DK>
+hipError_t launch(const kq_launch_linattn &a, const kq_launch_seqs &q, uint32_t max_rows,
+                  const kq_linattn_plan &plan, uint32_t *status, hipStream_t s) {
+    const uint64_t tiles = (uint64_t)a.value_heads * a.value_width / 32u * q.count;
+    if (plan.total != nullptr) return launch<DK, 8, 256, true>(a, q, max_rows, plan, status, s);
+    return tiles <= 256u ? launch<DK, 4, 64, false>(a, q, max_rows, plan, status, s)
+                         : launch<DK, 8, 256, false>(a, q, max_rows, plan, status, s);
 }
 
 }  // namespace
 
 hipError_t kq_linattn_recurrent(const kq_launch_linattn &a, const kq_launch_seqs &q,
-                                uint32_t max_rows, uint32_t *status, hipStream_t s) {
-    /* few waves (one sequence's row): half the columns each, which takes 48
-     * heads of 128 x 128 from 6.4 to 6.0 us; 61 sequences 81 -> 83 us */
-    const uint64_t tiles = (uint64_t)a.value_heads * a.value_width / 32u * q.count;
-    if (a.key_width == 128u)
-        return tiles <= 256u ? launch<128, 4>(a, q, max_rows, status, s)
-                             : launch<128, 8>(a, q, max_rows, status, s);
-    return tiles <= 256u ? launch<64, 4>(a, q, max_rows, status, s)
-                         : launch<64, 8>(a, q, max_rows, status, s);
+                                uint32_t max_rows, const kq_linattn_plan &plan, uint32_t *status,
+                                hipStream_t s) {
+    return a.key_width == 128u ? launch<128>(a, q, max_rows, plan, status, s)
+                               : launch<64>(a, q, max_rows, plan, status, s);
 }
 
 /* sequences up to this long run in the recurrent form */
@@ -200,7 +267,6 @@ extern "C" uint64_t kq_launch_linattn_scratch(const kq_launch_linattn *a, uint64
 extern "C" hipError_t kq_launch_linattn_run(const kq_launch_linattn *a, const kq_launch_seqs *q,
                                             void *scratch, uint32_t *status, hipStream_t s) {
     if (q->offsets == nullptr || q->tokens <= kShort)
-        return kq_linattn_recurrent(*a, *q, kShort, status, s);
-    const hipError_t e = kq_linattn_chunked(*a, *q, kShort, scratch, status, s);
-    return e == hipSuccess ? kq_linattn_recurrent(*a, *q, kShort, status, s) : e;
+        return kq_linattn_recurrent(*a, *q, kShort, kq_linattn_plan{}, status, s);
+    return kq_linattn_chunked(*a, *q, kShort, scratch, status, s);
 }

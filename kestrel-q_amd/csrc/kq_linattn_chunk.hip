@@ -16,8 +16,8 @@
  * Without the delta correction E = diag(n) V.
  *
  * Three launches:
- *   linattn_plan  cuts the sequences into chunks (on the device: the lengths
- *                 are there)
+ *   linattn_rows  the recurrent form over the short sequences, which also cuts
+ *                 the others into chunks (on the device: the lengths are there)
  *   linattn_prep  a workgroup for each chunk and key head: Q, K'^T as operands
  *                 of the matrix cores, and for each of its value heads M, W, B
  *   linattn_scan  a workgroup for each sequence, head and 32 columns of v:
@@ -48,7 +48,7 @@ typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef float f2 __attribute__((ext_vector_type(2)));
 typedef float f4 __attribute__((ext_vector_type(4)));
 
-constexpr uint32_t kC = 64;       /* rows of a chunk */
+constexpr uint32_t kC = kChunkRows;
 constexpr uint32_t kHeads = 3;    /* value heads that linattn_prep takes at a time */
 constexpr uint32_t kBlk = 20;     /* floats of an LDS row of a 16 x 16 block */
 constexpr uint32_t kMat = 12288;  /* bytes of a lower 64 x 64 operand, hi and lo */
@@ -61,9 +61,7 @@ constexpr float kMixUnit = 0x1p6f; /* of M: |q.k| <= 512 of such rows (128 value
 
 /* where the parts of the scratch lie */
 struct Work {
-    uint32_t *total;  /* chunks */
-    uint2 *seq;       /* of each sequence: its first chunk and their number */
-    uint4 *chunk;     /* first row, rows, sequence, number in it */
+    kq_linattn_plan plan;
     char *data;       /* operands of the chunks of a window */
     uint32_t window;  /* chunks */
     uint64_t chunk_bytes;
@@ -105,62 +103,6 @@ __device__ __forceinline__ int scale_exp(float m) {
     return e > 126 ? 126 : e;
 }
 __device__ __forceinline__ float pow2(int e) { return ldexpf(1.0f, e); }
-
-/* ------------------------------------------------------------------ */
-
-constexpr int kPlanThreads = 1024;
-
-__global__ __launch_bounds__(kPlanThreads) void linattn_plan(kq_launch_seqs q, uint32_t max_rows,
-                                                             Work w) {
-    __shared__ uint32_t first[kPlanThreads], number[kPlanThreads], begin[kPlanThreads],
-        rows[kPlanThreads], sums[kPlanThreads / 64];
-    __shared__ uint32_t refused;
-    const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6;
-    if (tid == 0u) refused = 0u;
-    __syncthreads();
-    bool bad = false;
-    for (uint32_t s = tid; s < q.count; s += kPlanThreads) kq::seq_span(q, s, bad);
-    if (bad) refused = 1u; /* the recurrent form's launch reports it */
-    __syncthreads();
-    const bool none = refused != 0u;
-    uint32_t at = 0u;
-    for (uint32_t base = 0u; base < q.count; base += kPlanThreads) {
-        const uint32_t s = base + tid;
-        uint32_t n = 0u;
-        if (s < q.count) {
-            const kq::SeqSpan sp = kq::seq_span(q, s, bad);
-            begin[tid] = sp.begin;
-            rows[tid] = sp.rows;
-            if (!none && sp.live && sp.rows > max_rows) n = (sp.rows + kC - 1u) / kC;
-        }
-        uint32_t x = n; /* inclusive sum over the workgroup */
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const uint32_t y = __shfl_up(x, o, KQ_WAVE);
-            if (lane >= (uint32_t)o) x += y;
-        }
-        if (lane == 63u) sums[wave] = x;
-        __syncthreads();
-        uint32_t before = at, all = at;
-        for (uint32_t k = 0; k < kPlanThreads / 64u; ++k) {
-            if (k < wave) before += sums[k];
-            all += sums[k];
-        }
-        first[tid] = before + x - n;
-        number[tid] = n;
-        if (s < q.count) w.seq[s] = make_uint2(before + x - n, n);
-        __syncthreads();
-        for (uint32_t i = wave; i < kPlanThreads && base + i < q.count; i += kPlanThreads / 64u)
-            for (uint32_t k = lane; k < number[i]; k += 64u) {
-                const uint32_t left = rows[i] - k * kC;
-                w.chunk[first[i] + k] =
-                    make_uint4(begin[i] + k * kC, left < kC ? left : kC, base + i, k);
-            }
-        at = all;
-        __syncthreads();
-    }
-    if (tid == 0u) *w.total = at;
-}
 
 /* ------------------------------------------------------------------ */
 
@@ -278,8 +220,8 @@ __global__ __launch_bounds__(256, 2) void linattn_prep(kq_launch_linattn a, Work
     __shared__ float bet[kHeads][kC], nks[kC], nqs[kC];
     __shared__ int pw[kHeads], pu[kHeads];
     const uint32_t c = base + blockIdx.x, kh = blockIdx.y;
-    if (c >= *w.total) return;
-    const uint4 ch = w.chunk[c];
+    if (c >= *w.plan.total) return;
+    const uint4 ch = w.plan.chunk[c];
     const uint32_t lane = threadIdx.x & 63u, r16 = lane & 15u, g4 = lane >> 4;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t per = a.value_heads / a.key_heads;
@@ -660,10 +602,10 @@ __global__ __launch_bounds__(64 * scan_waves(DELTA)) void linattn_scan(kq_launch
     __shared__ float vscale[2][kTile]; /* of V's columns, by 32 rows */
     /* the chunks of one sequence that lie in the window: from the window's
      * first chunk, or the sequence's */
-    if (base + blockIdx.y >= *w.total) return;
-    const uint4 ch = w.chunk[base + blockIdx.y];
+    if (base + blockIdx.y >= *w.plan.total) return;
+    const uint4 ch = w.plan.chunk[base + blockIdx.y];
     if (blockIdx.y != 0u && ch.w != 0u) return;
-    const uint2 mine = w.seq[ch.z];
+    const uint2 mine = w.plan.seq[ch.z];
     const uint32_t left_here = w.window - blockIdx.y, left_seq = mine.y - ch.w;
     const uint32_t last = (left_here < left_seq ? left_here : left_seq) - 1u;
     bool badseq = false, bad = false, badin = false;
@@ -1132,10 +1074,10 @@ Work carve(const kq_launch_linattn &a, uint64_t tokens, uint32_t count, uint32_t
     const uint64_t n = most_chunks(tokens, count, max_rows);
     const bool delta = a.beta != nullptr;
     char *p = (char *)(((uintptr_t)scratch + 255u) & ~(uintptr_t)255u);
-    w.total = (uint32_t *)p;
-    w.seq = (uint2 *)(p + 256u);
-    w.chunk = (uint4 *)((char *)w.seq + up256(8u * (uint64_t)count));
-    w.data = (char *)w.chunk + up256(16u * n);
+    w.plan.total = (uint32_t *)p;
+    w.plan.seq = (uint2 *)(p + 256u);
+    w.plan.chunk = (uint4 *)((char *)w.plan.seq + up256(8u * (uint64_t)count));
+    w.data = (char *)w.plan.chunk + up256(16u * n);
     w.key_bytes = 512u * a.key_width;
     w.value_at = w.key_bytes * a.key_heads;
     const uint32_t least = kMat + kRowF * 4u;
@@ -1185,8 +1127,7 @@ hipError_t kq_linattn_chunked(const kq_launch_linattn &a, const kq_launch_seqs &
     uint64_t bytes;
     const Work w = carve(a, q.tokens, q.count, max_rows, scratch, &bytes);
     const uint32_t chunks = (uint32_t)most_chunks(q.tokens, q.count, max_rows);
-    hipLaunchKernelGGL(linattn_plan, dim3(1), dim3(kPlanThreads), 0, s, q, max_rows, w);
-    const hipError_t e = hipGetLastError();
+    const hipError_t e = kq_linattn_recurrent(a, q, max_rows, w.plan, status, s);
     if (e != hipSuccess) return e;
     const bool delta = a.beta != nullptr;
     if (a.key_width == 128u)
