@@ -21,7 +21,9 @@
  *   linattn_prep  a workgroup for each chunk and key head: Q, K'^T as operands
  *                 of the matrix cores, and for each of its value heads M, W, B
  *   linattn_scan  a workgroup for each sequence, head and 32 columns of v:
- *                 S in registers from the first chunk to the last
+ *                 S in registers from the first chunk to the last; without the
+ *                 delta correction and with few such workgroups three launches
+ *                 over all chunks instead (linattn_sums, _states, _outs)
  *
  * A lane's eight values of an operand's long axis are 4 g .. 4 g + 3 of one 16
  * and the same four of the next (g = lane / 16), for both sides of a product:
@@ -1055,6 +1057,253 @@ __global__ __launch_bounds__(64 * scan_waves(DELTA)) void linattn_scan(kq_launch
     if (bad) kq_flag(status, KQ_DEV_NUMERIC);
 }
 
+/* ------------------------------------------------------------------ */
+
+/*
+ * Without the delta correction a chunk's rows add to the state what does not
+ * hang on it. Where the scan would have few workgroups, the work is split
+ * over the chunks instead:
+ *   linattn_sums    U = sum_j e^(G_64 - G_j) k'_j e_j^T of every chunk
+ *   linattn_states  S from chunk to chunk, into U's place
+ *   linattn_outs    the outputs of every chunk
+ * for a state read and written more a chunk.
+ */
+
+/* a workgroup's chunk, value head and 32 columns; four waves with 16 rows of
+ * the chunk each */
+struct Place {
+    uint4 ch;
+    uint32_t slot, h, col, fr;
+    char *data;
+    uint32_t kat, vat, fat, uat; /* Q, M, the factors, U */
+    bool live;
+    KqBuf buf;
+    __device__ __forceinline__ Place(const kq_launch_linattn &a, const kq_launch_seqs &q,
+                                     const Work &w, uint32_t base, uint32_t wave, uint32_t lane) {
+        live = base + blockIdx.y < *w.plan.total;
+        if (!live) return;
+        ch = w.plan.chunk[base + blockIdx.y];
+        bool bad = false;
+        const kq::SeqSpan sp = kq::seq_span(q, ch.z, bad);
+        live = sp.live;
+        slot = sp.slot;
+        uint32_t b = blockIdx.x; /* a head's to one XCD, as in the scan */
+        if (gridDim.x % 8u == 0u) b = (b % 8u) * (gridDim.x / 8u) + b / 8u;
+        const uint32_t tiles = a.value_width / kTile;
+        h = b / tiles;
+        col = (b % tiles) * kTile + (lane & 15u);
+        fr = 16u * wave + 4u * (lane >> 4);
+        data = w.data + (uint64_t)blockIdx.y * w.chunk_bytes;
+        kat = h / (a.value_heads / a.key_heads) * w.key_bytes;
+        vat = w.value_at + h * w.value_bytes;
+        fat = vat + kMat;
+        uat = fat + kRowF * 4u;
+        buf = kq_buf(data, (uint32_t)w.chunk_bytes);
+    }
+    __device__ __forceinline__ f4 factors(uint32_t i) const {
+        return __builtin_bit_cast(f4, kq_ld128(buf, fr * 4u, fat + i * kC * 4u));
+    }
+    /* the chunk's rows of v or of the output; rows past it are past the buffer */
+    __device__ __forceinline__ KqBuf rows(const float *p, uint64_t stride, uint32_t width) const {
+        return kq_buf(p + (uint64_t)ch.x * stride + h * width, ch.y * (uint32_t)stride * 4u);
+    }
+    __device__ __forceinline__ void load_v(const kq_launch_linattn &a, f4 (&V)[2]) const {
+        const KqBuf v = rows(a.v, a.vs, a.value_width);
+#pragma unroll
+        for (int ct = 0; ct < 2; ++ct)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                V[ct][r] = __uint_as_float(
+                    kq_ld32(v, ((fr + r) * (uint32_t)a.vs + col) * 4u, 64u * ct));
+    }
+};
+
+template <int DK>
+__global__ __launch_bounds__(256) void linattn_sums(kq_launch_linattn a, kq_launch_seqs q, Work w,
+                                                    uint32_t base, uint32_t *status) {
+    constexpr int NR = DK / 64;
+    __shared__ __attribute__((aligned(16))) char fbuf[8192];
+    __shared__ __attribute__((aligned(16))) float top[4];
+    const uint32_t lane = threadIdx.x & 63u, lane16 = lane * 16u;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const Place p(a, q, w, base, wave, lane);
+    if (!p.live) return;
+    f4 V[2];
+    p.load_v(a, V);
+    const f4 f0 = p.factors(0u), f1 = p.factors(1u);
+    Frag<2> T[NR];
+#pragma unroll
+    for (int t = 0; t < NR; ++t)
+        T[t].load(p.buf, lane16, p.kat + 256u * DK + (NR * wave + t) * 4096u);
+    bool badin = false;
+#pragma unroll
+    for (int ct = 0; ct < 2; ++ct)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            badin |= !kq_isfinite(V[ct][r]);
+            V[ct][r] = f0[r] * V[ct][r] * f1[r];
+        }
+    const float m = kq::lanes_max<63>(largest(largest(0.0f, V[0]), V[1]));
+    if (lane == 0u) top[wave] = m;
+    kq_lds_barrier();
+    Scale s;
+    s.set(top_of(top));
+#pragma unroll
+    for (int ct = 0; ct < 2; ++ct) put(fbuf, wave, ct, lane16, V[ct], s.s);
+    kq_lds_barrier();
+    float *u = (float *)(p.data + p.uat) +
+               (16u * NR * wave + 4u * (lane >> 4)) * a.value_width + p.col;
+#pragma unroll
+    for (int ct = 0; ct < 2; ++ct) {
+        Frag<2> B;
+        B.read(fbuf + ct * 2048u + lane16, 4096);
+#pragma unroll
+        for (int t = 0; t < NR; ++t) {
+            f4 x = f4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int ks = 0; ks < 2; ++ks)
+                x = mfma3(T[t].hi[ks], T[t].lo[ks], B.hi[ks], B.lo[ks], x);
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                u[(uint32_t)(16 * t + r) * a.value_width + 16u * ct] =
+                    x[r] * (s.inv * (1.0f / kUnit));
+        }
+    }
+    if (badin) kq_flag(status, KQ_DEV_INPUT);
+}
+
+/* grid (1024 values of the states, window): the first chunk of a sequence in
+ * the window goes on to its last there */
+__global__ __launch_bounds__(256) void linattn_states(kq_launch_linattn a, kq_launch_seqs q,
+                                                      Work w, uint32_t base, uint32_t *status) {
+    constexpr uint32_t kAhead = 8;
+    if (base + blockIdx.y >= *w.plan.total) return;
+    const uint4 ch = w.plan.chunk[base + blockIdx.y];
+    if (blockIdx.y != 0u && ch.w != 0u) return;
+    bool bad = false;
+    const kq::SeqSpan sp = kq::seq_span(q, ch.z, bad);
+    if (!sp.live) return;
+    const uint32_t left_here = w.window - blockIdx.y, left_seq = w.plan.seq[ch.z].y - ch.w;
+    const uint32_t n = left_here < left_seq ? left_here : left_seq;
+    const uint32_t size = a.key_width * a.value_width; /* a multiple of 1024 */
+    const uint32_t at = blockIdx.x * 1024u, h = at / size, i = at % size + 4u * threadIdx.x;
+    const size_t sat = ((size_t)sp.slot * a.value_heads + h) * size + i;
+    f4 S = f4{0.0f, 0.0f, 0.0f, 0.0f};
+    if (ch.w != 0u)
+        S = *(const f4 *)(a.state_out + sat);
+    else if (!sp.fresh)
+        S = *(const f4 *)(a.state + sat);
+    char *f = w.data + (uint64_t)blockIdx.y * w.chunk_bytes + w.value_at + h * w.value_bytes + kMat;
+    for (uint32_t c = 0; c < n; c += kAhead) {
+        f4 u[kAhead];
+        float c0[kAhead];
+#pragma unroll
+        for (uint32_t k = 0; k < kAhead; ++k) { /* the last again behind it */
+            const char *p = f + (uint64_t)(c + k < n ? c + k : n - 1u) * w.chunk_bytes;
+            u[k] = *(const f4 *)(p + kRowF * 4u + i * 4u);
+            c0[k] = *(const float *)(p + 4u * kC * 4u);
+        }
+#pragma unroll
+        for (uint32_t k = 0; k < kAhead; ++k) {
+            if (c + k >= n) break;
+            *(f4 *)(f + (uint64_t)(c + k) * w.chunk_bytes + kRowF * 4u + i * 4u) = S;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) S[r] = fmaf(c0[k], S[r], u[k][r]);
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < 4; ++r) bad |= !kq_isfinite(S[r]);
+    *(f4 *)(a.state_out + sat) = S;
+    if (bad) kq_flag(status, KQ_DEV_NUMERIC);
+}
+
+template <int DK>
+__global__ __launch_bounds__(256) void linattn_outs(kq_launch_linattn a, kq_launch_seqs q, Work w,
+                                                    uint32_t base, uint32_t *status) {
+    constexpr int KS = DK / 32, NR = DK / 64;
+    __shared__ __attribute__((aligned(16))) char sbuf[KS * 4096], ebuf[8192];
+    __shared__ __attribute__((aligned(16))) float top_s[4], top_e[4];
+    const uint32_t lane = threadIdx.x & 63u, lane16 = lane * 16u;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const Place p(a, q, w, base, wave, lane);
+    if (!p.live) return;
+    f4 S[NR][2], V[2];
+    const float *s = (const float *)(p.data + p.uat) +
+                     (16u * NR * wave + 4u * (lane >> 4)) * a.value_width + p.col;
+#pragma unroll
+    for (int t = 0; t < NR; ++t)
+#pragma unroll
+        for (int ct = 0; ct < 2; ++ct)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                S[t][ct][r] = s[(uint32_t)(16 * t + r) * a.value_width + 16u * ct];
+    p.load_v(a, V);
+    const f4 f0 = p.factors(0u), f2 = p.factors(2u), f3 = p.factors(3u);
+    Frag<KS> Q;
+    Frag<2> M;
+    Q.load(p.buf, lane16, p.kat + wave * KS * 2048u);
+    M.load(p.buf, lane16, p.vat + piece(wave, 0u)); /* rows 0 .. 31 have one piece */
+    float ms = 0.0f;
+#pragma unroll
+    for (int t = 0; t < NR; ++t) ms = largest(largest(ms, S[t][0]), S[t][1]);
+    ms = kq::lanes_max<63>(ms);
+#pragma unroll
+    for (int ct = 0; ct < 2; ++ct)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) V[ct][r] *= f0[r];
+    const float me = kq::lanes_max<63>(largest(largest(0.0f, V[0]), V[1]));
+    if (lane == 0u) {
+        top_s[wave] = ms;
+        top_e[wave] = me;
+    }
+    kq_lds_barrier();
+    Scale ss, se;
+    ss.set(top_of(top_s));
+    se.set(top_of(top_e));
+#pragma unroll
+    for (int ct = 0; ct < 2; ++ct) {
+#pragma unroll
+        for (int t = 0; t < NR; ++t) put(sbuf, NR * wave + t, ct, lane16, S[t][ct], ss.s);
+        put(ebuf, wave, ct, lane16, V[ct], se.s);
+    }
+    kq_lds_barrier();
+    const float ps = ss.inv * (1.0f / kUnit), pe = se.inv * (1.0f / kMixUnit);
+    const KqBuf y = p.rows(a.y, a.ys, a.value_width);
+    bool bad = false;
+#pragma unroll
+    for (int ct = 0; ct < 2; ++ct) {
+        f4 P = f4{0.0f, 0.0f, 0.0f, 0.0f}, O = P;
+        Frag<KS> B;
+        B.read(sbuf + ct * 2048u + lane16, 4096);
+        Frag<2> E;
+        E.read(ebuf + ct * 2048u + lane16, 4096);
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+            P = mfma3(Q.hi[ks], Q.lo[ks], B.hi[ks], B.lo[ks], P);
+        O = mfma3(M.hi[0], M.lo[0], E.hi[0], E.lo[0], O);
+        if (wave >= 2u) O = mfma3(M.hi[1], M.lo[1], E.hi[1], E.lo[1], O);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const float o = fmaf(f3[r], P[r] * ps, f2[r] * (O[r] * pe));
+            bad |= !kq_isfinite(o);
+            __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(o), y.r,
+                                                  (int)(((p.fr + r) * (uint32_t)a.ys + p.col) * 4u),
+                                                  64 * ct, 0);
+        }
+    }
+    if (bad) kq_flag(status, KQ_DEV_NUMERIC);
+}
+
+/* Whether a call without the delta correction is split over the chunks: if the
+ * scan's workgroups, those of 128 rows of S counted twice, are 64 at most.
+ * The scan and the three launches (4099 rows): 32 of 64 rows 99 and 44 us, 48
+ * of 64 (three sequences) 42 and 26; 64 of 128 125 and 112; 192 of 128 148
+ * and 268. */
+bool over_chunks(const kq_launch_linattn &a, uint32_t count) {
+    return a.beta == nullptr &&
+           (uint64_t)a.value_heads * (a.value_width / kTile) * (a.key_width / 64u) * count <= 64u;
+}
+
 uint64_t up256(uint64_t n) { return (n + 255u) & ~(uint64_t)255u; }
 
 /* chunks that sequences of more than max_rows rows can have at most */
@@ -1082,10 +1331,11 @@ Work carve(const kq_launch_linattn &a, uint64_t tokens, uint32_t count, uint32_t
     w.value_at = w.key_bytes * a.key_heads;
     const uint32_t least = kMat + kRowF * 4u;
     const uint32_t solved = least + 256u * a.key_width + kMat;
-    w.value_bytes = delta ? solved : least;
+    const uint32_t states = least + 4u * a.key_width * a.value_width;
+    w.value_bytes = delta ? solved : over_chunks(a, count) ? states : least;
     w.chunk_bytes = w.value_at + (uint64_t)w.value_bytes * a.value_heads;
-    /* room for the delta form, which the sizes alone do not tell */
-    const uint64_t most = w.value_at + (uint64_t)solved * a.value_heads;
+    /* room for any form: the sizes alone do not tell which */
+    const uint64_t most = w.value_at + (uint64_t)(solved > states ? solved : states) * a.value_heads;
     const uint64_t fit = kWindowBytes / most < 8u ? 8u : kWindowBytes / most;
     /* whole rounds of linattn_prep's workgroups, two on each of 256 CUs */
     const uint64_t round = a.key_heads < 512u ? 512u / a.key_heads : 1u;
@@ -1104,6 +1354,22 @@ hipError_t run(const kq_launch_linattn &a, const kq_launch_seqs &q, const Work &
                            dim3(w.window, a.key_heads), dim3(256), 0, s, a, w, base, status);
         hipError_t e = hipGetLastError();
         if (e != hipSuccess) return e;
+        if constexpr (!DELTA) {
+            if (over_chunks(a, q.count)) {
+                const dim3 grid(a.value_heads * (a.value_width / kTile), w.window);
+                hipLaunchKernelGGL(HIP_KERNEL_NAME(linattn_sums<DK>), grid, dim3(256), 0, s, a, q,
+                                   w, base, status);
+                hipLaunchKernelGGL(linattn_states,
+                                   dim3(a.value_heads * a.key_width * a.value_width / 1024u,
+                                        w.window),
+                                   dim3(256), 0, s, a, q, w, base, status);
+                hipLaunchKernelGGL(HIP_KERNEL_NAME(linattn_outs<DK>), grid, dim3(256), 0, s, a, q,
+                                   w, base, status);
+                e = hipGetLastError();
+                if (e != hipSuccess) return e;
+                continue;
+            }
+        }
         hipLaunchKernelGGL(HIP_KERNEL_NAME(linattn_scan<DK, DELTA>),
                            dim3(a.value_heads * (a.value_width / kTile), w.window),
                                dim3(64 * scan_waves(DELTA)), 0, s, a, q, w, base, status);

@@ -274,6 +274,41 @@ def test_attention_rounds(ctx, lengths, delta):
         check(a, a.got(ctx, off, slots, fresh, n), spans, slots, fresh)
 
 
+# without the delta correction and with few heads: chunks side by side
+@pytest.mark.parametrize("heads", [(1, 1, 64, 64), (1, 2, 128, 64), (2, 4, 64, 128),
+                                   (1, 3, 128, 128)], ids=str)
+@pytest.mark.parametrize("lengths", [[17], [64], [900], [70, 0, 200]], ids=str)
+def test_attention_chunks_at_once(ctx, heads, lengths):
+    say("chunks at once", heads, lengths)
+    off, spans, rows = table(lengths, lead=2, gap=1)
+    n = len(lengths)
+    a = Attention(n, *heads, rows, n + 1, delta=False, alpha=n != 1, pad=8)
+    slots = [n - i for i in range(n)]
+    fresh = [i % 2 for i in range(n)]
+    check(a, a.got(ctx, off, slots, fresh, n, pad=4), spans, slots, fresh)
+    check(a, a.got(ctx, off, slots, None, n, in_place=True), spans, slots, [0] * n, in_place=True)
+
+
+def test_attention_chunks_at_once_rounds(ctx):
+    # more chunks than a round of the work has (236), the state carried on
+    say("chunks at once, rounds")
+    off, spans, rows = table([15200, 33])
+    a = Attention(3, 1, 16, 64, 64, rows, 2, delta=False)
+    check(a, a.got(ctx, off, None, [1, 0], 2), spans, [0, 1], [1, 0])
+
+
+@pytest.mark.parametrize("where", ["q", "v", "state"])
+def test_attention_chunks_at_once_non_finite(ctx, where):
+    say("chunks at once, non-finite", where)
+    off, _, _ = table([200])
+    a = Attention(9, 1, 2, 64, 64, 200, 1, delta=False)
+    if where == "state":
+        a.state[0, 1, 5, 7] = np.nan
+    else:
+        a.qkv[150, 3 if where == "q" else 130] = np.inf
+    assert failing(ctx, a, off, None, None, 1) == "NUMERIC_DOMAIN"
+
+
 def test_attention_split_prompt_is_one(ctx):
     # a prompt in two calls, its state carried on, against the prompt in one
     say("split prompt")
