@@ -460,8 +460,9 @@ def expert_member_span(type_id, rows, cols, experts, expert_id) -> tuple[int, in
 
 
 def _ptr(x):
-    """The device address of a DeviceBuffer or of an int; None stays None."""
-    return C.c_void_p(x.ptr if hasattr(x, "ptr") else x)
+    """The device address of a DeviceBuffer; an int and None stay, which ctypes
+    takes as addresses (an object for each costs a call more than its checks)."""
+    return x if x is None or type(x) is int else x.ptr if hasattr(x, "ptr") else x
 
 
 def sequences(tokens: int, count: int, slot_count: int, offsets=None, slots=None,
