@@ -37,6 +37,13 @@
  * two to below 1 and its norm becomes a factor of the row; T, W, V, E and S
  * carry powers of two. Log decays are summed in 64 bits, since their
  * differences are what counts.
+ *
+ * 16,384 rows of one sequence, 16 key and 48 value heads of 128 x 128: 860 us,
+ * 105 TFLOP/s of the recurrent form's operations, which takes 33.4 ms for them. 690 us are the scan's, whose 256 steps
+ * hang on each other: 2.7 us a step, two LDS round trips through a barrier with
+ * 24 matrix instructions a wave behind each. 265 are linattn_prep's, bound by
+ * the bytes it writes. (Launches overlap; U = B V formed there as well made
+ * its writes, not the scan, the bound.) 513 rows: 47 us.
  */
 #include <type_traits>
 
@@ -1335,7 +1342,8 @@ Work carve(const kq_launch_linattn &a, uint64_t tokens, uint32_t count, uint32_t
     w.value_bytes = delta ? solved : over_chunks(a, count) ? states : least;
     w.chunk_bytes = w.value_at + (uint64_t)w.value_bytes * a.value_heads;
     /* room for any form: the sizes alone do not tell which */
-    const uint64_t most = w.value_at + (uint64_t)(solved > states ? solved : states) * a.value_heads;
+    const uint64_t most =
+        w.value_at + (uint64_t)(solved > states ? solved : states) * a.value_heads;
     const uint64_t fit = kWindowBytes / most < 8u ? 8u : kWindowBytes / most;
     /* whole rounds of linattn_prep's workgroups, two on each of 256 CUs */
     const uint64_t round = a.key_heads < 512u ? 512u / a.key_heads : 1u;

@@ -6,7 +6,13 @@
  *
  * Both kernels hold a row in registers between its sum of squares and its
  * scaling, so that memory is read once and written once; a few operations a
- * value leave them bound by memory (or, for few rows, by the launch).
+ * value leave them bound by memory (or, for few rows, by the launch). Groups
+ * of up to 256 values share a workgroup: 4099 rows of 48 heads of 128 with a
+ * SiLU gate take 55 us, 5.5 TB/s (a large copy: 5.1). 2499 tokens of 4
+ * branches of 2560, gated and with both norms, take 83.5 us: 4.3 TB/s, of
+ * which 4 bytes in 7 are written (two branches a workgroup 89 us, the next
+ * branch's loads during the norm before it 84.5, a thread for 4 x 4 values in
+ * place of 2 x 4 at this width 87.4).
  */
 #include "kq_device.h"
 #include "kq_launch.h"
