@@ -39,11 +39,19 @@ __device__ __forceinline__ Decay decay_of(float g) {
 
 }  // namespace kq
 
-/* the chunks of the sequences that the chunked form runs, in device memory */
+/* A chunk of a sequence that the chunked form runs: all that a workgroup has
+ * to know before its first loads, which a record of its own for the sequence
+ * would have wait for one more. */
+struct alignas(32) kq_linattn_chunk {
+    uint32_t row, rows;    /* its first, their number (0: no chunk) */
+    uint32_t number, left; /* which of its sequence; chunks from it to the last */
+    uint32_t slot, fresh;  /* the sequence's */
+    uint32_t ahead;        /* rows from its first to the sequence's end */
+    uint32_t none;
+};
 struct kq_linattn_plan {
-    uint32_t *total; /* their number; NULL for no plan */
-    uint2 *seq;      /* of each sequence: its first chunk and their number */
-    uint4 *chunk;    /* first row, rows, sequence, number in it */
+    kq_linattn_chunk *chunk; /* in device memory; NULL for no plan */
+    uint32_t chunks;         /* what the sizes of a call allow */
 };
 constexpr uint32_t kChunkRows = 64;
 

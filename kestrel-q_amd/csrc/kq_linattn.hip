@@ -68,7 +68,8 @@ __device__ __forceinline__ float inverse_norm(const float (&x)[R], float eps) {
 template <int NT>
 __device__ __forceinline__ void cut(const kq_launch_seqs &q, uint32_t max_rows,
                                     const kq_linattn_plan &w) {
-    __shared__ uint32_t first[NT], number[NT], begin[NT], rows[NT], sums[NT / 64];
+    __shared__ uint32_t first[NT], number[NT], begin[NT], rows[NT], slot[NT],
+        fresh[NT], sums[NT / 64];
     __shared__ uint32_t refused;
     const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6;
     if (tid == 0u) refused = 0u;
@@ -78,6 +79,9 @@ __device__ __forceinline__ void cut(const kq_launch_seqs &q, uint32_t max_rows,
     if (bad) refused = 1u; /* each sequence's own workgroups report it */
     __syncthreads();
     const bool none = refused != 0u;
+    /* the longest first, so that their scans, a workgroup after the other where
+     * there are more than the device holds, do not end last */
+    const bool sorted = q.count <= (uint32_t)NT;
     uint32_t at = 0u;
     for (uint32_t base = 0u; base < q.count; base += NT) {
         const uint32_t s = base + tid;
@@ -86,6 +90,8 @@ __device__ __forceinline__ void cut(const kq_launch_seqs &q, uint32_t max_rows,
             const kq::SeqSpan sp = kq::seq_span(q, s, bad);
             begin[tid] = sp.begin;
             rows[tid] = sp.rows;
+            slot[tid] = sp.slot;
+            fresh[tid] = sp.fresh;
             if (!none && sp.live && sp.rows > max_rows)
                 n = (sp.rows + kChunkRows - 1u) / kChunkRows;
         }
@@ -104,19 +110,26 @@ __device__ __forceinline__ void cut(const kq_launch_seqs &q, uint32_t max_rows,
         }
         first[tid] = before + x - n;
         number[tid] = n;
-        if (s < q.count) w.seq[s] = make_uint2(before + x - n, n);
+        if (sorted) {
+            __syncthreads();
+            uint32_t longer = 0u;
+            for (uint32_t j = 0; j < q.count; ++j)
+                longer += number[j] > n || (number[j] == n && j < tid) ? number[j] : 0u;
+            first[tid] = longer;
+        }
         __syncthreads();
         for (uint32_t i = wave; i < NT && base + i < q.count; i += NT / 64u)
-            for (uint32_t k = lane; k < number[i]; k += 64u) {
-                const uint32_t left = rows[i] - k * kChunkRows;
+            for (uint32_t k = lane; k < number[i] && first[i] + k < w.chunks; k += 64u) {
+                const uint32_t ahead = rows[i] - k * kChunkRows;
                 w.chunk[first[i] + k] =
-                    make_uint4(begin[i] + k * kChunkRows, left < kChunkRows ? left : kChunkRows,
-                               base + i, k);
+                    kq_linattn_chunk{begin[i] + k * kChunkRows,
+                                     ahead < kChunkRows ? ahead : kChunkRows,
+                                     k, number[i] - k, slot[i], fresh[i], ahead, 0u};
             }
         at = all;
         __syncthreads();
     }
-    if (tid == 0u) *w.total = at;
+    for (uint32_t i = at + tid; i < w.chunks; i += NT) w.chunk[i] = kq_linattn_chunk{};
 }
 
 /* grid (waves of columns of all heads / waves a workgroup, sequences): the
@@ -246,7 +259,7 @@ template <int DK>
 hipError_t launch(const kq_launch_linattn &a, const kq_launch_seqs &q, uint32_t max_rows,
                   const kq_linattn_plan &plan, uint32_t *status, hipStream_t s) {
     const uint64_t tiles = (uint64_t)a.value_heads * a.value_width / 32u * q.count;
-    if (plan.total != nullptr) return launch<DK, 8, 256, true>(a, q, max_rows, plan, status, s);
+    if (plan.chunk != nullptr) return launch<DK, 8, 256, true>(a, q, max_rows, plan, status, s);
     return tiles <= 256u ? launch<DK, 4, 64, false>(a, q, max_rows, plan, status, s)
                          : launch<DK, 8, 256, false>(a, q, max_rows, plan, status, s);
 }

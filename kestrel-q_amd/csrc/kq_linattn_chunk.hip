@@ -77,6 +77,11 @@ struct Work {
     uint32_t key_bytes, value_at, value_bytes;
 };
 
+/* chunk c of the call; one without rows behind the last */
+__device__ __forceinline__ kq_linattn_chunk chunk_at(const Work &w, uint32_t c) {
+    return c < w.plan.chunks ? w.plan.chunk[c] : kq_linattn_chunk{};
+}
+
 __device__ __forceinline__ f4 mfma(h8 a, h8 b, f4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
@@ -229,8 +234,8 @@ __global__ __launch_bounds__(256, 2) void linattn_prep(kq_launch_linattn a, Work
     __shared__ float bet[kHeads][kC], nks[kC], nqs[kC];
     __shared__ int pw[kHeads], pu[kHeads];
     const uint32_t c = base + blockIdx.x, kh = blockIdx.y;
-    if (c >= *w.plan.total) return;
-    const uint4 ch = w.plan.chunk[c];
+    const kq_linattn_chunk ch = chunk_at(w, c);
+    if (ch.rows == 0u) return;
     const uint32_t lane = threadIdx.x & 63u, r16 = lane & 15u, g4 = lane >> 4;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t per = a.value_heads / a.key_heads;
@@ -243,7 +248,7 @@ __global__ __launch_bounds__(256, 2) void linattn_prep(kq_launch_linattn a, Work
     float g_rate = 0.0f, g_bias = 0.0f, g_alpha = 0.0f, g_beta = 0.0f, g_b = 0.0f;
     double g_sum = 0.0, g_end = 0.0;
     auto load_gates = [&](uint32_t h) {
-        const uint64_t t = (uint64_t)ch.x + (lane < ch.y ? lane : 0u);
+        const uint64_t t = (uint64_t)ch.row + (lane < ch.rows ? lane : 0u);
         g_rate = a.rate[h];
         if (a.bias != nullptr) g_bias = a.bias[h];
         if (a.alpha != nullptr) g_alpha = a.alpha[t * a.as + h];
@@ -254,8 +259,8 @@ __global__ __launch_bounds__(256, 2) void linattn_prep(kq_launch_linattn a, Work
                  !kq_isfinite(g_alpha) || !kq_isfinite(g_beta);
         float g = g_rate;
         if (a.alpha != nullptr) g *= kq::softplus(g_alpha + g_bias);
-        g = lane < ch.y ? fmaxf(g, -1.0e30f) : 0.0f;
-        if (DELTA) g_b = lane < ch.y ? kq::sigmoid(g_beta) : 0.0f;
+        g = lane < ch.rows ? fmaxf(g, -1.0e30f) : 0.0f;
+        if (DELTA) g_b = lane < ch.rows ? kq::sigmoid(g_beta) : 0.0f;
         g_sum = kq_wave_scan_f64((double)g);
         g_end = kq_readlane_f64(g_sum, 63);
     };
@@ -271,8 +276,8 @@ __global__ __launch_bounds__(256, 2) void linattn_prep(kq_launch_linattn a, Work
         for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
             for (int e = 0; e < 8; ++e) x[ks][e] = y[ks][e] = 0.0f;
-        if (i < ch.y) {
-            const uint64_t t = (uint64_t)ch.x + i;
+        if (i < ch.rows) {
+            const uint64_t t = (uint64_t)ch.row + i;
             const float4 *kp = (const float4 *)(a.k + t * a.ks + kh * DK + 4u * g4);
             const float4 *qp = (const float4 *)(a.q + t * a.qs + kh * DK + 4u * g4);
 #pragma unroll
@@ -598,8 +603,7 @@ constexpr int scan_waves(bool delta) { return delta ? 12 : 8; }
 
 template <int DK, bool DELTA>
 __global__ __launch_bounds__(64 * scan_waves(DELTA)) void linattn_scan(kq_launch_linattn a,
-                                                                kq_launch_seqs q, Work w,
-                                                                uint32_t base,
+                                                                Work w, uint32_t base,
                                                                 uint32_t *status) {
     constexpr int KS = DK / 32, NR = DK / 64; /* steps over S's rows; row tiles of a solver */
     constexpr uint32_t kKeyImage = 256u * DK;
@@ -611,18 +615,14 @@ __global__ __launch_bounds__(64 * scan_waves(DELTA)) void linattn_scan(kq_launch
     __shared__ float vscale[2][kTile]; /* of V's columns, by 32 rows */
     /* the chunks of one sequence that lie in the window: from the window's
      * first chunk, or the sequence's */
-    if (base + blockIdx.y >= *w.plan.total) return;
-    const uint4 ch = w.plan.chunk[base + blockIdx.y];
-    if (blockIdx.y != 0u && ch.w != 0u) return;
-    const uint2 mine = w.plan.seq[ch.z];
-    const uint32_t left_here = w.window - blockIdx.y, left_seq = mine.y - ch.w;
-    const uint32_t last = (left_here < left_seq ? left_here : left_seq) - 1u;
-    bool badseq = false, bad = false, badin = false;
-    const kq::SeqSpan sp = kq::seq_span(q, ch.z, badseq);
-    if (!sp.live) return;
-    const uint32_t row0 = ch.w * kC, rows = sp.rows - row0; /* from the first chunk on */
-    const float *state = ch.w == 0u ? a.state : a.state_out; /* as the last window left it */
-    const bool fresh = sp.fresh && ch.w == 0u;
+    const kq_linattn_chunk ch = chunk_at(w, base + blockIdx.y);
+    if (ch.rows == 0u || (blockIdx.y != 0u && ch.number != 0u)) return;
+    const uint32_t left_here = w.window - blockIdx.y;
+    const uint32_t last = (left_here < ch.left ? left_here : ch.left) - 1u;
+    bool bad = false, badin = false;
+    const uint32_t rows = ch.ahead; /* from the first chunk on */
+    const float *state = ch.number == 0u ? a.state : a.state_out; /* as the last window left it */
+    const bool fresh = ch.fresh != 0u && ch.number == 0u;
     const uint32_t lane = threadIdx.x & 63u, r16 = lane & 15u, g4 = lane >> 4, lane16 = lane * 16u;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t rt = wave & 3u, fr = 16u * rt + 4u * g4; /* rows of the chunk */
@@ -659,7 +659,7 @@ __global__ __launch_bounds__(64 * scan_waves(DELTA)) void linattn_scan(kq_launch
     /* rows of v or of the output of chunk n, the call's column tile */
     auto rows_at = [&](const float *p, uint64_t stride, uint32_t n) {
         const uint32_t left = rows - n * kC; /* rows past it are past the buffer */
-        return kq_buf(p + ((uint64_t)sp.begin + row0 + n * kC) * stride + h * a.value_width,
+        return kq_buf(p + ((uint64_t)ch.row + n * kC) * stride + h * a.value_width,
                       (left < kC ? left : kC) * (uint32_t)stride * 4u);
     };
     Scale ss, se, sf;
@@ -668,7 +668,7 @@ __global__ __launch_bounds__(64 * scan_waves(DELTA)) void linattn_scan(kq_launch
     if (wave < 4u) {
         __builtin_amdgcn_s_setprio(3); /* the chain first */
         const uint32_t srow = 16u * NR * rt + 4u * g4;
-        const size_t sat = (((size_t)sp.slot * a.value_heads + h) * DK + srow) * a.value_width + col;
+        const size_t sat = (((size_t)ch.slot * a.value_heads + h) * DK + srow) * a.value_width + col;
         f4 S[NR][2];
 #pragma unroll
         for (int t = 0; t < NR; ++t)
@@ -1079,21 +1079,14 @@ __global__ __launch_bounds__(64 * scan_waves(DELTA)) void linattn_scan(kq_launch
 /* a workgroup's chunk, value head and 32 columns; four waves with 16 rows of
  * the chunk each */
 struct Place {
-    uint4 ch;
-    uint32_t slot, h, col, fr;
+    kq_linattn_chunk ch;
+    uint32_t h, col, fr;
     char *data;
     uint32_t kat, vat, fat, uat; /* Q, M, the factors, U */
-    bool live;
     KqBuf buf;
-    __device__ __forceinline__ Place(const kq_launch_linattn &a, const kq_launch_seqs &q,
-                                     const Work &w, uint32_t base, uint32_t wave, uint32_t lane) {
-        live = base + blockIdx.y < *w.plan.total;
-        if (!live) return;
-        ch = w.plan.chunk[base + blockIdx.y];
-        bool bad = false;
-        const kq::SeqSpan sp = kq::seq_span(q, ch.z, bad);
-        live = sp.live;
-        slot = sp.slot;
+    __device__ __forceinline__ Place(const kq_launch_linattn &a, const Work &w, uint32_t base,
+                                     uint32_t wave, uint32_t lane) {
+        ch = chunk_at(w, base + blockIdx.y);
         uint32_t b = blockIdx.x; /* a head's to one XCD, as in the scan */
         if (gridDim.x % 8u == 0u) b = (b % 8u) * (gridDim.x / 8u) + b / 8u;
         const uint32_t tiles = a.value_width / kTile;
@@ -1112,7 +1105,7 @@ struct Place {
     }
     /* the chunk's rows of v or of the output; rows past it are past the buffer */
     __device__ __forceinline__ KqBuf rows(const float *p, uint64_t stride, uint32_t width) const {
-        return kq_buf(p + (uint64_t)ch.x * stride + h * width, ch.y * (uint32_t)stride * 4u);
+        return kq_buf(p + (uint64_t)ch.row * stride + h * width, ch.rows * (uint32_t)stride * 4u);
     }
     __device__ __forceinline__ void load_v(const kq_launch_linattn &a, f4 (&V)[2]) const {
         const KqBuf v = rows(a.v, a.vs, a.value_width);
@@ -1126,15 +1119,15 @@ struct Place {
 };
 
 template <int DK>
-__global__ __launch_bounds__(256) void linattn_sums(kq_launch_linattn a, kq_launch_seqs q, Work w,
+__global__ __launch_bounds__(256) void linattn_sums(kq_launch_linattn a, Work w,
                                                     uint32_t base, uint32_t *status) {
     constexpr int NR = DK / 64;
     __shared__ __attribute__((aligned(16))) char fbuf[8192];
     __shared__ __attribute__((aligned(16))) float top[4];
     const uint32_t lane = threadIdx.x & 63u, lane16 = lane * 16u;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const Place p(a, q, w, base, wave, lane);
-    if (!p.live) return;
+    const Place p(a, w, base, wave, lane);
+    if (p.ch.rows == 0u) return;
     f4 V[2];
     p.load_v(a, V);
     const f4 f0 = p.factors(0u), f1 = p.factors(1u);
@@ -1181,24 +1174,21 @@ __global__ __launch_bounds__(256) void linattn_sums(kq_launch_linattn a, kq_laun
 
 /* grid (1024 values of the states, window): the first chunk of a sequence in
  * the window goes on to its last there */
-__global__ __launch_bounds__(256) void linattn_states(kq_launch_linattn a, kq_launch_seqs q,
-                                                      Work w, uint32_t base, uint32_t *status) {
+__global__ __launch_bounds__(256) void linattn_states(kq_launch_linattn a, Work w,
+                                                      uint32_t base, uint32_t *status) {
     constexpr uint32_t kAhead = 8;
-    if (base + blockIdx.y >= *w.plan.total) return;
-    const uint4 ch = w.plan.chunk[base + blockIdx.y];
-    if (blockIdx.y != 0u && ch.w != 0u) return;
+    const kq_linattn_chunk ch = chunk_at(w, base + blockIdx.y);
+    if (ch.rows == 0u || (blockIdx.y != 0u && ch.number != 0u)) return;
     bool bad = false;
-    const kq::SeqSpan sp = kq::seq_span(q, ch.z, bad);
-    if (!sp.live) return;
-    const uint32_t left_here = w.window - blockIdx.y, left_seq = w.plan.seq[ch.z].y - ch.w;
-    const uint32_t n = left_here < left_seq ? left_here : left_seq;
+    const uint32_t left_here = w.window - blockIdx.y;
+    const uint32_t n = left_here < ch.left ? left_here : ch.left;
     const uint32_t size = a.key_width * a.value_width; /* a multiple of 1024 */
     const uint32_t at = blockIdx.x * 1024u, h = at / size, i = at % size + 4u * threadIdx.x;
-    const size_t sat = ((size_t)sp.slot * a.value_heads + h) * size + i;
+    const size_t sat = ((size_t)ch.slot * a.value_heads + h) * size + i;
     f4 S = f4{0.0f, 0.0f, 0.0f, 0.0f};
-    if (ch.w != 0u)
+    if (ch.number != 0u)
         S = *(const f4 *)(a.state_out + sat);
-    else if (!sp.fresh)
+    else if (ch.fresh == 0u)
         S = *(const f4 *)(a.state + sat);
     char *f = w.data + (uint64_t)blockIdx.y * w.chunk_bytes + w.value_at + h * w.value_bytes + kMat;
     for (uint32_t c = 0; c < n; c += kAhead) {
@@ -1225,15 +1215,15 @@ __global__ __launch_bounds__(256) void linattn_states(kq_launch_linattn a, kq_la
 }
 
 template <int DK>
-__global__ __launch_bounds__(256) void linattn_outs(kq_launch_linattn a, kq_launch_seqs q, Work w,
+__global__ __launch_bounds__(256) void linattn_outs(kq_launch_linattn a, Work w,
                                                     uint32_t base, uint32_t *status) {
     constexpr int KS = DK / 32, NR = DK / 64;
     __shared__ __attribute__((aligned(16))) char sbuf[KS * 4096], ebuf[8192];
     __shared__ __attribute__((aligned(16))) float top_s[4], top_e[4];
     const uint32_t lane = threadIdx.x & 63u, lane16 = lane * 16u;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const Place p(a, q, w, base, wave, lane);
-    if (!p.live) return;
+    const Place p(a, w, base, wave, lane);
+    if (p.ch.rows == 0u) return;
     f4 S[NR][2], V[2];
     const float *s = (const float *)(p.data + p.uat) +
                      (16u * NR * wave + 4u * (lane >> 4)) * a.value_width + p.col;
@@ -1330,10 +1320,9 @@ Work carve(const kq_launch_linattn &a, uint64_t tokens, uint32_t count, uint32_t
     const uint64_t n = most_chunks(tokens, count, max_rows);
     const bool delta = a.beta != nullptr;
     char *p = (char *)(((uintptr_t)scratch + 255u) & ~(uintptr_t)255u);
-    w.plan.total = (uint32_t *)p;
-    w.plan.seq = (uint2 *)(p + 256u);
-    w.plan.chunk = (uint4 *)((char *)w.plan.seq + up256(8u * (uint64_t)count));
-    w.data = (char *)w.plan.chunk + up256(16u * n);
+    w.plan.chunk = (kq_linattn_chunk *)p;
+    w.plan.chunks = (uint32_t)n;
+    w.data = p + up256(sizeof(kq_linattn_chunk) * n);
     w.key_bytes = 512u * a.key_width;
     w.value_at = w.key_bytes * a.key_heads;
     const uint32_t least = kMat + kRowF * 4u;
@@ -1349,29 +1338,28 @@ Work carve(const kq_launch_linattn &a, uint64_t tokens, uint32_t count, uint32_t
     const uint64_t round = a.key_heads < 512u ? 512u / a.key_heads : 1u;
     const uint64_t whole = fit > round ? fit / round * round : fit;
     w.window = (uint32_t)(whole < n ? whole : n);
-    *bytes = 512u + up256(8u * (uint64_t)count) + up256(16u * n) +
-             w.window * most;
+    *bytes = 256u + up256(sizeof(kq_linattn_chunk) * n) + w.window * most;
     return w;
 }
 
 template <int DK, bool DELTA>
-hipError_t run(const kq_launch_linattn &a, const kq_launch_seqs &q, const Work &w, uint32_t chunks,
-               uint32_t *status, hipStream_t s) {
-    for (uint32_t base = 0u; base < chunks; base += w.window) {
+hipError_t run(const kq_launch_linattn &a, uint32_t count, const Work &w, uint32_t *status,
+               hipStream_t s) {
+    for (uint32_t base = 0u; base < w.plan.chunks; base += w.window) {
         hipLaunchKernelGGL(HIP_KERNEL_NAME(linattn_prep<DK, DELTA>),
                            dim3(w.window, a.key_heads), dim3(256), 0, s, a, w, base, status);
         hipError_t e = hipGetLastError();
         if (e != hipSuccess) return e;
         if constexpr (!DELTA) {
-            if (over_chunks(a, q.count)) {
+            if (over_chunks(a, count)) {
                 const dim3 grid(a.value_heads * (a.value_width / kTile), w.window);
-                hipLaunchKernelGGL(HIP_KERNEL_NAME(linattn_sums<DK>), grid, dim3(256), 0, s, a, q,
+                hipLaunchKernelGGL(HIP_KERNEL_NAME(linattn_sums<DK>), grid, dim3(256), 0, s, a,
                                    w, base, status);
                 hipLaunchKernelGGL(linattn_states,
                                    dim3(a.value_heads * a.key_width * a.value_width / 1024u,
                                         w.window),
-                                   dim3(256), 0, s, a, q, w, base, status);
-                hipLaunchKernelGGL(HIP_KERNEL_NAME(linattn_outs<DK>), grid, dim3(256), 0, s, a, q,
+                                   dim3(256), 0, s, a, w, base, status);
+                hipLaunchKernelGGL(HIP_KERNEL_NAME(linattn_outs<DK>), grid, dim3(256), 0, s, a,
                                    w, base, status);
                 e = hipGetLastError();
                 if (e != hipSuccess) return e;
@@ -1380,7 +1368,7 @@ hipError_t run(const kq_launch_linattn &a, const kq_launch_seqs &q, const Work &
         }
         hipLaunchKernelGGL(HIP_KERNEL_NAME(linattn_scan<DK, DELTA>),
                            dim3(a.value_heads * (a.value_width / kTile), w.window),
-                               dim3(64 * scan_waves(DELTA)), 0, s, a, q, w, base, status);
+                               dim3(64 * scan_waves(DELTA)), 0, s, a, w, base, status);
         e = hipGetLastError();
         if (e != hipSuccess) return e;
     }
@@ -1400,13 +1388,12 @@ hipError_t kq_linattn_chunked(const kq_launch_linattn &a, const kq_launch_seqs &
                               uint32_t max_rows, void *scratch, uint32_t *status, hipStream_t s) {
     uint64_t bytes;
     const Work w = carve(a, q.tokens, q.count, max_rows, scratch, &bytes);
-    const uint32_t chunks = (uint32_t)most_chunks(q.tokens, q.count, max_rows);
     const hipError_t e = kq_linattn_recurrent(a, q, max_rows, w.plan, status, s);
     if (e != hipSuccess) return e;
     const bool delta = a.beta != nullptr;
     if (a.key_width == 128u)
-        return delta ? run<128, true>(a, q, w, chunks, status, s)
-                     : run<128, false>(a, q, w, chunks, status, s);
-    return delta ? run<64, true>(a, q, w, chunks, status, s)
-                 : run<64, false>(a, q, w, chunks, status, s);
+        return delta ? run<128, true>(a, q.count, w, status, s)
+                     : run<128, false>(a, q.count, w, status, s);
+    return delta ? run<64, true>(a, q.count, w, status, s)
+                 : run<64, false>(a, q.count, w, status, s);
 }
