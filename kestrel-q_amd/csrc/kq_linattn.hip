@@ -68,8 +68,7 @@ __device__ __forceinline__ float inverse_norm(const float (&x)[R], float eps) {
 template <int NT>
 __device__ __forceinline__ void cut(const kq_launch_seqs &q, uint32_t max_rows,
                                     const kq_linattn_plan &w) {
-    __shared__ uint32_t first[NT], number[NT], begin[NT], rows[NT], slot[NT],
-        fresh[NT], sums[NT / 64];
+    __shared__ uint32_t number[NT], sums[NT / 64];
     __shared__ uint32_t refused;
     const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6;
     if (tid == 0u) refused = 0u;
@@ -86,12 +85,9 @@ __device__ __forceinline__ void cut(const kq_launch_seqs &q, uint32_t max_rows,
     for (uint32_t base = 0u; base < q.count; base += NT) {
         const uint32_t s = base + tid;
         uint32_t n = 0u;
+        kq::SeqSpan sp = {};
         if (s < q.count) {
-            const kq::SeqSpan sp = kq::seq_span(q, s, bad);
-            begin[tid] = sp.begin;
-            rows[tid] = sp.rows;
-            slot[tid] = sp.slot;
-            fresh[tid] = sp.fresh;
+            sp = kq::seq_span(q, s, bad);
             if (!none && sp.live && sp.rows > max_rows)
                 n = (sp.rows + kChunkRows - 1u) / kChunkRows;
         }
@@ -102,30 +98,31 @@ __device__ __forceinline__ void cut(const kq_launch_seqs &q, uint32_t max_rows,
             if (lane >= (uint32_t)o) x += y;
         }
         if (lane == 63u) sums[wave] = x;
+        number[tid] = n;
         __syncthreads();
-        uint32_t before = at, all = at;
+        uint32_t first = at + x - n, all = at;
         for (uint32_t k = 0; k < NT / 64u; ++k) {
-            if (k < wave) before += sums[k];
+            if (k < wave) first += sums[k];
             all += sums[k];
         }
-        first[tid] = before + x - n;
-        number[tid] = n;
         if (sorted) {
-            __syncthreads();
-            uint32_t longer = 0u;
+            first = 0u;
             for (uint32_t j = 0; j < q.count; ++j)
-                longer += number[j] > n || (number[j] == n && j < tid) ? number[j] : 0u;
-            first[tid] = longer;
+                first += number[j] > n || (number[j] == n && j < tid) ? number[j] : 0u;
         }
-        __syncthreads();
-        for (uint32_t i = wave; i < NT && base + i < q.count; i += NT / 64u)
-            for (uint32_t k = lane; k < number[i] && first[i] + k < w.chunks; k += 64u) {
-                const uint32_t ahead = rows[i] - k * kChunkRows;
-                w.chunk[first[i] + k] =
-                    kq_linattn_chunk{begin[i] + k * kChunkRows,
-                                     ahead < kChunkRows ? ahead : kChunkRows,
-                                     k, number[i] - k, slot[i], fresh[i], ahead, 0u};
+        /* the wave's sequences one after the other, a lane for a chunk */
+        for (uint64_t todo = __ballot(n != 0u); todo != 0ull; todo &= todo - 1ull) {
+            const int i = __builtin_ctzll(todo);
+            auto of = [&](uint32_t v) { return (uint32_t)__builtin_amdgcn_readlane((int)v, i); };
+            const uint32_t to = of(first), chunks = of(n), begin = of(sp.begin), rows = of(sp.rows);
+            const uint32_t slot = of(sp.slot), fresh = of(sp.fresh ? 1u : 0u);
+            for (uint32_t k = lane; k < chunks && to + k < w.chunks; k += 64u) {
+                const uint32_t ahead = rows - k * kChunkRows;
+                w.chunk[to + k] = kq_linattn_chunk{begin + k * kChunkRows,
+                                                   ahead < kChunkRows ? ahead : kChunkRows,
+                                                   k, chunks - k, slot, fresh, ahead, 0u};
             }
+        }
         at = all;
         __syncthreads();
     }

@@ -309,6 +309,19 @@ def test_attention_chunks_at_once_non_finite(ctx, where):
     assert failing(ctx, a, off, None, None, 1) == "NUMERIC_DOMAIN"
 
 
+def test_attention_many_sequences(ctx):
+    # more than a workgroup looks at at a time, chunks among them here and there
+    say("many sequences")
+    lengths = [1, 0, 2, 1] * 160 + [70, 1, 17, 1] + [1] * 300 + [200, 18]
+    off, spans, rows = table(lengths, lead=1, gap=2)
+    n = len(lengths)
+    a = Attention(31, 1, 2, 64, 64, rows, n)
+    slots = np.random.default_rng(31).permutation(n).tolist()
+    slots[100] = slots[641] = NO
+    fresh = [i % 5 == 0 for i in range(n)]
+    check(a, a.got(ctx, off, slots, fresh, n), spans, slots, fresh)
+
+
 def test_attention_split_prompt_is_one(ctx):
     # a prompt in two calls, its state carried on, against the prompt in one
     say("split prompt")
@@ -752,6 +765,87 @@ def put(ctx, ptr, a):
     a = np.ascontiguousarray(a)
     kq_hip.check(kq_hip.lib().kq_hip_upload(ctx._h, C.c_void_p(ptr), a.ctypes.data, a.nbytes,
                                             C.byref(d)), d)
+
+
+class Far:
+    """Rows 4 MiB apart: from the 1024th on past 32-bit offsets."""
+    STRIDE = 1 << 20
+
+    def __init__(self, ctx, c, a):
+        self.ctx, self.a = ctx, a
+        b = ctx.alloc(((a.shape[0] - 1) * self.STRIDE + a.shape[1]) * 4)
+        c.bufs.append(b)
+        self.ptr = b.ptr
+        for t in range(a.shape[0]):
+            put(ctx, self.ptr + 4 * t * self.STRIDE, a[t])
+
+    def down(self):
+        return np.stack([self.ctx.download(self.ptr + 4 * t * self.STRIDE, self.a.dtype,
+                                           self.a.shape[1]) for t in range(self.a.shape[0])])
+
+
+def far_slots(ctx, c, slots, held):
+    """A pool in which the slots named lie far apart: its address, slot by slot upload."""
+    size = held[0].nbytes
+    b = ctx.alloc((max(slots) + 1) * size)
+    c.bufs.append(b)
+    for s, h in zip(slots, held):
+        put(ctx, b.ptr + s * size, h)
+    return b.ptr, size
+
+
+@pytest.mark.parametrize("delta", [True, False])
+def test_far_rows_and_slots(delta):
+    # rows and states past 4 GiB of their arrays
+    say("far", delta)
+    lengths = [1000, 90, 10]
+    off, spans, rows = table(lengths)
+    with kq_hip.Context(0) as ctx, Call(ctx) as c:
+        ctx.set_commit_on_success(False)
+        hk, hv, dk, dv = dims = (2, 4, 64, 64) if delta else (1, 2, 64, 64)
+        a = Attention(21, *dims, rows, 3, delta=delta)
+        slots = [(9 << 29) // (hv * dk * dv), 7, (9 << 28) // (hv * dk * dv)]
+        x, y = Far(ctx, c, a.qkv), Far(ctx, c, np.full((rows, hv * dv), SENTINEL))
+        pool, size = far_slots(ctx, c, slots, a.state)
+        la, _, _ = a.describe(c, off, None, None, 3)
+        seqs = kq_hip.sequences(rows, 3, max(slots) + 1, c.up(off),
+                                c.up(np.asarray(slots, np.uint32)),
+                                c.up(np.asarray([0, 1, 0], np.uint32)))
+        inp = kq_hip.linear_attention_inputs(
+            x.ptr, Far.STRIDE, x.ptr + 4 * hk * dk, Far.STRIDE, x.ptr + 8 * hk * dk, Far.STRIDE,
+            c.up(a.alpha), hv + 3, c.up(a.beta), hv)
+        n = kq_hip.linear_attention_scratch_bytes(la, seqs)
+        ctx.linear_attention(la, seqs, inp, pool, pool, y.ptr, Far.STRIDE, c.scratch(n), n)
+        got = np.stack([ctx.download(pool + s * size, np.float32, a.state[0].size)
+                        .reshape(a.state[0].shape) for s in slots])
+        heads = y.down()
+        check(a, (heads.reshape(rows, hv, dv), got), spans, [0, 1, 2], [0, 1, 0], in_place=True)
+        # and the norm over them, in place
+        w = Gen(22).normal(dv)
+        ctx.gated_norm(kq_hip.gated_norm(hv, dv, 1e-6, c.up(w)), rows, y.ptr, Far.STRIDE, None, 0,
+                       y.ptr, Far.STRIDE)
+        h = heads.reshape(rows, hv, dv).astype(np.float64)
+        want = h / np.sqrt((h * h).mean(2, keepdims=True) + 1e-6) * w
+        assert (np.abs(y.down().reshape(rows, hv, dv) - want) <= 16 * U * np.abs(want)).all()
+
+
+def test_far_conv():
+    say("far conv")
+    lengths = [1000, 2, 98]
+    off, spans, rows = table(lengths)
+    with kq_hip.Context(0) as ctx, Call(ctx) as c:
+        ctx.set_commit_on_success(False)
+        v = Conv(23, 256, 4, rows, 3)
+        slots = [(9 << 29) // (3 * 256), 5, (9 << 28) // (3 * 256)]
+        x, y = Far(ctx, c, v.x), Far(ctx, c, np.full((rows, 256), SENTINEL))
+        pool, size = far_slots(ctx, c, slots, v.state)
+        cv, _ = v.describe(c, off, None, None, 3)
+        seqs = kq_hip.sequences(rows, 3, max(slots) + 1, c.up(off),
+                                c.up(np.asarray(slots, np.uint32)), None)
+        ctx.causal_conv(cv, seqs, x.ptr, Far.STRIDE, pool, pool, y.ptr, Far.STRIDE)
+        got = np.stack([ctx.download(pool + s * size, np.float32, v.state[0].size)
+                        .reshape(v.state[0].shape) for s in slots])
+        v.check((y.down(), got), spans, [0, 1, 2], [0, 0, 0], in_place=True)
 
 
 def hip_lib():
