@@ -17,7 +17,8 @@
  *
  * Three launches:
  *   linattn_rows  the recurrent form over the short sequences, which also cuts
- *                 the others into chunks (on the device: the lengths are there)
+ *                 the others into chunks (on the device: the lengths are there;
+ *                 not for a call's only sequence)
  *   linattn_prep  a workgroup for each chunk and key head: Q, K'^T as operands
  *                 of the matrix cores, and for each of its value heads M, W, B
  *   linattn_scan  a workgroup for each sequence, head and 32 columns of v:
@@ -71,6 +72,7 @@ constexpr float kMixUnit = 0x1p6f; /* of M: |q.k| <= 512 of such rows (128 value
 /* where the parts of the scratch lie */
 struct Work {
     kq_linattn_plan plan;
+    kq_launch_seqs one; /* a call of one sequence, which needs no plan; else count 0 */
     char *data;       /* operands of the chunks of a window */
     uint32_t window;  /* chunks */
     uint64_t chunk_bytes;
@@ -79,7 +81,31 @@ struct Work {
 
 /* chunk c of the call; one without rows behind the last */
 __device__ __forceinline__ kq_linattn_chunk chunk_at(const Work &w, uint32_t c) {
-    return c < w.plan.chunks ? w.plan.chunk[c] : kq_linattn_chunk{};
+    if (w.one.count == 0u) return c < w.plan.chunks ? w.plan.chunk[c] : kq_linattn_chunk{};
+    bool bad = false;
+    const kq::SeqSpan sp = kq::seq_span(w.one, 0u, bad);
+    kq_linattn_chunk r = {};
+    if (sp.live && c * kC < sp.rows) {
+        r.row = sp.begin + c * kC;
+        r.ahead = sp.rows - c * kC;
+        r.rows = r.ahead < kC ? r.ahead : kC;
+        r.number = c;
+        r.left = (r.ahead + kC - 1u) / kC;
+        r.slot = sp.slot;
+        r.fresh = sp.fresh ? 1u : 0u;
+    }
+    return r;
+}
+
+/* Whether chunk c, which has no rows, is the first of a call's only sequence,
+ * without rows: its state is passed on. Says so if the sequence is refused. */
+__device__ __forceinline__ bool passes(const Work &w, uint32_t c, kq::SeqSpan &sp,
+                                       uint32_t *status) {
+    if (w.one.count == 0u || c != 0u) return false;
+    bool bad = false;
+    sp = kq::seq_span(w.one, 0u, bad);
+    if (bad) kq_flag(status, KQ_DEV_SEQUENCE);
+    return sp.live;
 }
 
 __device__ __forceinline__ f4 mfma(h8 a, h8 b, f4 c) {
@@ -616,7 +642,22 @@ __global__ __launch_bounds__(64 * scan_waves(DELTA)) void linattn_scan(kq_launch
     /* the chunks of one sequence that lie in the window: from the window's
      * first chunk, or the sequence's */
     const kq_linattn_chunk ch = chunk_at(w, base + blockIdx.y);
-    if (ch.rows == 0u || (blockIdx.y != 0u && ch.number != 0u)) return;
+    if (ch.rows == 0u) {
+        kq::SeqSpan sp;
+        if (passes(w, base + blockIdx.y, sp, status)) {
+            const uint32_t at = blockIdx.x * (DK * kTile); /* a part of the state each */
+            const size_t from = (size_t)sp.slot * a.value_heads * DK * a.value_width + at;
+            bool odd = false;
+            for (uint32_t i = threadIdx.x; i < DK * kTile; i += blockDim.x) {
+                const float x = sp.fresh ? 0.0f : a.state[from + i];
+                odd |= !kq_isfinite(x);
+                a.state_out[from + i] = x;
+            }
+            if (odd) kq_flag(status, KQ_DEV_NUMERIC);
+        }
+        return;
+    }
+    if (blockIdx.y != 0u && ch.number != 0u) return;
     const uint32_t left_here = w.window - blockIdx.y;
     const uint32_t last = (left_here < ch.left ? left_here : ch.left) - 1u;
     bool bad = false, badin = false;
@@ -1177,11 +1218,19 @@ __global__ __launch_bounds__(256) void linattn_sums(kq_launch_linattn a, Work w,
 __global__ __launch_bounds__(256) void linattn_states(kq_launch_linattn a, Work w,
                                                       uint32_t base, uint32_t *status) {
     constexpr uint32_t kAhead = 8;
-    const kq_linattn_chunk ch = chunk_at(w, base + blockIdx.y);
-    if (ch.rows == 0u || (blockIdx.y != 0u && ch.number != 0u)) return;
+    kq_linattn_chunk ch = chunk_at(w, base + blockIdx.y);
+    uint32_t n = 0u;
+    if (ch.rows == 0u) {
+        kq::SeqSpan sp;
+        if (!passes(w, base + blockIdx.y, sp, status)) return;
+        ch.slot = sp.slot;
+        ch.fresh = sp.fresh ? 1u : 0u;
+    } else {
+        if (blockIdx.y != 0u && ch.number != 0u) return;
+        const uint32_t left_here = w.window - blockIdx.y;
+        n = left_here < ch.left ? left_here : ch.left;
+    }
     bool bad = false;
-    const uint32_t left_here = w.window - blockIdx.y;
-    const uint32_t n = left_here < ch.left ? left_here : ch.left;
     const uint32_t size = a.key_width * a.value_width; /* a multiple of 1024 */
     const uint32_t at = blockIdx.x * 1024u, h = at / size, i = at % size + 4u * threadIdx.x;
     const size_t sat = ((size_t)ch.slot * a.value_heads + h) * size + i;
@@ -1316,7 +1365,7 @@ constexpr uint64_t kWindowBytes = 160u << 20;
 
 Work carve(const kq_launch_linattn &a, uint64_t tokens, uint32_t count, uint32_t max_rows,
            void *scratch, uint64_t *bytes) {
-    Work w;
+    Work w = {};
     const uint64_t n = most_chunks(tokens, count, max_rows);
     const bool delta = a.beta != nullptr;
     char *p = (char *)(((uintptr_t)scratch + 255u) & ~(uintptr_t)255u);
@@ -1387,9 +1436,13 @@ uint64_t kq_linattn_chunked_scratch(const kq_launch_linattn &a, uint64_t tokens,
 hipError_t kq_linattn_chunked(const kq_launch_linattn &a, const kq_launch_seqs &q,
                               uint32_t max_rows, void *scratch, uint32_t *status, hipStream_t s) {
     uint64_t bytes;
-    const Work w = carve(a, q.tokens, q.count, max_rows, scratch, &bytes);
-    const hipError_t e = kq_linattn_recurrent(a, q, max_rows, w.plan, status, s);
-    if (e != hipSuccess) return e;
+    Work w = carve(a, q.tokens, q.count, max_rows, scratch, &bytes);
+    if (q.count == 1u) { /* a prompt of its own: no launch for its plan, 4.5 us */
+        w.one = q;
+    } else {
+        const hipError_t e = kq_linattn_recurrent(a, q, max_rows, w.plan, status, s);
+        if (e != hipSuccess) return e;
+    }
     const bool delta = a.beta != nullptr;
     if (a.key_width == 128u)
         return delta ? run<128, true>(a, q.count, w, status, s)

@@ -322,6 +322,37 @@ def test_attention_many_sequences(ctx):
     check(a, a.got(ctx, off, slots, fresh, n), spans, slots, fresh)
 
 
+# a call's only sequence among rows of nobody
+@pytest.mark.parametrize("lead,length,gap", [(0, 0, 40), (30, 0, 0), (3, 5, 30), (20, 200, 7)])
+@pytest.mark.parametrize("heads", [(2, 6, 128, 128), (1, 2, 64, 64)], ids=str)
+@pytest.mark.parametrize("delta", [True, False])
+def test_attention_one_sequence(ctx, heads, lead, length, gap, delta):
+    say("one sequence", heads, lead, length, gap, delta)
+    off, spans, rows = table([length], lead=lead, gap=gap)
+    a = Attention(41, *heads, rows, 3, delta=delta)
+    for slot in (2, NO):
+        for fresh in (0, 1):
+            check(a, a.got(ctx, off, [slot], [fresh], 1), spans, [slot], [fresh])
+        check(a, a.got(ctx, off, [slot], None, 1, in_place=True), spans, [slot], [0], in_place=True)
+
+
+@pytest.mark.parametrize("off,slot", [([5, 2], 0), ([0, 51], 0), ([60, 70], 0), ([0, 50], 3),
+                                      ([0xFFFFFFF0, 50], 0)], ids=str)
+@pytest.mark.parametrize("delta", [True, False])
+def test_attention_one_bad_sequence(ctx, off, slot, delta):
+    say("one bad sequence", off, slot, delta)
+    a = Attention(42, 1, 2, 64, 64, 50, 3, delta=delta)
+    assert failing(ctx, a, off, [slot], None, 1) == "INVALID_ARGUMENT"
+
+
+@pytest.mark.parametrize("delta", [True, False])
+def test_attention_one_empty_sequence_non_finite(ctx, delta):
+    say("one empty sequence, non-finite", delta)
+    a = Attention(43, 1, 2, 64, 64, 50, 2, delta=delta)
+    a.state[1, 1, 63, 63] = np.inf
+    assert failing(ctx, a, [9, 9], [1], None, 1) == "NUMERIC_DOMAIN"
+
+
 def test_attention_split_prompt_is_one(ctx):
     # a prompt in two calls, its state carried on, against the prompt in one
     say("split prompt")
