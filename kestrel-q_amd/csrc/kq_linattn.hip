@@ -249,16 +249,19 @@ hipError_t launch(const kq_launch_linattn &a, const kq_launch_seqs &q, uint32_t 
     return hipGetLastError();
 }
 
-/* Workgroups of four waves. Few waves (one sequence's row): half the columns
- * each and one a workgroup, so that they spread over the device, which takes
- * 48 heads of 128 x 128 from 6.4 to 5.6 us; 61 sequences 81 -> 83 us. */
+/* Workgroups of four waves with 32 columns each. For few sequences 16 columns
+ * and, for the fewest, one wave a workgroup, so that they spread over the
+ * device. 48 heads of 128 x 128, in us, with 16 columns and one wave, 16 and
+ * four, 32 and four: one sequence 5.9, 6.3, -; two 8.2, 6.7, 7.6; four 10.6,
+ * 9.3, 9.8; eight 15.7, 13.7, 13.4; 32 58, 50, 44. */
 template <int DK>
 hipError_t launch(const kq_launch_linattn &a, const kq_launch_seqs &q, uint32_t max_rows,
                   const kq_linattn_plan &plan, uint32_t *status, hipStream_t s) {
     const uint64_t tiles = (uint64_t)a.value_heads * a.value_width / 32u * q.count;
     if (plan.chunk != nullptr) return launch<DK, 8, 256, true>(a, q, max_rows, plan, status, s);
-    return tiles <= 256u ? launch<DK, 4, 64, false>(a, q, max_rows, plan, status, s)
-                         : launch<DK, 8, 256, false>(a, q, max_rows, plan, status, s);
+    if (tiles <= 256u) return launch<DK, 4, 64, false>(a, q, max_rows, plan, status, s);
+    if (tiles <= 1024u) return launch<DK, 4, 256, false>(a, q, max_rows, plan, status, s);
+    return launch<DK, 8, 256, false>(a, q, max_rows, plan, status, s);
 }
 
 }  // namespace
