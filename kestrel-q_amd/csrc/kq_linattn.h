@@ -12,15 +12,9 @@
 namespace kq {
 
 /* a row's log decay g <= 0 of a head */
-__device__ __forceinline__ float log_decay(const kq_launch_linattn &a, uint64_t t, uint32_t h,
-                                           float rate, float bias, bool &badin) {
-    float g = rate;
-    if (a.alpha != nullptr) {
-        const float x = a.alpha[t * a.as + h];
-        badin |= !kq_isfinite(x);
-        g = rate * softplus(x + bias);
-    }
-    return fmaxf(g, -1.0e30f);
+__device__ __forceinline__ float log_decay(const kq_launch_linattn &a, float alpha, float rate,
+                                           float bias) {
+    return fmaxf(a.alpha != nullptr ? rate * softplus(alpha + bias) : rate, -1.0e30f);
 }
 
 /* S e^g as c0 S + c1 S. A decay near 1 that is rounded to 32 bits is off by

@@ -25,14 +25,12 @@ namespace {
 
 typedef float f4 __attribute__((ext_vector_type(4)));
 
-/* one row of a lane: its part of q and k, its columns of v, the head's gates */
+/* one row of a lane: its part of q and k, its columns of v */
 template <int R>
 struct Row {
-    float q[R], k[R], v[4], beta;
-    kq::Decay e;
+    float q[R], k[R], v[4];
     __device__ __forceinline__ void load(const kq_launch_linattn &a, uint64_t t, uint32_t qk,
-                                         uint32_t vc, uint32_t h, float rate, float bias,
-                                         bool &badin) {
+                                         uint32_t vc) {
         const float4 *qp = (const float4 *)(a.q + t * a.qs + qk);
         const float4 *kp = (const float4 *)(a.k + t * a.ks + qk);
 #pragma unroll
@@ -43,9 +41,6 @@ struct Row {
         }
         const float4 x = *(const float4 *)(a.v + t * a.vs + vc);
         v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
-        beta = a.beta != nullptr ? a.beta[t * a.bs + h] : 0.0f;
-        badin |= !kq_isfinite(beta);
-        e = kq::decay_of(kq::log_decay(a, t, h, rate, bias, badin));
     }
 };
 
@@ -57,7 +52,7 @@ __device__ __forceinline__ float inverse_norm(const float (&x)[R], float eps) {
 #pragma unroll
     for (int i = 0; i < R; ++i) s = fmaf(x[i], x[i], s);
     s = kq::lanes_sum<SUM>(s);
-    if (s < 3.0e38f) return 1.0f / sqrtf(s + eps); /* the same way in every lane */
+    if (s < 3.0e38f) return kq::inverse_root(s + eps); /* the same way in every lane */
     s = 0.0f;
 #pragma unroll
     for (int i = 0; i < R; ++i) s = fmaf(x[i] * 0x1p-96f, x[i] * 0x1p-96f, s);
@@ -130,7 +125,7 @@ __device__ __forceinline__ void cut(const kq_launch_seqs &q, uint32_t max_rows,
 }
 
 /* grid (waves of columns of all heads / waves a workgroup, sequences): the
- * sequences of at most max_rows rows. With a plan (CUT) one workgroup more in
+ * sequences of at most max_rows (64) rows. With a plan (CUT) one workgroup more in
  * x, the first of which cuts the others into chunks: a launch of its own for
  * that takes 5 us. */
 template <int DK, int CG, int NT, bool CUT>
@@ -163,6 +158,14 @@ __global__ __launch_bounds__(NT) void linattn_rows(kq_launch_linattn a, kq_launc
     const uint32_t vc = h * a.value_width + col;
     const size_t at = (((size_t)sp.slot * a.value_heads + h) * DK + row0) * a.value_width + col;
 
+    /* the gates: a lane for each row */
+    const uint64_t mine = (uint64_t)sp.begin + (lane < sp.rows ? lane : 0u);
+    float alpha = 0.0f, beta = 0.0f;
+    if (sp.rows != 0u) {
+        if (a.alpha != nullptr) alpha = a.alpha[mine * a.as + h];
+        if (a.beta != nullptr) beta = a.beta[mine * a.bs + h];
+    }
+    const float rate = a.rate[h], bias = a.bias != nullptr ? a.bias[h] : 0.0f;
     float S[R][4];
     if (!sp.fresh) {
 #pragma unroll
@@ -174,15 +177,21 @@ __global__ __launch_bounds__(NT) void linattn_rows(kq_launch_linattn a, kq_launc
 #pragma unroll
         for (int i = 0; i < R; ++i) S[i][0] = S[i][1] = S[i][2] = S[i][3] = 0.0f;
     }
-    const float rate = a.rate[h], bias = a.bias != nullptr ? a.bias[h] : 0.0f;
-    bool badin = !kq_isfinite(rate) || rate > 0.0f || !kq_isfinite(bias), bad = false;
     Row<R> next;
-    if (sp.rows != 0u) next.load(a, sp.begin, qk, vc, h, rate, bias, badin);
+    if (sp.rows != 0u) next.load(a, sp.begin, qk, vc);
+    bool badin = !kq_isfinite(rate) || rate > 0.0f || !kq_isfinite(bias), bad = false;
+    badin |= !kq_isfinite(alpha) || !kq_isfinite(beta);
+    const kq::Decay e = kq::decay_of(kq::log_decay(a, alpha, rate, bias));
+    const float part = kq::sigmoid(beta);
     for (uint32_t n = 0; n < sp.rows; ++n) {
         Row<R> r = next;
         const uint64_t t = (uint64_t)sp.begin + n;
-        if (n + 1u < sp.rows) next.load(a, t + 1u, qk, vc, h, rate, bias, badin);
-        const float c0 = r.e.c0, c1 = r.e.c1;
+        if (n + 1u < sp.rows) next.load(a, t + 1u, qk, vc);
+        auto of = [&](float x) {
+            return __uint_as_float(
+                (uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(x), (int)n));
+        };
+        const float c0 = of(e.c0), c1 = of(e.c1), b = of(part);
         float nq = a.scale, nk = 1.0f;
         if (a.normalize != 0u) {
             nq *= inverse_norm<R, SUM>(r.q, a.epsilon);
@@ -209,7 +218,6 @@ __global__ __launch_bounds__(NT) void linattn_rows(kq_launch_linattn a, kq_launc
             sk[c] = kq::lanes_sum<SUM>(sk[c]);
             sq[c] = kq::lanes_sum<SUM>(sq[c]);
         }
-        const float b = a.beta != nullptr ? kq::sigmoid(r.beta) : 1.0f;
         float d[4], o[4];
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
@@ -273,7 +281,7 @@ hipError_t kq_linattn_recurrent(const kq_launch_linattn &a, const kq_launch_seqs
                                : launch<64>(a, q, max_rows, plan, status, s);
 }
 
-/* sequences up to this long run in the recurrent form: 2 us a row, against about
+/* sequences up to this long (64: a lane for each row) run in the recurrent form: 2 us a row, against about
  * 35 us for one chunk's three launches */
 constexpr uint32_t kShort = 16u;
 

@@ -79,6 +79,12 @@ __device__ __forceinline__ float inverse_of(float d) {
     return fmaf(fmaf(-d, r, 1.0f), r, r);
 }
 
+/* 1 / sqrt(x), x normal: the hardware's and one Newton step */
+__device__ __forceinline__ float inverse_root(float x) {
+    const float r = __builtin_amdgcn_rsqf(x);
+    return fmaf(0.5f * r, fmaf(-x * r, r, 1.0f), r);
+}
+
 /* ln(1 + e^x) of a finite sum x that may have left the range */
 __device__ __forceinline__ float softplus(float x) {
     x = fminf(x, 0x1.fffffep127f);
