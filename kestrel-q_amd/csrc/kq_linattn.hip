@@ -192,31 +192,59 @@ __global__ __launch_bounds__(NT) void linattn_rows(kq_launch_linattn a, kq_launc
                 (uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(x), (int)n));
         };
         const float c0 = of(e.c0), c1 = of(e.c1), b = of(part);
-        float nq = a.scale, nk = 1.0f;
-        if (a.normalize != 0u) {
-            nq *= inverse_norm<R, SUM>(r.q, a.epsilon);
-            nk = inverse_norm<R, SUM>(r.k, a.epsilon);
-        }
-        float qkv = 0.0f, sk[4], sq[4];
+        /* sums over the rows of S, of q and k as they are: all exchanges side by
+         * side, then the norms as factors */
+        float q2, k2, qkv, sk[4], sq[4];
+        auto sums = [&]() {
+            q2 = k2 = qkv = 0.0f;
 #pragma unroll
-        for (int c = 0; c < 4; ++c) sk[c] = sq[c] = 0.0f;
+            for (int c = 0; c < 4; ++c) sk[c] = sq[c] = 0.0f;
 #pragma unroll
-        for (int i = 0; i < R; ++i) {
-            badin |= !kq_isfinite(r.q[i]) || !kq_isfinite(r.k[i]);
-            r.q[i] *= nq;
-            r.k[i] *= nk;
-            qkv = fmaf(r.q[i], r.k[i], qkv);
+            for (int i = 0; i < R; ++i) {
+                q2 = fmaf(r.q[i], r.q[i], q2);
+                k2 = fmaf(r.k[i], r.k[i], k2);
+                qkv = fmaf(r.q[i], r.k[i], qkv);
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    sk[c] = fmaf(r.k[i], S[i][c], sk[c]);
+                    sq[c] = fmaf(r.q[i], S[i][c], sq[c]);
+                }
+            }
+            q2 = kq::lanes_sum<SUM>(q2);
+            k2 = kq::lanes_sum<SUM>(k2);
+            qkv = kq::lanes_sum<SUM>(qkv);
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
-                sk[c] = fmaf(r.k[i], S[i][c], sk[c]);
-                sq[c] = fmaf(r.q[i], S[i][c], sq[c]);
+                sk[c] = kq::lanes_sum<SUM>(sk[c]);
+                sq[c] = kq::lanes_sum<SUM>(sq[c]);
+            }
+        };
+        sums();
+        float nq = a.scale, nk = 1.0f;
+        /* the same way in every lane */
+        if (a.normalize != 0u && q2 > 1e-24f && q2 < 1e12f && k2 > 1e-24f && k2 < 1e12f) {
+            nq *= kq::inverse_root(q2 + a.epsilon);
+            nk = kq::inverse_root(k2 + a.epsilon);
+        } else {
+#pragma unroll
+            for (int i = 0; i < R; ++i) badin |= !kq_isfinite(r.q[i]) || !kq_isfinite(r.k[i]);
+            if (a.normalize != 0u) { /* sums as they are could leave the type's range */
+                nq *= inverse_norm<R, SUM>(r.q, a.epsilon);
+                nk = inverse_norm<R, SUM>(r.k, a.epsilon);
+#pragma unroll
+                for (int i = 0; i < R; ++i) {
+                    r.q[i] *= nq;
+                    r.k[i] *= nk;
+                }
+                sums();
+                nq = nk = 1.0f;
             }
         }
-        qkv = kq::lanes_sum<SUM>(qkv);
+        qkv *= nq * nk;
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-            sk[c] = kq::lanes_sum<SUM>(sk[c]);
-            sq[c] = kq::lanes_sum<SUM>(sq[c]);
+            sk[c] *= nk;
+            sq[c] *= nq;
         }
         float d[4], o[4];
 #pragma unroll
@@ -230,7 +258,8 @@ __global__ __launch_bounds__(NT) void linattn_rows(kq_launch_linattn a, kq_launc
 #pragma unroll
         for (int i = 0; i < R; ++i)
 #pragma unroll
-            for (int c = 0; c < 4; ++c) S[i][c] = fmaf(r.k[i], d[c], fmaf(c1, S[i][c], c0 * S[i][c]));
+            for (int c = 0; c < 4; ++c)
+                S[i][c] = fmaf(r.k[i], d[c] * nk, fmaf(c1, S[i][c], c0 * S[i][c]));
         if (lane < CG)
             *(float4 *)(a.y + t * a.ys + vc) = make_float4(o[0], o[1], o[2], o[3]);
     }
