@@ -13,11 +13,11 @@
  * rg R .. rg R + R - 1 of columns 4 cg .. 4 cg + 3, and every sum over the rows
  * is finished by lane exchanges, without LDS or a barrier. For one row a
  * sequence the state's read and write are the bound: 131,072 bytes a head of
- * 128 x 128, against 100 KFLOP. 61 sequences of 48 such heads take 79 us, 4.9
+ * 128 x 128, against 100 KFLOP. 61 sequences of 48 such heads take 74 us, 5.2
  * TB/s (a large copy: 5.1).
  *
- * Sequences of up to 16 rows run here too, a row after the other in 2 us each;
- * longer ones have chunks (kq_linattn_chunk.hip).
+ * Sequences of up to 16 rows run here too, a row after the other in 1.2 us
+ * each; longer ones have chunks (kq_linattn_chunk.hip).
  */
 #include "kq_linattn.h"
 
@@ -289,15 +289,15 @@ hipError_t launch(const kq_launch_linattn &a, const kq_launch_seqs &q, uint32_t 
 /* Workgroups of four waves with 32 columns each. For few sequences 16 columns
  * and, for the fewest, one wave a workgroup, so that they spread over the
  * device. 48 heads of 128 x 128, in us, with 16 columns and one wave, 16 and
- * four, 32 and four: one sequence 5.9, 6.3, -; two 8.2, 6.7, 7.6; four 10.6,
- * 9.3, 9.8; eight 15.7, 13.7, 13.4; 32 58, 50, 44. */
+ * four, 32 and four: one sequence 5.4, 5.6, 6.7; two 7.3, 6.1, 7.0; four 9.5,
+ * 8.1, 9.0; six 12.5, 10.1, 11.5; eight 14.0, 12.4, 12.0; 32 55, 48, 39. */
 template <int DK>
 hipError_t launch(const kq_launch_linattn &a, const kq_launch_seqs &q, uint32_t max_rows,
                   const kq_linattn_plan &plan, uint32_t *status, hipStream_t s) {
     const uint64_t tiles = (uint64_t)a.value_heads * a.value_width / 32u * q.count;
     if (plan.chunk != nullptr) return launch<DK, 8, 256, true>(a, q, max_rows, plan, status, s);
     if (tiles <= 256u) return launch<DK, 4, 64, false>(a, q, max_rows, plan, status, s);
-    if (tiles <= 1024u) return launch<DK, 4, 256, false>(a, q, max_rows, plan, status, s);
+    if (tiles <= 1280u) return launch<DK, 4, 256, false>(a, q, max_rows, plan, status, s);
     return launch<DK, 8, 256, false>(a, q, max_rows, plan, status, s);
 }
 
@@ -310,8 +310,8 @@ hipError_t kq_linattn_recurrent(const kq_launch_linattn &a, const kq_launch_seqs
                                : launch<64>(a, q, max_rows, plan, status, s);
 }
 
-/* sequences up to this long (64: a lane for each row) run in the recurrent form: 2 us a row, against about
- * 35 us for one chunk's three launches */
+/* sequences up to this long (64: a lane for each row) run in the recurrent form: 1.2
+ * us a row, against 26 to 35 us for a chunk's launches */
 constexpr uint32_t kShort = 16u;
 
 extern "C" uint64_t kq_launch_linattn_scratch(const kq_launch_linattn *a, uint64_t tokens,

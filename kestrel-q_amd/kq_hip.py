@@ -857,7 +857,7 @@ class Context:
     def causal_conv(self, conv: CausalConv, seqs: Sequences, x, x_stride: int, state, state_out,
                     y, y_stride: int) -> None:
         d = Diagnostic()
-        check(lib().kq_hip_causal_conv_f32(self._h, C.byref(conv), C.byref(seqs), _ptr(x),
+        check(lib().kq_hip_causal_conv_f32(self.handle, C.byref(conv), C.byref(seqs), _ptr(x),
                                            x_stride, _ptr(state), _ptr(state_out), _ptr(y),
                                            y_stride, C.byref(d)), d)
 
@@ -865,7 +865,7 @@ class Context:
                          inputs: LinearAttentionInputs, state, state_out, y, y_stride: int,
                          scratch=None, scratch_bytes: int = 0) -> None:
         d = Diagnostic()
-        check(lib().kq_hip_linear_attention_f32(self._h, C.byref(attention), C.byref(seqs),
+        check(lib().kq_hip_linear_attention_f32(self.handle, C.byref(attention), C.byref(seqs),
                                                 C.byref(inputs), _ptr(state), _ptr(state_out),
                                                 _ptr(y), y_stride, _ptr(scratch), scratch_bytes,
                                                 C.byref(d)), d)
@@ -873,14 +873,14 @@ class Context:
     def gated_norm(self, norm: GatedNorm, tokens: int, x, x_stride: int, gate, gate_stride: int,
                    y, y_stride: int) -> None:
         d = Diagnostic()
-        check(lib().kq_hip_gated_norm_f32(self._h, C.byref(norm), tokens, _ptr(x), x_stride,
+        check(lib().kq_hip_gated_norm_f32(self.handle, C.byref(norm), tokens, _ptr(x), x_stride,
                                           _ptr(gate), gate_stride, _ptr(y), y_stride,
                                           C.byref(d)), d)
 
     def block_join(self, join: BlockJoin, tokens: int, block_output, gate, residual, branch_gate,
                    residual_out, normalized=None) -> None:
         d = Diagnostic()
-        check(lib().kq_hip_block_join_f32(self._h, C.byref(join), tokens, _ptr(block_output),
+        check(lib().kq_hip_block_join_f32(self.handle, C.byref(join), tokens, _ptr(block_output),
                                           _ptr(gate), _ptr(residual), _ptr(branch_gate),
                                           _ptr(residual_out), _ptr(normalized), C.byref(d)), d)
 
