@@ -990,6 +990,62 @@ def test_prompt_graph_replays():
         h.hipGraphExecDestroy(graph)
 
 
+@pytest.mark.parametrize("count,dims,delta", [(1, (2, 4, 128, 64), True), (1, (1, 2, 64, 128), False),
+                                              (2, (1, 2, 64, 64), False)], ids=str)
+def test_attention_graph_lengths(count, dims, delta):
+    """Captured calls whose lengths change between replays, down to none."""
+    say("graph lengths", count, dims, delta)
+    with kq_hip.Context(0) as ctx, Call(ctx) as c:
+        a = Attention(31, *dims, 300, 2, delta=delta)
+        hk, hv, dk, dv = dims
+        off = c.up(np.zeros(count + 1, np.uint32))
+        la, _, inp = a.describe(c, None, None, None, 1)
+        seqs = kq_hip.sequences(300, count, 2, off)
+        st, so = c.up(a.state), c.up(np.zeros_like(a.state))
+        out = np.full((300, hv * dv), SENTINEL)
+        y = c.up(out)
+        n = kq_hip.linear_attention_scratch_bytes(la, seqs)
+        scr = c.scratch(n)
+        ctx.set_async(True)
+        h, graph = capture(ctx, lambda: ctx.linear_attention(la, seqs, inp, st, so, y, hv * dv, scr,
+                                                             n))
+        for lengths in ([300, 0], [0, 150], [5, 100], [129, 171], [0, 0], [64, 16]):
+            o, spans, _ = table(lengths[:count], lead=0)
+            put(ctx, off, o)
+            put(ctx, so, np.full_like(a.state, SENTINEL))
+            put(ctx, y, out)
+            assert h.hipGraphLaunch(graph, C.c_void_p(ctx.stream)) == 0
+            ctx.synchronize()
+            check(a, (c.down(y, out).reshape(300, hv, dv), c.down(so, a.state)), spans,
+                  list(range(count)), [0] * count)
+        ctx.set_async(False)
+        h.hipGraphExecDestroy(graph)
+
+
+def test_conv_graph_lengths():
+    say("conv graph lengths")
+    with kq_hip.Context(0) as ctx, Call(ctx) as c:
+        v = Conv(32, 260, 4, 90, 3)
+        off = c.up(np.zeros(4, np.uint32))
+        cv, _ = v.describe(c, None, None, None, 1)
+        seqs = kq_hip.sequences(90, 3, 3, off)
+        x, st, so = c.up(v.x), c.up(v.state), c.up(np.zeros_like(v.state))
+        out = np.full((90, 260), SENTINEL)
+        y = c.up(out)
+        ctx.set_async(True)
+        h, graph = capture(ctx, lambda: ctx.causal_conv(cv, seqs, x, 260, st, so, y, 260))
+        for lengths in ([90, 0, 0], [1, 2, 3], [0, 0, 0], [30, 17, 43], [0, 16, 74]):
+            o, spans, _ = table(lengths)
+            put(ctx, off, o)
+            put(ctx, so, np.full_like(v.state, SENTINEL))
+            put(ctx, y, out)
+            assert h.hipGraphLaunch(graph, C.c_void_p(ctx.stream)) == 0
+            ctx.synchronize()
+            v.check((c.down(y, out), c.down(so, v.state)), spans, [0, 1, 2], [0, 0, 0])
+        ctx.set_async(False)
+        h.hipGraphExecDestroy(graph)
+
+
 def test_same_inputs_same_bits(ctx):
     # no sum depends on the order in which workgroups run
     say("same bits")
