@@ -139,32 +139,43 @@ __global__ __launch_bounds__(NT) void linattn_rows(kq_launch_linattn a, kq_launc
     constexpr int RG = 64 / CG, R = DK / RG, SUM = 63 & ~(CG - 1);
     const uint32_t lane = threadIdx.x & 63u;
     const uint32_t s = blockIdx.y;
-    bool badseq = false;
-    const kq::SeqSpan sp = kq::seq_span(q, s, badseq);
-    if (blockIdx.x == 0u) {
-        if (sp.live && q.slots != nullptr)
-            for (uint32_t j = threadIdx.x; j < s; j += NT) badseq |= q.slots[j] == sp.slot;
-        if (badseq) kq_flag(status, KQ_DEV_SEQUENCE);
-    }
-    if (!sp.live || sp.rows > max_rows) return;
-    const uint32_t tiles = a.value_width / (4u * CG);
+    constexpr uint32_t kTile = 4u * CG; /* columns of a wave */
+    const uint32_t shift = (a.value_width == 128u ? 7u : 6u) - (kTile == 32u ? 5u : 4u);
     const uint32_t w = __builtin_amdgcn_readfirstlane(blockIdx.x * (NT / 64) +
                                                       (threadIdx.x >> 6));
-    const uint32_t h = w / tiles;
-    if (h >= a.value_heads) return;
-    const uint32_t col = (w % tiles) * (4u * CG) + (lane % CG) * 4u;
+    const uint32_t h = w >> shift;
+    const uint32_t col = (w & ((1u << shift) - 1u)) * kTile + (lane % CG) * 4u;
     const uint32_t row0 = (lane / CG) * R;
     const uint32_t qk = h / (a.value_heads / a.key_heads) * DK + row0;
     const uint32_t vc = h * a.value_width + col;
-    const size_t at = (((size_t)sp.slot * a.value_heads + h) * DK + row0) * a.value_width + col;
-
-    /* the gates: a lane for each row */
-    const uint64_t mine = (uint64_t)sp.begin + (lane < sp.rows ? lane : 0u);
+    /* where each sequence has one row, its loads do not wait for its slot */
+    const bool single = q.offsets == nullptr;
     float alpha = 0.0f, beta = 0.0f;
-    if (sp.rows != 0u) {
-        if (a.alpha != nullptr) alpha = a.alpha[mine * a.as + h];
-        if (a.beta != nullptr) beta = a.beta[mine * a.bs + h];
+    Row<R> next;
+    auto load_gates = [&](uint64_t t) {
+        if (a.alpha != nullptr) alpha = a.alpha[t * a.as + h];
+        if (a.beta != nullptr) beta = a.beta[t * a.bs + h];
+    };
+    if (single && h < a.value_heads) {
+        load_gates(s);
+        next.load(a, s, qk, vc);
     }
+    bool badseq = false;
+    const kq::SeqSpan sp = kq::seq_span(q, s, badseq);
+    /* by a workgroup of the sequence, every thread, behind its loads */
+    auto check_slot = [&]() {
+        if (blockIdx.x != 0u) return;
+        if (sp.live && q.slots != nullptr)
+            for (uint32_t j = threadIdx.x; j < s; j += NT) badseq |= q.slots[j] == sp.slot;
+        if (badseq) kq_flag(status, KQ_DEV_SEQUENCE);
+    };
+    if (!sp.live || sp.rows > max_rows || h >= a.value_heads) {
+        check_slot();
+        return;
+    }
+    const size_t at = (((size_t)sp.slot * a.value_heads + h) * DK + row0) * a.value_width + col;
+    if (!single && sp.rows != 0u) /* the gates: a lane for each row */
+        load_gates((uint64_t)sp.begin + (lane < sp.rows ? lane : 0u));
     const float rate = a.rate[h], bias = a.bias != nullptr ? a.bias[h] : 0.0f;
     float S[R][4];
     if (!sp.fresh) {
@@ -177,8 +188,7 @@ __global__ __launch_bounds__(NT) void linattn_rows(kq_launch_linattn a, kq_launc
 #pragma unroll
         for (int i = 0; i < R; ++i) S[i][0] = S[i][1] = S[i][2] = S[i][3] = 0.0f;
     }
-    Row<R> next;
-    if (sp.rows != 0u) next.load(a, sp.begin, qk, vc);
+    if (!single && sp.rows != 0u) next.load(a, sp.begin, qk, vc);
     bool badin = !kq_isfinite(rate) || rate > 0.0f || !kq_isfinite(bias), bad = false;
     badin |= !kq_isfinite(alpha) || !kq_isfinite(beta);
     const kq::Decay e = kq::decay_of(kq::log_decay(a, alpha, rate, bias));
@@ -272,6 +282,7 @@ __global__ __launch_bounds__(NT) void linattn_rows(kq_launch_linattn a, kq_launc
 #pragma unroll
         for (int c = 0; c < 4; ++c) bad |= !kq_isfinite(S[i][c]);
     }
+    check_slot();
     if (badin) kq_flag(status, KQ_DEV_INPUT);
     if (bad) kq_flag(status, KQ_DEV_NUMERIC);
 }

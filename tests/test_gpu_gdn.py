@@ -476,6 +476,23 @@ def test_bad_sequences(ctx, off, slots, scale):
 # -------------------------------------------------------------- convolution
 
 
+@pytest.mark.parametrize("first,second", [(0, 1), (63, 299), (64, 65), (150, 298), (255, 256),
+                                          (200, 299)])
+@pytest.mark.parametrize("rows", ["one each", "mixed"])
+def test_slot_taken_among_many(ctx, first, second, rows):
+    # one head: a workgroup has more threads than columns, and all of them look
+    say("slot taken", first, second, rows)
+    n = 300
+    lengths = [1] * n if rows == "one each" else [i % 3 for i in range(n)]
+    off, _, total = table(lengths)
+    off = None if rows == "one each" else off
+    slots = np.random.default_rng(1).permutation(n).tolist()
+    slots[second] = slots[first]
+    a = Attention(51, 1, 1, 64, 64, total, n)
+    assert failing(ctx, a, off, slots, None, n) == "INVALID_ARGUMENT"
+    assert Conv(52, 12, 4, total, n).failing(ctx, off, slots, None, n) == "INVALID_ARGUMENT"
+
+
 class Conv:
     def __init__(self, seed, channels, taps, rows, pool, bias=False, silu=True, pad=0):
         g = Gen(seed)
