@@ -189,9 +189,9 @@ __global__ __launch_bounds__(kThreads) void conv_rows(kq_launch_conv c, kq_launc
     if (mine) badin |= !w.load(c, ch);
     if (part < q.count) {
         const kq::SeqSpan sp = kq::seq_span(q, part, badseq);
-        if (sp.live && blockIdx.x == 0u) badseq |= kq::seq_slot_taken<kThreads>(q, part, sp.slot);
         if (sp.live && mine)
             head_rows<K, V>(c, sp, ch, x, xs, state, state_out, y, ys, w, badin, bad);
+        if (sp.live && blockIdx.x == 0u) badseq |= kq::seq_slot_taken<kThreads>(q, part, sp.slot);
     } else {
         const uint32_t tokens = (uint32_t)q.tokens;
         const uint32_t t0 = (part - q.count) * kRows; /* past the rows: none to do */
@@ -250,28 +250,26 @@ __global__ __launch_bounds__(kThreads) void conv_step(kq_launch_conv c, kq_launc
     const uint32_t s = blockIdx.y;
     bool badseq = false, badin = false, bad = false;
     const kq::SeqSpan sp = kq::seq_span(q, s, badseq);
-    if (blockIdx.x == 0u) {
-        if (sp.live) badseq |= kq::seq_slot_taken<kThreads>(q, s, sp.slot);
-        if (badseq) kq_flag(status, KQ_DEV_SEQUENCE);
-    }
     const uint32_t ch = (blockIdx.x * kThreads + threadIdx.x) * V;
-    if (ch >= c.channels || !sp.live) return;
-    const size_t at = (size_t)sp.slot * (K - 1) * c.channels + ch;
-    const float *row = x + (size_t)sp.begin * xs + ch;
-    const Vec<V> in = load<V>(row);
-    Vec<V> hist[K - 1];
-    read_state<K, V>(hist, sp.fresh, state + at, c.channels);
-    Taps<K, V> w;
-    badin |= !w.load(c, ch);
-    badin |= !finite(in);
+    if (sp.live && ch < c.channels) {
+        const size_t at = (size_t)sp.slot * (K - 1) * c.channels + ch;
+        const Vec<V> in = load<V>(x + (size_t)sp.begin * xs + ch);
+        Vec<V> hist[K - 1];
+        read_state<K, V>(hist, sp.fresh, state + at, c.channels);
+        Taps<K, V> w;
+        badin |= !w.load(c, ch);
+        badin |= !finite(in);
 #pragma unroll
-    for (int j = 0; j < K - 1; ++j) badin |= !finite(hist[j]);
-    const Vec<V> out = w.apply(hist, in, c.silu != 0u);
-    bad |= !finite(out);
-    store(y + (size_t)sp.begin * ys + ch, out);
+        for (int j = 0; j < K - 1; ++j) badin |= !finite(hist[j]);
+        const Vec<V> out = w.apply(hist, in, c.silu != 0u);
+        bad |= !finite(out);
+        store(y + (size_t)sp.begin * ys + ch, out);
 #pragma unroll
-    for (int j = 0; j < K - 1; ++j)
-        store(state_out + at + (size_t)j * c.channels, j + 1 < K - 1 ? hist[j + 1] : in);
+        for (int j = 0; j < K - 1; ++j)
+            store(state_out + at + (size_t)j * c.channels, j + 1 < K - 1 ? hist[j + 1] : in);
+    }
+    if (sp.live && blockIdx.x == 0u) badseq |= kq::seq_slot_taken<kThreads>(q, s, sp.slot);
+    if (badseq) kq_flag(status, KQ_DEV_SEQUENCE);
     if (badin) kq_flag(status, KQ_DEV_INPUT);
     if (bad) kq_flag(status, KQ_DEV_NUMERIC);
 }

@@ -40,12 +40,13 @@
  * differences are what counts.
  *
  * 16,384 rows of one sequence, 16 key and 48 value heads of 128 x 128: 860 us,
- * 105 TFLOP/s of the recurrent form's operations, which takes 33.4 ms for them. 690 us are the scan's, whose 256 steps
- * hang on each other: 2.6 us a step, two LDS round trips through a barrier with
- * 24 matrix instructions a wave behind each (2.07 us with a third of the heads:
- * the L2s give a workgroup 120 KB a step). 265 are linattn_prep's, bound by
- * the bytes it writes. (Launches overlap; U = B V formed there as well made
- * its writes, not the scan, the bound.) 513 rows: 43 us.
+ * 105 TFLOP/s of the recurrent form's operations, which at 1.2 us a row would
+ * take 20 ms for them. 690 us are the scan's, whose 256 steps hang on each
+ * other: 2.6 us a step, two LDS round trips through a barrier with 24 matrix
+ * instructions a wave behind each (2.07 us with a third of the heads: the L2s
+ * give a workgroup 120 KB a step). 265 are linattn_prep's, bound by the bytes
+ * it writes. (Launches overlap; U = B V formed there as well made its writes,
+ * not the scan, the bound.) 513 rows: 43 us.
  */
 #include <type_traits>
 
