@@ -1013,12 +1013,12 @@ __global__ __launch_bounds__(64 * scan_waves(DELTA)) void linattn_scan(kq_launch
         const uint32_t ct = rt & 1u, ks = rt >> 1;
         auto load_v = [&](float(&v)[8], uint32_t n) {
             const KqBuf vr = rows_at(a.v, a.vs, n < last ? n : last);
-            const uint32_t at = (4u * g4 * (uint32_t)a.vs + col) * 4u;
+            /* the row in the lane's offset, which alone is held against the buffer's end */
+            const uint32_t at = ((32u * ks + 4u * g4) * (uint32_t)a.vs + col) * 4u;
 #pragma unroll
             for (uint32_t e = 0; e < 8u; ++e)
                 v[e] = __uint_as_float(
-                    kq_ld32(vr, at + (16u * (e / 4u) + e % 4u) * (uint32_t)a.vs * 4u,
-                            128u * ks * (uint32_t)a.vs + 64u * ct));
+                    kq_ld32(vr, at + (16u * (e / 4u) + e % 4u) * (uint32_t)a.vs * 4u, 64u * ct));
         };
         auto put_v = [&](float(&v)[8]) {
             float m = 0.0f;

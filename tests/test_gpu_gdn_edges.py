@@ -1,0 +1,41 @@
+"""The operators between a GDN layer's projections and its residual where
+values or places are at an edge: what lies behind a sequence's rows, decays
+that differ by orders of magnitude, long memories, small columns beside large
+ones, the ends of the type's range. Against binary64 (tests/gdn64.py), with
+the bars of tests/test_gpu_gdn.py where no other is derived here.
+"""
+import numpy as np
+import pytest
+
+import gdn64
+import kq_hip
+from test_gpu_gdn import (NO, SENTINEL, U, Attention, Call, Conv, Gen, check, ctx,  # noqa: F401
+                          failing, near, say, table)
+
+pytestmark = pytest.mark.gpu
+
+
+# What follows a sequence in the arrays (rows of nobody, rows of a sequence taken
+# out) is never looked at: not its values, not their size, not whether they are
+# numbers.
+@pytest.mark.parametrize("tail", [1, 31, 32, 33, 63])
+@pytest.mark.parametrize("heads,delta", [((2, 4, 128, 128), True), ((1, 2, 64, 64), True),
+                                         ((16, 48, 128, 128), True), ((1, 2, 64, 64), False),
+                                         ((2, 4, 128, 128), False)], ids=str)
+@pytest.mark.parametrize("behind", [np.nan, 1e30])
+def test_attention_rows_behind_a_tail(ctx, tail, heads, delta, behind):  # noqa: F811
+    say("behind a tail", tail, heads, delta, behind)
+    for lengths, slots in (([64 + tail], [1]), ([tail], [0]), ([tail, 40, 128 + tail], [2, NO, 0])):
+        off, spans, rows = table(lengths, lead=1, gap=70)
+        n = len(lengths)
+        a = Attention(tail, *heads, rows, 3, delta=delta)
+        mine = np.zeros(rows, bool)
+        for (b, e), s in zip(spans, slots):
+            mine[b:e] = s != NO
+        clean = a.got(ctx, off, slots, None, n)
+        for x in (a.qkv, a.alpha, a.beta):
+            if x is not None:
+                x[~mine] = behind
+        got = a.got(ctx, off, slots, None, n)
+        assert np.array_equal(got[0], clean[0]) and np.array_equal(got[1], clean[1])
+        check(a, got, spans, slots, [0] * n)
