@@ -11,10 +11,13 @@
 
 namespace kq {
 
-/* a row's log decay g <= 0 of a head */
+/* A row's log decay g <= 0 of a head. From -104 on e^g is 0 in binary32; held
+ * at -1024, a decay is as strong as any, and 64 of them summed in 64 bits leave
+ * the decays of the rows between them to 2^-33: a difference of the sums that
+ * does not span a strong row would otherwise have lost its own terms. */
 __device__ __forceinline__ float log_decay(const kq_launch_linattn &a, float alpha, float rate,
                                            float bias) {
-    return fmaxf(a.alpha != nullptr ? rate * softplus(alpha + bias) : rate, -1.0e30f);
+    return fmaxf(a.alpha != nullptr ? rate * softplus(alpha + bias) : rate, -1024.0f);
 }
 
 /* S e^g as c0 S + c1 S. A decay near 1 that is rounded to 32 bits is off by

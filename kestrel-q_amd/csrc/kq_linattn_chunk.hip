@@ -285,9 +285,7 @@ __global__ __launch_bounds__(256, 2) void linattn_prep(kq_launch_linattn a, Work
     auto form_gates = [&]() {
         badin |= !kq_isfinite(g_rate) || g_rate > 0.0f || !kq_isfinite(g_bias) ||
                  !kq_isfinite(g_alpha) || !kq_isfinite(g_beta);
-        float g = g_rate;
-        if (a.alpha != nullptr) g *= kq::softplus(g_alpha + g_bias);
-        g = lane < ch.rows ? fmaxf(g, -1.0e30f) : 0.0f;
+        const float g = lane < ch.rows ? kq::log_decay(a, g_alpha, g_rate, g_bias) : 0.0f;
         if (DELTA) g_b = lane < ch.rows ? kq::sigmoid(g_beta) : 0.0f;
         g_sum = kq_wave_scan_f64((double)g);
         g_end = kq_readlane_f64(g_sum, 63);

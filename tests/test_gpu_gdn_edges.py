@@ -39,3 +39,28 @@ def test_attention_rows_behind_a_tail(ctx, tail, heads, delta, behind):  # noqa:
         got = a.got(ctx, off, slots, None, n)
         assert np.array_equal(got[0], clean[0]) and np.array_equal(got[1], clean[1])
         check(a, got, spans, slots, [0] * n)
+
+
+def near_parts(got, want):
+    """Every head's rows, 64 at a time, by themselves."""
+    for b in range(0, len(got), 64):
+        for h in range(got.shape[1]):
+            near(got[b:b + 64, h], want[b:b + 64, h])
+
+
+# Rows that wipe a head's state out (a gate that resets it) between ordinary rows.
+@pytest.mark.parametrize("alpha", [1e3, 1e10, 1e12, 1e15, 1e17, 1e30])
+@pytest.mark.parametrize("heads", [(2, 4, 128, 64), (1, 2, 64, 64)], ids=str)
+@pytest.mark.parametrize("delta", [True, False])
+def test_attention_decays_behind_a_strong_one(ctx, alpha, heads, delta):  # noqa: F811
+    say("behind a strong decay", alpha, heads, delta)
+    off, spans, rows = table([200, 90, 12])
+    a = Attention(61, *heads, rows, 3, delta=delta)
+    for t in (3, 20, 21, 70, 100, 150, 203, 230, 295):
+        a.alpha[t, :heads[1] - (t % 2)] = np.float32(alpha) * np.float32(1 + t / 64)
+    got = a.got(ctx, off, None, None, 3)
+    wy, ws = a.want(spans, [0, 1, 2], [0] * 3)
+    near_parts(got[0], wy)
+    for s in range(3):
+        for h in range(heads[1]):
+            near(got[1][s, h], ws[s, h])
