@@ -33,6 +33,23 @@ __device__ __forceinline__ Decay decay_of(float g) {
     d.c1 = g > -0.5f ? expm1f(g) : exp_neg(g);
     return d;
 }
+/* of many rows, g their sum. e^g - 1 is Taylor's sum to g^8, whose rest is
+ * 2^-26 of it at -1/2. */
+__device__ __forceinline__ Decay decay_of(double g) {
+    const float x = fmaxf((float)g, -0.5f);
+    float s = 1.0f / 40320.0f;
+    s = fmaf(s, x, 1.0f / 5040.0f);
+    s = fmaf(s, x, 1.0f / 720.0f);
+    s = fmaf(s, x, 1.0f / 120.0f);
+    s = fmaf(s, x, 1.0f / 24.0f);
+    s = fmaf(s, x, 1.0f / 6.0f);
+    s = fmaf(s, x, 0.5f);
+    s = fmaf(s * x, x, x);
+    Decay d;
+    d.c0 = g > -0.5 ? 1.0f : 0.0f;
+    d.c1 = g > -0.5 ? s : exp_of(g);
+    return d;
+}
 
 }  // namespace kq
 

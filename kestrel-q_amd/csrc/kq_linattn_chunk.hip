@@ -12,7 +12,9 @@
  *   E = B V - W S
  *   O = diag(e^G) Q S + M E,          M_ij = e^(G_i - G_j) q_i.k'_j      (j <= i)
  *   S' = e^(G_64) S + sum_j e^(G_64 - G_j) k'_j e_j^T
- * and what hangs on the chunk before is four products with S and E.
+ * and what hangs on the chunk before is four products with S and E. e^(G_64)
+ * is kept as kq::Decay has it: rounded to 32 bits it would be off the same way
+ * chunk after chunk, 8e-6 of a state after 256 of them.
  * Without the delta correction E = diag(n) V.
  *
  * Three launches:
@@ -392,7 +394,8 @@ __global__ __launch_bounds__(256, 2) void linattn_prep(kq_launch_linattn a, Work
             f[kC + lane] = kq::exp_of(end - G);
             f[2 * kC + lane] = nqs[lane];
             f[3 * kC + lane] = from * nqs[lane];
-            if (lane == 0u) f[4 * kC] = kq::exp_of(end);
+            const kq::Decay e = kq::decay_of(end);
+            if (lane == 0u) *(f2 *)&f[4 * kC] = f2{e.c0, e.c1};
         }
         __syncthreads();
         for (uint32_t hh = 0; hh < nh; ++hh) {
@@ -458,8 +461,8 @@ __global__ __launch_bounds__(256, 2) void linattn_prep(kq_launch_linattn a, Work
                 pw[wave] = p;
                 pu[wave] = scale_exp(mu);
                 float *f = (float *)(vb0 + wave * w.value_bytes + kMat) + 4 * kC;
-                f[1] = pow2(kWDown - p);
-                f[2] = pow2(-pu[wave]);
+                f[2] = pow2(kWDown - p);
+                f[3] = pow2(-pu[wave]);
             }
         }
         __syncthreads();
@@ -723,7 +726,7 @@ __global__ __launch_bounds__(64 * scan_waves(DELTA)) void linattn_scan(kq_launch
         Frag<KS> W;
         Frag<2> T[NR];
         f4 V[2], f0, f1; /* B V, or V with the factors n; e^(G_64 - G) */
-        float iw = 0.0f, c0;
+        float iw = 0.0f, c0, c1;
         uint32_t io[4]; /* the wave's rows of v, in bytes */
         if (!DELTA)
 #pragma unroll
@@ -733,7 +736,7 @@ __global__ __launch_bounds__(64 * scan_waves(DELTA)) void linattn_scan(kq_launch
         };
         auto load_v = [&](KqBuf c, uint32_t n) {
             if (DELTA) {
-                iw = scalar(c, 1u);
+                iw = scalar(c, 2u);
             } else {
                 f0 = factors(c, 0u);
                 const KqBuf v = rows_at(a.v, a.vs, n);
@@ -745,11 +748,16 @@ __global__ __launch_bounds__(64 * scan_waves(DELTA)) void linattn_scan(kq_launch
             }
             f1 = factors(c, 1u);
         };
+        auto load_decay = [&](KqBuf c) {
+            const f2 e = __builtin_bit_cast(f2, kq_ld64(c, 0u, fat + 4u * kC * 4u));
+            c0 = e.x;
+            c1 = e.y;
+        };
         auto load_t = [&](KqBuf c) {
 #pragma unroll
             for (int t = 0; t < NR; ++t)
                 T[t].load(c, lane16, kat + kKeyImage + (NR * rt + t) * 4096u);
-            c0 = scalar(c, 0u);
+            load_decay(c);
         };
         /* S as an operand */
         char *sbuf = sbufs[0];
@@ -839,7 +847,7 @@ __global__ __launch_bounds__(64 * scan_waves(DELTA)) void linattn_scan(kq_launch
             };
             put_ef();
             kq_lds_barrier();
-            /* 2: S' = e^G S + K'^T F */
+            /* 2: S' = e^G S + K'^T F, e^G in two parts (kq::Decay) */
             f4 x[NR][2];
             {
                 const uint32_t all = told_of(told_ef);
@@ -866,9 +874,14 @@ __global__ __launch_bounds__(64 * scan_waves(DELTA)) void linattn_scan(kq_launch
 #pragma unroll
                     for (int t = 0; t < NR; ++t)
 #pragma unroll
-                        for (int ct = 0; ct < 2; ++ct)
+                        for (int ct = 0; ct < 2; ++ct) {
                             x[t][ct] = mfma3(T[t].hi[ks], T[t].lo[ks], B[ct].hi[ks], B[ct].lo[ks],
                                              x[t][ct]);
+                            if (ks == 1) /* beside the products */
+#pragma unroll
+                                for (int r = 0; r < 4; ++r)
+                                    S[t][ct][r] = fmaf(c1, S[t][ct][r], c0 * S[t][ct][r]);
+                        }
 #pragma unroll
                     for (int t = 0; t < NR; ++t)
                         T[t].load1(next, lane16, kat + kKeyImage + (NR * rt + t) * 4096u, ks);
@@ -883,9 +896,8 @@ __global__ __launch_bounds__(64 * scan_waves(DELTA)) void linattn_scan(kq_launch
                 for (int ct = 0; ct < 2; ++ct)
 #pragma unroll
                     for (int r = 0; r < 4; ++r)
-                        S[t][ct][r] = fmaf(x[t][ct][r], jf, c0 * S[t][ct][r]);
-            __builtin_amdgcn_sched_barrier(0); /* c0 has been used: no copy that would wait */
-            c0 = scalar(next, 0u);
+                        S[t][ct][r] = fmaf(x[t][ct][r], jf, S[t][ct][r]);
+            load_decay(next);
             sbuf = sbufs[(n + 1u) & 1u];
             share_s();
         }
@@ -1037,7 +1049,7 @@ __global__ __launch_bounds__(64 * scan_waves(DELTA)) void linattn_scan(kq_launch
             const KqBuf c = chunk(n < last ? n : last);
             load_lower(B2[i], c, wat + kKeyImage, 0);
             load_lower(B2[i], c, wat + kKeyImage, 1);
-            ib[i] = scalar(c, 2u);
+            ib[i] = scalar(c, 3u);
         };
         /* B V of chunk n from vbuf; then B of chunk n + 2 */
         auto times_v = [&](int i, uint32_t n) {
@@ -1242,19 +1254,19 @@ __global__ __launch_bounds__(256) void linattn_states(kq_launch_linattn a, Work 
     char *f = w.data + (uint64_t)blockIdx.y * w.chunk_bytes + w.value_at + h * w.value_bytes + kMat;
     for (uint32_t c = 0; c < n; c += kAhead) {
         f4 u[kAhead];
-        float c0[kAhead];
+        f2 e[kAhead]; /* e^G in two parts */
 #pragma unroll
         for (uint32_t k = 0; k < kAhead; ++k) { /* the last again behind it */
             const char *p = f + (uint64_t)(c + k < n ? c + k : n - 1u) * w.chunk_bytes;
             u[k] = *(const f4 *)(p + kRowF * 4u + i * 4u);
-            c0[k] = *(const float *)(p + 4u * kC * 4u);
+            e[k] = *(const f2 *)(p + 4u * kC * 4u);
         }
 #pragma unroll
         for (uint32_t k = 0; k < kAhead; ++k) {
             if (c + k >= n) break;
             *(f4 *)(f + (uint64_t)(c + k) * w.chunk_bytes + kRowF * 4u + i * 4u) = S;
 #pragma unroll
-            for (int r = 0; r < 4; ++r) S[r] = fmaf(c0[k], S[r], u[k][r]);
+            for (int r = 0; r < 4; ++r) S[r] = fmaf(e[k].x, S[r], fmaf(e[k].y, S[r], u[k][r]));
         }
     }
 #pragma unroll

@@ -64,3 +64,26 @@ def test_attention_decays_behind_a_strong_one(ctx, alpha, heads, delta):  # noqa
     for s in range(3):
         for h in range(heads[1]):
             near(got[1][s, h], ws[s, h])
+
+
+def awkward_rates(n):
+    r = np.linspace(-1e-4, -1e-5, 4000).astype(np.float32)
+    e = np.exp(64.0 * r.astype(np.float64))
+    off = (e.astype(np.float32) - e) / e
+    return r[np.argsort(off)[[0, -1, 1, -2][:n]]]
+
+
+@pytest.mark.parametrize("count", [1, 17])
+@pytest.mark.parametrize("delta", [True, False])
+def test_attention_long_memory(ctx, delta, count):  # noqa: F811
+    say("long memory", delta, count)
+    off, spans, rows = table([16384] + [1] * (count - 1))
+    a = Attention(62, 1, 4, 64, 64, rows, count, delta=delta, alpha=False)
+    a.qkv[:, 64:96] = 0
+    a.rate[:] = awkward_rates(4)
+    got = a.got(ctx, off, None, None, count)
+    wy, ws = a.want(spans, list(range(count)), [0] * count)
+    for h in range(4):
+        near(got[1][0, h, :32], ws[0, h, :32])
+        near(got[1][0, h, 32:], ws[0, h, 32:])
+    near_parts(got[0], wy)
