@@ -40,15 +40,15 @@ static uint64_t rows_span(uint64_t rows, uint64_t stride, uint64_t width) {
     return rows == 0u ? 0u : (rows - 1u) * stride + width;
 }
 
-/* outputs against everything else; NULL buffers overlap nothing. An output
- * may equal the input at its index in `may` (NULL: none). */
-static int aliased(const span *outs, uint32_t n, const span *ins, uint32_t m,
-                   const void *const *may) {
+/* Outputs against everything else; NULL buffers overlap nothing. The first
+ * output may be the first input, which lies there alone: any other one is
+ * read where something else is written. */
+static int aliased(const span *outs, uint32_t n, const span *ins, uint32_t m) {
     for (uint32_t i = 0; i < n; ++i) {
         for (uint32_t j = i + 1u; j < n; ++j)
             if (overlap(outs[i], outs[j])) return 1;
         for (uint32_t j = 0; j < m; ++j) {
-            if (may != NULL && outs[i].p == may[i] && ins[j].p == may[i]) continue;
+            if (i == 0u && j == 0u && outs[0].p == ins[0].p) continue;
             if (overlap(outs[i], ins[j])) return 1;
         }
     }
@@ -125,8 +125,7 @@ kq_status kq_hip_causal_conv_f32(kq_hip_context *c, const kq_hip_causal_conv *v,
                              {q->offsets, (uint64_t)q->sequence_count + 1u},
                              {q->slots, q->sequence_count},
                              {q->fresh, q->sequence_count}};
-        const void *const may[2] = {state, NULL};
-        if (aliased(outs, 2u, ins, 7u, may))
+        if (aliased(outs, 2u, ins, 7u))
             return kq_fail(diag, KQ_STATUS_ALIASING_VIOLATION,
                            "convolution outputs overlap; state_out may only be the state itself");
     }
@@ -249,8 +248,7 @@ kq_status kq_hip_linear_attention_f32(kq_hip_context *c, const kq_hip_linear_att
                               {q->offsets, (uint64_t)q->sequence_count + 1u},
                               {q->slots, q->sequence_count},
                               {q->fresh, q->sequence_count}};
-        const void *const may[3] = {state, NULL, NULL};
-        if (aliased(outs, 3u, ins, 11u, may))
+        if (aliased(outs, 3u, ins, 11u))
             return kq_fail(diag, KQ_STATUS_ALIASING_VIOLATION,
                            "linear attention outputs or scratch overlap; state_out may only be the "
                            "state itself");
@@ -386,8 +384,7 @@ kq_status kq_hip_block_join_f32(kq_hip_context *c, const kq_hip_block_join *v, u
                              {branch_gate, tokens * v->branch_count},
                              {v->post_weight, v->hidden_size},
                              {v->pre_weight, (uint64_t)v->branch_count * v->hidden_size}};
-        const void *const may[2] = {residual, NULL};
-        if (aliased(outs, 2u, ins, 6u, may))
+        if (aliased(outs, 2u, ins, 6u))
             return kq_fail(diag, KQ_STATUS_ALIASING_VIOLATION,
                            "block join outputs overlap; residual_out may only be the residual");
     }

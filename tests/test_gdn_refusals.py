@@ -173,3 +173,19 @@ def test_scratch_bytes():
     assert f(a, seqs(3, 3, 5, None)) == 0  # one row a sequence: none
     assert f(a, seqs(0)) == 0              # refused
     assert f(kq_hip.linear_attention(16, 40, 128, 128, 0.1, at(4)), seqs()) == 0
+
+
+# an output that is the input it may be, where another input lies there too: that
+# one is read by other workgroups than those that write it
+def test_second_input_at_the_output():
+    assert conv(x=at(1), state=at(1), out=at(1))[0] == "ALIASING_VIOLATION"
+    assert conv(kq_hip.causal_conv(64, 4, at(1)), state=at(1), out=at(1))[0] == "ALIASING_VIOLATION"
+    i = kq_hip.linear_attention_inputs(at(1), 128, at(10), 128, at(11), 256)
+    assert attn(i=i, state=at(1), out=at(1))[0] == "ALIASING_VIOLATION"
+    assert attn(q=seqs(slots=at(1)), state=at(1), out=at(1))[0] == "ALIASING_VIOLATION"
+    assert join(block=at(2), out=at(2))[0] == "ALIASING_VIOLATION"
+    assert join(gate=at(2), out=at(2))[0] == "ALIASING_VIOLATION"
+    assert join(branch=at(2), out=at(2))[0] == "ALIASING_VIOLATION"
+    # the other inputs may lie together
+    assert passes(join(block=at(2), gate=at(2)))
+    assert passes(join(block=at(1), gate=at(1), out=at(2)))
