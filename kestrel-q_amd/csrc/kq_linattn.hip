@@ -44,19 +44,26 @@ struct Row {
     }
 };
 
-/* 1 / n(x) for a lane's part of x, where SUM are the bits of the lanes that
- * hold the rest. Squares past the type's range are formed of x 2^-96. */
+/* x = scale x / n(x) for a lane's part of x, where SUM are the bits of the lanes
+ * that hold the rest. Where squares leave the type's range x is taken 2^-96
+ * times: 1 / n(x) itself could be a number of fewer bits. */
 template <int R, int SUM>
-__device__ __forceinline__ float inverse_norm(const float (&x)[R], float eps) {
-    float s = 0.0f;
+__device__ __forceinline__ void normalize(float (&x)[R], float eps, float scale) {
+    auto squares = [&]() {
+        float s = 0.0f;
 #pragma unroll
-    for (int i = 0; i < R; ++i) s = fmaf(x[i], x[i], s);
-    s = kq::lanes_sum<SUM>(s);
-    if (s < 3.0e38f) return kq::inverse_root(s + eps); /* the same way in every lane */
-    s = 0.0f;
+        for (int i = 0; i < R; ++i) s = fmaf(x[i], x[i], s);
+        return kq::lanes_sum<SUM>(s);
+    };
+    float s = squares();
+    float f = kq::inverse_root(s + eps);
+    if (!(s < 3.0e38f)) { /* the same way in every lane */
 #pragma unroll
-    for (int i = 0; i < R; ++i) s = fmaf(x[i] * 0x1p-96f, x[i] * 0x1p-96f, s);
-    return 0x1p-96f / sqrtf(kq::lanes_sum<SUM>(s));
+        for (int i = 0; i < R; ++i) x[i] *= 0x1p-96f;
+        f = 1.0f / sqrtf(squares());
+    }
+#pragma unroll
+    for (int i = 0; i < R; ++i) x[i] = x[i] * f * scale;
 }
 
 /* the plan, by one workgroup of NT threads */
@@ -239,13 +246,8 @@ __global__ __launch_bounds__(NT) void linattn_rows(kq_launch_linattn a, kq_launc
 #pragma unroll
             for (int i = 0; i < R; ++i) badin |= !kq_isfinite(r.q[i]) || !kq_isfinite(r.k[i]);
             if (a.normalize != 0u) { /* sums as they are could leave the type's range */
-                nq *= inverse_norm<R, SUM>(r.q, a.epsilon);
-                nk = inverse_norm<R, SUM>(r.k, a.epsilon);
-#pragma unroll
-                for (int i = 0; i < R; ++i) {
-                    r.q[i] *= nq;
-                    r.k[i] *= nk;
-                }
+                normalize<R, SUM>(r.q, a.epsilon, a.scale);
+                normalize<R, SUM>(r.k, a.epsilon, 1.0f);
                 sums();
                 nq = nk = 1.0f;
             }

@@ -87,3 +87,21 @@ def test_attention_long_memory(ctx, delta, count):  # noqa: F811
         near(got[1][0, h, :32], ws[0, h, :32])
         near(got[1][0, h, 32:], ws[0, h, 32:])
     near_parts(got[0], wy)
+
+
+def awkward_size(n):
+    m = np.linspace(2.4e38, 3.4e38, 20001).astype(np.float32)
+    want = 1.0 / (m.astype(np.float64) * np.sqrt(n))
+    off = np.abs(want.astype(np.float32).astype(np.float64) - want) / want
+    return m[np.argmax(off)], off.max()
+
+
+@pytest.mark.parametrize("rows", [1, 7, 40])
+@pytest.mark.parametrize("dk", [64, 128])
+def test_attention_largest_keys(ctx, rows, dk):  # noqa: F811
+    m, off_ = awkward_size(dk)
+    say("largest keys", rows, dk, m, off_)
+    off, spans, _ = table([rows])
+    a = Attention(63, 1, 2, dk, 64, rows, 1)
+    a.qkv[:, :2 * dk] = np.sign(a.qkv[:, :2 * dk]) * m
+    check(a, a.got(ctx, off, None, None, 1), spans, [0], [0])
