@@ -155,10 +155,10 @@ __device__ __forceinline__ void head_rows(const kq_launch_conv &c, const kq::Seq
     read_state<K, V>(hist, sp.fresh, state + at, c.channels);
     if (sp.rows != 0u)
 #pragma unroll
-        for (int j = 0; j < K - 1; ++j) {
+        for (int j = 0; j < K - 1; ++j)
             in[j] = load<V>(x + (j < (int)sp.rows ? (size_t)j * xs : 0u));
-            badin |= !finite(hist[j]);
-        }
+#pragma unroll
+    for (int j = 0; j < K - 1; ++j) badin |= !finite(hist[j]); /* passed on, without rows */
     write_state<K, V>(hist, x, xs, sp.rows, state_out + at, c.channels);
 #pragma unroll
     for (int t = 0; t < K - 1; ++t) {

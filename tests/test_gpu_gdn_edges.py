@@ -105,3 +105,11 @@ def test_attention_largest_keys(ctx, rows, dk):  # noqa: F811
     a = Attention(63, 1, 2, dk, 64, rows, 1)
     a.qkv[:, :2 * dk] = np.sign(a.qkv[:, :2 * dk]) * m
     check(a, a.got(ctx, off, None, None, 1), spans, [0], [0])
+
+
+@pytest.mark.parametrize("channels", [64, 67])
+def test_conv_empty_sequence_non_finite(ctx, channels):  # noqa: F811
+    say("conv, empty sequence", channels)
+    v = Conv(64, channels, 4, 20, 2)
+    v.state[1, 2, 33] = np.inf
+    assert v.failing(ctx, [0, 20, 20], [0, 1], None, 2) == "NUMERIC_DOMAIN"
