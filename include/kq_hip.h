@@ -830,8 +830,9 @@ kq_status kq_hip_gated_norm_f32(kq_hip_context *context, const kq_hip_gated_norm
  *             times act(gate[t]) with a gate activation
  *   r[t][b] = residual[t][b] + (residual_scale * branch_gate[t][b]) y[t]
  *   n[t][b] = rms(r[t][b]) (pre_offset + pre_weight[b])
- * for the branches b of a token (1: an ordinary residual; the gated
- * residual's branches and write gates: kq_hip_gr_write_f32). block_output and
+ * for the branches b of a token (1: an ordinary residual; the gated residual's
+ * branches and write gates, where r has kq_hip_gr_write_f32's bits with
+ * residual_scale 1 and neither post_weight nor a gate). block_output and
  * gate [tokens][hidden], residual, residual_out and normalized
  * [tokens][branches][hidden], branch_gate [tokens][branches] (NULL: ones).
  * pre_weight [branches][hidden] and normalized go together: both or neither.

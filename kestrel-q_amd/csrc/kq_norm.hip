@@ -204,7 +204,8 @@ __global__ __launch_bounds__(L) void block_join(kq_launch_join a, uint32_t per,
 #pragma unroll
                 for (int k = 0; k < V; ++k) {
                     badin |= !kq_isfinite(r[p * V + k]);
-                    r[p * V + k] = fmaf(cs, y[p * V + k], r[p * V + k]);
+                    /* a rounded product and a sum: gr_write's bits */
+                    r[p * V + k] = r[p * V + k] + cs * y[p * V + k];
                     bad |= !kq_isfinite(r[p * V + k]);
                 }
                 st<V>(a.residual_out + at + i, r + p * V);

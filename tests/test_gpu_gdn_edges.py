@@ -113,3 +113,24 @@ def test_conv_empty_sequence_non_finite(ctx, channels):  # noqa: F811
     v = Conv(64, channels, 4, 20, 2)
     v.state[1, 2, 33] = np.inf
     assert v.failing(ctx, [0, 20, 20], [0, 1], None, 2) == "NUMERIC_DOMAIN"
+
+
+# The join in the place of the gated residual's write leaves the same bits.
+@pytest.mark.parametrize("tokens", [1, 9, 600])
+@pytest.mark.parametrize("hidden", [2560, 640, 36])
+def test_join_is_gr_write(ctx, hidden, tokens):  # noqa: F811
+    say("join as gr_write", hidden, tokens)
+    g, b = Gen(65), 4
+    block, res = g.normal(tokens, hidden), g.normal(tokens, b, hidden)
+    gate = 2 * gdn64.sigmoid(g.normal(tokens, b)).astype(np.float32)
+    with Call(ctx) as c:
+        out, same, norm = (c.up(np.empty_like(res)) for _ in range(3))
+        pb, pr, pg = c.up(block), c.up(res), c.up(gate)
+        ctx.gr_write(kq_hip.gr_dims(b, hidden, 1), pr, pb, pg, tokens, same)
+        want = c.down(same, res)
+        assert np.array_equal(want, res + block[:, None] * gate[:, :, None])
+        ctx.block_join(kq_hip.block_join(b, hidden, 1e-6), tokens, pb, None, pr, pg, out)
+        assert np.array_equal(c.down(out, res), want)
+        j = kq_hip.block_join(b, hidden, 1e-6, pre=c.up(g.normal(b, hidden)), pre_offset=1.0)
+        ctx.block_join(j, tokens, pb, None, pr, pg, pr, norm)
+        assert np.array_equal(c.down(pr, res), want)
