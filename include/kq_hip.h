@@ -755,7 +755,10 @@ kq_status kq_hip_causal_conv_f32(kq_hip_context *context, const kq_hip_causal_co
  * floats between rows, up to 2^22; query, key, value, output, the states and the
  * scratch 16-byte aligned, and the strides of the four in fours.
  * Long sequences run in chunks of 64 rows on the matrix cores, single
- * rows and short sequences in the recurrent form.
+ * rows and short sequences in the recurrent form. In chunks the factors of a
+ * sum are held to 2^-22 of themselves or 2^-27 of the largest one of their
+ * column of the state (d: 2^-31 of the largest one of its column's 64 rows), and
+ * the columns of a value, like the heads, to themselves in either form.
  * Non-finite inputs and results and rates above 0 give NUMERIC_DOMAIN. */
 typedef struct kq_hip_linear_attention {
     uint32_t key_heads;

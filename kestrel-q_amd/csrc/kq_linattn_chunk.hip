@@ -581,38 +581,64 @@ __device__ __forceinline__ float largest(float m, const f4 &x) {
     return fmaxf(fmaxf(m, fmaxf(fabsf(x[0]), fabsf(x[1]))), fmaxf(fabsf(x[2]), fabsf(x[3])));
 }
 
-/* The scale of an operand that the workgroup's waves share, from one chunk
- * to the next: a power of two under which the largest value lay at 2^13 when
- * it was set. It holds while that value stays within 2^10 .. 2^15: values
- * down to 2^-13 of the largest keep 22 bits, the others an error of 2^-35 of
- * it. A wave tells of its part only whether it has values past the range,
- * values at its upper end, values at all. */
-struct Scale {
-    float s, inv;
-    __device__ __forceinline__ void set(float m) {
-        const int e = scale_exp(m) - 2;
-        s = pow2(e);
-        inv = pow2(-e);
-    }
-    __device__ __forceinline__ uint32_t tell(float m) const {
-        const float y = m * s;
-        return (__ballot(!(y < 32768.0f)) != 0ull ? 1u : 0u) |
-               (__ballot(y >= 1024.0f) != 0ull ? 2u : 0u) | (__ballot(m > 0.0f) != 0ull ? 4u : 0u);
-    }
-    static __device__ __forceinline__ bool holds(uint32_t told) {
-        return (told & 1u) == 0u && (told & 6u) != 4u;
-    }
-};
-
-__device__ __forceinline__ float top_of(const float *p) {
-    const f4 a = *(const f4 *)p;
+/* The largest values of column r16 over a wave's rows, for sets of 16 columns:
+ * row g4 of the lanes has set g4 & 1 of two, set g4 of four. Rows of lanes are
+ * exchanged between two sets, so that each step halves what is left. */
+__device__ __forceinline__ float swap_max16(float a, float b) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(a), __float_as_uint(b), false,
+                                                    false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float swap_max32(float a, float b) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(a), __float_as_uint(b), false,
+                                                    false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float tops(float m0, float m1) {
+    const float x = swap_max16(m0, m1);
+    return swap_max32(x, x);
+}
+__device__ __forceinline__ float tops(float m0, float m1, float m2, float m3) {
+    return swap_max16(swap_max32(m0, m2), swap_max32(m1, m3));
+}
+/* over the four waves that hold the rows */
+__device__ __forceinline__ float top_of(const f4 &a) {
     return fmaxf(fmaxf(a[0], a[1]), fmaxf(a[2], a[3]));
 }
 
-__device__ __forceinline__ uint32_t told_of(const uint32_t *p) {
-    const uint4 a = *(const uint4 *)p;
-    return (uint32_t)__builtin_amdgcn_readfirstlane((int)(a.x | a.y | a.z | a.w));
+/* of a power of two */
+__device__ __forceinline__ float inverse(float power) {
+    return __uint_as_float((254u << 23) - __float_as_uint(power));
 }
+
+/* The scales of an operand's columns, which all waves hold from one chunk to
+ * the next: a lane for each column, of two or four sets (`tops`). A column has
+ * its own, since what one column of v is multiplied by says nothing of its
+ * neighbours': under one scale for 32 a column 2^-k of the largest would be
+ * off by 2^(k - 35) of itself. They hold while every column's largest value
+ * lies between `low` and 2^15, or is zero. Values from 2^-2 on keep 22 bits,
+ * smaller ones an error of 2^-25: 2^-31 of the column's largest for E, whose
+ * rows are in the outputs one by one. For S and F, which are in sums over all
+ * rows, 2^-27 will do: decays that leave a chunk's last few rows move their
+ * largest values far (each time a barrier more: 64 steps of four heads 118 us
+ * with E's limits, 111 with these).
+ */
+struct Scales {
+    float s, low;
+    int back; /* from 2^14 .. 2^15 to where a largest value is set */
+    __device__ __forceinline__ Scales(bool sums)
+        : s(1.0f), low(sums ? 4.0f : 64.0f), back(sums ? 7 : 5) {}
+    /* the same in all waves */
+    __device__ __forceinline__ bool hold(float m) const {
+        const float y = m * s;
+        return __ballot(!(y < 32768.0f) || (y < low && m > 0.0f)) == 0ull;
+    }
+    __device__ __forceinline__ void set(float m) { s = pow2(scale_exp(m) - back); }
+    /* of column r16 of a set */
+    __device__ __forceinline__ float of(uint32_t set, uint32_t r16) const {
+        return __shfl(s, (int)(16u * set + r16), KQ_WAVE);
+    }
+};
 
 /*
  * Waves 0 .. 3 (the solvers) run the chain S -> E -> S': W S and E for 16 rows
@@ -638,9 +664,8 @@ __global__ __launch_bounds__(64 * scan_waves(DELTA)) void linattn_scan(kq_launch
     constexpr uint32_t kKeyImage = 256u * DK;
     __shared__ __attribute__((aligned(16))) char sbufs[2][KS * 4096], ebufs[2][8192], fbuf[8192],
         vbuf[DELTA ? 8192 : 16], ubufs[2][DELTA ? 8192 : 16]; /* V; B V in 32 bits */
-    /* what the solvers tell of S, of E and F; their largest values, of S, E, F */
-    __shared__ __attribute__((aligned(16))) uint32_t told_s[4], told_ef[4];
-    __shared__ __attribute__((aligned(16))) float top_s[4], top_e[4], top_f[4];
+    /* the columns' largest values in each solver's rows, of S; of E, then F */
+    __shared__ __attribute__((aligned(16))) float top_s[kTile][4], top_ef[2 * kTile][4];
     __shared__ float vscale[2][kTile]; /* of V's columns, by 32 rows */
     /* the chunks of one sequence that lie in the window: from the window's
      * first chunk, or the sequence's */
@@ -706,8 +731,29 @@ __global__ __launch_bounds__(64 * scan_waves(DELTA)) void linattn_scan(kq_launch
         return kq_buf(p + ((uint64_t)ch.row + n * kC) * stride + h * a.value_width,
                       (left < kC ? left : kC) * (uint32_t)stride * 4u);
     };
-    Scale ss, se, sf;
-    ss.s = ss.inv = se.s = se.inv = sf.s = sf.inv = 1.0f;
+    /* of S, of E and F; and of the lane's columns, by column tile: */
+    Scales own_s(true), own_ef(lane >= kTile);
+    float ss[2] = {1.0f, 1.0f}, se[2] = {1.0f, 1.0f}, sf[2] = {1.0f, 1.0f};
+    /* From the largest values that a phase left behind its barrier: whether the
+     * scales are set anew, which all waves find alike, so that all of them take
+     * the barrier more behind which the operand is there again. */
+    auto moved_s = [&](f4 t) {
+        const float m = top_of(t);
+        if (own_s.hold(m)) return false;
+        own_s.set(m);
+        for (uint32_t ct = 0; ct < 2u; ++ct) ss[ct] = own_s.of(ct, r16);
+        return true;
+    };
+    auto moved_ef = [&](f4 t) {
+        const float m = top_of(t);
+        if (own_ef.hold(m)) return false;
+        own_ef.set(m);
+        for (uint32_t ct = 0; ct < 2u; ++ct) {
+            se[ct] = own_ef.of(ct, r16);
+            sf[ct] = own_ef.of(2u + ct, r16);
+        }
+        return true;
+    };
 
     if (wave < 4u) {
         __builtin_amdgcn_s_setprio(3); /* the chain first */
@@ -765,17 +811,16 @@ __global__ __launch_bounds__(64 * scan_waves(DELTA)) void linattn_scan(kq_launch
 #pragma unroll
             for (int t = 0; t < NR; ++t)
 #pragma unroll
-                for (int ct = 0; ct < 2; ++ct) put(sbuf, NR * rt + t, ct, lane16, S[t][ct], ss.s);
+                for (int ct = 0; ct < 2; ++ct) put(sbuf, NR * rt + t, ct, lane16, S[t][ct], ss[ct]);
         };
-        float ms = 0.0f;
         auto share_s = [&]() {
-            ms = 0.0f;
+            float m[2] = {0.0f, 0.0f};
 #pragma unroll
             for (int t = 0; t < NR; ++t)
 #pragma unroll
-                for (int ct = 0; ct < 2; ++ct) ms = largest(ms, S[t][ct]);
-            const uint32_t told = ss.tell(ms);
-            if (lane == 0u) told_s[rt] = told;
+                for (int ct = 0; ct < 2; ++ct) m[ct] = largest(m[ct], S[t][ct]);
+            const float top = tops(m[0], m[1]);
+            if (lane < kTile) top_s[lane][rt] = top;
             put_s();
         };
         const KqBuf first = chunk(0u);
@@ -795,18 +840,22 @@ __global__ __launch_bounds__(64 * scan_waves(DELTA)) void linattn_scan(kq_launch
             /* 1: E, and F with the decay to the chunk's end */
             f4 E[2], F[2];
             zero(E);
-            if (!Scale::holds(told_of(told_s))) { /* the same in all waves */
-                const float m = kq::lanes_max<63>(ms);
-                if (lane == 0u) top_s[rt] = m;
-                kq_lds_barrier();
-                ss.set(top_of(top_s));
-                put_s();
-                kq_lds_barrier();
+            Frag<2> B[2]; /* two steps' at a time */
+            auto read_s = [&]() {
+                if (DELTA)
+#pragma unroll
+                    for (int ct = 0; ct < 2; ++ct) B[ct].read(sbuf + ct * 2048u + lane16, 4096);
+            };
+            {
+                const f4 t = *(const f4 *)top_s[lane & 31u];
+                read_s(); /* under way meanwhile */
+                if (moved_s(t)) {
+                    put_s();
+                    kq_lds_barrier();
+                    read_s();
+                }
             }
             if (DELTA) {
-                Frag<2> B[2]; /* two steps' at a time */
-#pragma unroll
-                for (int ct = 0; ct < 2; ++ct) B[ct].read(sbuf + ct * 2048u + lane16, 4096);
 #pragma unroll
                 for (int ct = 0; ct < 2; ++ct)
                     V[ct] = *(const f4 *)(ubufs[n & 1u] + (ct * 4u + rt) * 1024u + lane16);
@@ -825,24 +874,22 @@ __global__ __launch_bounds__(64 * scan_waves(DELTA)) void linattn_scan(kq_launch
                     __builtin_amdgcn_sched_barrier(0);
                 }
             }
-            const float is = ss.inv * iw;
+            const float is[2] = {inverse(ss[0]) * iw, inverse(ss[1]) * iw};
 #pragma unroll
             for (int ct = 0; ct < 2; ++ct)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     if (!DELTA) badin |= !kq_isfinite(V[ct][r]);
-                    E[ct][r] = DELTA ? fmaf(-is, E[ct][r], V[ct][r]) : f0[r] * V[ct][r];
+                    E[ct][r] = DELTA ? fmaf(-is[ct], E[ct][r], V[ct][r]) : f0[r] * V[ct][r];
                     F[ct][r] = E[ct][r] * f1[r];
                 }
-            const float me = largest(largest(0.0f, E[0]), E[1]);
-            const float mf = largest(largest(0.0f, F[0]), F[1]);
-            const uint32_t told = se.tell(me) | sf.tell(mf) << 8;
-            if (lane == 0u) told_ef[rt] = told;
+            top_ef[lane][rt] = tops(largest(0.0f, E[0]), largest(0.0f, E[1]), largest(0.0f, F[0]),
+                                    largest(0.0f, F[1]));
             auto put_ef = [&]() {
 #pragma unroll
                 for (int ct = 0; ct < 2; ++ct) {
-                    put(fbuf, rt, ct, lane16, F[ct], sf.s);
-                    put(ebuf, rt, ct, lane16, E[ct], se.s);
+                    put(fbuf, rt, ct, lane16, F[ct], sf[ct]);
+                    put(ebuf, rt, ct, lane16, E[ct], se[ct]);
                 }
             };
             put_ef();
@@ -850,22 +897,18 @@ __global__ __launch_bounds__(64 * scan_waves(DELTA)) void linattn_scan(kq_launch
             /* 2: S' = e^G S + K'^T F, e^G in two parts (kq::Decay) */
             f4 x[NR][2];
             {
-                const uint32_t all = told_of(told_ef);
-                if (!Scale::holds(all) || !Scale::holds(all >> 8)) {
-                    const float m0 = kq::lanes_max<63>(me), m1 = kq::lanes_max<63>(mf);
-                    if (lane == 0u) {
-                        top_e[rt] = m0;
-                        top_f[rt] = m1;
-                    }
-                    kq_lds_barrier();
-                    se.set(top_of(top_e));
-                    sf.set(top_of(top_f));
+                Frag<2> B[2];
+                auto read_f = [&]() {
+#pragma unroll
+                    for (int ct = 0; ct < 2; ++ct) B[ct].read(fbuf + ct * 2048u + lane16, 4096);
+                };
+                const f4 t = *(const f4 *)top_ef[lane];
+                read_f();
+                if (moved_ef(t)) {
                     put_ef();
                     kq_lds_barrier();
+                    read_f();
                 }
-                Frag<2> B[2];
-#pragma unroll
-                for (int ct = 0; ct < 2; ++ct) B[ct].read(fbuf + ct * 2048u + lane16, 4096);
                 __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                 for (int t = 0; t < NR; ++t) zero(x[t]);
@@ -889,14 +932,14 @@ __global__ __launch_bounds__(64 * scan_waves(DELTA)) void linattn_scan(kq_launch
                 }
             }
             load_v(next, more);
-            const float jf = sf.inv * (1.0f / kUnit);
+            const float jf[2] = {inverse(sf[0]) * (1.0f / kUnit), inverse(sf[1]) * (1.0f / kUnit)};
 #pragma unroll
             for (int t = 0; t < NR; ++t)
 #pragma unroll
                 for (int ct = 0; ct < 2; ++ct)
 #pragma unroll
                     for (int r = 0; r < 4; ++r)
-                        S[t][ct][r] = fmaf(x[t][ct][r], jf, S[t][ct][r]);
+                        S[t][ct][r] = fmaf(x[t][ct][r], jf[ct], S[t][ct][r]);
             load_decay(next);
             sbuf = sbufs[(n + 1u) & 1u];
             share_s();
@@ -920,7 +963,7 @@ __global__ __launch_bounds__(64 * scan_waves(DELTA)) void linattn_scan(kq_launch
 #pragma unroll
         for (int r = 0; r < 4; ++r) io[r] = ((fr + r) * (uint32_t)a.ys + col) * 4u;
         f4 P[2];
-        float ps = 0.0f;
+        float ps[2] = {0.0f, 0.0f};
         zero(P);
         /* M E and the output of chunk n; the operands of chunk n + 1 */
         auto write = [&](uint32_t n, KqBuf next) {
@@ -939,13 +982,14 @@ __global__ __launch_bounds__(64 * scan_waves(DELTA)) void linattn_scan(kq_launch
                 load_lower(M, next, vat, ks);
                 __builtin_amdgcn_sched_barrier(0);
             }
-            const float pe = se.inv * (1.0f / kMixUnit);
+            const float pe[2] = {inverse(se[0]) * (1.0f / kMixUnit),
+                                 inverse(se[1]) * (1.0f / kMixUnit)};
             const KqBuf y = rows_at(a.y, a.ys, n);
 #pragma unroll
             for (int ct = 0; ct < 2; ++ct)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    const float o = fmaf(f1[r], P[ct][r] * ps, f0[r] * (O[ct][r] * pe));
+                    const float o = fmaf(f1[r], P[ct][r] * ps[ct], f0[r] * (O[ct][r] * pe[ct]));
                     bad |= !kq_isfinite(o);
                     __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(o), y.r, (int)io[r],
                                                           64 * ct, 0);
@@ -967,22 +1011,12 @@ __global__ __launch_bounds__(64 * scan_waves(DELTA)) void linattn_scan(kq_launch
         }
         auto check_s = [&]() {
             kq_lds_barrier();
-            if (!Scale::holds(told_of(told_s))) {
-                kq_lds_barrier();
-                ss.set(top_of(top_s));
-                kq_lds_barrier();
-            }
+            if (moved_s(*(const f4 *)top_s[lane & 31u])) kq_lds_barrier();
         };
         /* 2: Q S */
         auto second = [&](uint32_t n) {
             kq_lds_barrier();
-            const uint32_t all = told_of(told_ef);
-            if (!Scale::holds(all) || !Scale::holds(all >> 8)) {
-                kq_lds_barrier();
-                se.set(top_of(top_e));
-                sf.set(top_of(top_f));
-                kq_lds_barrier();
-            }
+            if (moved_ef(*(const f4 *)top_ef[lane])) kq_lds_barrier();
             const KqBuf next = chunk(n < last ? n + 1u : n);
             const char *sb = sbufs[n & 1u] + lane16;
             Frag<2> B[2];
@@ -1002,7 +1036,7 @@ __global__ __launch_bounds__(64 * scan_waves(DELTA)) void linattn_scan(kq_launch
                 Q.load1(next, lane16, kat + rt * KS * 2048u, ks);
                 __builtin_amdgcn_sched_barrier(0);
             }
-            ps = ss.inv * (1.0f / kUnit);
+            for (int ct = 0; ct < 2; ++ct) ps[ct] = inverse(ss[ct]) * (1.0f / kUnit);
         };
         check_s();
         second(0u);
@@ -1090,18 +1124,11 @@ __global__ __launch_bounds__(64 * scan_waves(DELTA)) void linattn_scan(kq_launch
         /* chunk n, with the registers of B of chunk n + 1 and of V of chunk n + 2 */
         auto body = [&](int ib1, int iv, uint32_t n) {
             kq_lds_barrier();
-            if (!Scale::holds(told_of(told_s))) {
-                kq_lds_barrier();
-                kq_lds_barrier();
-            }
+            if (moved_s(*(const f4 *)top_s[lane & 31u])) kq_lds_barrier();
             /* 1 (behind the last chunk, B V of it again) */
             times_v(ib1, n + 1u);
             kq_lds_barrier();
-            const uint32_t all = told_of(told_ef);
-            if (!Scale::holds(all) || !Scale::holds(all >> 8)) {
-                kq_lds_barrier();
-                kq_lds_barrier();
-            }
+            if (moved_ef(*(const f4 *)top_ef[lane])) kq_lds_barrier();
             /* 2 */
             put_v(v[iv]);
             load_v(v[iv], n + 4u);
@@ -1176,7 +1203,7 @@ __global__ __launch_bounds__(256) void linattn_sums(kq_launch_linattn a, Work w,
                                                     uint32_t base, uint32_t *status) {
     constexpr int NR = DK / 64;
     __shared__ __attribute__((aligned(16))) char fbuf[8192];
-    __shared__ __attribute__((aligned(16))) float top[4];
+    __shared__ __attribute__((aligned(16))) float top[kTile][4]; /* of each wave's rows */
     const uint32_t lane = threadIdx.x & 63u, lane16 = lane * 16u;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const Place p(a, w, base, wave, lane);
@@ -1196,13 +1223,15 @@ __global__ __launch_bounds__(256) void linattn_sums(kq_launch_linattn a, Work w,
             badin |= !kq_isfinite(V[ct][r]);
             V[ct][r] = f0[r] * V[ct][r] * f1[r];
         }
-    const float m = kq::lanes_max<63>(largest(largest(0.0f, V[0]), V[1]));
-    if (lane == 0u) top[wave] = m;
+    const float m = tops(largest(0.0f, V[0]), largest(0.0f, V[1]));
+    if (lane < kTile) top[lane][wave] = m;
     kq_lds_barrier();
-    Scale s;
-    s.set(top_of(top));
+    float s[2]; /* of the lane's columns */
 #pragma unroll
-    for (int ct = 0; ct < 2; ++ct) put(fbuf, wave, ct, lane16, V[ct], s.s);
+    for (int ct = 0; ct < 2; ++ct) {
+        s[ct] = pow2(scale_exp(top_of(*(const f4 *)top[16 * ct + (lane & 15u)])));
+        put(fbuf, wave, ct, lane16, V[ct], s[ct]);
+    }
     kq_lds_barrier();
     float *u = (float *)(p.data + p.uat) +
                (16u * NR * wave + 4u * (lane >> 4)) * a.value_width + p.col;
@@ -1219,7 +1248,7 @@ __global__ __launch_bounds__(256) void linattn_sums(kq_launch_linattn a, Work w,
 #pragma unroll
             for (int r = 0; r < 4; ++r)
                 u[(uint32_t)(16 * t + r) * a.value_width + 16u * ct] =
-                    x[r] * (s.inv * (1.0f / kUnit));
+                    x[r] * (inverse(s[ct]) * (1.0f / kUnit));
         }
     }
     if (badin) kq_flag(status, KQ_DEV_INPUT);
@@ -1280,7 +1309,7 @@ __global__ __launch_bounds__(256) void linattn_outs(kq_launch_linattn a, Work w,
                                                     uint32_t base, uint32_t *status) {
     constexpr int KS = DK / 32, NR = DK / 64;
     __shared__ __attribute__((aligned(16))) char sbuf[KS * 4096], ebuf[8192];
-    __shared__ __attribute__((aligned(16))) float top_s[4], top_e[4];
+    __shared__ __attribute__((aligned(16))) float top[2 * kTile][4]; /* of S, then E */
     const uint32_t lane = threadIdx.x & 63u, lane16 = lane * 16u;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const Place p(a, w, base, wave, lane);
@@ -1301,36 +1330,33 @@ __global__ __launch_bounds__(256) void linattn_outs(kq_launch_linattn a, Work w,
     Frag<2> M;
     Q.load(p.buf, lane16, p.kat + wave * KS * 2048u);
     M.load(p.buf, lane16, p.vat + piece(wave, 0u)); /* rows 0 .. 31 have one piece */
-    float ms = 0.0f;
-#pragma unroll
-    for (int t = 0; t < NR; ++t) ms = largest(largest(ms, S[t][0]), S[t][1]);
-    ms = kq::lanes_max<63>(ms);
-#pragma unroll
-    for (int ct = 0; ct < 2; ++ct)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) V[ct][r] *= f0[r];
-    const float me = kq::lanes_max<63>(largest(largest(0.0f, V[0]), V[1]));
-    if (lane == 0u) {
-        top_s[wave] = ms;
-        top_e[wave] = me;
-    }
-    kq_lds_barrier();
-    Scale ss, se;
-    ss.set(top_of(top_s));
-    se.set(top_of(top_e));
+    float ms[2] = {0.0f, 0.0f}, me[2];
 #pragma unroll
     for (int ct = 0; ct < 2; ++ct) {
 #pragma unroll
-        for (int t = 0; t < NR; ++t) put(sbuf, NR * wave + t, ct, lane16, S[t][ct], ss.s);
-        put(ebuf, wave, ct, lane16, V[ct], se.s);
+        for (int t = 0; t < NR; ++t) ms[ct] = largest(ms[ct], S[t][ct]);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) V[ct][r] *= f0[r];
+        me[ct] = largest(0.0f, V[ct]);
+    }
+    top[lane][wave] = tops(ms[0], ms[1], me[0], me[1]);
+    kq_lds_barrier();
+    float ss[2], se[2]; /* of the lane's columns */
+#pragma unroll
+    for (int ct = 0; ct < 2; ++ct) {
+        ss[ct] = pow2(scale_exp(top_of(*(const f4 *)top[16 * ct + (lane & 15u)])));
+        se[ct] = pow2(scale_exp(top_of(*(const f4 *)top[kTile + 16 * ct + (lane & 15u)])));
+#pragma unroll
+        for (int t = 0; t < NR; ++t) put(sbuf, NR * wave + t, ct, lane16, S[t][ct], ss[ct]);
+        put(ebuf, wave, ct, lane16, V[ct], se[ct]);
     }
     kq_lds_barrier();
-    const float ps = ss.inv * (1.0f / kUnit), pe = se.inv * (1.0f / kMixUnit);
     const KqBuf y = p.rows(a.y, a.ys, a.value_width);
     bool bad = false;
 #pragma unroll
     for (int ct = 0; ct < 2; ++ct) {
         f4 P = f4{0.0f, 0.0f, 0.0f, 0.0f}, O = P;
+        const float ps = inverse(ss[ct]) * (1.0f / kUnit), pe = inverse(se[ct]) * (1.0f / kMixUnit);
         Frag<KS> B;
         B.read(sbuf + ct * 2048u + lane16, 4096);
         Frag<2> E;

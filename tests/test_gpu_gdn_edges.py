@@ -134,3 +134,78 @@ def test_join_is_gr_write(ctx, hidden, tokens):  # noqa: F811
         j = kq_hip.block_join(b, hidden, 1e-6, pre=c.up(g.normal(b, hidden)), pre_offset=1.0)
         ctx.block_join(j, tokens, pb, None, pr, pg, pr, norm)
         assert np.array_equal(c.down(pr, res), want)
+
+
+def terms(a, b, rows, slot):
+    """Of outputs q.S of a sequence from row b on, the 2-norms of the terms q_i S_i: what
+    an output's error is a fraction of. Its own size is about that, but for cancellation,
+    which leaves one output in ten at a tenth; a norm over few rows shows that."""
+    hk, hv, dk, dv = a.dims
+    q = a.parts()[0].astype(np.float64)
+    q = q / np.sqrt((q * q).sum(-1, keepdims=True) + a.eps) * float(a.scale)
+    out = []
+    for t in rows:
+        S = a.want([(b, t + 1)], [slot], [0])[1][slot]
+        out.append(np.sqrt((q[t].repeat(hv // hk, 0)[:, :, None] ** 2 * S * S).sum(1)))
+    return np.array(out)
+
+
+# Columns of v have nothing to do with each other: each keeps its own bits, however
+# small beside its neighbours (factors of 2^-spread .. 1), and from chunk to chunk
+# as they grow and fall.
+@pytest.mark.parametrize("spread", [8, 24, 60])
+@pytest.mark.parametrize("lengths", [[17], [150], [70, 12, 130]], ids=str)
+@pytest.mark.parametrize("heads,delta", [((2, 4, 128, 64), True), ((1, 2, 64, 64), True),
+                                         ((2, 4, 128, 64), False), ((1, 9, 128, 128), False)],
+                         ids=str)
+def test_attention_columns(ctx, spread, lengths, heads, delta):  # noqa: F811
+    say("columns", spread, lengths, heads, delta)
+    off, spans, rows = table(lengths)
+    n, (hk, hv, dk, dv) = len(lengths), heads
+    g = Gen(67)
+    a = Attention(66, *heads, rows, n, delta=delta)
+    f = np.float32(2.0) ** -np.round(g.uniform(0, spread, hv, dv))
+    # and each chunk's values by up to 2^6 either way, a column by itself
+    wave = np.float32(2.0) ** np.round(g.uniform(-6, 6, rows // 64 + 1, hv, dv))
+    a.qkv[:, 2 * hk * dk:a.width] *= (f * np.repeat(wave, 64, 0)[:rows]).reshape(rows, -1)
+    a.state *= f[None, :, None, :]
+    got = a.got(ctx, off, None, None, n)
+    wy, ws = a.want(spans, list(range(n)), [0] * n)
+    for s, (b, e) in enumerate(spans):
+        for x in range(b, e, 64):  # 64 rows at a time, and the state
+            x = slice(x, min(x + 64, e))
+            size = np.linalg.norm(wy[x], axis=0)
+            if x.stop - x.start < 16:
+                t = terms(a, b, range(x.start, x.stop), s)
+                size = np.maximum(size, np.linalg.norm(t, axis=0))
+            err = np.linalg.norm(got[0][x] - wy[x], axis=0) / size
+            assert err.max() <= 2e-6, (s, x, err.max())
+        err = np.linalg.norm(got[1][s] - ws[s], axis=1) / np.linalg.norm(ws[s], axis=1)
+        say("   worst column of the state", err.max())
+        assert err.max() <= 2e-6, (s, err.max())
+
+
+# Rows of one column share a scale in their chunk, under which a value's error is
+# 2^-22 of it or 2^-31 of the column's largest: rows 2^k below those behind them.
+@pytest.mark.parametrize("k", [10, 20, 30])
+@pytest.mark.parametrize("heads,delta", [((2, 4, 128, 64), True), ((1, 2, 64, 64), True),
+                                         ((2, 4, 128, 64), False), ((1, 9, 128, 128), False)],
+                         ids=str)
+def test_attention_rows_before_large_ones(ctx, k, heads, delta):  # noqa: F811
+    say("before large rows", k, heads, delta)
+    off, spans, rows = table([160])
+    hk, hv, dk, dv = heads
+    a = Attention(68, *heads, rows, 1, delta=delta)
+    v = a.qkv[:, 2 * hk * dk:a.width]
+    v[100:] *= np.float32(2.0 ** k)
+    got = a.got(ctx, off, None, None, 1)
+    wy, ws = a.want(spans, [0], [0])
+    near(got[0][:64], wy[:64])
+    near(got[0][100:], wy[100:])
+    near(got[1], ws)
+    # |d| is at most twice |v| and what the state gives; a row takes up to 64 of them
+    # times |q.k| <= dk^-1/2
+    floor = 64 * dk ** -0.5 * 2.0 ** -31 * 4 * np.abs(v).max()
+    y = wy[64:100]
+    bar = 3e-5 * np.maximum(np.abs(y), np.sqrt((y * y).mean())) + floor
+    assert (np.abs(got[0][64:100] - y) <= bar).all()
