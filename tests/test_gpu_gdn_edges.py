@@ -209,3 +209,47 @@ def test_attention_rows_before_large_ones(ctx, k, heads, delta):  # noqa: F811
     y = wy[64:100]
     bar = 3e-5 * np.maximum(np.abs(y), np.sqrt((y * y).mean())) + floor
     assert (np.abs(got[0][64:100] - y) <= bar).all()
+
+
+# The heads, and 64 rows at a time, by themselves where they differ most in size.
+@pytest.mark.parametrize("rows", [16, 17, 200])
+@pytest.mark.parametrize("what", ["decays", "values", "keys", "no decay"])
+@pytest.mark.parametrize("delta", [True, False])
+def test_attention_parts_of_different_size(ctx, what, rows, delta):  # noqa: F811
+    say("parts", what, rows, delta)
+    off, spans, _ = table([rows])
+    hk, hv, dk, dv = heads = (2, 4, 128, 64)
+    a = Attention(69, *heads, rows, 1, delta=delta, normalize=what != "keys")
+    qk = 2 * hk * dk
+    if what == "decays":  # a head forgets at once, another hardly
+        a.rate[:] = [-1e30, -200.0, -1.0, -1e-6]
+    elif what == "values":  # heads 2^60 apart, their states with them
+        f = np.float32(2.0) ** np.array([0, -20, 20, 40], np.float32)
+        a.qkv[:, qk:a.width] *= np.repeat(f, dv)
+        a.state *= f[None, :, None, None]
+    elif what == "keys":  # rows of q, k and v of very different sizes, not normalized
+        f = np.float32(10.0) ** Gen(70).uniform(-3, 0, rows, 1)
+        a.qkv[:, :hk * dk] *= f
+        a.qkv[:, hk * dk:qk] *= f[::-1]
+        a.qkv[:, qk:a.width] *= f[::-1] ** -1
+    else:
+        a.rate[:] = 0.0
+    got = a.got(ctx, off, None, None, 1)
+    wy, ws = a.want(spans, [0], [0])
+    near_parts(got[0], wy)
+    for h in range(hv):
+        near(got[1][0, h], ws[0, h])
+
+
+# Rows and states of sequences taken out of a call of single rows are nobody's
+def test_single_rows_taken_out(ctx):  # noqa: F811
+    say("single rows taken out")
+    slots = [2, NO, 0, NO, 4, 1]
+    spans = [(i, i + 1) for i in range(6)]
+    a = Attention(71, 2, 6, 128, 128, 6, 5)
+    v = Conv(72, 260, 4, 6, 5, bias=True)
+    for t in (1, 3):
+        a.qkv[t], a.alpha[t], a.beta[t], v.x[t] = np.nan, np.inf, np.nan, np.nan
+    a.state[3], v.state[3] = np.nan, np.nan
+    check(a, a.got(ctx, None, slots, None, 6), spans, slots, [0] * 6)
+    v.check(v.got(ctx, None, slots, None, 6), spans, slots, [0] * 6)
