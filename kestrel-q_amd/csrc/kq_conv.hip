@@ -8,9 +8,10 @@
  * holds V neighbouring channels and walks a block of rows with the last K-1
  * inputs in registers, so that each input is read once (plus K-1 rows at a
  * walk's start, from a cache). Bound by memory: 2 K operations and a sigmoid
- * for a value of 8 bytes moved. 4097 rows of 10,240 channels take 67 us, 5.0
- * TB/s, what a large copy reaches; walks of 32 or 64 rows 72 us (fewer loads
- * under way). One row a sequence, 32 x 10,240: 4.4 us, mostly the launch.
+ * for a value of 8 bytes moved. 4097 rows of 10,240 channels take 66 us, 5.1
+ * TB/s, what a large copy reaches; walks of 32 rows 5 us more, of 64 rows 9
+ * (fewer loads under way). One row a sequence, 32 x 10,240: 4.4 us, mostly the
+ * launch.
  *
  * A state may be written in place. Everything that reads it is therefore
  * done by the workgroup that also writes it: those of a sequence take its
@@ -58,7 +59,7 @@ __device__ __forceinline__ void store(float *p, const Vec<V> &r) {
 }
 
 /* the next launch reads these rows, from other XCDs' caches as a rule: not
- * kept in this one's (68 against 71 us in walks of 32 rows) */
+ * kept in this one's (for 4097 rows of 10,240 channels 7 us less) */
 template <int V>
 __device__ __forceinline__ void store_nt(float *p, const Vec<V> &r) {
     if constexpr (V == 4)

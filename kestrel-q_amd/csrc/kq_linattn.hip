@@ -303,7 +303,10 @@ hipError_t launch(const kq_launch_linattn &a, const kq_launch_seqs &q, uint32_t 
  * and, for the fewest, one wave a workgroup, so that they spread over the
  * device. 48 heads of 128 x 128, in us, with 16 columns and one wave, 16 and
  * four, 32 and four: one sequence 5.4, 5.6, 6.7; two 7.3, 6.1, 7.0; four 9.5,
- * 8.1, 9.0; six 12.5, 10.1, 11.5; eight 14.0, 12.4, 12.0; 32 55, 48, 39. */
+ * 8.1, 9.0; six 12.5, 10.1, 11.5; eight 14.0, 12.4, 12.0; 32 55, 48, 39.
+ * With a plan 32 columns always, since what takes long there are many rows:
+ * 16 and 32 columns for 32 sequences of one row 41 and 36, 61 of one 92 and 79,
+ * 32 of four 46 and 41, but two of 16 rows 26 and 32. */
 template <int DK>
 hipError_t launch(const kq_launch_linattn &a, const kq_launch_seqs &q, uint32_t max_rows,
                   const kq_linattn_plan &plan, uint32_t *status, hipStream_t s) {
@@ -323,8 +326,13 @@ hipError_t kq_linattn_recurrent(const kq_launch_linattn &a, const kq_launch_seqs
                                : launch<64>(a, q, max_rows, plan, status, s);
 }
 
-/* sequences up to this long (64: a lane for each row) run in the recurrent form: 1.2
- * us a row, against 26 to 35 us for a chunk's launches */
+/* Sequences up to this long (64: a lane for each row) run in the recurrent form:
+ * 1.2 us a row, against a chunk's launches. In the recurrent form and in chunks,
+ * in us, 48 heads of 128 x 128: one sequence of 17 rows 24 and 24, of 24 32 and 25;
+ * eight of 17 48 and 61, of 24 63 and 62, of 32 82 and 62; 32 of 17 120 and 209, of
+ * 24 163 and 212, of 32 223 and 215. So 16 is the limit of one sequence; many
+ * would gain from twice that, which a call's counts alone, with the lengths on
+ * the device, do not tell. */
 constexpr uint32_t kShort = 16u;
 
 extern "C" uint64_t kq_launch_linattn_scratch(const kq_launch_linattn *a, uint64_t tokens,

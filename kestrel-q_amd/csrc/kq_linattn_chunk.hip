@@ -35,20 +35,21 @@
  *
  * Operands are two fp16 numbers hi + lo (22 bits) in three products
  * hi hi + hi lo + lo hi with binary32 sums: off by at most 2^-22 of a
- * product, 5 times the rate of binary32 products on these cores. The ranges
- * that fp16 lacks are kept outside: a row of k or q is scaled by a power of
- * two to below 1 and its norm becomes a factor of the row; T, W, V, E and S
- * carry powers of two. Log decays are summed in 64 bits, since their
- * differences are what counts.
+ * product, 2.5 times the rate of binary32 products (8192^3 in the vendor
+ * library: 1134 TFLOP/s in 16 bits, a third of which is 378, against 154 in 32).
+ * The ranges that fp16 lacks are kept outside: a row of k or q is scaled by a
+ * power of two to below 1 and its norm becomes a factor of the row; T and W
+ * carry a power of two, V, E, F and S one for each column. Log decays are summed
+ * in 64 bits, since their differences are what counts.
  *
- * 16,384 rows of one sequence, 16 key and 48 value heads of 128 x 128: 860 us,
+ * 16,384 rows of one sequence, 16 key and 48 value heads of 128 x 128: 852 us,
  * 105 TFLOP/s of the recurrent form's operations, which at 1.2 us a row would
  * take 20 ms for them. 690 us are the scan's, whose 256 steps hang on each
  * other: 2.6 us a step, two LDS round trips through a barrier with 24 matrix
  * instructions a wave behind each (2.07 us with a third of the heads: the L2s
  * give a workgroup 120 KB a step). 265 are linattn_prep's, bound by the bytes
  * it writes. (Launches overlap; U = B V formed there as well made its writes,
- * not the scan, the bound.) 513 rows: 43 us.
+ * not the scan, the bound.) 513 rows: 43.7 us.
  */
 #include <type_traits>
 

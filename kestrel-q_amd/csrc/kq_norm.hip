@@ -100,45 +100,45 @@ __global__ __launch_bounds__(L <= 64 ? 256 : L) void gated_norm(kq_launch_norm a
     bool badin = false, bad = false;
     for (uint64_t row = (uint64_t)blockIdx.x * kRows + (L <= 64 ? threadIdx.x / L : 0u);
          row < rows; row += (uint64_t)gridDim.x * kRows) { /* the threads of a row together */
-    const uint64_t t = row / a.groups;
-    const uint32_t g = (uint32_t)(row - t * a.groups);
-    const size_t at = (size_t)g * a.width;
-    const float *xr = x + (size_t)t * xs + at;
-    const float *gr = gate + (a.gate != kNone ? (size_t)t * gs + at : 0u);
-    const float *w = a.weight != nullptr ? a.weight + (a.per_group != 0u ? at : 0u) : nullptr;
-    float *yr = y + (size_t)t * ys + at;
-    float v[P * V], m[P * V], gv[P * V];
+        const uint64_t t = row / a.groups;
+        const uint32_t g = (uint32_t)(row - t * a.groups);
+        const size_t at = (size_t)g * a.width;
+        const float *xr = x + (size_t)t * xs + at;
+        const float *gr = gate + (a.gate != kNone ? (size_t)t * gs + at : 0u);
+        const float *w = a.weight != nullptr ? a.weight + (a.per_group != 0u ? at : 0u) : nullptr;
+        float *yr = y + (size_t)t * ys + at;
+        float v[P * V], m[P * V], gv[P * V];
 #pragma unroll
-    for (int p = 0; p < P; ++p) {
-        const uint32_t i = (l + p * L) * V;
+        for (int p = 0; p < P; ++p) {
+            const uint32_t i = (l + p * L) * V;
 #pragma unroll
-        for (int k = 0; k < V; ++k) v[p * V + k] = 0.0f, m[p * V + k] = 0.0f, gv[p * V + k] = 0.0f;
-        if (i < a.width) {
-            ld<V>(xr + i, v + p * V);
-            if (a.gate != kNone) ld<V>(gr + i, gv + p * V);
-            if (w != nullptr) ld<V>(w + i, m + p * V);
-        }
-    }
-#pragma unroll
-    for (int k = 0; k < P * V; ++k) 
-        badin |= !(kq_isfinite(v[k]) && kq_isfinite(m[k]) && kq_isfinite(gv[k]));
-    const float inv = row_inverse<L>(v, a.width, a.epsilon, red);
-#pragma unroll
-    for (int p = 0; p < P; ++p) {
-        const uint32_t i = (l + p * L) * V;
-        if (i < a.width) {
-            float o[V];
-#pragma unroll
-            for (int k = 0; k < V; ++k) {
-                const int j = p * V + k;
-                o[k] = v[j] * inv;
-                if (w != nullptr) o[k] *= a.offset + m[j];
-                if (a.gate != kNone) o[k] *= act(a.gate, gv[j]);
-                bad |= !kq_isfinite(o[k]);
+            for (int k = 0; k < V; ++k) v[p * V + k] = 0.0f, m[p * V + k] = 0.0f, gv[p * V + k] = 0.0f;
+            if (i < a.width) {
+                ld<V>(xr + i, v + p * V);
+                if (a.gate != kNone) ld<V>(gr + i, gv + p * V);
+                if (w != nullptr) ld<V>(w + i, m + p * V);
             }
-            st<V>(yr + i, o);
         }
-    }
+#pragma unroll
+        for (int k = 0; k < P * V; ++k)
+            badin |= !(kq_isfinite(v[k]) && kq_isfinite(m[k]) && kq_isfinite(gv[k]));
+        const float inv = row_inverse<L>(v, a.width, a.epsilon, red);
+#pragma unroll
+        for (int p = 0; p < P; ++p) {
+            const uint32_t i = (l + p * L) * V;
+            if (i < a.width) {
+                float o[V];
+#pragma unroll
+                for (int k = 0; k < V; ++k) {
+                    const int j = p * V + k;
+                    o[k] = v[j] * inv;
+                    if (w != nullptr) o[k] *= a.offset + m[j];
+                    if (a.gate != kNone) o[k] *= act(a.gate, gv[j]);
+                    bad |= !kq_isfinite(o[k]);
+                }
+                st<V>(yr + i, o);
+            }
+        }
     }
     if (badin) kq_flag(status, KQ_DEV_INPUT);
     if (bad) kq_flag(status, KQ_DEV_NUMERIC);
@@ -281,7 +281,11 @@ extern "C" hipError_t kq_launch_block_join(const kq_launch_join *a, uint64_t tok
     const bool v4 = h % 4u == 0u && by16(a->block) && by16(a->post) &&
                     (a->gate_kind == kNone || by16(a->gate)) && by16(a->residual) &&
                     by16(a->residual_out) && by16(a->pre) && by16(a->normalized);
-    /* few tokens: a workgroup for each branch */
+    /* Few tokens: a workgroup for each branch, which forms the block's norm for
+     * itself. 4 branches of 2560 with both norms and a gate, a workgroup a
+     * branch and one for all of them: 64 tokens 5.6 and 9.8 us, 256 9.8 and 13.5,
+     * 384 14.0 and 15.4, 500 18.0 and 15.9, 512 17.1 and 16.0, 1024 41.6 and
+     * 33.2. */
     const uint32_t per = tokens >= 512u ? a->branches : 1u;
     const dim3 grid((uint32_t)tokens, (a->branches + per - 1u) / per);
 #define KQ_JOIN(L, V, P)                                                                         \
@@ -291,6 +295,8 @@ extern "C" hipError_t kq_launch_block_join(const kq_launch_join *a, uint64_t tok
         return hipGetLastError();                                                                \
     } while (0)
     if (v4) {
+        /* 2499 tokens of 4 branches, 256 and 320 threads: 1536 values 56 and 67 us,
+         * 2048 65 and 72, 2304 80.5 and 77.9, 2560 87.5 and 83.6 */
         if (h <= 1024u) KQ_JOIN(256, 4, 1);
         if (h <= 2048u) KQ_JOIN(256, 4, 2);
         if (h <= 2560u) KQ_JOIN(320, 4, 2);
