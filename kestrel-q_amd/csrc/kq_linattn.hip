@@ -238,8 +238,11 @@ __global__ __launch_bounds__(NT) void linattn_rows(kq_launch_linattn a, kq_launc
         };
         sums();
         float nq = a.scale, nk = 1.0f;
-        /* the same way in every lane */
-        if (a.normalize != 0u && q2 > 1e-24f && q2 < 1e12f && k2 > 1e-24f && k2 < 1e12f) {
+        /* sums with S may leave the range before their norm divides them */
+        const float most = ((fabsf(sk[0]) + fabsf(sk[1])) + (fabsf(sk[2]) + fabsf(sk[3]))) +
+                           ((fabsf(sq[0]) + fabsf(sq[1])) + (fabsf(sq[2]) + fabsf(sq[3])));
+        const bool fits = most < 3.0e38f && q2 > 1e-24f && q2 < 1e12f && k2 > 1e-24f && k2 < 1e12f;
+        if (a.normalize != 0u && __ballot(!fits) == 0ull) { /* the same way in every lane */
             nq *= kq::inverse_root(q2 + a.epsilon);
             nk = kq::inverse_root(k2 + a.epsilon);
         } else {

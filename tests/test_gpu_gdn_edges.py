@@ -253,3 +253,17 @@ def test_single_rows_taken_out(ctx):  # noqa: F811
     a.state[3], v.state[3] = np.nan, np.nan
     check(a, a.got(ctx, None, slots, None, 6), spans, slots, [0] * 6)
     v.check(v.got(ctx, None, slots, None, 6), spans, slots, [0] * 6)
+
+
+# States and values near the type's largest: what leaves the range is a sum with
+# rows of q and k that are not yet divided by their norm, not the result.
+@pytest.mark.parametrize("rows", [1, 12, 40])
+@pytest.mark.parametrize("delta", [True, False])
+def test_attention_largest_states(ctx, rows, delta):  # noqa: F811
+    say("largest states", rows, delta)
+    off, spans, _ = table([rows])
+    a = Attention(73, 2, 4, 128, 64, rows, 1, delta=delta)
+    a.qkv[:, :2 * 2 * 128] *= np.float32(30.0)
+    a.qkv[:, 2 * 2 * 128:a.width] *= np.float32(1e36)
+    a.state *= np.float32(3e37)
+    check(a, a.got(ctx, None if rows == 1 else off, None, None, 1), spans, [0], [0])
