@@ -9,8 +9,8 @@ import pytest
 
 import gdn64
 import kq_hip
-from test_gpu_gdn import (NO, SENTINEL, U, Attention, Call, Conv, Gen, check, ctx,  # noqa: F401
-                          failing, near, say, table)
+from test_gpu_gdn import (NO, Attention, Call, Conv, Gen, check, ctx, near, say,  # noqa: F401
+                          table)
 
 pytestmark = pytest.mark.gpu
 
