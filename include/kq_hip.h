@@ -800,6 +800,164 @@ kq_status kq_hip_linear_attention_f32(kq_hip_context *context,
                                       kq_diagnostic *diagnostic);
 
 /* ------------------------------------------------------------------ */
+/* Softmax attention over a paged cache: the rotation of queries and keys by
+ * their positions, the cache that keeps the keys and values of the sequences
+ * above between calls, and the attention of a call's rows over it.
+ *
+ * Rotary positions: the first `dims` values of a head, in pairs (x_i, x_j),
+ * turned by the angle of their position,
+ *   y_i = magnitude (x_i cos a - x_j sin a)
+ *   y_j = magnitude (x_i sin a + x_j cos a),  a = position frequencies[i];
+ * the head's other values are passed on. Angles are formed in binary64: one
+ * of 2^24 radians is held to 2^-27 of a radian.
+ * HALVES: pair i is (i, i + dims / 2); PAIRS: (2 i, 2 i + 1). */
+typedef enum kq_hip_rotary_layout {
+    KQ_HIP_ROTARY_HALVES = 0,
+    KQ_HIP_ROTARY_PAIRS
+} kq_hip_rotary_layout;
+
+typedef struct kq_hip_rotary {
+    uint32_t dims;             /* even, 2 .. 1024 and at most the head's width */
+    uint32_t layout;           /* kq_hip_rotary_layout */
+    float magnitude;           /* of cos and sin; 1: a plain rotation */
+    const double *frequencies; /* device [dims / 2], radians a position */
+} kq_hip_rotary;
+
+/* How the frequencies are made: base^(-2 i / dims), each divided by its
+ * divisor (a file's rope_freqs; host [dims / 2] or NULL: ones), then
+ *   NONE    as they are
+ *   LINEAR  divided by factor
+ *   BANDS   those that turn at least `fast` times in the original context as
+ *           they are, at most `slow` times divided by factor, and between
+ *           both, along the index i of the plain frequencies, a straight line
+ *           from one to the other. magnitude: 0.1 ln(factor) + 1. */
+typedef enum kq_hip_rotary_scaling_kind {
+    KQ_HIP_ROTARY_SCALING_NONE = 0,
+    KQ_HIP_ROTARY_SCALING_LINEAR,
+    KQ_HIP_ROTARY_SCALING_BANDS
+} kq_hip_rotary_scaling_kind;
+
+typedef struct kq_hip_rotary_scaling {
+    double base;             /* above 1 */
+    uint32_t kind;           /* kq_hip_rotary_scaling_kind */
+    double factor;           /* LINEAR, BANDS: at least 1 */
+    double original_context; /* BANDS: tokens, at least 1 */
+    double fast, slow;       /* BANDS: turns, fast > slow > 0 (32 and 1) */
+    const float *divisors;   /* host [dims / 2], finite and above 0, or NULL */
+} kq_hip_rotary_scaling;
+
+/* Host only: the frequencies [dims / 2] to upload, and the magnitude. */
+kq_status kq_hip_rotary_frequencies(const kq_hip_rotary_scaling *scaling, uint32_t dims,
+                                    double *host_frequencies, float *magnitude,
+                                    kq_diagnostic *diagnostic);
+
+/* The rotation of `heads` heads of `width` values in each of token_count rows;
+ * positions: device [token_count], NULL: row t has position t. width 1 ..
+ * 1024, rows of at most 2^22 values; strides count floats between rows, up to
+ * 2^22; 4-byte alignment, frequencies 8 (16 bytes, with width, dims / 2 and
+ * strides in fours, is faster). The output may be the input, with its stride.
+ * Non-finite inputs and results give NUMERIC_DOMAIN. */
+kq_status kq_hip_rotary_f32(kq_hip_context *context, const kq_hip_rotary *rotary, uint32_t heads,
+                            uint32_t width, uint64_t token_count,
+                            const uint32_t *device_positions, const float *device_input,
+                            uint64_t input_stride, float *device_output, uint64_t output_stride,
+                            kq_diagnostic *diagnostic);
+
+/* A cache of one layer's keys and values in pages of page_tokens tokens:
+ * keys and values device [page_count][heads][page_tokens][width], F16 or BF16.
+ * A sequence's slot (kq_hip_sequences; slot_count rows) is its line of
+ * `table`, which names the pages of its tokens in order, and its entry of
+ * `lengths`, the tokens that the cache holds of it before this call's rows;
+ * with `fresh` it holds none, whatever the entry. Row j of the sequence is the
+ * token at position length + j. The lengths are the same for every layer of a
+ * step; the caller adds the step's rows behind the last one.
+ * Only the entries of pages that hold the sequence's tokens are read, and
+ * pages may be shared by sequences that do not write them. Pages that do not
+ * exist and sequences longer than their line of the table are found on the
+ * device: INVALID_ARGUMENT, and nothing is read or written through them. */
+#define KQ_HIP_TYPE_F16 1u /* GGUF's number; its files' tensors are not read in it here */
+
+typedef struct kq_hip_paged_cache {
+    uint32_t type_id;     /* KQ_HIP_TYPE_F16 or KQ_GGUF_TYPE_BF16 */
+    uint32_t heads;       /* 1 .. 256 */
+    uint32_t width;       /* 64, 128 or 256 */
+    uint32_t page_tokens; /* 16, 32, 64, 128 or 256 */
+    uint32_t page_count;
+    uint32_t table_pages; /* entries of a line; table_pages page_tokens <= 2^24 */
+    void *keys;
+    void *values;
+    const uint32_t *table;   /* device [slot_count][table_pages] */
+    const uint32_t *lengths; /* device [slot_count] */
+} kq_hip_paged_cache;
+
+/* The call's new rows: keys and values [tokens][heads][width] for the pages,
+ * and, with query_heads above 0, queries [tokens][query_heads][width], which
+ * are only turned. query_output may be the query, with its stride. */
+typedef struct kq_hip_cache_rows {
+    const float *key;
+    uint64_t key_stride;
+    const float *value;
+    uint64_t value_stride;
+    uint32_t query_heads; /* 0 .. 256 */
+    const float *query;
+    uint64_t query_stride;
+    float *query_output;
+    uint64_t query_output_stride;
+} kq_hip_cache_rows;
+
+/* Writes the rows of the sequences into their pages, keys and queries turned
+ * by `rotary` at their positions (NULL: as they are), rounded to the cache's
+ * type. Strides count floats between rows, up to 2^22; rows, queries and the
+ * cache 16-byte aligned, strides in fours. Non-finite inputs, and values
+ * beyond the cache's type, give NUMERIC_DOMAIN. After a failure the places of
+ * the call's rows hold anything (no copy of the cache is made); those of
+ * earlier tokens are never written. Queries of rows that belong to no sequence
+ * keep what query_output held. */
+kq_status kq_hip_cache_append_f32(kq_hip_context *context, const kq_hip_paged_cache *cache,
+                                  const kq_hip_sequences *sequences,
+                                  const kq_hip_cache_rows *rows, const kq_hip_rotary *rotary,
+                                  kq_diagnostic *diagnostic);
+
+/* Attention of a call's rows over the cache, which holds them already: query
+ * head h of the row at position p reads key head h / (query_heads / heads),
+ *   y = act(gate) sum_t w_t value_t / (sum_t w_t + exp(sinks[h])),
+ *   w_t = exp(scale query . key_t)
+ * over the sequence's positions t <= p (causal) or all of them with this
+ * call's, with a window only t > p - window. sinks NULL: no such term. Both
+ * factors of a weight's product are held in full: results are those of
+ * binary32 products over the cache's values.
+ * Offsets as in kq_hip_sequences; a slot may be named more than once here.
+ * Rows that belong to no sequence keep what the output held. Strides count
+ * floats between rows, up to 2^22; queries, gate, output, cache and scratch
+ * 16-byte aligned, strides in fours. Non-finite queries, gates and results
+ * give NUMERIC_DOMAIN; what the pages hold behind a sequence's tokens is not
+ * looked at. */
+typedef struct kq_hip_paged_attention {
+    uint32_t query_heads; /* 1 .. 256, a multiple of the cache's heads */
+    float scale;
+    uint32_t causal;      /* 0 or 1 */
+    uint32_t window;      /* tokens, 0: no window */
+    const float *sinks;   /* device [query_heads] or NULL */
+    uint32_t gate_activation; /* KQ_HIP_ACTIVATION_NONE or _SIGMOID */
+} kq_hip_paged_attention;
+
+/* Device scratch of a call with these sizes (only counts are looked at, and
+ * whether offsets is NULL); 0 for arguments that the call refuses. Calls that
+ * may run at the same time need scratch of their own. */
+uint64_t kq_hip_paged_attention_scratch_bytes(const kq_hip_paged_attention *attention,
+                                              const kq_hip_paged_cache *cache,
+                                              const kq_hip_sequences *sequences);
+kq_status kq_hip_paged_attention_f32(kq_hip_context *context,
+                                     const kq_hip_paged_attention *attention,
+                                     const kq_hip_paged_cache *cache,
+                                     const kq_hip_sequences *sequences,
+                                     const float *device_query, uint64_t query_stride,
+                                     const float *device_gate, uint64_t gate_stride,
+                                     float *device_output, uint64_t output_stride,
+                                     void *device_scratch, uint64_t scratch_bytes,
+                                     kq_diagnostic *diagnostic);
+
+/* ------------------------------------------------------------------ */
 /* Norms around a block, with its gate and its residual. rms(x) below is
  * x / sqrt(mean(x^2) + epsilon). */
 

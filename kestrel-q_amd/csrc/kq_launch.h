@@ -399,6 +399,48 @@ uint64_t kq_launch_linattn_scratch(const kq_launch_linattn *a, uint64_t tokens, 
 hipError_t kq_launch_linattn_run(const kq_launch_linattn *a, const kq_launch_seqs *seqs,
                                  void *scratch, uint32_t *status, hipStream_t stream);
 
+/* rotary positions, appending to a paged cache (kq_rotary.hip) */
+typedef struct kq_launch_rotary {
+    uint32_t dims, pairs; /* dims 0: no rotation */
+    float magnitude;
+    const double *frequencies;
+} kq_launch_rotary;
+hipError_t kq_launch_rotary_rows(const kq_launch_rotary *r, uint32_t heads, uint32_t width,
+                                 uint64_t tokens, const uint32_t *positions, const float *x,
+                                 uint64_t xs, float *y, uint64_t ys, uint32_t *status,
+                                 hipStream_t stream);
+typedef struct kq_launch_paged {
+    uint32_t bf16, heads, width, page_shift, page_count, table_pages;
+    void *keys, *values;
+    const uint32_t *table, *lengths;
+} kq_launch_paged;
+typedef struct kq_launch_append {
+    const float *k, *v, *q;
+    float *qo;
+    uint64_t ks, vs, qs, qos;
+    uint32_t query_heads;
+} kq_launch_append;
+hipError_t kq_launch_cache_append(const kq_launch_paged *cache, const kq_launch_seqs *seqs,
+                                  const kq_launch_append *rows, const kq_launch_rotary *rotary,
+                                  uint32_t *status, hipStream_t stream);
+
+/* attention over a paged cache (kq_paged_attn.hip) */
+typedef struct kq_launch_pattn {
+    uint32_t query_heads;
+    float scale;
+    uint32_t causal, window;
+    const float *sinks;
+    uint32_t gated;
+    const float *q, *gate;
+    float *y;
+    uint64_t qs, gs, ys;
+} kq_launch_pattn;
+uint64_t kq_launch_pattn_scratch(const kq_launch_pattn *a, const kq_launch_paged *cache,
+                                 const kq_launch_seqs *seqs);
+hipError_t kq_launch_pattn_run(const kq_launch_pattn *a, const kq_launch_paged *cache,
+                               const kq_launch_seqs *seqs, void *scratch, uint32_t *status,
+                               hipStream_t stream);
+
 /* norms around a block (kq_norm.hip) */
 typedef struct kq_launch_norm {
     uint32_t groups, width;

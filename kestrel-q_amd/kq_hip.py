@@ -21,6 +21,7 @@ HERE = Path(__file__).resolve().parent
 LIB_PATH = Path(os.environ.get("KQ_HIP_LIB", HERE / "_build" / "libkq_hip.so"))
 
 TYPE_F32, TYPE_Q8_0, TYPE_Q4_K, TYPE_Q6_K = 0, 8, 12, 14
+TYPE_F16 = 1
 TYPE_Q5_1, TYPE_Q5_K, TYPE_IQ4_NL, TYPE_BF16 = 7, 13, 20, 30
 TYPE_IDS = {"F32": TYPE_F32, "Q8_0": TYPE_Q8_0, "Q4_K": TYPE_Q4_K, "Q6_K": TYPE_Q6_K,
             "Q5_1": TYPE_Q5_1, "Q5_K": TYPE_Q5_K, "IQ4_NL": TYPE_IQ4_NL, "BF16": TYPE_BF16}
@@ -107,6 +108,40 @@ class BlockJoin(C.Structure):
 
 NO_SLOT = 0xFFFFFFFF
 ACTIVATIONS = {"none": 0, "sigmoid": 1, "silu": 2}
+
+
+class Rotary(C.Structure):
+    _fields_ = [("dims", C.c_uint32), ("layout", C.c_uint32), ("magnitude", C.c_float),
+                ("frequencies", C.c_void_p)]
+
+
+class RotaryScaling(C.Structure):
+    _fields_ = [("base", C.c_double), ("kind", C.c_uint32), ("factor", C.c_double),
+                ("original_context", C.c_double), ("fast", C.c_double), ("slow", C.c_double),
+                ("divisors", C.POINTER(C.c_float))]
+
+
+class PagedCache(C.Structure):
+    _fields_ = [("type_id", C.c_uint32), ("heads", C.c_uint32), ("width", C.c_uint32),
+                ("page_tokens", C.c_uint32), ("page_count", C.c_uint32),
+                ("table_pages", C.c_uint32), ("keys", C.c_void_p), ("values", C.c_void_p),
+                ("table", C.c_void_p), ("lengths", C.c_void_p)]
+
+
+class CacheRows(C.Structure):
+    _fields_ = [("key", C.c_void_p), ("key_stride", C.c_uint64), ("value", C.c_void_p),
+                ("value_stride", C.c_uint64), ("query_heads", C.c_uint32),
+                ("query", C.c_void_p), ("query_stride", C.c_uint64),
+                ("query_output", C.c_void_p), ("query_output_stride", C.c_uint64)]
+
+
+class PagedAttention(C.Structure):
+    _fields_ = [("query_heads", C.c_uint32), ("scale", C.c_float), ("causal", C.c_uint32),
+                ("window", C.c_uint32), ("sinks", C.c_void_p), ("gate_activation", C.c_uint32)]
+
+
+ROTARY_LAYOUTS = {"halves": 0, "pairs": 1}
+ROTARY_SCALINGS = {"none": 0, "linear": 1, "bands": 2}
 
 
 class MoeWeights(C.Structure):
@@ -384,6 +419,13 @@ SIGNATURES = {
     "kq_hip_linear_attention_scratch_bytes": (C.c_uint64, [_P, _P]),
     "kq_hip_linear_attention_f32": (C.c_int, [_P, _P, _P, _P, _P, _P, _P, C.c_uint64, _P,
                                               C.c_uint64, _P]),
+    "kq_hip_rotary_frequencies": (C.c_int, [_P, C.c_uint32, _P, _P, _P]),
+    "kq_hip_rotary_f32": (C.c_int, [_P, _P, C.c_uint32, C.c_uint32, C.c_uint64, _P, _P, C.c_uint64,
+                                    _P, C.c_uint64, _P]),
+    "kq_hip_cache_append_f32": (C.c_int, [_P, _P, _P, _P, _P, _P]),
+    "kq_hip_paged_attention_scratch_bytes": (C.c_uint64, [_P, _P, _P]),
+    "kq_hip_paged_attention_f32": (C.c_int, [_P, _P, _P, _P, _P, C.c_uint64, _P, C.c_uint64, _P,
+                                             C.c_uint64, _P, C.c_uint64, _P]),
     "kq_hip_gated_norm_f32": (C.c_int, [_P, _P, C.c_uint64, _P, C.c_uint64, _P, C.c_uint64, _P,
                                         C.c_uint64, _P]),
     "kq_hip_block_join_f32": (C.c_int, [_P, _P, C.c_uint64, _P, _P, _P, _P, _P, _P, _P]),
@@ -494,6 +536,51 @@ def linear_attention_inputs(query, query_stride: int, key, key_stride: int, valu
 
 def linear_attention_scratch_bytes(attention: LinearAttention, seqs: Sequences) -> int:
     return lib().kq_hip_linear_attention_scratch_bytes(C.byref(attention), C.byref(seqs))
+
+
+def rotary(dims: int, frequencies, layout: str = "halves", magnitude: float = 1.0) -> Rotary:
+    """frequencies: device [dims / 2] float64, radians a position."""
+    return Rotary(dims, ROTARY_LAYOUTS[layout], magnitude, _ptr(frequencies))
+
+
+def rotary_frequencies(dims: int, base: float, scaling: str = "none", factor: float = 1.0,
+                       original_context: float = 0.0, fast: float = 32.0, slow: float = 1.0,
+                       divisors=None) -> tuple[np.ndarray, float]:
+    """(frequencies [dims / 2] float64 to upload, magnitude)."""
+    div = None if divisors is None else np.ascontiguousarray(divisors, np.float32)
+    if div is not None and div.size < dims // 2:
+        raise ValueError("a divisor for each pair")
+    sc = RotaryScaling(base, ROTARY_SCALINGS[scaling], factor, original_context, fast, slow,
+                       None if div is None else div.ctypes.data_as(C.POINTER(C.c_float)))
+    out, m, d = np.empty(max(dims // 2, 1), np.float64), C.c_float(), Diagnostic()
+    check(lib().kq_hip_rotary_frequencies(C.byref(sc), dims, out.ctypes.data, C.byref(m),
+                                          C.byref(d)), d)
+    return out, m.value
+
+
+def paged_cache(type_id: int, heads: int, width: int, page_tokens: int, page_count: int,
+                table_pages: int, keys, values, table, lengths) -> PagedCache:
+    """Device arrays: keys and values [page_count][heads][page_tokens][width], table
+    [slots][table_pages], lengths [slots]: tokens before the call's rows."""
+    return PagedCache(type_id, heads, width, page_tokens, page_count, table_pages, _ptr(keys),
+                      _ptr(values), _ptr(table), _ptr(lengths))
+
+
+def cache_rows(key, key_stride: int, value, value_stride: int, query_heads: int = 0, query=None,
+               query_stride: int = 0, query_output=None, query_output_stride: int = 0) -> CacheRows:
+    return CacheRows(_ptr(key), key_stride, _ptr(value), value_stride, query_heads, _ptr(query),
+                     query_stride, _ptr(query_output), query_output_stride)
+
+
+def paged_attention(query_heads: int, scale: float, causal: bool = True, window: int = 0,
+                    sinks=None, gate: str = "none") -> PagedAttention:
+    return PagedAttention(query_heads, scale, int(causal), window, _ptr(sinks), ACTIVATIONS[gate])
+
+
+def paged_attention_scratch_bytes(attention: PagedAttention, cache: PagedCache,
+                                  seqs: Sequences) -> int:
+    return lib().kq_hip_paged_attention_scratch_bytes(C.byref(attention), C.byref(cache),
+                                                      C.byref(seqs))
 
 
 def gated_norm(groups: int, width: int, epsilon: float, weight=None, weight_offset: float = 0.0,
@@ -869,6 +956,30 @@ class Context:
                                                 C.byref(inputs), _ptr(state), _ptr(state_out),
                                                 _ptr(y), y_stride, _ptr(scratch), scratch_bytes,
                                                 C.byref(d)), d)
+
+    def rotary(self, rotary: Rotary, heads: int, width: int, tokens: int, positions, x,
+               x_stride: int, y, y_stride: int) -> None:
+        d = Diagnostic()
+        check(lib().kq_hip_rotary_f32(self.handle, C.byref(rotary), heads, width, tokens,
+                                      _ptr(positions), _ptr(x), x_stride, _ptr(y), y_stride,
+                                      C.byref(d)), d)
+
+    def cache_append(self, cache: PagedCache, seqs: Sequences, rows: CacheRows,
+                     rotary: Rotary | None = None) -> None:
+        d = Diagnostic()
+        check(lib().kq_hip_cache_append_f32(self.handle, C.byref(cache), C.byref(seqs),
+                                            C.byref(rows),
+                                            None if rotary is None else C.byref(rotary),
+                                            C.byref(d)), d)
+
+    def paged_attention(self, attention: PagedAttention, cache: PagedCache, seqs: Sequences, query,
+                        query_stride: int, gate, gate_stride: int, y, y_stride: int, scratch,
+                        scratch_bytes: int) -> None:
+        d = Diagnostic()
+        check(lib().kq_hip_paged_attention_f32(self.handle, C.byref(attention), C.byref(cache),
+                                               C.byref(seqs), _ptr(query), query_stride,
+                                               _ptr(gate), gate_stride, _ptr(y), y_stride,
+                                               _ptr(scratch), scratch_bytes, C.byref(d)), d)
 
     def gated_norm(self, norm: GatedNorm, tokens: int, x, x_stride: int, gate, gate_stride: int,
                    y, y_stride: int) -> None:
