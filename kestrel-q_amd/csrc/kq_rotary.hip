@@ -21,7 +21,7 @@
 namespace {
 
 constexpr uint32_t kThreads = 256;
-constexpr uint32_t kTokens = 4; /* of a workgroup: a wave looks up each */
+constexpr int kTokens = 4; /* of a workgroup: a wave looks up each */
 constexpr uint32_t kMaxHalf = 512;
 
 struct Turn {
@@ -58,14 +58,10 @@ __device__ __forceinline__ Turn turn_of(uint32_t position, double frequency, flo
 /* V neighbouring values */
 template <int V>
 struct Vec {
+    typedef float fv __attribute__((ext_vector_type(V)));
     float v[V];
     __device__ __forceinline__ void load(const float *p) {
-        if constexpr (V == 4) {
-            const float4 q = *(const float4 *)p;
-            v[0] = q.x; v[1] = q.y; v[2] = q.z; v[3] = q.w;
-        } else {
-            v[0] = *p;
-        }
+        *this = __builtin_bit_cast(Vec<V>, *(const fv *)p);
     }
     __device__ __forceinline__ bool finite() const {
         bool ok = true;
@@ -75,163 +71,204 @@ struct Vec {
     }
 };
 
-/* where results go: fp32 rows */
-struct ToRows {
-    template <int V>
-    __device__ __forceinline__ void store(float *p, const Vec<V> &x, bool &bad) const {
-        if constexpr (V == 4)
-            *(float4 *)p = make_float4(x.v[0], x.v[1], x.v[2], x.v[3]);
-        else
-            *p = x.v[0];
-        bad |= !x.finite();
-    }
-};
-
-/* or a page, rounded to its type */
-template <typename T>
-struct ToPage {
-    template <int V>
-    __device__ __forceinline__ void store(T *p, const Vec<V> &x, bool &bad) const {
-        typedef T tv __attribute__((ext_vector_type(V)));
-        tv r;
-        bool ok = true;
+/* Results go past the caches: what reads them next runs on other XCDs, and the
+ * call's inputs would make room for them (8191 rows of 24 heads of 128: 56 us
+ * where ordinary stores took 71). Rows are fp32, pages of the cache's type. */
+template <int V, typename T>
+__device__ __forceinline__ void store(T *p, const Vec<V> &x, bool &bad) {
+    typedef T tv __attribute__((ext_vector_type(V)));
+    tv r;
+    bool ok = true;
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-            r[i] = (T)x.v[i];
-            ok &= kq_isfinite((float)r[i]);
-        }
-        bad |= !ok;
-        *(tv *)p = r;
+    for (int i = 0; i < V; ++i) {
+        r[i] = (T)x.v[i];
+        ok &= kq_isfinite((float)r[i]);
     }
-};
-
-/* The cosines and sines of tokens [0, n) of the workgroup at their positions */
-__device__ __forceinline__ void make_turns(const kq_launch_rotary &r, uint32_t n,
-                                           const uint32_t *position, float (*co)[kMaxHalf],
-                                           float (*si)[kMaxHalf], bool &badin) {
-    const uint32_t half = r.dims / 2u;
-    for (uint32_t i = threadIdx.x; i < half; i += kThreads) {
-        const double f = r.frequencies[i];
-        badin |= !isfinite(f);
-        for (uint32_t t = 0; t < n; ++t) {
-            const Turn c = turn_of(position[t], f, r.magnitude);
-            co[t][i] = c.c;
-            si[t][i] = c.s;
-        }
-    }
+    bad |= !ok;
+    __builtin_nontemporal_store(r, (tv *)p);
 }
 
-/* Heads of up to kTokens rows, turned: from[t] a row's heads, to(t, head) where
- * the head goes; NULL rows are left out. A unit is V pairs (2 V values), or V
- * values that are passed on. */
-template <int V, typename Out, typename To>
-__device__ __forceinline__ void turn_heads(const kq_launch_rotary &r, uint32_t heads,
-                                           uint32_t width, const float *const (&from)[kTokens],
-                                           const Out &out, To to, const float (*co)[kMaxHalf],
-                                           const float (*si)[kMaxHalf], bool &badin, bool &bad) {
-    const uint32_t half = r.dims / 2u;
-    const uint32_t turned = half / V, units = turned + (width - r.dims) / V;
-    for (uint32_t u = threadIdx.x; u < heads * units; u += kThreads) {
-        const uint32_t head = u / units, k = u - head * units;
-        const uint32_t base = head * width;
-        if (k < turned) {
-            const uint32_t a = r.pairs ? 2u * V * k : V * k;
-            const uint32_t b = r.pairs ? a + V : a + half;
-            Vec<V> x[kTokens], y[kTokens];
-#pragma unroll
-            for (uint32_t t = 0; t < kTokens; ++t)
-                if (from[t] != nullptr) {
-                    x[t].load(from[t] + base + a);
-                    y[t].load(from[t] + base + b);
-                }
-#pragma unroll
-            for (uint32_t t = 0; t < kTokens; ++t) {
-                if (from[t] == nullptr) continue;
-                badin |= !x[t].finite() || !y[t].finite();
-                Vec<V> c, s, p, q;
-                c.load(&co[t][V * k]);
-                s.load(&si[t][V * k]);
-                if (r.pairs && V > 1) {
-                    /* x, y: pairs side by side */
-#pragma unroll
-                    for (int i = 0; i < V; ++i) {
-                        const float e = i < V / 2 ? x[t].v[(2 * i) % V] : y[t].v[(2 * i) % V];
-                        const float o = i < V / 2 ? x[t].v[(2 * i + 1) % V] : y[t].v[(2 * i + 1) % V];
-                        const float re = fmaf(e, c.v[i], -(o * s.v[i]));
-                        const float im = fmaf(e, s.v[i], o * c.v[i]);
-                        if (i < V / 2) {
-                            p.v[(2 * i) % V] = re;
-                            p.v[(2 * i + 1) % V] = im;
-                        } else {
-                            q.v[(2 * i) % V] = re;
-                            q.v[(2 * i + 1) % V] = im;
-                        }
-                    }
-                } else {
-#pragma unroll
-                    for (int i = 0; i < V; ++i) {
-                        p.v[i] = fmaf(x[t].v[i], c.v[i], -(y[t].v[i] * s.v[i]));
-                        q.v[i] = fmaf(x[t].v[i], s.v[i], y[t].v[i] * c.v[i]);
-                    }
-                }
-                out.store(to(t, head) + a, p, bad);
-                out.store(to(t, head) + b, q, bad);
-            }
-        } else {
-            const uint32_t a = r.dims + (k - turned) * V;
-            Vec<V> x[kTokens];
-#pragma unroll
-            for (uint32_t t = 0; t < kTokens; ++t)
-                if (from[t] != nullptr) x[t].load(from[t] + base + a);
-#pragma unroll
-            for (uint32_t t = 0; t < kTokens; ++t) {
-                if (from[t] == nullptr) continue;
-                badin |= !x[t].finite();
-                out.store(to(t, head) + a, x[t], bad);
-            }
+/* The cosines and sines of n tokens at their positions */
+template <int TOK>
+struct Turns {
+    float c[TOK][kMaxHalf], s[TOK][kMaxHalf];
+
+    template <typename At>
+    __device__ __forceinline__ void make(const kq_launch_rotary &r, uint32_t n, At position,
+                                         bool &badin) {
+        const uint32_t half = r.dims / 2u;
+        for (uint32_t i = threadIdx.x; i < n * half; i += kThreads) {
+            const uint32_t t = TOK == 1 ? 0u : i / half, k = i - t * half;
+            const double f = r.frequencies[k];
+            badin |= !isfinite(f);
+            const Turn x = turn_of(position(t), f, r.magnitude);
+            c[t][k] = x.c;
+            s[t][k] = x.s;
         }
     }
+};
+
+/* Heads of rows that turn, or are passed on (dims 0), in units: V pairs of two
+ * vectors (HALVES), or one vector of V values. The lanes' vectors of a load lie
+ * side by side, and the stores' too, which go past the caches. */
+struct Heads {
+    const float *rows;
+    uint64_t stride;
+    uint32_t count, width, dims, pairs;
+};
+
+/* values that turn in a unit */
+template <int V>
+__device__ __forceinline__ uint32_t unit_turns(const Heads &h) {
+    return V == 1 || !h.pairs ? 2u * V : V;
+}
+template <int V>
+__device__ __forceinline__ uint32_t units_of(const Heads &h) {
+    return h.dims / unit_turns<V>(h) + (h.width - h.dims) / V;
 }
 
 template <int V>
-__global__ __launch_bounds__(kThreads) void rotary_rows(kq_launch_rotary r, uint32_t heads,
-                                                        uint32_t width, uint32_t tokens,
-                                                        const uint32_t *__restrict__ positions,
-                                                        const float *x, uint64_t xs, float *y,
-                                                        uint64_t ys, uint32_t *status) {
-    __shared__ __attribute__((aligned(16))) float co[kTokens][kMaxHalf], si[kTokens][kMaxHalf];
-    const uint32_t t0 = blockIdx.x * kTokens;
-    const uint32_t n = tokens - t0 < kTokens ? tokens - t0 : kTokens;
-    uint32_t at[kTokens];
-    const float *from[kTokens];
-    bool badin = false, bad = false;
-#pragma unroll
-    for (uint32_t t = 0; t < kTokens; ++t) {
-        at[t] = t < n ? (positions != nullptr ? positions[t0 + t] : t0 + t) : 0u;
-        from[t] = t < n ? x + (size_t)(t0 + t) * xs : nullptr;
+struct Unit {
+    uint32_t head, a, b, turn; /* turn: its first pair, ~0: passed on */
+    bool two;
+
+    __device__ __forceinline__ Unit(const Heads &h, uint32_t u) {
+        const uint32_t each = units_of<V>(h), values = unit_turns<V>(h), turned = h.dims / values;
+        head = u / each;
+        const uint32_t k = u - head * each;
+        if (k < turned) {
+            turn = k * (values / 2u);
+            two = values == 2u * V;
+            a = h.pairs ? values * k : V * k;
+            b = h.pairs ? a + 1u : a + h.dims / 2u;
+        } else {
+            turn = ~0u;
+            two = false;
+            a = b = h.dims + (k - turned) * V;
+        }
     }
-    make_turns(r, n, at, co, si, badin);
+};
+
+template <int V, int TOK>
+struct Values {
+    Vec<V> a[TOK], b[TOK];
+
+    __device__ __forceinline__ void load(const Heads &h, const Unit<V> &u, uint32_t t0, uint32_t n) {
+        const float *p = h.rows + (size_t)t0 * h.stride + u.head * h.width;
+#pragma unroll
+        for (uint32_t t = 0; t < TOK; ++t) {
+            if (t >= n) break;
+            a[t].load(p + t * h.stride + u.a);
+            if (u.two) b[t].load(p + t * h.stride + u.b);
+        }
+    }
+
+    /* the turned values of token t */
+    __device__ __forceinline__ void turned(const Unit<V> &u, const Turns<TOK> &turns, uint32_t t,
+                                           Vec<V> &p, Vec<V> &q) const {
+        if (V > 1 && !u.two) { /* V / 2 pairs side by side */
+            Vec<(V + 1) / 2> c, s;
+            c.load(&turns.c[t][u.turn]);
+            s.load(&turns.s[t][u.turn]);
+#pragma unroll
+            for (int i = 0; i < V / 2; ++i) {
+                const float e = a[t].v[2 * i], o = a[t].v[(2 * i + 1) % V];
+                p.v[2 * i] = fmaf(e, c.v[i], -(o * s.v[i]));
+                p.v[(2 * i + 1) % V] = fmaf(e, s.v[i], o * c.v[i]);
+            }
+        } else {
+            Vec<V> c, s;
+            c.load(&turns.c[t][u.turn]);
+            s.load(&turns.s[t][u.turn]);
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                p.v[i] = fmaf(a[t].v[i], c.v[i], -(b[t].v[i] * s.v[i]));
+                q.v[i] = fmaf(a[t].v[i], s.v[i], b[t].v[i] * c.v[i]);
+            }
+        }
+    }
+
+    /* unit u's values of the n tokens, those that `some` names, to to(t) */
+    template <typename Some, typename To>
+    __device__ __forceinline__ void put(const Heads &h, const Unit<V> &u, const Turns<TOK> &turns,
+                                        uint32_t n, Some some, To to, bool &badin,
+                                        bool &bad) const {
+#pragma unroll
+        for (uint32_t t = 0; t < TOK; ++t) {
+            if (t >= n) break;
+            if (!some(t)) continue;
+            badin |= !a[t].finite() || (u.two && !b[t].finite());
+            Vec<V> p = a[t], q = b[t];
+            if (u.turn != ~0u) turned(u, turns, t, p, q);
+            auto *at = to(t) + (size_t)u.head * h.width;
+            store(at + u.a, p, bad);
+            if (u.two) store(at + u.b, q, bad);
+        }
+    }
+};
+
+template <int V, int TOK>
+__global__ __launch_bounds__(kThreads) void rotary_rows(kq_launch_rotary r, Heads h,
+                                                        uint32_t tokens,
+                                                        const uint32_t *__restrict__ positions,
+                                                        float *y, uint64_t ys, uint32_t *status) {
+    __shared__ __attribute__((aligned(16))) Turns<TOK> turns;
+    const uint32_t t0 = blockIdx.x * TOK;
+    const uint32_t n = tokens - t0 < TOK ? tokens - t0 : TOK;
+    const uint32_t units = h.count * units_of<V>(h);
+    bool badin = false, bad = false;
+    uint32_t at = blockIdx.y * kThreads + threadIdx.x;
+    const uint32_t step = gridDim.y * kThreads;
+    Values<V, TOK> x;
+    /* the first values are under way while the turns are formed */
+    if (at < units) x.load(h, Unit<V>(h, at), t0, n);
+    turns.make(
+        r, n, [&](uint32_t t) { return positions != nullptr ? positions[t0 + t] : t0 + t; }, badin);
     __syncthreads();
-    turn_heads<V>(
-        r, heads, width, from, ToRows{},
-        [&](uint32_t t, uint32_t head) { return y + (size_t)(t0 + t) * ys + head * width; }, co, si,
-        badin, bad);
+    while (at < units) {
+        const Unit<V> u(h, at);
+        x.put(
+            h, u, turns, n, [](uint32_t) { return true; },
+            [&](uint32_t t) { return y + (size_t)(t0 + t) * ys; }, badin, bad);
+        at += step;
+        if (at < units) x.load(h, Unit<V>(h, at), t0, n);
+    }
     if (badin) kq_flag(status, KQ_DEV_INPUT);
     if (bad) kq_flag(status, KQ_DEV_NUMERIC);
 }
 
-template <typename T, int V>
+/* Keys, then queries, then values of a row. Where a row goes hangs on its
+ * sequence, slot, length and page, one load after the other: the first values
+ * are asked for before. */
+template <typename T, int V, int TOK>
 __global__ __launch_bounds__(kThreads) void append_rows(kq_launch_paged c, kq_launch_seqs q,
                                                         kq_launch_append a, kq_launch_rotary r,
                                                         uint32_t *status) {
-    __shared__ __attribute__((aligned(16))) float co[kTokens][kMaxHalf], si[kTokens][kMaxHalf];
-    __shared__ uint32_t pos_of[kTokens], page_of[kTokens];
-    const uint32_t t0 = blockIdx.x * kTokens, tokens = (uint32_t)q.tokens;
-    const uint32_t n = tokens - t0 < kTokens ? tokens - t0 : kTokens;
+    __shared__ __attribute__((aligned(16))) Turns<TOK> turns;
+    __shared__ uint32_t pos_of[TOK], page_of[TOK];
+    const uint32_t t0 = blockIdx.x * TOK, tokens = (uint32_t)q.tokens;
+    const uint32_t n = tokens - t0 < TOK ? tokens - t0 : TOK;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64u);
+    const Heads keys = {a.k, a.ks, c.heads, c.width, r.dims, r.pairs};
+    const Heads queries = {a.q, a.qs, a.query_heads, c.width, r.dims, r.pairs};
+    const Heads values = {a.v, a.vs, c.heads, c.width, 0u, 0u};
+    const uint32_t nk = c.heads * units_of<V>(keys), nq = nk + a.query_heads * units_of<V>(queries);
+    const uint32_t units = nq + c.heads * units_of<V>(values);
     bool badin = false, bad = false, badseq = false;
+    uint32_t at = blockIdx.y * kThreads + threadIdx.x;
+    const uint32_t step = gridDim.y * kThreads;
+    Values<V, TOK> x;
+    auto load = [&]() {
+        if (at < nk)
+            x.load(keys, Unit<V>(keys, at), t0, n);
+        else if (at < nq)
+            x.load(queries, Unit<V>(queries, at - nk), t0, n);
+        else if (at < units)
+            x.load(values, Unit<V>(values, at - nq), t0, n);
+    };
+    load();
     /* wave w: where row t0 + w goes */
-    if (wave < kTokens) {
+    if (wave < TOK) {
         uint32_t page = ~0u, pos = 0u;
         const uint32_t t = t0 + wave;
         if (wave < n) {
@@ -252,51 +289,59 @@ __global__ __launch_bounds__(kThreads) void append_rows(kq_launch_paged c, kq_la
         }
     }
     __syncthreads();
-    uint32_t at[kTokens];
-    size_t place[kTokens];
-    const float *from[kTokens];
+    if (r.dims != 0u) turns.make(r, n, [&](uint32_t t) { return pos_of[t]; }, badin);
+    __syncthreads();
     const uint32_t mask = (1u << c.page_shift) - 1u;
     const size_t head_values = (size_t)c.width << c.page_shift;
-#pragma unroll
-    for (uint32_t t = 0; t < kTokens; ++t) {
-        at[t] = pos_of[t];
-        const uint32_t page = page_of[t];
-        from[t] = page != ~0u ? a.k + (size_t)(t0 + t) * a.ks : nullptr;
-        place[t] = page != ~0u ? page * c.heads * head_values + (size_t)(at[t] & mask) * c.width : 0u;
+    auto some = [&](uint32_t t) { return page_of[t] != ~0u; };
+    while (at < units) {
+        if (at < nk || at >= nq) {
+            const Heads &h = at < nk ? keys : values;
+            const Unit<V> u(h, at < nk ? at : at - nq);
+            T *pool = (T *)(at < nk ? c.keys : c.values) + u.head * (head_values - c.width);
+            x.put(
+                h, u, turns, n, some,
+                [&](uint32_t t) {
+                    return pool + page_of[t] * c.heads * head_values +
+                           (size_t)(pos_of[t] & mask) * c.width;
+                },
+                badin, bad);
+        } else {
+            x.put(
+                queries, Unit<V>(queries, at - nk), turns, n, some,
+                [&](uint32_t t) { return a.qo + (size_t)(t0 + t) * a.qos; }, badin, bad);
+        }
+        at += step;
+        load();
     }
-    if (r.dims != 0u) make_turns(r, n, at, co, si, badin);
-    __syncthreads();
-    turn_heads<V>(
-        r, c.heads, c.width, from, ToPage<T>{},
-        [&](uint32_t t, uint32_t head) { return (T *)c.keys + place[t] + head * head_values; }, co,
-        si, badin, bad);
-    if (a.query_heads != 0u) {
-#pragma unroll
-        for (uint32_t t = 0; t < kTokens; ++t)
-            if (from[t] != nullptr) from[t] = a.q + (size_t)(t0 + t) * a.qs;
-        turn_heads<V>(
-            r, a.query_heads, c.width, from, ToRows{},
-            [&](uint32_t t, uint32_t head) {
-                return a.qo + (size_t)(t0 + t) * a.qos + head * c.width;
-            },
-            co, si, badin, bad);
-    }
-#pragma unroll
-    for (uint32_t t = 0; t < kTokens; ++t)
-        if (from[t] != nullptr) from[t] = a.v + (size_t)(t0 + t) * a.vs;
-    r.dims = 0u;
-    turn_heads<4>(
-        r, c.heads, c.width, from, ToPage<T>{},
-        [&](uint32_t t, uint32_t head) { return (T *)c.values + place[t] + head * head_values; }, co,
-        si, badin, bad);
     /* every sequence is looked at, those without rows too, and its slot */
-    for (uint32_t s = blockIdx.x; s < q.count; s += gridDim.x) {
-        const kq::PagedSeq sp = kq::paged_seq(q, c, s, badseq);
-        if (sp.live) badseq |= kq::seq_slot_taken<kThreads>(q, s, sp.slot);
-    }
+    if (blockIdx.y == 0u)
+        for (uint32_t s = blockIdx.x; s < q.count; s += gridDim.x) {
+            const kq::PagedSeq sp = kq::paged_seq(q, c, s, badseq);
+            if (sp.live) badseq |= kq::seq_slot_taken<kThreads>(q, s, sp.slot);
+        }
     if (badseq) kq_flag(status, KQ_DEV_SEQUENCE);
     if (badin) kq_flag(status, KQ_DEV_INPUT);
     if (bad) kq_flag(status, KQ_DEV_NUMERIC);
+}
+
+/* Tokens of a workgroup: one while that does not fill the device (61 rows of 20
+ * heads: 4.6 us, 10.2 with four), then four, whose turns are formed together.
+ * Beside each other in y, workgroups for the row's values, so that a thread has
+ * few to walk through: 8191 rows of 24 heads take 38.2 us, 5.3 TB/s, where one
+ * workgroup for them took 43; 4099 rows of 48 heads into pages 40.3, 4.6 TB/s,
+ * and 46. */
+struct Shape {
+    bool one;
+    dim3 grid;
+};
+Shape shape_of(uint64_t tokens, uint64_t units) {
+    Shape s;
+    s.one = tokens < 1024u;
+    const uint64_t across = (units + kThreads - 1u) / kThreads, most = s.one ? 8u : 4u;
+    s.grid = dim3((uint32_t)(s.one ? tokens : (tokens + kTokens - 1u) / kTokens),
+                  (uint32_t)(across < most ? across : most));
+    return s;
 }
 
 }  // namespace
@@ -306,37 +351,59 @@ extern "C" hipError_t kq_launch_rotary_rows(const kq_launch_rotary *r, uint32_t 
                                             const uint32_t *positions, const float *x, uint64_t xs,
                                             float *y, uint64_t ys, uint32_t *status,
                                             hipStream_t s) {
-    const bool v4 = r->dims % 8u == 0u && width % 4u == 0u && xs % 4u == 0u && ys % 4u == 0u &&
+    const bool v4 = r->dims % (r->pairs ? 4u : 8u) == 0u && width % 4u == 0u && xs % 4u == 0u && ys % 4u == 0u &&
                     (((uintptr_t)x | (uintptr_t)y) & 15u) == 0u;
-    const dim3 grid((uint32_t)((tokens + kTokens - 1u) / kTokens));
-    if (v4)
-        hipLaunchKernelGGL(HIP_KERNEL_NAME(rotary_rows<4>), grid, dim3(kThreads), 0, s, *r, heads,
-                           width, (uint32_t)tokens, positions, x, xs, y, ys, status);
-    else
-        hipLaunchKernelGGL(HIP_KERNEL_NAME(rotary_rows<1>), grid, dim3(kThreads), 0, s, *r, heads,
-                           width, (uint32_t)tokens, positions, x, xs, y, ys, status);
+    const Heads h = {x, xs, heads, width, r->dims, r->pairs};
+    const Shape g = shape_of(tokens, (uint64_t)heads * width / (v4 ? 4u : 1u));
+#define KQ_ROTARY(V, TOK)                                                                          \
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(rotary_rows<V, TOK>), g.grid, dim3(kThreads), 0, s, *r, h,  \
+                       (uint32_t)tokens, positions, y, ys, status)
+    if (g.one) {
+        if (v4)
+            KQ_ROTARY(4, 1);
+        else
+            KQ_ROTARY(1, 1);
+    } else {
+        if (v4)
+            KQ_ROTARY(4, kTokens);
+        else
+            KQ_ROTARY(1, kTokens);
+    }
+#undef KQ_ROTARY
     return hipGetLastError();
 }
+
+namespace {
+
+template <typename T>
+hipError_t append(const kq_launch_paged &c, const kq_launch_seqs &q, const kq_launch_append &a,
+                  const kq_launch_rotary &r, uint32_t *status, hipStream_t s) {
+    const bool v4 = r.dims % (r.pairs ? 4u : 8u) == 0u;
+    const Shape g =
+        shape_of(q.tokens, (uint64_t)(2u * c.heads + a.query_heads) * c.width / (v4 ? 4u : 1u));
+#define KQ_APPEND(V, TOK)                                                                         \
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(append_rows<T, V, TOK>), g.grid, dim3(kThreads), 0, s, c, q, \
+                       a, r, status)
+    if (g.one) {
+        if (v4)
+            KQ_APPEND(4, 1);
+        else
+            KQ_APPEND(1, 1);
+    } else {
+        if (v4)
+            KQ_APPEND(4, kTokens);
+        else
+            KQ_APPEND(1, kTokens);
+    }
+#undef KQ_APPEND
+    return hipGetLastError();
+}
+
+}  // namespace
 
 extern "C" hipError_t kq_launch_cache_append(const kq_launch_paged *c, const kq_launch_seqs *q,
                                              const kq_launch_append *a, const kq_launch_rotary *r,
                                              uint32_t *status, hipStream_t s) {
-    const dim3 grid((uint32_t)((q->tokens + kTokens - 1u) / kTokens));
-    const bool v4 = r->dims % 8u == 0u;
-#define KQ_APPEND(T, V)                                                                          \
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(append_rows<T, V>), grid, dim3(kThreads), 0, s, *c, *q, *a, \
-                       *r, status)
-    if (c->bf16) {
-        if (v4)
-            KQ_APPEND(__bf16, 4);
-        else
-            KQ_APPEND(__bf16, 1);
-    } else {
-        if (v4)
-            KQ_APPEND(_Float16, 4);
-        else
-            KQ_APPEND(_Float16, 1);
-    }
-#undef KQ_APPEND
-    return hipGetLastError();
+    return c->bf16 ? append<__bf16>(*c, *q, *a, *r, status, s)
+                   : append<_Float16>(*c, *q, *a, *r, status, s);
 }
