@@ -20,8 +20,9 @@ constexpr uint32_t kTile = 64;       /* keys of a tile */
 constexpr uint32_t kFew = 16;        /* rows of an item whose waves share out its keys */
 constexpr uint32_t kMany = 128;      /* rows of an item whose waves share out its rows */
 constexpr uint32_t kLeast = 2;       /* tiles of a part */
-constexpr uint32_t kTarget = 1024;   /* parts that the device is filled with */
-constexpr uint32_t kSlots = 2u * kTarget;
+constexpr uint32_t kShort = 8;       /* tiles of a part of few rows that are worth a second round */
+constexpr uint32_t kParts = 1024;    /* of few rows; of many half of them */
+constexpr uint32_t kSlots = 2u * kParts;
 constexpr uint32_t kByLane = 64;     /* sequences that each wave plans by itself */
 constexpr float kSlack = 8.0f;       /* by which a row's largest exponent may pass its stand-in */
 constexpr float kLowest = -0x1.fffffep127f;
@@ -35,8 +36,8 @@ struct Args {
     uint32_t slots;
     double exponent;    /* scale log2(e) */
     float *partial;     /* slots of [slot_rows][width] sums, then tops, then totals */
-    uint32_t *plan;     /* [0]: tiles a part, [1]: parts; then first parts, then first slots of
-                           the sequences */
+    uint32_t *plan;     /* tiles a part of few rows, parts, tiles a part of many rows; then first
+                           parts, then first slots of the sequences */
 };
 
 /* ---------------------------------------------------------------- the plan */
@@ -71,10 +72,28 @@ __device__ __forceinline__ uint64_t cost_of(const Args &g, const Need &n) {
     return (uint64_t)n.blocks * g.c.heads * n.tiles;
 }
 
-/* tiles a part, of all sequences' cost: kTarget parts, not too short ones */
-__device__ __forceinline__ uint32_t part_tiles(uint64_t cost) {
-    const double t = ceil((double)cost * (1.0 / (double)kTarget));
-    return t < (double)kLeast ? kLeast : (uint32_t)t;
+/* Tiles a part: items are cut so that the device is full and its workgroups'
+ * ends do not lie far apart. */
+struct Lengths {
+    uint32_t few, many;
+};
+
+__device__ __forceinline__ uint32_t tiles_for(uint64_t cost, uint32_t parts) {
+    return (uint32_t)ceil((double)cost / (double)parts);
+}
+
+__device__ __forceinline__ Lengths part_tiles(uint64_t cost) {
+    const uint32_t fine = tiles_for(cost, kParts), coarse = tiles_for(cost, kParts / 2u);
+    Lengths l;
+    l.few = coarse < kShort ? coarse : fine > kShort ? fine : kShort;
+    l.many = coarse;
+    l.few = l.few < kLeast ? kLeast : l.few;
+    l.many = l.many < kLeast ? kLeast : l.many;
+    return l;
+}
+
+__device__ __forceinline__ uint32_t length_of(const Lengths &l, uint32_t block) {
+    return block == kFew ? l.few : l.many;
 }
 
 __device__ __forceinline__ uint32_t parts_of(const Need &n, uint32_t length) {
@@ -125,16 +144,16 @@ __device__ __forceinline__ Part part_of(const Args &g, const kq::PagedSeq &s, co
     return p;
 }
 
-__device__ __forceinline__ uint64_t lanes_add(uint64_t v) {
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) v += __shfl_xor(v, d, KQ_WAVE);
+/* sums over the first `count` lanes (lane 0's is theirs), and over those before
+ * a lane; the others hold zeros */
+__device__ __forceinline__ uint64_t lanes_add(uint64_t v, uint32_t count) {
+    for (uint32_t d = 1u; d < count; d *= 2u) v += __shfl_xor(v, d, KQ_WAVE);
     return v;
 }
-__device__ __forceinline__ uint32_t lanes_before(uint32_t v) {
+__device__ __forceinline__ uint32_t lanes_before(uint32_t v, uint32_t count) {
     uint32_t sum = v;
     const uint32_t lane = threadIdx.x & 63u;
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
+    for (uint32_t d = 1u; d < count; d *= 2u) {
         const uint32_t o = __shfl_up(sum, d, KQ_WAVE);
         if (lane >= (uint32_t)d) sum += o;
     }
@@ -156,10 +175,13 @@ __device__ __forceinline__ Part find_part(const Args &g, uint32_t index, bool re
         if (lane < g.q.count) s = kq::paged_seq(g.q, g.c, lane, bad);
         if (report && bad) kq_flag(status, KQ_DEV_SEQUENCE);
         const Need n = need_of(g, s);
-        const uint32_t length = part_tiles(lanes_add(cost_of(g, n)));
-        const uint32_t each = parts_of(n, length), mine = n.blocks * g.c.heads * each;
-        const uint32_t first = lanes_before(mine);
-        const uint32_t first_slot = lanes_before(each > 1u ? mine : 0u);
+        const uint64_t cost = lanes_add(cost_of(g, n), g.q.count);
+        const Lengths length = part_tiles(
+            (uint64_t)__builtin_amdgcn_readfirstlane((uint32_t)(cost >> 32)) << 32 |
+            __builtin_amdgcn_readfirstlane((uint32_t)cost));
+        const uint32_t each = parts_of(n, length_of(length, rows_of_block(g, s.rows))), mine = n.blocks * g.c.heads * each;
+        const uint32_t first = lanes_before(mine, g.q.count);
+        const uint32_t first_slot = lanes_before(each > 1u ? mine : 0u, g.q.count);
         const uint64_t m = __ballot(index >= first && index - first < mine);
         if (m == 0ull) return p;
         const int at = __builtin_amdgcn_readfirstlane((int)__builtin_ctzll(m));
@@ -169,16 +191,17 @@ __device__ __forceinline__ Part find_part(const Args &g, uint32_t index, bool re
         w.past = __builtin_amdgcn_readlane(s.past, at);
         w.slot = __builtin_amdgcn_readlane(s.slot, at);
         w.live = true;
-        return part_of(g, w, need_of(g, w), __builtin_amdgcn_readfirstlane(length),
+        return part_of(g, w, need_of(g, w), length_of(length, rows_of_block(g, w.rows)),
                        index - __builtin_amdgcn_readlane(first, at),
                        __builtin_amdgcn_readlane(first_slot, at));
     } else {
         if (index >= g.plan[1]) return p;
-        const uint32_t *first = g.plan + 2u, *slots = first + g.q.count + 1u;
+        const uint32_t *first = g.plan + 3u, *slots = first + g.q.count + 1u;
         const uint32_t s = kq::wave_find(first, g.q.count, index);
         const kq::PagedSeq w = kq::paged_seq(g.q, g.c, s, bad);
         const Need n = need_of(g, w);
-        const uint32_t length = g.plan[0], u = index - first[s];
+        const uint32_t u = index - first[s];
+        const uint32_t length = g.plan[rows_of_block(g, w.rows) == kFew ? 0 : 2];
         if (u >= n.blocks * g.c.heads * parts_of(n, length)) return p; /* offsets not in order */
         return part_of(g, w, n, length, u, slots[s]);
     }
@@ -194,24 +217,25 @@ __global__ __launch_bounds__(1024) void plan_many(Args g, uint32_t *status) {
     for (uint32_t s = threadIdx.x; s < g.q.count; s += 1024u)
         cost += cost_of(g, need_of(g, kq::paged_seq(g.q, g.c, s, bad)));
     if (bad) kq_flag(status, KQ_DEV_SEQUENCE);
-    cost = lanes_add(cost);
+    cost = lanes_add(cost, 64u);
     if (lane == 0u) sums[wave] = cost;
     __syncthreads();
     cost = 0u;
     for (int w = 0; w < 16; ++w) cost += sums[w];
-    const uint32_t length = part_tiles(cost);
-    uint32_t *first = g.plan + 2u, *slot = first + g.q.count + 1u;
+    const Lengths length = part_tiles(cost);
+    uint32_t *first = g.plan + 3u, *slot = first + g.q.count + 1u;
     uint32_t parts_before = 0u, slots_before = 0u;
     for (uint32_t base = 0u; base < g.q.count; base += 1024u) {
         const uint32_t s = base + threadIdx.x;
         uint32_t mine = 0u, held = 0u;
         if (s < g.q.count) {
-            const Need n = need_of(g, kq::paged_seq(g.q, g.c, s, bad));
-            const uint32_t each = parts_of(n, length);
+            const kq::PagedSeq q = kq::paged_seq(g.q, g.c, s, bad);
+            const Need n = need_of(g, q);
+            const uint32_t each = parts_of(n, length_of(length, rows_of_block(g, q.rows)));
             mine = n.blocks * g.c.heads * each;
             held = each > 1u ? mine : 0u;
         }
-        const uint32_t p = lanes_before(mine), h = lanes_before(held);
+        const uint32_t p = lanes_before(mine, 64u), h = lanes_before(held, 64u);
         if (lane == 63u) {
             parts[wave] = p + mine;
             slots[wave] = h + held;
@@ -235,7 +259,8 @@ __global__ __launch_bounds__(1024) void plan_many(Args g, uint32_t *status) {
         __syncthreads();
     }
     if (threadIdx.x == 0u) {
-        g.plan[0] = length;
+        g.plan[0] = length.few;
+        g.plan[2] = length.many;
         g.plan[1] = parts_before;
         first[g.q.count] = parts_before;
         slot[g.q.count] = slots_before;
@@ -300,7 +325,7 @@ __device__ __forceinline__ void split(const float (&x)[8], e8<BF> (&t)[Type<BF>:
     }
 }
 
-/* A row's queries, as operands: the exponent's factor put in in binary64, and
+/* A row's queries, as operands: the exponent's factor put in to 48 bits, and
  * the row's largest value brought to 2^TOP by a power of two. */
 template <bool BF, int STEPS>
 struct Query {
@@ -312,7 +337,8 @@ struct Query {
 template <bool BF, int STEPS, int LANES, typename At>
 __device__ __forceinline__ void load_query(Query<BF, STEPS> &q, bool some, double factor, At at,
                                            bool &badin) {
-    float v[STEPS][8], top = 0.0f;
+    float v[STEPS][8];
+    uint32_t most = 0u; /* of the values' bits without the sign: orders them, and finds a NaN */
 #pragma unroll
     for (int s = 0; s < STEPS; ++s) {
         if (some) {
@@ -323,24 +349,29 @@ __device__ __forceinline__ void load_query(Query<BF, STEPS> &q, bool some, doubl
 #pragma unroll
             for (int i = 0; i < 8; ++i) v[s][i] = 0.0f;
         }
+    }
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s)
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            badin |= !kq_isfinite(v[s][i]);
-            top = fmaxf(top, fabsf(v[s][i]));
+            const uint32_t b = __float_as_uint(v[s][i]) & 0x7fffffffu;
+            most = b > most ? b : most;
         }
-    }
-    top = kq::lanes_max<LANES>(top);
+    badin |= most >= 0x7f800000u;
+    float top = kq::lanes_max<LANES>(__uint_as_float(most < 0x7f800000u ? most : 0u));
     /* the largest value's exponent, 0 for a row of zeros */
     int e = 0;
-    if (top > 0.0f && kq_isfinite(top)) e = ilogb((double)top * fabs(factor));
+    if (top > 0.0f) e = ilogb((double)top * fabs(factor));
     e = e < -100 ? -100 : e > 126 ? 126 : e;
+    /* the factor as two numbers: its own rounding would be the same for all keys */
     const double scale = __builtin_ldexp(factor, Type<BF>::TOP - e);
+    const float high = (float)scale, low = (float)(scale - (double)high);
     q.unscale = __builtin_ldexpf(1.0f, e - Type<BF>::TOP);
 #pragma unroll
     for (int s = 0; s < STEPS; ++s) {
         float x[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = (float)((double)v[s][i] * scale);
+        for (int i = 0; i < 8; ++i) x[i] = fmaf(v[s][i], high, v[s][i] * low);
         split<BF>(x, q.x[s]);
     }
 }
@@ -400,40 +431,43 @@ __device__ __forceinline__ void keep(const Args &g, float *slot, uint32_t row, u
 
 /* ------------------------------------------------------------------ pages */
 
-/* 16 keys from key `at` on (a multiple of 16) of the item's head: a descriptor
- * of the page's part, and the byte where the keys begin in it. `some`: whether
- * any of them is asked for; otherwise, and for a page that is none, nothing can
- * be read through it. */
+/* Pages of 16 keys from key `at` on (a multiple of 16), by scalar loads: the
+ * vector loads under way are not waited for. `some`: whether any of the keys is
+ * asked for; otherwise, and for a page that is none, the descriptor that comes
+ * of it lets nothing be read. */
+__device__ __forceinline__ uint32_t page_at(const Args &g, const Part &p, uint32_t at) {
+    typedef const __attribute__((address_space(4))) uint32_t *scalar_ptr;
+    const bool some = at < p.key1 && at + 16u > p.key0;
+    return some ? ((scalar_ptr)g.c.table)[(size_t)p.seq.slot * g.c.table_pages +
+                                          (at >> g.c.page_shift)]
+                : ~0u;
+}
+
 struct Place {
     const char *kp, *vp;
     uint32_t bytes, off;
-    __device__ __forceinline__ kq_i4v k() const { return dma_rsrc(kp, bytes); }
-    __device__ __forceinline__ kq_i4v v() const { return dma_rsrc(vp, bytes); }
 };
 
 template <int D>
-__device__ __forceinline__ Place place_of(const Args &g, const Part &p, uint32_t at, bool some,
+__device__ __forceinline__ Place place_of(const Args &g, const Part &p, uint32_t at, uint32_t page,
                                           bool &bad) {
     Place r;
-    uint32_t page = 0u, bytes = (D * 2u) << g.c.page_shift;
-    if (some) page = g.c.table[(size_t)p.seq.slot * g.c.table_pages + (at >> g.c.page_shift)];
-    if (page >= g.c.page_count) {
-        bad = true;
-        some = false;
-        page = 0u;
-    }
-    page = __builtin_amdgcn_readfirstlane(page);
-    const uint64_t off = ((uint64_t)page * g.c.heads + p.head) * bytes;
-    if (!some) bytes = 0u;
-    bytes = __builtin_amdgcn_readfirstlane(bytes);
+    const uint32_t bytes = (D * 2u) << g.c.page_shift;
+    const bool there = page < g.c.page_count;
+    bad |= !there && at < p.key1 && at + 16u > p.key0;
+    const uint64_t off = ((uint64_t)(there ? page : 0u) * g.c.heads + p.head) * bytes;
     r.kp = (const char *)g.c.keys + off;
     r.vp = (const char *)g.c.values + off;
-    r.bytes = bytes;
+    r.bytes = there ? bytes : 0u;
     r.off = (at & ((1u << g.c.page_shift) - 1u)) * (D * 2u);
     return r;
 }
 
-constexpr uint32_t kOut = 0xfffffff0u; /* an offset that no page has */
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_of(const char *p, uint32_t bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc((void *)p, 0, bytes, 0x00020000);
+}
+
+constexpr uint32_t kOut = 0x80000000u; /* an offset that no page has, nor what is added to it */
 
 /* ------------------------------------------------- few rows: keys shared out */
 
@@ -444,9 +478,19 @@ __device__ __forceinline__ uint32_t few_piece(uint32_t r, uint32_t c) {
     return D == 64 ? c ^ (2u * ((r >> 1) & 3u)) : c ^ (2u * (r & 7u));
 }
 
+/* 4 x 32 rows of V, or what the waves hand each other: sums of 16 rows, tops, totals */
 template <int D>
-constexpr uint32_t lds_bytes() {
-    return 512u * D; /* 4 waves x 2 x 32 rows of V, or 2 x 64 rows of K and V */
+constexpr uint32_t few_bytes() {
+    return kWaves * (16u * (D + 4u) * 4u + 128u);
+}
+template <int D>
+constexpr uint32_t many_bytes() {
+    return 512u * D; /* 2 x 64 rows of K and V */
+}
+/* workgroups a CU that registers allow */
+template <bool BF, int D>
+constexpr int few_side() {
+    return D == 256 ? 2 : D == 128 ? 3 : 4;
 }
 
 /* Up to 16 rows: a wave takes every fourth 32 keys, S' = K Q' and O' = V' P' of
@@ -466,51 +510,72 @@ __device__ __forceinline__ void few_rows(const Args &g, const Part &p, char *lds
 
     Query<BF, STEPS> q;
     const float *qp = g.a.q + (size_t)(p.seq.begin + token) * g.a.qs + (size_t)h * D + 8u * quarter;
-    load_query<BF, STEPS, 48>(q, some, g.exponent, [&](int s) { return qp + 32 * s; }, badin);
 
     f4 o[BLOCKS];
 #pragma unroll
     for (int b = 0; b < BLOCKS; ++b) o[b] = f4{0.0f, 0.0f, 0.0f, 0.0f};
     float top = kLowest, total = 0.0f;
 
-    const uint32_t mine = lds_addr(lds) + wave * (128u * D); /* 2 x 32 rows of V */
-    e8<BF> k[2][2][STEPS];
+    char *const mine = lds + wave * (64u * D); /* 32 rows of V */
+    const uint32_t mine_at = lds_addr(mine);
     uint32_t key = p.t0 * kTile + wave * 32u;
     const uint32_t end = p.t1 * kTile < p.key1 ? p.t1 * kTile : p.key1;
+    const bool any = key < end;
+    e8<BF> k[2][STEPS];
+    uint32_t page[2];
+    Place place[2];
 
-    auto load = [&](uint32_t at, uint32_t buf, e8<BF> (&kk)[2][STEPS]) {
+    auto pages = [&](uint32_t at) {
+#pragma unroll
+        for (uint32_t b = 0; b < 2u; ++b) page[b] = page_at(g, p, at + 16u * b);
+    };
+    auto places = [&](uint32_t at) {
+#pragma unroll
+        for (uint32_t b = 0; b < 2u; ++b)
+            place[b] = place_of<D>(g, p, at + 16u * b, page[b], badseq);
+    };
+    auto load_k = [&](uint32_t at) {
 #pragma unroll
         for (uint32_t b = 0; b < 2u; ++b) {
-            const uint32_t a16 = at + 16u * b;
-            const Place pl = place_of<D>(g, p, a16, a16 < p.key1 && a16 + 16u > p.key0, badseq);
-            /* V's 16 rows: D / 32 pieces of 1 KiB */
+            const uint32_t r = at + 16u * b + n;
+            const uint32_t off = r < p.key1 && r >= p.key0
+                                     ? place[b].off + n * (2u * D) + 16u * quarter : kOut;
+            const auto keys = buffer_of(place[b].kp, place[b].bytes);
 #pragma unroll
-            for (uint32_t j = 0; j < D / 32u; ++j) {
+            for (uint32_t s = 0; s < STEPS; ++s)
+                k[b][s] = __builtin_bit_cast(
+                    e8<BF>, __builtin_amdgcn_raw_buffer_load_b128(keys, off + 64u * s, 0, 0));
+        }
+    };
+    auto load_v = [&](uint32_t at) {
+#pragma unroll
+        for (uint32_t b = 0; b < 2u; ++b) {
+            const auto values = buffer_of(place[b].vp, place[b].bytes);
+#pragma unroll
+            for (uint32_t j = 0; j < D / 32u; ++j) { /* pieces of 1 KiB */
                 const uint32_t o16 = j * 64u + lane, r = o16 / (D / 8u), c = o16 % (D / 8u);
-                const bool in = a16 + r < p.key1 && a16 + r >= p.key0;
-                dma16(pl.v(), in ? pl.off + r * (2u * D) + few_piece<D>(r, c) * 16u : kOut,
-                      mine + buf * (64u * D) + b * (32u * D) + j * 1024u);
-            }
-            const bool in = a16 + n < p.key1 && a16 + n >= p.key0;
-            const auto keys = __builtin_amdgcn_make_buffer_rsrc((void *)pl.kp, 0, pl.bytes, 0x00020000);
-#pragma unroll
-            for (int s = 0; s < STEPS; ++s) {
-                const auto w = __builtin_amdgcn_raw_buffer_load_b128(
-                    keys, in ? pl.off + n * (2u * D) + 64u * s + 16u * quarter : kOut, 0, 0);
-                kk[b][s] = __builtin_bit_cast(e8<BF>, w);
+                const uint32_t key = at + 16u * b + r;
+                const uint32_t off = key < p.key1 && key >= p.key0
+                                         ? place[b].off + r * (2u * D) + few_piece<D>(r, c) * 16u
+                                         : kOut;
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(
+                    values,
+                    (__attribute__((address_space(3))) void *)(mine + b * (32u * D) + j * 1024u), 16,
+                    off, 0, 0, 0);
             }
         }
     };
-    auto compute = [&](uint32_t at, uint32_t buf, const e8<BF> (&kk)[2][STEPS]) {
-        f4 s[2];
+    auto scores = [&](f4 (&s)[2]) {
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
             s[b] = f4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int t = 0; t < STEPS; ++t)
 #pragma unroll
-                for (int m = 0; m < TERMS; ++m) s[b] = mma(kk[b][t], q.x[t][m], s[b]);
+                for (int m = 0; m < TERMS; ++m) s[b] = mma(k[b][t], q.x[t][m], s[b]);
         }
+    };
+    auto weights = [&](uint32_t at, const f4 (&s)[2], e8<BF> (&pw)[TERMS]) {
         float w[8];
         float peak = kLowest;
 #pragma unroll
@@ -535,12 +600,13 @@ __device__ __forceinline__ void few_rows(const Args &g, const Part &p, char *lds
             sum += w[i];
         }
         total += sum;
-        e8<BF> pw[TERMS];
         split<BF>(w, pw);
+    };
+    auto gather = [&](const e8<BF> (&pw)[TERMS]) {
 #pragma unroll
         for (uint32_t b = 0; b < BLOCKS; ++b) {
             const uint32_t r = 4u * quarter + n / 4u;
-            const uint32_t a = mine + buf * (64u * D) + r * (2u * D) +
+            const uint32_t a = mine_at + r * (2u * D) +
                                few_piece<D>(r, 2u * b + (n % 4u) / 2u) * 16u + (n & 1u) * 8u;
             const e8<BF> v = join8<BF>(transposed(a), transposed(a + 32u * D));
 #pragma unroll
@@ -548,22 +614,33 @@ __device__ __forceinline__ void few_rows(const Args &g, const Part &p, char *lds
         }
     };
 
-    if (key < end) {
-        load(key, 0u, k[0]);
-        for (;;) {
-            wait_vm<0>();
-            if (key + 128u < end) load(key + 128u, 1u, k[1]);
-            compute(key, 0u, k[0]);
-            key += 128u;
-            if (key >= end) break;
-            wait_lgkm0();
-            wait_vm<0>();
-            if (key + 128u < end) load(key + 128u, 0u, k[0]);
-            compute(key, 1u, k[1]);
-            key += 128u;
-            if (key >= end) break;
-            wait_lgkm0();
+    if (any) {
+        pages(key);
+        places(key);
+        load_k(key);
+        load_v(key);
+        if (key + 128u < end) pages(key + 128u);
+    }
+    load_query<BF, STEPS, 48>(q, some, g.exponent, [&](int s) { return qp + 32 * s; }, badin);
+    /* K of the next keys is asked for when this one's is used, V likewise: while
+     * one waits the CU's other workgroups read */
+    while (key < end) {
+        const uint32_t next = key + 128u;
+        f4 s[2];
+        e8<BF> pw[TERMS];
+        scores(s);
+        if (next < end) {
+            places(next);
+            load_k(next);
+            if (next + 128u < end) pages(next + 128u);
         }
+        weights(key, s, pw);
+        gather(pw);
+        if (next < end) {
+            wait_lgkm0(); /* V is read */
+            load_v(next);
+        }
+        key = next;
     }
     total = kq::lanes_sum<48>(total);
 
@@ -660,15 +737,16 @@ __device__ __forceinline__ void many_rows(const Args &g, const Part &p, char *ld
     /* the wave's 16 keys of a tile, K and V: D / 32 pieces of 1 KiB each */
     auto load = [&](uint32_t t, uint32_t buf) {
         const uint32_t a16 = t * kTile + wave * 16u;
-        const Place pl = place_of<D>(g, p, a16, a16 < p.key1 && a16 + 16u > p.key0, badseq);
+        const Place pl = place_of<D>(g, p, a16, page_at(g, p, a16), badseq);
+        const kq_i4v keys = dma_rsrc(pl.kp, pl.bytes), values = dma_rsrc(pl.vp, pl.bytes);
         const uint32_t to = base + buf * (256u * D) + wave * (32u * D);
 #pragma unroll
         for (uint32_t j = 0; j < D / 32u; ++j) {
             const uint32_t o16 = j * 64u + lane, r = o16 / (D / 8u), c = o16 % (D / 8u);
             const bool in = a16 + r < p.key1 && a16 + r >= p.key0;
             const uint32_t a = pl.off + r * (2u * D);
-            dma16(pl.k(), in ? a + k_piece<D>(r, c) * 16u : kOut, to + j * 1024u);
-            dma16(pl.v(), in ? a + v_piece<D>(r, c) * 16u : kOut, to + 128u * D + j * 1024u);
+            dma16(keys, in ? a + k_piece<D>(r, c) * 16u : kOut, to + j * 1024u);
+            dma16(values, in ? a + v_piece<D>(r, c) * 16u : kOut, to + 128u * D + j * 1024u);
         }
     };
     auto compute = [&](uint32_t t, uint32_t buf) {
@@ -759,9 +837,23 @@ __device__ __forceinline__ void many_rows(const Args &g, const Part &p, char *ld
         }
 }
 
+/* calls whose items all have few rows, as where every sequence decodes */
+template <bool BF, int D, bool MANY>
+__global__ __launch_bounds__(kThreads, (few_side<BF, D>())) void attend_few(Args g,
+                                                                            uint32_t *status) {
+    __shared__ __attribute__((aligned(16))) char lds[few_bytes<D>()];
+    const Part p = find_part<MANY>(g, blockIdx.x, blockIdx.x == 0u, status);
+    if (!p.live) return;
+    bool badin = false, bad = false, badseq = false;
+    few_rows<BF, D>(g, p, lds, badin, bad, badseq);
+    if (badseq) kq_flag(status, KQ_DEV_SEQUENCE);
+    if (badin) kq_flag(status, KQ_DEV_INPUT);
+    if (bad) kq_flag(status, KQ_DEV_NUMERIC);
+}
+
 template <bool BF, int D, bool MANY>
 __global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void attend(Args g, uint32_t *status) {
-    __shared__ __attribute__((aligned(16))) char lds[lds_bytes<D>()];
+    __shared__ __attribute__((aligned(16))) char lds[many_bytes<D>()];
     const Part p = find_part<MANY>(g, blockIdx.x, blockIdx.x == 0u, status);
     if (!p.live) return;
     bool badin = false, bad = false, badseq = false;
@@ -849,12 +941,13 @@ Sizes sizes_of(const kq_launch_pattn &a, const kq_launch_paged &c, const kq_laun
     z.slot_rows = (single ? group : rows) <= kFew ? kFew : kMany;
     z.items = c.heads * (single ? q.count * ((group + z.slot_rows - 1u) / z.slot_rows)
                                 : rows / kMany + q.count);
-    z.parts = kTarget + z.items;
-    /* an item of w tiles has at most w / kLeast + 1 parts */
+    /* all items' tiles / tiles a part <= kParts, and an item of w tiles has at
+     * most w / kLeast + 1 parts; only items of two parts or more have slots */
     const uint64_t tiles = (((uint64_t)c.table_pages << c.page_shift) + kTile - 1u) / kTile;
     const uint64_t most = z.items * (tiles / kLeast + 1u);
+    z.parts = most < kParts + z.items ? most : kParts + z.items;
     z.slots = most < kSlots ? most : kSlots;
-    z.plan_bytes = q.count > kByLane ? ((2u + 2u * (q.count + 1u)) * 4u + 255u) / 256u * 256u : 0u;
+    z.plan_bytes = q.count > kByLane ? ((3u + 2u * (q.count + 1u)) * 4u + 255u) / 256u * 256u : 0u;
     z.bytes = z.plan_bytes + z.slots * z.slot_rows * (c.width + 2u) * 4u;
     return z;
 }
@@ -866,9 +959,13 @@ hipError_t launch(const Args &g, uint32_t parts, uint32_t *status, hipStream_t s
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess) return e;
     }
-#define KQ_ATTEND(BF, D)                                                                    \
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(attend<BF, D, MANY>), dim3(parts), dim3(kThreads), 0, s, g, \
-                       status)
+#define KQ_ATTEND(BF, D)                                                                     \
+    if (g.slot_rows == kFew)                                                                 \
+        hipLaunchKernelGGL(HIP_KERNEL_NAME(attend_few<BF, D, MANY>), dim3(parts), dim3(kThreads), \
+                           0, s, g, status);                                                 \
+    else                                                                                     \
+        hipLaunchKernelGGL(HIP_KERNEL_NAME(attend<BF, D, MANY>), dim3(parts), dim3(kThreads), 0, s, \
+                           g, status)
     switch (g.c.width * 2u + (g.c.bf16 ? 1u : 0u)) {
     case 128u: KQ_ATTEND(false, 64); break;
     case 129u: KQ_ATTEND(true, 64); break;
