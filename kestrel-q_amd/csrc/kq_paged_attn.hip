@@ -15,7 +15,7 @@ typedef short s4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) char lds_char;
 
-constexpr int kThreads = 256, kWaves = 4;
+constexpr int kThreads = 256;
 constexpr uint32_t kTile = 64;       /* keys of a tile */
 constexpr uint32_t kFew = 16;        /* rows of an item whose waves share out its keys */
 constexpr uint32_t kMany = 128;      /* rows of an item whose waves share out its rows */
@@ -307,22 +307,37 @@ __device__ __forceinline__ f16v mma(e8<true> a, e8<true> b, f16v c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
 }
 
-/* x[0..7] as TERMS operands whose sum it is */
+/* x[0..7] as TERMS operands whose sum it is: pairs at a time, which one
+ * instruction rounds and packs */
 template <bool BF>
 __device__ __forceinline__ void split(const float (&x)[8], e8<BF> (&t)[Type<BF>::TERMS]) {
-    typedef typename Type<BF>::e E;
+    typedef float f2 __attribute__((ext_vector_type(2)));
+    e2<BF> p[Type<BF>::TERMS][4];
 #pragma unroll
-    for (int i = 0; i < 8; i += 2) {
-        float a = x[i], b = x[i + 1];
+    for (int i = 0; i < 4; ++i) {
+        f2 v = f2{x[2 * i], x[2 * i + 1]};
 #pragma unroll
         for (int k = 0; k < Type<BF>::TERMS; ++k) {
-            const E p = (E)a, q = (E)b;
-            t[k][i] = p;
-            t[k][i + 1] = q;
-            a -= (float)p;
-            b -= (float)q;
+            p[k][i] = __builtin_convertvector(v, e2<BF>);
+            if constexpr (BF) {
+                const uint32_t u = __builtin_bit_cast(uint32_t, p[k][i]);
+                v -= f2{__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u)};
+            } else {
+                /* x less its rounded value, without converting that back */
+                const uint32_t u = __builtin_bit_cast(uint32_t, p[k][i]);
+                if (k + 1 < Type<BF>::TERMS) {
+                    f2 r;
+                    asm("v_fma_mix_f32 %0, -%1, 1.0, %2 op_sel_hi:[1,0,0]"
+                        : "=v"(r.x) : "v"(u), "v"(v.x));
+                    asm("v_fma_mix_f32 %0, -%1, 1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]"
+                        : "=v"(r.y) : "v"(u), "v"(v.y));
+                    v = r;
+                }
+            }
         }
     }
+#pragma unroll
+    for (int k = 0; k < Type<BF>::TERMS; ++k) t[k] = __builtin_bit_cast(e8<BF>, p[k]);
 }
 
 /* A row's queries, as operands: the exponent's factor put in to 48 bits, and
@@ -431,13 +446,14 @@ __device__ __forceinline__ void keep(const Args &g, float *slot, uint32_t row, u
 
 /* ------------------------------------------------------------------ pages */
 
-/* Pages of 16 keys from key `at` on (a multiple of 16), by scalar loads: the
- * vector loads under way are not waited for. `some`: whether any of the keys is
+/* Pages of KEYS keys from key `at` on (16 or 8, a multiple of that), by scalar
+ * loads: the vector loads under way are not waited for. `some`: whether any of the keys is
  * asked for; otherwise, and for a page that is none, the descriptor that comes
  * of it lets nothing be read. */
+template <uint32_t KEYS>
 __device__ __forceinline__ uint32_t page_at(const Args &g, const Part &p, uint32_t at) {
     typedef const __attribute__((address_space(4))) uint32_t *scalar_ptr;
-    const bool some = at < p.key1 && at + 16u > p.key0;
+    const bool some = at < p.key1 && at + KEYS > p.key0;
     return some ? ((scalar_ptr)g.c.table)[(size_t)p.seq.slot * g.c.table_pages +
                                           (at >> g.c.page_shift)]
                 : ~0u;
@@ -448,13 +464,13 @@ struct Place {
     uint32_t bytes, off;
 };
 
-template <int D>
+template <int D, uint32_t KEYS>
 __device__ __forceinline__ Place place_of(const Args &g, const Part &p, uint32_t at, uint32_t page,
                                           bool &bad) {
     Place r;
     const uint32_t bytes = (D * 2u) << g.c.page_shift;
     const bool there = page < g.c.page_count;
-    bad |= !there && at < p.key1 && at + 16u > p.key0;
+    bad |= !there && at < p.key1 && at + KEYS > p.key0;
     const uint64_t off = ((uint64_t)(there ? page : 0u) * g.c.heads + p.head) * bytes;
     r.kp = (const char *)g.c.keys + off;
     r.vp = (const char *)g.c.values + off;
@@ -478,10 +494,10 @@ __device__ __forceinline__ uint32_t few_piece(uint32_t r, uint32_t c) {
     return D == 64 ? c ^ (2u * ((r >> 1) & 3u)) : c ^ (2u * (r & 7u));
 }
 
-/* 4 x 32 rows of V, or what the waves hand each other: sums of 16 rows, tops, totals */
-template <int D>
+/* 32 rows of V a wave, or what the waves hand each other: sums of 16 rows, tops, totals */
+template <int D, int W>
 constexpr uint32_t few_bytes() {
-    return kWaves * (16u * (D + 4u) * 4u + 128u);
+    return W * (16u * (D + 4u) * 4u + 128u);
 }
 template <int D>
 constexpr uint32_t many_bytes() {
@@ -493,9 +509,9 @@ constexpr int few_side() {
     return D == 256 ? 2 : D == 128 ? 3 : 4;
 }
 
-/* Up to 16 rows: a wave takes every fourth 32 keys, S' = K Q' and O' = V' P' of
+/* Up to 16 rows: a wave takes every W-th 32 keys, S' = K Q' and O' = V' P' of
  * 16 x 16 x 32 products, and the waves' results are joined in LDS. */
-template <bool BF, int D>
+template <bool BF, int D, int W>
 __device__ __forceinline__ void few_rows(const Args &g, const Part &p, char *lds, bool &badin,
                                          bool &bad, bool &badseq) {
     constexpr int STEPS = D / 32, BLOCKS = D / 16, TERMS = Type<BF>::TERMS;
@@ -527,12 +543,12 @@ __device__ __forceinline__ void few_rows(const Args &g, const Part &p, char *lds
 
     auto pages = [&](uint32_t at) {
 #pragma unroll
-        for (uint32_t b = 0; b < 2u; ++b) page[b] = page_at(g, p, at + 16u * b);
+        for (uint32_t b = 0; b < 2u; ++b) page[b] = page_at<16u>(g, p, at + 16u * b);
     };
     auto places = [&](uint32_t at) {
 #pragma unroll
         for (uint32_t b = 0; b < 2u; ++b)
-            place[b] = place_of<D>(g, p, at + 16u * b, page[b], badseq);
+            place[b] = place_of<D, 16u>(g, p, at + 16u * b, page[b], badseq);
     };
     auto load_k = [&](uint32_t at) {
 #pragma unroll
@@ -619,20 +635,20 @@ __device__ __forceinline__ void few_rows(const Args &g, const Part &p, char *lds
         places(key);
         load_k(key);
         load_v(key);
-        if (key + 128u < end) pages(key + 128u);
+        if (key + 32u * W < end) pages(key + 32u * W);
     }
     load_query<BF, STEPS, 48>(q, some, g.exponent, [&](int s) { return qp + 32 * s; }, badin);
     /* K of the next keys is asked for when this one's is used, V likewise: while
      * one waits the CU's other workgroups read */
     while (key < end) {
-        const uint32_t next = key + 128u;
+        const uint32_t next = key + 32u * W;
         f4 s[2];
         e8<BF> pw[TERMS];
         scores(s);
         if (next < end) {
             places(next);
             load_k(next);
-            if (next + 128u < end) pages(next + 128u);
+            if (next + 32u * W < end) pages(next + 32u * W);
         }
         weights(key, s, pw);
         gather(pw);
@@ -645,7 +661,7 @@ __device__ __forceinline__ void few_rows(const Args &g, const Part &p, char *lds
     total = kq::lanes_sum<48>(total);
 
     /* the waves' tops, totals and sums [wave][row][d], then 16 rows by all */
-    float *tops = (float *)lds, *totals = tops + kWaves * 16, *sums = totals + kWaves * 16;
+    float *tops = (float *)lds, *totals = tops + W * 16, *sums = totals + W * 16;
     constexpr uint32_t kRow = D + 4u; /* rows 16 bytes apart in the banks */
     __syncthreads();
     if (quarter == 0u) {
@@ -657,15 +673,15 @@ __device__ __forceinline__ void few_rows(const Args &g, const Part &p, char *lds
         *(f4 *)(sums + (wave * 16u + n) * kRow + 16u * b + 4u * quarter) = o[b];
     __syncthreads();
     float *slot = p.parts > 1u ? slot_at(g, p.slot + p.part * p.step) : nullptr;
-    for (uint32_t i = threadIdx.x; i < p.rows * (D / 4u); i += kThreads) {
+    for (uint32_t i = threadIdx.x; i < p.rows * (D / 4u); i += 64u * W) {
         const uint32_t r = i / (D / 4u), d = i % (D / 4u) * 4u;
         float t = tops[r];
 #pragma unroll
-        for (int w = 1; w < kWaves; ++w) t = fmaxf(t, tops[w * 16 + r]);
+        for (int w = 1; w < W; ++w) t = fmaxf(t, tops[w * 16 + r]);
         f4 v = f4{0.0f, 0.0f, 0.0f, 0.0f};
         float l = 0.0f;
 #pragma unroll
-        for (int w = 0; w < kWaves; ++w) {
+        for (int w = 0; w < W; ++w) {
             const float f = __builtin_amdgcn_exp2f(tops[w * 16 + r] - t);
             l = fmaf(totals[w * 16 + r], f, l);
             const f4 x = *(const f4 *)(sums + (w * 16u + r) * kRow + d);
@@ -681,26 +697,54 @@ __device__ __forceinline__ void few_rows(const Args &g, const Part &p, char *lds
 
 /* ------------------------------------------------ many rows: rows shared out */
 
-/* where the 16-byte piece c of a row of K (read down 16 rows), or of V (read
- * 64 bytes of 8 rows, transposed) lies */
+/* Up to 128 rows: M of them a wave, whose K and V come into LDS once for all,
+ * two buffers of 64 keys. S' = K Q' and O' = V' P' of products of M x M: 32 (4
+ * waves) moves half the bytes out of LDS that 16 (8 waves) does, and 16 holds a
+ * head of 256 in the registers of two waves a SIMD, one of which multiplies
+ * while the other has exponentials to form. */
 template <int D>
-__device__ __forceinline__ uint32_t k_piece(uint32_t r, uint32_t c) {
-    return D == 64 ? c ^ ((r >> 1) & 7u) : c ^ (r & 15u);
-}
-template <int D>
-__device__ __forceinline__ uint32_t v_piece(uint32_t r, uint32_t c) {
-    return D == 64 ? c ^ (((r >> 1) & 1u) << 2) : c ^ ((r & 3u) << 2);
-}
+struct Many {
+    static constexpr int M = D == 256 ? 16 : 32;
+    static constexpr int W = kMany / M, THREADS = 64 * W;
+    static constexpr int KEYS = 64 / W;         /* that a wave brings in */
+    static constexpr int REGS = M * M / 64;     /* values of a block that a lane holds */
+    static constexpr int STEPS = D * M / 512;   /* products along a head */
+    static constexpr int BLOCKS = D / M;        /* of O */
+    static constexpr uint32_t ROW = 2 * D;      /* bytes */
+    static constexpr uint32_t LDS = 4u * kTile * ROW;
+    typedef float acc __attribute__((ext_vector_type(REGS)));
 
-/* Up to 128 rows, 32 of them a wave: K and V come into LDS once for all, two
- * buffers of 64 keys; S' = K Q' and O' = V' P' of 32 x 32 x 16 products. */
+    /* 16-byte pieces of a row's bytes are held at piece c ^ these: K's are read
+     * down 16 rows, V's 64 (32) bytes of 8 (16) rows at a time, transposed */
+    static __device__ __forceinline__ uint32_t k_swap(uint32_t r) {
+        return D == 64 ? (r >> 1) & 7u : r & 15u;
+    }
+    static __device__ __forceinline__ uint32_t v_swap(uint32_t r) {
+        if (M == 16) return few_piece<D>(r, 0u);
+        return D == 64 ? ((r >> 1) & 1u) << 2 : (r & 3u) << 2;
+    }
+    /* where a lane's piece `at` (of four values) of a partial result's rows lies */
+    static __device__ __forceinline__ uint32_t column(uint32_t piece, uint32_t lane) {
+        return M == 16 ? 16u * piece + 4u * (lane / 16u)
+                       : 32u * (piece / 4u) + 8u * (piece % 4u) + 4u * (lane / 32u);
+    }
+};
+
+template <uint32_t I>
+struct Buffer {
+    static constexpr uint32_t value = I;
+};
+
 template <bool BF, int D>
 __device__ __forceinline__ void many_rows(const Args &g, const Part &p, char *lds, bool &badin,
                                           bool &bad, bool &badseq) {
-    constexpr int STEPS = D / 16, BLOCKS = D / 32, TERMS = Type<BF>::TERMS;
+    typedef Many<D> T;
+    typedef typename T::acc acc;
+    constexpr int M = T::M, REGS = T::REGS, STEPS = T::STEPS, BLOCKS = T::BLOCKS;
+    constexpr int TERMS = Type<BF>::TERMS, SETS = kTile / M, LANES = M == 32 ? 32 : 48;
     const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64u);
-    const uint32_t n = lane & 31u, half = lane >> 5;
-    const uint32_t r0 = wave * 32u;
+    const uint32_t n = lane % M, part = lane / M;
+    const uint32_t r0 = wave * M;
     const bool some = r0 + n < p.rows;
     const uint32_t row = p.row0 + r0 + n, token = some ? row / g.group : 0u;
     const uint32_t h = p.head * g.group + (some ? row % g.group : 0u);
@@ -711,7 +755,7 @@ __device__ __forceinline__ void many_rows(const Args &g, const Part &p, char *ld
     const bool awake = r0 < p.rows;
     uint32_t see0 = 0u, see1 = 0u, all0 = 0u, all1 = 0u; /* any row; every row */
     if (awake) {
-        const uint32_t rl = (r0 + 32u < p.rows ? r0 + 31u : p.rows - 1u) + p.row0;
+        const uint32_t rl = (r0 + M < p.rows ? r0 + M - 1u : p.rows - 1u) + p.row0;
         const uint32_t ta = (p.row0 + r0) / g.group, tb = rl / g.group;
         const uint32_t pa = p.seq.past + ta + 1u, pb = p.seq.past + tb + 1u;
         see1 = g.a.causal ? pb : p.seq.past + p.seq.rows;
@@ -722,64 +766,76 @@ __device__ __forceinline__ void many_rows(const Args &g, const Part &p, char *ld
         }
     }
 
-    Query<BF, STEPS> q;
-    const float *qp = g.a.q + (size_t)(p.seq.begin + token) * g.a.qs + (size_t)h * D + 8u * half;
-    load_query<BF, STEPS, 32>(q, some, g.exponent, [&](int s) { return qp + 16 * s; }, badin);
+    const uint32_t base = lds_addr(lds);
+    /* the wave's keys of a tile, K and V: pieces of 1 KiB */
+    auto load = [&](uint32_t t, uint32_t buf) {
+        const uint32_t at = t * kTile + wave * T::KEYS;
+        const Place pl = place_of<D, T::KEYS>(g, p, at, page_at<T::KEYS>(g, p, at), badseq);
+        const kq_i4v keys = dma_rsrc(pl.kp, pl.bytes), values = dma_rsrc(pl.vp, pl.bytes);
+        const uint32_t to = base + buf * (2u * kTile * T::ROW) + wave * (T::KEYS * T::ROW);
+#pragma unroll
+        for (uint32_t j = 0; j < T::KEYS * T::ROW / 1024u; ++j) {
+            const uint32_t o16 = j * 64u + lane, r = o16 / (D / 8u), c = o16 % (D / 8u);
+            const uint32_t rt = wave * T::KEYS + r; /* of the tile */
+            const bool in = at + r < p.key1 && at + r >= p.key0;
+            const uint32_t a = pl.off + r * T::ROW;
+            dma16(keys, in ? a + (c ^ T::k_swap(rt)) * 16u : kOut, to + j * 1024u);
+            dma16(values, in ? a + (c ^ T::v_swap(rt)) * 16u : kOut,
+                  to + kTile * T::ROW + j * 1024u);
+        }
+    };
+    load(p.t0, 0u);
 
-    f16v o[BLOCKS];
+    Query<BF, STEPS> q;
+    const float *qp = g.a.q + (size_t)(p.seq.begin + token) * g.a.qs + (size_t)h * D + 8u * part;
+    load_query<BF, STEPS, LANES>(q, some, g.exponent, [&](int s) { return qp + 512 / M * s; }, badin);
+
+    acc o[BLOCKS];
 #pragma unroll
     for (int b = 0; b < BLOCKS; ++b)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) o[b][i] = 0.0f;
+        for (int i = 0; i < REGS; ++i) o[b][i] = 0.0f;
     float top = kLowest, total = 0.0f;
 
-    const uint32_t base = lds_addr(lds);
-    /* the wave's 16 keys of a tile, K and V: D / 32 pieces of 1 KiB each */
-    auto load = [&](uint32_t t, uint32_t buf) {
-        const uint32_t a16 = t * kTile + wave * 16u;
-        const Place pl = place_of<D>(g, p, a16, page_at(g, p, a16), badseq);
-        const kq_i4v keys = dma_rsrc(pl.kp, pl.bytes), values = dma_rsrc(pl.vp, pl.bytes);
-        const uint32_t to = base + buf * (256u * D) + wave * (32u * D);
+    /* K: row n of a block, 16 bytes; V: row `vr` of 16 (M 32: of 8), 8 bytes */
+    const uint32_t k_at = base + n * T::ROW + (T::k_swap(n) ^ part) * 16u;
+    const uint32_t vr = 4u * part + n % 16u / 4u;
+    const uint32_t v_at = base + kTile * T::ROW + vr * T::ROW +
+                          (T::v_swap(vr) ^ (n / 16u * 2u) ^ (n % 4u / 2u)) * 16u + (n & 1u) * 8u;
+    auto compute = [&](uint32_t t, auto buffer) {
+        constexpr uint32_t BUF = decltype(buffer)::value * 2u * kTile * T::ROW;
+        const uint32_t at = t * kTile;
+        acc s[SETS];
 #pragma unroll
-        for (uint32_t j = 0; j < D / 32u; ++j) {
-            const uint32_t o16 = j * 64u + lane, r = o16 / (D / 8u), c = o16 % (D / 8u);
-            const bool in = a16 + r < p.key1 && a16 + r >= p.key0;
-            const uint32_t a = pl.off + r * (2u * D);
-            dma16(keys, in ? a + k_piece<D>(r, c) * 16u : kOut, to + j * 1024u);
-            dma16(values, in ? a + v_piece<D>(r, c) * 16u : kOut, to + 128u * D + j * 1024u);
+        for (int b = 0; b < SETS; ++b)
+#pragma unroll
+            for (int i = 0; i < REGS; ++i) s[b][i] = 0.0f;
+#pragma unroll
+        for (uint32_t st = 0; st < STEPS; ++st) {
+            e8<BF> k[SETS];
+#pragma unroll
+            for (uint32_t b = 0; b < SETS; ++b)
+                k[b] = __builtin_bit_cast(
+                    e8<BF>, *(__attribute__((address_space(3))) u4 *)(uintptr_t)(
+                                (k_at ^ (64u / M * st * 16u)) + BUF + b * M * T::ROW));
+#pragma unroll
+            for (int m = 0; m < TERMS; ++m)
+#pragma unroll
+                for (uint32_t b = 0; b < SETS; ++b) s[b] = mma(k[b], q.x[st][m], s[b]);
         }
-    };
-    auto compute = [&](uint32_t t, uint32_t buf) {
-        const uint32_t kb = base + buf * (256u * D), vb = kb + 128u * D, at = t * kTile;
-        f16v s[2];
-#pragma unroll
-        for (int b = 0; b < 2; ++b)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) s[b][i] = 0.0f;
-#pragma unroll
-        for (uint32_t st = 0; st < STEPS; ++st)
-#pragma unroll
-            for (uint32_t b = 0; b < 2u; ++b) {
-                const uint32_t r = 32u * b + n;
-                const u4 w = *(__attribute__((address_space(3))) u4 *)(uintptr_t)(
-                    kb + r * (2u * D) + k_piece<D>(r, 2u * st + half) * 16u);
-                const e8<BF> k = __builtin_bit_cast(e8<BF>, w);
-#pragma unroll
-                for (int m = 0; m < TERMS; ++m) s[b] = mma(k, q.x[st][m], s[b]);
-            }
         if (at + kTile > all1 || at < all0) {
 #pragma unroll
-            for (uint32_t b = 0; b < 2u; ++b)
+            for (uint32_t b = 0; b < SETS; ++b)
 #pragma unroll
-                for (uint32_t i = 0; i < 16u; ++i) {
-                    const uint32_t key = at + 32u * b + 8u * (i / 4u) + 4u * half + i % 4u;
+                for (uint32_t i = 0; i < REGS; ++i) {
+                    const uint32_t key = at + M * b + 256u / M * (i / 4u) + 4u * part + i % 4u;
                     s[b][i] = key < last && key >= from ? s[b][i] : -INFINITY;
                 }
         }
         float peak = s[0][0];
 #pragma unroll
-        for (int i = 1; i < 32; ++i) peak = fmaxf(peak, s[i / 16][i % 16]);
-        peak = fmaxf(kq::lanes_max<32>(peak) * q.unscale, kLowest) - Type<BF>::LIFT;
+        for (int i = 1; i < SETS * REGS; ++i) peak = fmaxf(peak, s[i / REGS][i % REGS]);
+        peak = fmaxf(kq::lanes_max<LANES>(peak) * q.unscale, kLowest) - Type<BF>::LIFT;
         if (__any(peak > top + kSlack)) {
             const float next = fmaxf(top, peak);
             const float f = __builtin_amdgcn_exp2f(top - next);
@@ -789,76 +845,92 @@ __device__ __forceinline__ void many_rows(const Args &g, const Part &p, char *ld
             for (int b = 0; b < BLOCKS; ++b) o[b] *= f;
         }
         float sum = 0.0f;
+        constexpr uint32_t CHUNK = 512u / M; /* keys of a product */
 #pragma unroll
-        for (uint32_t c = 0; c < 4u; ++c) { /* 16 keys */
+        for (uint32_t c = 0; c < kTile / CHUNK; ++c) {
             float w[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                w[i] = __builtin_amdgcn_exp2f(fmaf(s[c / 2u][8u * (c % 2u) + i], q.unscale, -top));
+            for (uint32_t i = 0; i < 8u; ++i) {
+                /* M 32: half of a block; M 16: four values of each of two */
+                const uint32_t x = 8u * c + i;
+                w[i] = __builtin_amdgcn_exp2f(fmaf(s[x / REGS][x % REGS], q.unscale, -top));
                 sum += w[i];
             }
             e8<BF> pw[TERMS];
             split<BF>(w, pw);
 #pragma unroll
             for (uint32_t b = 0; b < BLOCKS; ++b) {
-                const uint32_t r = 16u * c + 4u * half + (n % 16u) / 4u;
-                const uint32_t a = vb + r * (2u * D) +
-                                   v_piece<D>(r, 4u * b + 2u * (n / 16u) + (n % 4u) / 2u) * 16u +
-                                   (n & 1u) * 8u;
-                const e8<BF> v = join8<BF>(transposed(a), transposed(a + 16u * D));
+                const uint32_t a = (v_at ^ (b * M * 2u)) + BUF + c * CHUNK * T::ROW;
+                const e8<BF> v = join8<BF>(transposed(a), transposed(a + CHUNK / 2u * T::ROW));
 #pragma unroll
                 for (int m = 0; m < TERMS; ++m) o[b] = mma(v, pw[m], o[b]);
             }
         }
         total += sum;
     };
-
-    load(p.t0, 0u);
-    for (uint32_t t = p.t0; t < p.t1; ++t) {
-        const uint32_t buf = (t - p.t0) & 1u;
+    auto step = [&](uint32_t t, auto buffer) {
         wait_vm<0>();
         __syncthreads(); /* the tile is there; the other buffer is read */
-        if (t + 1u < p.t1) load(t + 1u, buf ^ 1u);
-        if (awake && t * kTile < see1 && t * kTile + kTile > see0) compute(t, buf);
+        if (t + 1u < p.t1) load(t + 1u, 1u - decltype(buffer)::value);
+        if (t * kTile < see1 && t * kTile + kTile > see0) compute(t, buffer);
+    };
+    uint32_t t = p.t0;
+    for (; t + 1u < p.t1; t += 2u) {
+        step(t, Buffer<0u>{});
+        step(t + 1u, Buffer<1u>{});
+    }
+    if (t < p.t1) step(t, Buffer<0u>{});
+    total = kq::lanes_sum<LANES>(total);
+    if (p.parts > 1u) {
+        /* lane by lane, as join_parts reads it */
+        float *slot = slot_at(g, p.slot + p.part * p.step);
+        f4 *to = (f4 *)slot + wave * (M * D / 4u) + lane;
+#pragma unroll
+        for (uint32_t k = 0; k < BLOCKS * REGS / 4u; ++k) {
+            const uint32_t b = k / (REGS / 4u), i = k % (REGS / 4u) * 4u;
+            to[k * 64u] = f4{o[b][i], o[b][i + 1], o[b][i + 2], o[b][i + 3]};
+        }
+        if (part == 0u) {
+            float *m = slot + (size_t)kMany * D;
+            m[r0 + n] = top;
+            m[kMany + r0 + n] = total;
+        }
+        return;
     }
     if (!some) return;
-    total = kq::lanes_sum<32>(total);
-    float *slot = p.parts > 1u ? slot_at(g, p.slot + p.part * p.step) : nullptr;
 #pragma unroll
-    for (uint32_t b = 0; b < BLOCKS; ++b)
-#pragma unroll
-        for (uint32_t i = 0; i < 4u; ++i) {
-            const f4 v = f4{o[b][4 * i], o[b][4 * i + 1], o[b][4 * i + 2], o[b][4 * i + 3]};
-            const uint32_t d = 32u * b + 8u * i + 4u * half;
-            if (slot != nullptr)
-                keep(g, slot, r0 + n, d, D, v, top, total);
-            else
-                put(g, p.seq, p.head, row, d, D, v, top, total, badin, bad);
-        }
+    for (uint32_t k = 0; k < BLOCKS * REGS / 4u; ++k) {
+        const uint32_t b = k / (REGS / 4u), i = k % (REGS / 4u) * 4u;
+        put(g, p.seq, p.head, row, T::column(k, lane), D,
+            f4{o[b][i], o[b][i + 1], o[b][i + 2], o[b][i + 3]}, top, total, badin, bad);
+    }
 }
 
 /* calls whose items all have few rows, as where every sequence decodes */
 template <bool BF, int D, bool MANY>
 __global__ __launch_bounds__(kThreads, (few_side<BF, D>())) void attend_few(Args g,
                                                                             uint32_t *status) {
-    __shared__ __attribute__((aligned(16))) char lds[few_bytes<D>()];
+    __shared__ __attribute__((aligned(16))) char lds[few_bytes<D, 4>()];
     const Part p = find_part<MANY>(g, blockIdx.x, blockIdx.x == 0u, status);
     if (!p.live) return;
     bool badin = false, bad = false, badseq = false;
-    few_rows<BF, D>(g, p, lds, badin, bad, badseq);
+    few_rows<BF, D, 4>(g, p, lds, badin, bad, badseq);
     if (badseq) kq_flag(status, KQ_DEV_SEQUENCE);
     if (badin) kq_flag(status, KQ_DEV_INPUT);
     if (bad) kq_flag(status, KQ_DEV_NUMERIC);
 }
 
 template <bool BF, int D, bool MANY>
-__global__ __launch_bounds__(kThreads, D == 256 ? 1 : 2) void attend(Args g, uint32_t *status) {
-    __shared__ __attribute__((aligned(16))) char lds[many_bytes<D>()];
+__global__ __launch_bounds__(Many<D>::THREADS, 2) void attend(Args g, uint32_t *status) {
+    constexpr int W = Many<D>::W;
+    constexpr uint32_t BYTES = Many<D>::LDS > few_bytes<D, W>() ? Many<D>::LDS : few_bytes<D, W>();
+    /* a row's pieces are found by flipping address bits below its size */
+    __shared__ __attribute__((aligned(1024))) char lds[BYTES];
     const Part p = find_part<MANY>(g, blockIdx.x, blockIdx.x == 0u, status);
     if (!p.live) return;
     bool badin = false, bad = false, badseq = false;
     if (p.block == kFew)
-        few_rows<BF, D>(g, p, lds, badin, bad, badseq);
+        few_rows<BF, D, W>(g, p, lds, badin, bad, badseq);
     else
         many_rows<BF, D>(g, p, lds, badin, bad, badseq);
     if (badseq) kq_flag(status, KQ_DEV_SEQUENCE);
@@ -875,7 +947,11 @@ __global__ __launch_bounds__(kThreads) void join_parts(Args g, uint32_t *status)
     const Part p = find_part<MANY>(g, blockIdx.x, false, status);
     if (!p.live || p.parts < 2u) return;
     bool badin = false, bad = false;
-    const uint32_t width = g.c.width, pieces = p.rows * (width / 4u);
+    /* pieces of four values, in the slots' order: by rows, or by waves and lanes */
+    const uint32_t width = g.c.width, tall = width == 256u ? Many<256>::M : Many<128>::M;
+    const bool by_rows = p.block == kFew;
+    const uint32_t pieces =
+        (by_rows ? p.rows : (p.rows + tall - 1u) / tall * tall) * (width / 4u);
     const uint32_t a = (uint32_t)((uint64_t)pieces * p.part / p.parts);
     const uint32_t b = (uint32_t)((uint64_t)pieces * (p.part + 1u) / p.parts);
     /* side by side: pieces in the threads' low bits, parts in the high ones */
@@ -885,15 +961,21 @@ __global__ __launch_bounds__(kThreads) void join_parts(Args g, uint32_t *status)
     const uint32_t mine = threadIdx.x % wide, group = threadIdx.x / wide;
     for (uint32_t at = a; at < b; at += wide) {
         const uint32_t i = at + mine;
-        const uint32_t row = i / (width / 4u), d = i % (width / 4u) * 4u;
+        uint32_t row = i / (width / 4u), d = i % (width / 4u) * 4u;
+        if (!by_rows) {
+            const uint32_t lane = i % 64u, piece = i / 64u % (tall * width / 256u);
+            row = i / (tall * width / 4u) * tall + lane % tall;
+            d = tall == 16u ? Many<256>::column(piece, lane) : Many<128>::column(piece, lane);
+        }
+        const bool mine_too = i < b && row < p.rows;
         f4 v = f4{0.0f, 0.0f, 0.0f, 0.0f};
         float top = kLowest, total = 0.0f;
-        if (i < b)
+        if (mine_too)
             for (uint32_t k = group; k < p.parts; k += groups) {
                 const float *slot = slot_at(g, p.slot + k * p.step);
                 const float *m = slot + (size_t)g.slot_rows * width;
                 const float t = m[row], l = m[g.slot_rows + row];
-                const f4 x = *(const f4 *)(slot + (size_t)row * width + d);
+                const f4 x = *((const f4 *)slot + i);
                 const float next = fmaxf(top, t);
                 const float f = __builtin_amdgcn_exp2f(top - next), e = __builtin_amdgcn_exp2f(t - next);
                 top = next;
@@ -918,7 +1000,7 @@ __global__ __launch_bounds__(kThreads) void join_parts(Args g, uint32_t *status)
                 for (int c = 0; c < 4; ++c) v[c] = fmaf(v[c], f, x[c] * e);
             }
         }
-        if (group == 0u && i < b)
+        if (group == 0u && mine_too)
             put(g, p.seq, p.head, p.row0 + row, d, width, v, top, total, badin, bad);
     }
     if (badin) kq_flag(status, KQ_DEV_INPUT);
@@ -964,8 +1046,8 @@ hipError_t launch(const Args &g, uint32_t parts, uint32_t *status, hipStream_t s
         hipLaunchKernelGGL(HIP_KERNEL_NAME(attend_few<BF, D, MANY>), dim3(parts), dim3(kThreads), \
                            0, s, g, status);                                                 \
     else                                                                                     \
-        hipLaunchKernelGGL(HIP_KERNEL_NAME(attend<BF, D, MANY>), dim3(parts), dim3(kThreads), 0, s, \
-                           g, status)
+        hipLaunchKernelGGL(HIP_KERNEL_NAME(attend<BF, D, MANY>), dim3(parts),                \
+                           dim3(Many<D>::THREADS), 0, s, g, status)
     switch (g.c.width * 2u + (g.c.bf16 ? 1u : 0u)) {
     case 128u: KQ_ATTEND(false, 64); break;
     case 129u: KQ_ATTEND(true, 64); break;
