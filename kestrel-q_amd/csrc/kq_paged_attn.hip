@@ -35,6 +35,7 @@ struct Args {
     uint32_t slot_rows; /* rows that a slot of the partial results holds */
     uint32_t slots;
     double exponent;    /* scale log2(e) */
+    struct Item *items; /* of each workgroup, for the join */
     float *partial;     /* slots of [slot_rows][width] sums, then tops, then totals */
     uint32_t *plan;     /* tiles a part of few rows, parts, tiles a part of many rows; then first
                            parts, then first slots of the sequences */
@@ -96,8 +97,12 @@ __device__ __forceinline__ uint32_t length_of(const Lengths &l, uint32_t block) 
     return block == kFew ? l.few : l.many;
 }
 
-__device__ __forceinline__ uint32_t parts_of(const Need &n, uint32_t length) {
-    return n.tiles == 0u ? 0u : (n.tiles + length - 1u) / length;
+/* parts of so many tiles, the nearest number: an item a little longer than a
+ * part stays whole. Of `length` and 1.5 times that, and at least 2, tiles. */
+__device__ __forceinline__ uint32_t parts_of(uint32_t tiles, uint32_t length) {
+    if (tiles == 0u) return 0u;
+    const uint32_t n = (tiles + length / 2u) / length;
+    return n == 0u ? 1u : n;
 }
 
 /* One part of the work */
@@ -111,20 +116,48 @@ struct Part {
     uint32_t key0, key1;  /* keys that any of the item's rows sees */
     uint32_t slot, step;  /* of the item's first part, and between two parts */
     bool live;
+
+    /* what all lanes hold alike goes into scalar registers, as the descriptors
+     * of the loads into LDS need it */
+    __device__ __forceinline__ void pin() {
+        uint32_t *const all[] = {&seq.begin, &seq.rows, &seq.past, &seq.slot, &row0, &rows, &block,
+                                 &head, &part, &parts, &t0, &t1, &key0, &key1, &slot, &step};
+#pragma unroll
+        for (uint32_t *x : all) *x = __builtin_amdgcn_readfirstlane(*x);
+    }
 };
+
+/* What the join has to know of a part: its item's rows, and where its item's
+ * partial results lie. Every workgroup of the first launch leaves one. */
+struct __attribute__((aligned(16))) Item {
+    uint32_t begin, row0, rows, head_few; /* rows 0: nothing to join; few: the upper half */
+    uint32_t part, parts, slot, step;
+};
+
+__device__ __forceinline__ void leave(const Args &g, const Part &p) {
+    if (threadIdx.x == 0u) {
+        Item t = {0u, 0u, 0u, 0u, 0u, 0u, 0u, 0u};
+        if (p.live && p.parts > 1u)
+            t = {p.seq.begin, p.row0, p.rows, p.head | (p.block == kFew ? 1u << 16 : 0u),
+                 p.part, p.parts, p.slot, p.step};
+        g.items[blockIdx.x] = t;
+    }
+}
 
 __device__ __forceinline__ Part part_of(const Args &g, const kq::PagedSeq &s, const Need &n,
                                         uint32_t length, uint32_t u, uint32_t first_slot) {
     Part p;
     p.seq = s;
     p.block = rows_of_block(g, s.rows);
-    const uint32_t parts = parts_of(n, length);
-    p.head = u % g.c.heads;
-    u /= g.c.heads;
-    p.part = u % parts;
-    u /= parts;
-    /* the last rows, which see the most keys, first */
-    p.row0 = (n.blocks - 1u - u) * p.block;
+    /* Workgroups go to the XCDs in turn, so neighbours in number should have
+     * work alike: heads, then blocks, whose last rows see the most keys and go
+     * first, then parts, of which an item may have fewer than its sequence. (With
+     * the parts before the blocks 2049 rows of 4 heads of 256 took 323 us in place
+     * of 224: one half of the XCDs had the second parts, most of them none.) */
+    const uint32_t items = n.blocks * g.c.heads, item = u % items;
+    p.part = u / items;
+    p.head = item % g.c.heads;
+    p.row0 = (n.blocks - 1u - item / g.c.heads) * p.block;
     const uint32_t all = s.rows * g.group;
     p.rows = all - p.row0 < p.block ? all - p.row0 : p.block;
     const uint32_t ta = p.row0 / g.group, tb = (p.row0 + p.rows - 1u) / g.group;
@@ -132,40 +165,58 @@ __device__ __forceinline__ Part part_of(const Args &g, const kq::PagedSeq &s, co
     p.key0 = 0u;
     if (g.a.window != 0u && s.past + ta + 1u > g.a.window) p.key0 = s.past + ta + 1u - g.a.window;
     const uint32_t a = p.key0 / kTile, tiles = (p.key1 + kTile - 1u) / kTile - a;
-    p.parts = (tiles + length - 1u) / length;
-    const uint32_t each = (tiles + p.parts - 1u) / p.parts;
-    p.t0 = a + p.part * each;
-    p.t1 = p.t0 + each < a + tiles ? p.t0 + each : a + tiles;
-    p.slot = first_slot + u * parts * g.c.heads + p.head;
-    p.step = g.c.heads;
+    p.parts = parts_of(tiles, length);
+    const uint32_t each = tiles / p.parts, more = tiles % p.parts;
+    p.t0 = a + p.part * each + (p.part < more ? p.part : more);
+    p.t1 = p.t0 + each + (p.part < more ? 1u : 0u);
+    p.slot = first_slot + item;
+    p.step = items;
     /* offsets that overlap could ask for more slots than there are */
     p.live = p.part < p.parts &&
              (p.parts == 1u || p.slot + (p.parts - 1u) * p.step < g.slots);
     return p;
 }
 
-/* sums over the first `count` lanes (lane 0's is theirs), and over those before
- * a lane; the others hold zeros */
-__device__ __forceinline__ uint64_t lanes_add(uint64_t v, uint32_t count) {
-    for (uint32_t d = 1u; d < count; d *= 2u) v += __shfl_xor(v, d, KQ_WAVE);
-    return v;
+
+/* x of the lane that CTRL (a DPP control) names, 0 where there is none or ROWS
+ * leaves the row of 16 lanes out */
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t lane_from(uint32_t x) {
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, ROWS, 0xf, false);
 }
-__device__ __forceinline__ uint32_t lanes_before(uint32_t v, uint32_t count) {
-    uint32_t sum = v;
-    const uint32_t lane = threadIdx.x & 63u;
-    for (uint32_t d = 1u; d < count; d *= 2u) {
-        const uint32_t o = __shfl_up(sum, d, KQ_WAVE);
-        if (lane >= (uint32_t)d) sum += o;
-    }
-    return sum - v;
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t lane_add(uint32_t x) {
+    return x + lane_from<CTRL, ROWS>(x);
+}
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint64_t lane_add(uint64_t x) {
+    return x + ((uint64_t)lane_from<CTRL, ROWS>((uint32_t)(x >> 32)) << 32 |
+                lane_from<CTRL, ROWS>((uint32_t)x));
+}
+/* v of the lanes up to and with this one: within rows of 16, then row 0's end to
+ * row 1 and 2's to 3, then the lower half's end to the upper half */
+template <typename T>
+__device__ __forceinline__ T lanes_through(T v) {
+    v = lane_add<0x111, 0xf>(v);
+    v = lane_add<0x112, 0xf>(v);
+    v = lane_add<0x114, 0xf>(v);
+    v = lane_add<0x118, 0xf>(v);
+    v = lane_add<0x142, 0xa>(v);
+    return lane_add<0x143, 0xc>(v);
+}
+__device__ __forceinline__ uint32_t lanes_before(uint32_t v) { return lanes_through(v) - v; }
+/* v of all lanes */
+__device__ __forceinline__ uint64_t lanes_add(uint64_t v) {
+    v = lanes_through(v);
+    return (uint64_t)__builtin_amdgcn_readlane((uint32_t)(v >> 32), 63) << 32 |
+           __builtin_amdgcn_readlane((uint32_t)v, 63);
 }
 
 /* Part `index` of the call, the same in all lanes. Up to kByLane sequences:
  * a lane looks at each, and every wave adds up for itself. More: plan_many
  * has done so. */
 template <bool MANY>
-__device__ __forceinline__ Part find_part(const Args &g, uint32_t index, bool report,
-                                          uint32_t *status) {
+__device__ __forceinline__ Part find_part(const Args &g, uint32_t index, uint32_t *status) {
     Part p;
     p.live = false;
     bool bad = false;
@@ -173,15 +224,12 @@ __device__ __forceinline__ Part find_part(const Args &g, uint32_t index, bool re
         const uint32_t lane = threadIdx.x & 63u;
         kq::PagedSeq s = {0u, 0u, 0u, 0u, false};
         if (lane < g.q.count) s = kq::paged_seq(g.q, g.c, lane, bad);
-        if (report && bad) kq_flag(status, KQ_DEV_SEQUENCE);
+        if (index == 0u && bad) kq_flag(status, KQ_DEV_SEQUENCE);
         const Need n = need_of(g, s);
-        const uint64_t cost = lanes_add(cost_of(g, n), g.q.count);
-        const Lengths length = part_tiles(
-            (uint64_t)__builtin_amdgcn_readfirstlane((uint32_t)(cost >> 32)) << 32 |
-            __builtin_amdgcn_readfirstlane((uint32_t)cost));
-        const uint32_t each = parts_of(n, length_of(length, rows_of_block(g, s.rows))), mine = n.blocks * g.c.heads * each;
-        const uint32_t first = lanes_before(mine, g.q.count);
-        const uint32_t first_slot = lanes_before(each > 1u ? mine : 0u, g.q.count);
+        const Lengths length = part_tiles(lanes_add(cost_of(g, n)));
+        const uint32_t each = parts_of(n.tiles, length_of(length, rows_of_block(g, s.rows))), mine = n.blocks * g.c.heads * each;
+        const uint32_t first = lanes_before(mine);
+        const uint32_t first_slot = lanes_before(each > 1u ? mine : 0u);
         const uint64_t m = __ballot(index >= first && index - first < mine);
         if (m == 0ull) return p;
         const int at = __builtin_amdgcn_readfirstlane((int)__builtin_ctzll(m));
@@ -202,7 +250,7 @@ __device__ __forceinline__ Part find_part(const Args &g, uint32_t index, bool re
         const Need n = need_of(g, w);
         const uint32_t u = index - first[s];
         const uint32_t length = g.plan[rows_of_block(g, w.rows) == kFew ? 0 : 2];
-        if (u >= n.blocks * g.c.heads * parts_of(n, length)) return p; /* offsets not in order */
+        if (u >= n.blocks * g.c.heads * parts_of(n.tiles, length)) return p; /* offsets not in order */
         return part_of(g, w, n, length, u, slots[s]);
     }
 }
@@ -217,7 +265,7 @@ __global__ __launch_bounds__(1024) void plan_many(Args g, uint32_t *status) {
     for (uint32_t s = threadIdx.x; s < g.q.count; s += 1024u)
         cost += cost_of(g, need_of(g, kq::paged_seq(g.q, g.c, s, bad)));
     if (bad) kq_flag(status, KQ_DEV_SEQUENCE);
-    cost = lanes_add(cost, 64u);
+    cost = lanes_add(cost);
     if (lane == 0u) sums[wave] = cost;
     __syncthreads();
     cost = 0u;
@@ -231,11 +279,11 @@ __global__ __launch_bounds__(1024) void plan_many(Args g, uint32_t *status) {
         if (s < g.q.count) {
             const kq::PagedSeq q = kq::paged_seq(g.q, g.c, s, bad);
             const Need n = need_of(g, q);
-            const uint32_t each = parts_of(n, length_of(length, rows_of_block(g, q.rows)));
+            const uint32_t each = parts_of(n.tiles, length_of(length, rows_of_block(g, q.rows)));
             mine = n.blocks * g.c.heads * each;
             held = each > 1u ? mine : 0u;
         }
-        const uint32_t p = lanes_before(mine, 64u), h = lanes_before(held, 64u);
+        const uint32_t p = lanes_before(mine), h = lanes_before(held);
         if (lane == 63u) {
             parts[wave] = p + mine;
             slots[wave] = h + held;
@@ -406,11 +454,11 @@ __device__ __forceinline__ e8<BF> join8(s4 a, s4 b) {
 
 /* A piece of four values of a row, all keys in: the sink, the division and the
  * gate, and where it goes */
-__device__ __forceinline__ void put(const Args &g, const kq::PagedSeq &s, uint32_t head,
+__device__ __forceinline__ void put(const Args &g, uint32_t begin, uint32_t head,
                                     uint32_t row, uint32_t d, uint32_t width, f4 o, float top,
                                     float total, bool &badin, bool &bad) {
     const uint32_t h = head * g.group + row % g.group;
-    const size_t token = s.begin + row / g.group;
+    const size_t token = begin + row / g.group;
     if (g.a.sinks != nullptr)
         total += __builtin_amdgcn_exp2f((float)((double)g.a.sinks[h] * 1.4426950408889634 - top));
     const float inv = total > 0.0f ? 1.0f / total : total; /* a NaN stays one */
@@ -691,7 +739,7 @@ __device__ __forceinline__ void few_rows(const Args &g, const Part &p, char *lds
         if (slot != nullptr)
             keep(g, slot, r, d, D, v, t, l);
         else
-            put(g, p.seq, p.head, p.row0 + r, d, D, v, t, l, badin, bad);
+            put(g, p.seq.begin, p.head, p.row0 + r, d, D, v, t, l, badin, bad);
     }
 }
 
@@ -901,7 +949,7 @@ __device__ __forceinline__ void many_rows(const Args &g, const Part &p, char *ld
 #pragma unroll
     for (uint32_t k = 0; k < BLOCKS * REGS / 4u; ++k) {
         const uint32_t b = k / (REGS / 4u), i = k % (REGS / 4u) * 4u;
-        put(g, p.seq, p.head, row, T::column(k, lane), D,
+        put(g, p.seq.begin, p.head, row, T::column(k, lane), D,
             f4{o[b][i], o[b][i + 1], o[b][i + 2], o[b][i + 3]}, top, total, badin, bad);
     }
 }
@@ -911,8 +959,10 @@ template <bool BF, int D, bool MANY>
 __global__ __launch_bounds__(kThreads, (few_side<BF, D>())) void attend_few(Args g,
                                                                             uint32_t *status) {
     __shared__ __attribute__((aligned(16))) char lds[few_bytes<D, 4>()];
-    const Part p = find_part<MANY>(g, blockIdx.x, blockIdx.x == 0u, status);
+    Part p = find_part<MANY>(g, blockIdx.x, status);
+    leave(g, p);
     if (!p.live) return;
+    p.pin();
     bool badin = false, bad = false, badseq = false;
     few_rows<BF, D, 4>(g, p, lds, badin, bad, badseq);
     if (badseq) kq_flag(status, KQ_DEV_SEQUENCE);
@@ -921,13 +971,15 @@ __global__ __launch_bounds__(kThreads, (few_side<BF, D>())) void attend_few(Args
 }
 
 template <bool BF, int D, bool MANY>
-__global__ __launch_bounds__(Many<D>::THREADS, 2) void attend(Args g, uint32_t *status) {
+__global__ __launch_bounds__(Many<D>::THREADS, D == 64 ? 3 : 2) void attend(Args g, uint32_t *status) {
     constexpr int W = Many<D>::W;
     constexpr uint32_t BYTES = Many<D>::LDS > few_bytes<D, W>() ? Many<D>::LDS : few_bytes<D, W>();
     /* a row's pieces are found by flipping address bits below its size */
     __shared__ __attribute__((aligned(1024))) char lds[BYTES];
-    const Part p = find_part<MANY>(g, blockIdx.x, blockIdx.x == 0u, status);
+    Part p = find_part<MANY>(g, blockIdx.x, status);
+    leave(g, p);
     if (!p.live) return;
+    p.pin();
     bool badin = false, bad = false, badseq = false;
     if (p.block == kFew)
         few_rows<BF, D, W>(g, p, lds, badin, bad, badseq);
@@ -938,70 +990,93 @@ __global__ __launch_bounds__(Many<D>::THREADS, 2) void attend(Args g, uint32_t *
     if (bad) kq_flag(status, KQ_DEV_NUMERIC);
 }
 
+/* four values of a row over some keys, with the exponent they are held by and
+ * the weights' sum */
+struct Sum {
+    f4 v;
+    float top, total;
+
+    __device__ __forceinline__ void clear() {
+        v = f4{0.0f, 0.0f, 0.0f, 0.0f};
+        top = kLowest;
+        total = 0.0f;
+    }
+    __device__ __forceinline__ void add(const Sum &o) {
+        const float next = fmaxf(top, o.top);
+        const float f = __builtin_amdgcn_exp2f(top - next), e = __builtin_amdgcn_exp2f(o.top - next);
+        top = next;
+        total = fmaf(total, f, o.total * e);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) v[c] = fmaf(v[c], f, o.v[c] * e);
+    }
+};
+constexpr uint32_t kAtOnce = 4;
+constexpr uint32_t kShares = 4; /* workgroups that share out a part's share where rows are many */
+
 /* The parts of items that have several, joined: the workgroup of each part
  * takes its share of the item's values over all parts. */
-template <bool MANY>
 __global__ __launch_bounds__(kThreads) void join_parts(Args g, uint32_t *status) {
-    __shared__ f4 sums[kThreads];
-    __shared__ float tops[kThreads], totals[kThreads];
-    const Part p = find_part<MANY>(g, blockIdx.x, false, status);
-    if (!p.live || p.parts < 2u) return;
+    __shared__ Sum sums[kThreads];
+    const Item p = g.items[blockIdx.x];
+    if (p.rows == 0u) return;
     bool badin = false, bad = false;
     /* pieces of four values, in the slots' order: by rows, or by waves and lanes */
     const uint32_t width = g.c.width, tall = width == 256u ? Many<256>::M : Many<128>::M;
-    const bool by_rows = p.block == kFew;
+    const bool by_rows = p.head_few >> 16 != 0u;
     const uint32_t pieces =
         (by_rows ? p.rows : (p.rows + tall - 1u) / tall * tall) * (width / 4u);
-    const uint32_t a = (uint32_t)((uint64_t)pieces * p.part / p.parts);
-    const uint32_t b = (uint32_t)((uint64_t)pieces * (p.part + 1u) / p.parts);
+    const uint32_t share = p.part * gridDim.y + blockIdx.y, shares = p.parts * gridDim.y;
+    const uint32_t a = (uint32_t)((uint64_t)pieces * share / shares);
+    const uint32_t b = (uint32_t)((uint64_t)pieces * (share + 1u) / shares);
     /* side by side: pieces in the threads' low bits, parts in the high ones */
     uint32_t wide = 1u;
     while (wide < b - a && wide < (uint32_t)kThreads) wide *= 2u;
     const uint32_t groups = kThreads / wide;
     const uint32_t mine = threadIdx.x % wide, group = threadIdx.x / wide;
-    for (uint32_t at = a; at < b; at += wide) {
-        const uint32_t i = at + mine;
-        uint32_t row = i / (width / 4u), d = i % (width / 4u) * 4u;
-        if (!by_rows) {
-            const uint32_t lane = i % 64u, piece = i / 64u % (tall * width / 256u);
-            row = i / (tall * width / 4u) * tall + lane % tall;
-            d = tall == 16u ? Many<256>::column(piece, lane) : Many<128>::column(piece, lane);
-        }
-        const bool mine_too = i < b && row < p.rows;
-        f4 v = f4{0.0f, 0.0f, 0.0f, 0.0f};
-        float top = kLowest, total = 0.0f;
-        if (mine_too)
-            for (uint32_t k = group; k < p.parts; k += groups) {
-                const float *slot = slot_at(g, p.slot + k * p.step);
-                const float *m = slot + (size_t)g.slot_rows * width;
-                const float t = m[row], l = m[g.slot_rows + row];
-                const f4 x = *((const f4 *)slot + i);
-                const float next = fmaxf(top, t);
-                const float f = __builtin_amdgcn_exp2f(top - next), e = __builtin_amdgcn_exp2f(t - next);
-                top = next;
-                total = fmaf(total, f, l * e);
+    /* kAtOnce pieces of a thread have their loads under way together */
+    for (uint32_t at = a; at < b; at += wide * kAtOnce) {
+        uint32_t i[kAtOnce], row[kAtOnce], d[kAtOnce];
+        bool have[kAtOnce];
+        Sum v[kAtOnce];
 #pragma unroll
-                for (int c = 0; c < 4; ++c) v[c] = fmaf(v[c], f, x[c] * e);
+        for (uint32_t u = 0; u < kAtOnce; ++u) {
+            i[u] = at + u * wide + mine;
+            row[u] = i[u] / (width / 4u);
+            d[u] = i[u] % (width / 4u) * 4u;
+            if (!by_rows) {
+                const uint32_t lane = i[u] % 64u, piece = i[u] / 64u % (tall * width / 256u);
+                row[u] = i[u] / (tall * width / 4u) * tall + lane % tall;
+                d[u] = tall == 16u ? Many<256>::column(piece, lane) : Many<128>::column(piece, lane);
             }
-        for (uint32_t step = groups / 2u; step != 0u; step /= 2u) {
-            __syncthreads();
-            sums[threadIdx.x] = v;
-            tops[threadIdx.x] = top;
-            totals[threadIdx.x] = total;
-            __syncthreads();
-            if (group < step) {
-                const uint32_t o = threadIdx.x + step * wide;
-                const float t = tops[o], next = fmaxf(top, t);
-                const float f = __builtin_amdgcn_exp2f(top - next), e = __builtin_amdgcn_exp2f(t - next);
-                top = next;
-                total = fmaf(total, f, totals[o] * e);
-                const f4 x = sums[o];
-#pragma unroll
-                for (int c = 0; c < 4; ++c) v[c] = fmaf(v[c], f, x[c] * e);
-            }
+            have[u] = i[u] < b && row[u] < p.rows;
+            v[u].clear();
         }
-        if (group == 0u && mine_too)
-            put(g, p.seq, p.head, p.row0 + row, d, width, v, top, total, badin, bad);
+        for (uint32_t k = group; k < p.parts; k += groups) {
+            const float *slot = slot_at(g, p.slot + k * p.step);
+            const float *m = slot + (size_t)g.slot_rows * width;
+            Sum x[kAtOnce];
+#pragma unroll
+            for (uint32_t u = 0; u < kAtOnce; ++u)
+                if (have[u]) {
+                    x[u].top = m[row[u]];
+                    x[u].total = m[g.slot_rows + row[u]];
+                    x[u].v = *((const f4 *)slot + i[u]);
+                }
+#pragma unroll
+            for (uint32_t u = 0; u < kAtOnce; ++u)
+                if (have[u]) v[u].add(x[u]);
+        }
+        for (uint32_t step = groups / 2u; step != 0u; step /= 2u) { /* then kAtOnce 1 is enough */
+            __syncthreads();
+            sums[threadIdx.x] = v[0];
+            __syncthreads();
+            if (group < step) v[0].add(sums[threadIdx.x + step * wide]);
+        }
+#pragma unroll
+        for (uint32_t u = 0; u < kAtOnce; ++u)
+            if (group == 0u && have[u])
+                put(g, p.begin, p.head_few & 0xffffu, p.row0 + row[u], d[u], width, v[u].v, v[u].top, v[u].total,
+                    badin, bad);
     }
     if (badin) kq_flag(status, KQ_DEV_INPUT);
     if (bad) kq_flag(status, KQ_DEV_NUMERIC);
@@ -1012,7 +1087,7 @@ __global__ __launch_bounds__(kThreads) void join_parts(Args g, uint32_t *status)
 struct Sizes {
     uint64_t items, parts, slots;
     uint32_t slot_rows;
-    uint64_t plan_bytes, bytes;
+    uint64_t plan_bytes, item_bytes, bytes;
 };
 
 /* What a call can need, whatever the device holds */
@@ -1030,7 +1105,8 @@ Sizes sizes_of(const kq_launch_pattn &a, const kq_launch_paged &c, const kq_laun
     z.parts = most < kParts + z.items ? most : kParts + z.items;
     z.slots = most < kSlots ? most : kSlots;
     z.plan_bytes = q.count > kByLane ? ((3u + 2u * (q.count + 1u)) * 4u + 255u) / 256u * 256u : 0u;
-    z.bytes = z.plan_bytes + z.slots * z.slot_rows * (c.width + 2u) * 4u;
+    z.item_bytes = (z.parts * sizeof(Item) + 255u) / 256u * 256u;
+    z.bytes = z.plan_bytes + z.item_bytes + z.slots * z.slot_rows * (c.width + 2u) * 4u;
     return z;
 }
 
@@ -1060,8 +1136,8 @@ hipError_t launch(const Args &g, uint32_t parts, uint32_t *status, hipStream_t s
 #undef KQ_ATTEND
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(join_parts<MANY>), dim3(parts), dim3(kThreads), 0, s, g,
-                       status);
+    hipLaunchKernelGGL(join_parts, dim3(parts, g.slot_rows == kFew ? 1u : kShares),
+                       dim3(kThreads), 0, s, g, status);
     return hipGetLastError();
 }
 
@@ -1085,7 +1161,8 @@ extern "C" hipError_t kq_launch_pattn_run(const kq_launch_pattn *a, const kq_lau
     g.slots = (uint32_t)z.slots;
     g.exponent = (double)a->scale * 1.4426950408889634;
     g.plan = (uint32_t *)scratch;
-    g.partial = (float *)((char *)scratch + z.plan_bytes);
+    g.items = (Item *)((char *)scratch + z.plan_bytes);
+    g.partial = (float *)((char *)scratch + z.plan_bytes + z.item_bytes);
     return q->count > kByLane ? launch<true>(g, (uint32_t)z.parts, status, s)
                               : launch<false>(g, (uint32_t)z.parts, status, s);
 }
