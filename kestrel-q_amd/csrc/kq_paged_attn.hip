@@ -22,7 +22,7 @@ constexpr uint32_t kMany = 128;      /* rows of an item whose waves share out it
 constexpr uint32_t kLeast = 2;       /* tiles of a part */
 constexpr uint32_t kShort = 8;       /* tiles of a part of few rows that are worth a second round */
 constexpr uint32_t kParts = 1024;    /* of few rows; of many half of them */
-constexpr uint32_t kSlots = 2u * kParts;
+constexpr uint32_t kSlots = (4u * kParts + 2u) / 3u;
 constexpr uint32_t kByLane = 64;     /* sequences that each wave plans by itself */
 constexpr float kSlack = 8.0f;       /* by which a row's largest exponent may pass its stand-in */
 constexpr float kLowest = -0x1.fffffep127f;
@@ -37,8 +37,8 @@ struct Args {
     double exponent;    /* scale log2(e) */
     struct Item *items; /* of each workgroup, for the join */
     float *partial;     /* slots of [slot_rows][width] sums, then tops, then totals */
-    uint32_t *plan;     /* tiles a part of few rows, parts, tiles a part of many rows; then first
-                           parts, then first slots of the sequences */
+    uint32_t *plan;     /* tiles a part of few rows, parts, tiles a part of many rows, slots; with
+                           more sequences than kByLane their first parts, then first slots */
 };
 
 /* ---------------------------------------------------------------- the plan */
@@ -115,6 +115,7 @@ struct Part {
     uint32_t t0, t1;      /* its tiles */
     uint32_t key0, key1;  /* keys that any of the item's rows sees */
     uint32_t slot, step;  /* of the item's first part, and between two parts */
+    bool slotted;         /* whether the sequence's parts have slots */
     bool live;
 
     /* what all lanes hold alike goes into scalar registers, as the descriptors
@@ -127,20 +128,21 @@ struct Part {
     }
 };
 
-/* What the join has to know of a part: its item's rows, and where its item's
- * partial results lie. Every workgroup of the first launch leaves one. */
+/* What the join has to know of a part that has a slot: its item's rows, and
+ * where its item's partial results lie. The part's workgroup leaves it, by slot;
+ * plan[3] says how many slots there are. */
 struct __attribute__((aligned(16))) Item {
     uint32_t begin, row0, rows, head_few; /* rows 0: nothing to join; few: the upper half */
     uint32_t part, parts, slot, step;
 };
 
 __device__ __forceinline__ void leave(const Args &g, const Part &p) {
-    if (threadIdx.x == 0u) {
-        Item t = {0u, 0u, 0u, 0u, 0u, 0u, 0u, 0u};
-        if (p.live && p.parts > 1u)
-            t = {p.seq.begin, p.row0, p.rows, p.head | (p.block == kFew ? 1u << 16 : 0u),
-                 p.part, p.parts, p.slot, p.step};
-        g.items[blockIdx.x] = t;
+    const uint32_t at = p.slot + p.part * p.step;
+    if (threadIdx.x == 0u && p.slotted && at < g.slots) {
+        Item t = {p.seq.begin, p.row0, p.rows, p.head | (p.block == kFew ? 1u << 16 : 0u),
+                  p.part, p.parts, p.slot, p.step};
+        if (!p.live || p.parts == 1u) t.rows = 0u;
+        g.items[at] = t;
     }
 }
 
@@ -171,6 +173,7 @@ __device__ __forceinline__ Part part_of(const Args &g, const kq::PagedSeq &s, co
     p.t1 = p.t0 + each + (p.part < more ? 1u : 0u);
     p.slot = first_slot + item;
     p.step = items;
+    p.slotted = parts_of(n.tiles, length) > 1u;
     /* offsets that overlap could ask for more slots than there are */
     p.live = p.part < p.parts &&
              (p.parts == 1u || p.slot + (p.parts - 1u) * p.step < g.slots);
@@ -218,7 +221,7 @@ __device__ __forceinline__ uint64_t lanes_add(uint64_t v) {
 template <bool MANY>
 __device__ __forceinline__ Part find_part(const Args &g, uint32_t index, uint32_t *status) {
     Part p;
-    p.live = false;
+    p.live = p.slotted = false;
     bool bad = false;
     if constexpr (!MANY) {
         const uint32_t lane = threadIdx.x & 63u;
@@ -227,9 +230,12 @@ __device__ __forceinline__ Part find_part(const Args &g, uint32_t index, uint32_
         if (index == 0u && bad) kq_flag(status, KQ_DEV_SEQUENCE);
         const Need n = need_of(g, s);
         const Lengths length = part_tiles(lanes_add(cost_of(g, n)));
-        const uint32_t each = parts_of(n.tiles, length_of(length, rows_of_block(g, s.rows))), mine = n.blocks * g.c.heads * each;
+        const uint32_t each = parts_of(n.tiles, length_of(length, rows_of_block(g, s.rows)));
+        const uint32_t mine = n.blocks * g.c.heads * each;
         const uint32_t first = lanes_before(mine);
-        const uint32_t first_slot = lanes_before(each > 1u ? mine : 0u);
+        const uint32_t held = each > 1u ? mine : 0u, slots = lanes_through(held);
+        const uint32_t first_slot = slots - held;
+        if (index == 0u && lane == 63u) g.plan[3] = slots; /* for the join */
         const uint64_t m = __ballot(index >= first && index - first < mine);
         if (m == 0ull) return p;
         const int at = __builtin_amdgcn_readfirstlane((int)__builtin_ctzll(m));
@@ -244,7 +250,7 @@ __device__ __forceinline__ Part find_part(const Args &g, uint32_t index, uint32_
                        __builtin_amdgcn_readlane(first_slot, at));
     } else {
         if (index >= g.plan[1]) return p;
-        const uint32_t *first = g.plan + 3u, *slots = first + g.q.count + 1u;
+        const uint32_t *first = g.plan + 4u, *slots = first + g.q.count + 1u;
         const uint32_t s = kq::wave_find(first, g.q.count, index);
         const kq::PagedSeq w = kq::paged_seq(g.q, g.c, s, bad);
         const Need n = need_of(g, w);
@@ -271,7 +277,7 @@ __global__ __launch_bounds__(1024) void plan_many(Args g, uint32_t *status) {
     cost = 0u;
     for (int w = 0; w < 16; ++w) cost += sums[w];
     const Lengths length = part_tiles(cost);
-    uint32_t *first = g.plan + 3u, *slot = first + g.q.count + 1u;
+    uint32_t *first = g.plan + 4u, *slot = first + g.q.count + 1u;
     uint32_t parts_before = 0u, slots_before = 0u;
     for (uint32_t base = 0u; base < g.q.count; base += 1024u) {
         const uint32_t s = base + threadIdx.x;
@@ -309,6 +315,7 @@ __global__ __launch_bounds__(1024) void plan_many(Args g, uint32_t *status) {
     if (threadIdx.x == 0u) {
         g.plan[0] = length.few;
         g.plan[2] = length.many;
+        g.plan[3] = slots_before;
         g.plan[1] = parts_before;
         first[g.q.count] = parts_before;
         slot[g.q.count] = slots_before;
@@ -678,14 +685,19 @@ __device__ __forceinline__ void few_rows(const Args &g, const Part &p, char *lds
         }
     };
 
-    if (any) {
-        pages(key);
+    /* the first keys are under way while the queries are split, if registers hold both */
+    constexpr bool AHEAD = !(BF && D == 256);
+    auto begin = [&]() {
+        if (!any) return;
         places(key);
         load_k(key);
         load_v(key);
         if (key + 32u * W < end) pages(key + 32u * W);
-    }
+    };
+    if (any) pages(key);
+    if (AHEAD) begin();
     load_query<BF, STEPS, 48>(q, some, g.exponent, [&](int s) { return qp + 32 * s; }, badin);
+    if (!AHEAD) begin();
     /* K of the next keys is asked for when this one's is used, V likewise: while
      * one waits the CU's other workgroups read */
     while (key < end) {
@@ -1011,12 +1023,12 @@ struct Sum {
     }
 };
 constexpr uint32_t kAtOnce = 4;
-constexpr uint32_t kShares = 4; /* workgroups that share out a part's share where rows are many */
 
 /* The parts of items that have several, joined: the workgroup of each part
  * takes its share of the item's values over all parts. */
 __global__ __launch_bounds__(kThreads) void join_parts(Args g, uint32_t *status) {
     __shared__ Sum sums[kThreads];
+    if (blockIdx.x >= g.plan[3]) return;
     const Item p = g.items[blockIdx.x];
     if (p.rows == 0u) return;
     bool badin = false, bad = false;
@@ -1098,14 +1110,16 @@ Sizes sizes_of(const kq_launch_pattn &a, const kq_launch_paged &c, const kq_laun
     z.slot_rows = (single ? group : rows) <= kFew ? kFew : kMany;
     z.items = c.heads * (single ? q.count * ((group + z.slot_rows - 1u) / z.slot_rows)
                                 : rows / kMany + q.count);
-    /* all items' tiles / tiles a part <= kParts, and an item of w tiles has at
-     * most w / kLeast + 1 parts; only items of two parts or more have slots */
+    /* An item of w tiles has at most w / kLeast + 1/2 parts, at least one. All
+     * tiles by the tiles a part are at most kParts. Only sequences whose items may
+     * have two parts or more have slots: of w tiles, at least 3/2 parts long,
+     * which makes at most 4/3 of their length by a part's. */
     const uint64_t tiles = (((uint64_t)c.table_pages << c.page_shift) + kTile - 1u) / kTile;
-    const uint64_t most = z.items * (tiles / kLeast + 1u);
+    const uint64_t most = z.items * ((tiles + kLeast / 2u) / kLeast + 1u);
     z.parts = most < kParts + z.items ? most : kParts + z.items;
     z.slots = most < kSlots ? most : kSlots;
-    z.plan_bytes = q.count > kByLane ? ((3u + 2u * (q.count + 1u)) * 4u + 255u) / 256u * 256u : 0u;
-    z.item_bytes = (z.parts * sizeof(Item) + 255u) / 256u * 256u;
+    z.plan_bytes = ((4u + (q.count > kByLane ? 2u * (q.count + 1u) : 0u)) * 4u + 255u) / 256u * 256u;
+    z.item_bytes = (z.slots * sizeof(Item) + 255u) / 256u * 256u;
     z.bytes = z.plan_bytes + z.item_bytes + z.slots * z.slot_rows * (c.width + 2u) * 4u;
     return z;
 }
@@ -1136,7 +1150,8 @@ hipError_t launch(const Args &g, uint32_t parts, uint32_t *status, hipStream_t s
 #undef KQ_ATTEND
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    hipLaunchKernelGGL(join_parts, dim3(parts, g.slot_rows == kFew ? 1u : kShares),
+    /* where rows are many, a part's share is shared out again: kAtOnce pieces a thread */
+    hipLaunchKernelGGL(join_parts, dim3(g.slots, g.slot_rows == kFew ? 1u : g.c.width / 64u),
                        dim3(kThreads), 0, s, g, status);
     return hipGetLastError();
 }
