@@ -3,6 +3,8 @@
  * on gfx950 (include/kq_hip.h, kq_hip_paged_attention_f32).
  */
 #include "kq_device.h"
+#include <math.h>
+
 #include "kq_dma.h"
 #include "kq_launch.h"
 #include "kq_paged.h"
@@ -34,7 +36,8 @@ struct Args {
     uint32_t group;     /* query heads of a key head */
     uint32_t slot_rows; /* rows that a slot of the partial results holds */
     uint32_t slots;
-    double exponent;    /* scale log2(e) */
+    float factor_high, factor_low; /* scale log2(e), 1 .. 2 and its exponent */
+    int factor_exponent;
     struct Item *items; /* of each workgroup, for the join */
     float *partial;     /* slots of [slot_rows][width] sums, then tops, then totals */
     uint32_t *plan;     /* tiles a part of few rows, parts, tiles a part of many rows, slots; with
@@ -79,12 +82,9 @@ struct Lengths {
     uint32_t few, many;
 };
 
-__device__ __forceinline__ uint32_t tiles_for(uint64_t cost, uint32_t parts) {
-    return (uint32_t)ceil((double)cost / (double)parts);
-}
-
 __device__ __forceinline__ Lengths part_tiles(uint64_t cost) {
-    const uint32_t fine = tiles_for(cost, kParts), coarse = tiles_for(cost, kParts / 2u);
+    const uint32_t fine = (uint32_t)((cost + kParts - 1u) / kParts);
+    const uint32_t coarse = (uint32_t)((cost + kParts / 2u - 1u) / (kParts / 2u));
     Lengths l;
     l.few = coarse < kShort ? coarse : fine > kShort ? fine : kShort;
     l.many = coarse;
@@ -137,8 +137,9 @@ struct __attribute__((aligned(16))) Item {
 };
 
 __device__ __forceinline__ void leave(const Args &g, const Part &p) {
+    if (threadIdx.x != 0u || !p.slotted) return;
     const uint32_t at = p.slot + p.part * p.step;
-    if (threadIdx.x == 0u && p.slotted && at < g.slots) {
+    if (at < g.slots) {
         Item t = {p.seq.begin, p.row0, p.rows, p.head | (p.block == kFew ? 1u << 16 : 0u),
                   p.part, p.parts, p.slot, p.step};
         if (!p.live || p.parts == 1u) t.rows = 0u;
@@ -156,13 +157,19 @@ __device__ __forceinline__ Part part_of(const Args &g, const kq::PagedSeq &s, co
      * first, then parts, of which an item may have fewer than its sequence. (With
      * the parts before the blocks 2049 rows of 4 heads of 256 took 323 us in place
      * of 224: one half of the XCDs had the second parts, most of them none.) */
-    const uint32_t items = n.blocks * g.c.heads, item = u % items;
+    const uint32_t items = n.blocks * g.c.heads, all = s.rows * g.group;
+    uint32_t item = u % items, ta = 0u, tb = s.rows - 1u;
     p.part = u / items;
-    p.head = item % g.c.heads;
-    p.row0 = (n.blocks - 1u - item / g.c.heads) * p.block;
-    const uint32_t all = s.rows * g.group;
-    p.rows = all - p.row0 < p.block ? all - p.row0 : p.block;
-    const uint32_t ta = p.row0 / g.group, tb = (p.row0 + p.rows - 1u) / g.group;
+    p.head = item;
+    p.row0 = 0u;
+    p.rows = all;
+    if (n.blocks != 1u) {
+        p.head = item % g.c.heads;
+        p.row0 = (n.blocks - 1u - item / g.c.heads) * p.block;
+        p.rows = all - p.row0 < p.block ? all - p.row0 : p.block;
+        ta = p.row0 / g.group;
+        tb = (p.row0 + p.rows - 1u) / g.group;
+    }
     p.key1 = g.a.causal ? s.past + tb + 1u : s.past + s.rows;
     p.key0 = 0u;
     if (g.a.window != 0u && s.past + ta + 1u > g.a.window) p.key0 = s.past + ta + 1u - g.a.window;
@@ -174,7 +181,6 @@ __device__ __forceinline__ Part part_of(const Args &g, const kq::PagedSeq &s, co
     p.slot = first_slot + item;
     p.step = items;
     p.slotted = parts_of(n.tiles, length) > 1u;
-    /* offsets that overlap could ask for more slots than there are */
     p.live = p.part < p.parts &&
              (p.parts == 1u || p.slot + (p.parts - 1u) * p.step < g.slots);
     return p;
@@ -217,7 +223,9 @@ __device__ __forceinline__ uint64_t lanes_add(uint64_t v) {
 
 /* Part `index` of the call, the same in all lanes. Up to kByLane sequences:
  * a lane looks at each, and every wave adds up for itself. More: plan_many
- * has done so. */
+ * has done so. Offsets, slots and lengths that break the rules leave no part at
+ * all: where they hold, the rows of all sequences are at most the call's tokens,
+ * which the host's sizes go by. */
 template <bool MANY>
 __device__ __forceinline__ Part find_part(const Args &g, uint32_t index, uint32_t *status) {
     Part p;
@@ -227,7 +235,13 @@ __device__ __forceinline__ Part find_part(const Args &g, uint32_t index, uint32_
         const uint32_t lane = threadIdx.x & 63u;
         kq::PagedSeq s = {0u, 0u, 0u, 0u, false};
         if (lane < g.q.count) s = kq::paged_seq(g.q, g.c, lane, bad);
-        if (index == 0u && bad) kq_flag(status, KQ_DEV_SEQUENCE);
+        if (__any(bad)) { /* refused: nothing runs, and there is nothing to join */
+            if (index == 0u) {
+                if (bad) kq_flag(status, KQ_DEV_SEQUENCE);
+                g.plan[3] = 0u;
+            }
+            return p;
+        }
         const Need n = need_of(g, s);
         const Lengths length = part_tiles(lanes_add(cost_of(g, n)));
         const uint32_t each = parts_of(n.tiles, length_of(length, rows_of_block(g, s.rows)));
@@ -253,11 +267,8 @@ __device__ __forceinline__ Part find_part(const Args &g, uint32_t index, uint32_
         const uint32_t *first = g.plan + 4u, *slots = first + g.q.count + 1u;
         const uint32_t s = kq::wave_find(first, g.q.count, index);
         const kq::PagedSeq w = kq::paged_seq(g.q, g.c, s, bad);
-        const Need n = need_of(g, w);
-        const uint32_t u = index - first[s];
-        const uint32_t length = g.plan[rows_of_block(g, w.rows) == kFew ? 0 : 2];
-        if (u >= n.blocks * g.c.heads * parts_of(n.tiles, length)) return p; /* offsets not in order */
-        return part_of(g, w, n, length, u, slots[s]);
+        return part_of(g, w, need_of(g, w), g.plan[rows_of_block(g, w.rows) == kFew ? 0 : 2],
+                       index - first[s], slots[s]);
     }
 }
 
@@ -271,6 +282,10 @@ __global__ __launch_bounds__(1024) void plan_many(Args g, uint32_t *status) {
     for (uint32_t s = threadIdx.x; s < g.q.count; s += 1024u)
         cost += cost_of(g, need_of(g, kq::paged_seq(g.q, g.c, s, bad)));
     if (bad) kq_flag(status, KQ_DEV_SEQUENCE);
+    if (__syncthreads_or(bad)) {
+        if (threadIdx.x == 0u) g.plan[1] = g.plan[3] = 0u;
+        return;
+    }
     cost = lanes_add(cost);
     if (lane == 0u) sums[wave] = cost;
     __syncthreads();
@@ -331,9 +346,9 @@ template <bool BF>
 struct Type {
     typedef _Float16 e;
     static constexpr int TERMS = 2;
-    /* fp16's own range is short: a row's largest query is brought to 2^13, and
+    /* fp16's own range is short: a row's largest query is brought to 2^12 .. 2^14, and
      * weights are held times 2^7, at most 2^15 with the slack */
-    static constexpr int TOP = 13;
+    static constexpr int TOP = 12;
     static constexpr float LIFT = 7.0f;
 };
 template <>
@@ -396,52 +411,60 @@ __device__ __forceinline__ void split(const float (&x)[8], e8<BF> (&t)[Type<BF>:
 }
 
 /* A row's queries, as operands: the exponent's factor put in to 48 bits, and
- * the row's largest value brought to 2^TOP by a power of two. */
+ * the row's largest value brought to 2^TOP .. 2^(TOP + 2) by a power of two. */
 template <bool BF, int STEPS>
 struct Query {
     e8<BF> x[STEPS][Type<BF>::TERMS];
     float unscale;
 };
 
-/* at(step): 8 values of the row from there on; LANES: the lanes that share a row */
-template <bool BF, int STEPS, int LANES, typename At>
-__device__ __forceinline__ void load_query(Query<BF, STEPS> &q, bool some, double factor, At at,
-                                           bool &badin) {
-    float v[STEPS][8];
-    uint32_t most = 0u; /* of the values' bits without the sign: orders them, and finds a NaN */
-#pragma unroll
-    for (int s = 0; s < STEPS; ++s) {
-        if (some) {
-            const float4 a = *(const float4 *)at(s), b = *(const float4 *)(at(s) + 4);
-            v[s][0] = a.x; v[s][1] = a.y; v[s][2] = a.z; v[s][3] = a.w;
-            v[s][4] = b.x; v[s][5] = b.y; v[s][6] = b.z; v[s][7] = b.w;
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[s][i] = 0.0f;
-        }
-    }
+template <int STEPS>
+struct Raw {
+    float4 v[STEPS][2];
+};
+
+/* at(step): 8 values of the row from there on */
+template <int STEPS, typename At>
+__device__ __forceinline__ void fetch_query(Raw<STEPS> &r, bool some, At at) {
 #pragma unroll
     for (int s = 0; s < STEPS; ++s)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const uint32_t b = __float_as_uint(v[s][i]) & 0x7fffffffu;
-            most = b > most ? b : most;
-        }
+        for (int i = 0; i < 2; ++i)
+            r.v[s][i] = some ? *(const float4 *)(at(s) + 4 * i) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+}
+
+/* LANES: the lanes that share a row */
+template <bool BF, int STEPS, int LANES>
+__device__ __forceinline__ void split_query(const Args &g, const Raw<STEPS> &r, Query<BF, STEPS> &q,
+                                            bool &badin) {
+    constexpr int TOP = Type<BF>::TOP;
+    uint32_t most = 0u; /* of the values' bits without the sign: orders them, and finds a NaN */
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s)
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                const uint32_t b = __float_as_uint((&r.v[s][i].x)[c]) & 0x7fffffffu;
+                most = b > most ? b : most;
+            }
     badin |= most >= 0x7f800000u;
-    float top = kq::lanes_max<LANES>(__uint_as_float(most < 0x7f800000u ? most : 0u));
+    const float top = kq::lanes_max<LANES>(__uint_as_float(most < 0x7f800000u ? most : 0u));
     /* the largest value's exponent, 0 for a row of zeros */
-    int e = 0;
-    if (top > 0.0f) e = ilogb((double)top * fabs(factor));
-    e = e < -100 ? -100 : e > 126 ? 126 : e;
+    int e = (int)(__float_as_uint(top) >> 23) - 127;
+    e = top == 0.0f ? 0 : e < -100 ? -100 : e;
     /* the factor as two numbers: its own rounding would be the same for all keys */
-    const double scale = __builtin_ldexp(factor, Type<BF>::TOP - e);
-    const float high = (float)scale, low = (float)(scale - (double)high);
-    q.unscale = __builtin_ldexpf(1.0f, e - Type<BF>::TOP);
+    const float high = __builtin_ldexpf(g.factor_high, TOP - e);
+    const float low = __builtin_ldexpf(g.factor_low, TOP - e);
+    q.unscale = __builtin_ldexpf(1.0f, e + g.factor_exponent - TOP);
 #pragma unroll
     for (int s = 0; s < STEPS; ++s) {
         float x[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = fmaf(v[s][i], high, v[s][i] * low);
+        for (int i = 0; i < 8; ++i) {
+            const float v = (&r.v[s][i / 4].x)[i % 4];
+            x[i] = fmaf(v, high, v * low);
+        }
         split<BF>(x, q.x[s]);
     }
 }
@@ -468,8 +491,8 @@ __device__ __forceinline__ void put(const Args &g, uint32_t begin, uint32_t head
     const size_t token = begin + row / g.group;
     if (g.a.sinks != nullptr)
         total += __builtin_amdgcn_exp2f((float)((double)g.a.sinks[h] * 1.4426950408889634 - top));
-    const float inv = total > 0.0f ? 1.0f / total : total; /* a NaN stays one */
-    o *= inv;
+    bad |= !(total > 0.0f); /* of a row's keys one at least has a weight of its slack */
+    o *= 1.0f / total;
     const size_t at = (size_t)h * width + d;
     if (g.a.gated) {
         const float4 e = *(const float4 *)(g.a.gate + token * g.a.gs + at);
@@ -695,8 +718,10 @@ __device__ __forceinline__ void few_rows(const Args &g, const Part &p, char *lds
         if (key + 32u * W < end) pages(key + 32u * W);
     };
     if (any) pages(key);
+    Raw<STEPS> raw;
+    fetch_query(raw, some, [&](int s) { return qp + 32 * s; });
     if (AHEAD) begin();
-    load_query<BF, STEPS, 48>(q, some, g.exponent, [&](int s) { return qp + 32 * s; }, badin);
+    split_query<BF, STEPS, 48>(g, raw, q, badin);
     if (!AHEAD) begin();
     /* K of the next keys is asked for when this one's is used, V likewise: while
      * one waits the CU's other workgroups read */
@@ -848,7 +873,9 @@ __device__ __forceinline__ void many_rows(const Args &g, const Part &p, char *ld
 
     Query<BF, STEPS> q;
     const float *qp = g.a.q + (size_t)(p.seq.begin + token) * g.a.qs + (size_t)h * D + 8u * part;
-    load_query<BF, STEPS, LANES>(q, some, g.exponent, [&](int s) { return qp + 512 / M * s; }, badin);
+    Raw<STEPS> raw;
+    fetch_query(raw, some, [&](int s) { return qp + 512 / M * s; });
+    split_query<BF, STEPS, LANES>(g, raw, q, badin);
 
     acc o[BLOCKS];
 #pragma unroll
@@ -1028,9 +1055,8 @@ constexpr uint32_t kAtOnce = 4;
  * takes its share of the item's values over all parts. */
 __global__ __launch_bounds__(kThreads) void join_parts(Args g, uint32_t *status) {
     __shared__ Sum sums[kThreads];
-    if (blockIdx.x >= g.plan[3]) return;
-    const Item p = g.items[blockIdx.x];
-    if (p.rows == 0u) return;
+    const Item p = g.items[blockIdx.x]; /* behind the last slot, whatever lies there */
+    if (blockIdx.x >= g.plan[3] || p.rows == 0u) return;
     bool badin = false, bad = false;
     /* pieces of four values, in the slots' order: by rows, or by waves and lanes */
     const uint32_t width = g.c.width, tall = width == 256u ? Many<256>::M : Many<128>::M;
@@ -1174,7 +1200,11 @@ extern "C" hipError_t kq_launch_pattn_run(const kq_launch_pattn *a, const kq_lau
     g.group = a->query_heads / c->heads;
     g.slot_rows = z.slot_rows;
     g.slots = (uint32_t)z.slots;
-    g.exponent = (double)a->scale * 1.4426950408889634;
+    int exponent = 0;
+    const double factor = 2.0 * frexp((double)a->scale * 1.4426950408889634, &exponent);
+    g.factor_high = (float)factor;
+    g.factor_low = (float)(factor - (double)g.factor_high);
+    g.factor_exponent = exponent - 1;
     g.plan = (uint32_t *)scratch;
     g.items = (Item *)((char *)scratch + z.plan_bytes);
     g.partial = (float *)((char *)scratch + z.plan_bytes + z.item_bytes);
