@@ -1,10 +1,38 @@
 /*
  * kq_paged_attn.hip — softmax attention of a call's rows over a paged cache
  * on gfx950 (include/kq_hip.h, kq_hip_paged_attention_f32).
+ *
+ * One pass over a row's keys with the largest exponent so far, M, and the sum of
+ * weights, both binary32:
+ *   s_t = scale log2(e) q . k_t,  w_t = 2^(s_t - M),  l = sum w_t,
+ *   y = (sum w_t v_t) / (l + 2^(sink log2(e) - M))
+ * M follows a row's largest s only when that has passed it by 2^kSlack, so that
+ * the sums are rarely scaled; what they are held by cancels in the end. Partial
+ * sums (of waves, of parts of a long context) are added by their M.
+ *
+ * Products run on the matrix cores with keys and values as they lie in the cache.
+ * The queries and the weights, which are binary32, are two fp16 (three bf16)
+ * numbers each, whose products add up in one accumulator: twice (three times) the
+ * matrix work buys results off by 2-9 x 10^-7 of their 2-norm, as those of
+ * binary32 products are, where one fp16 term would leave 2 x 10^-4. S' = K Q' and
+ * O' = V' P': a lane has one row's scores, whose weights are the next product's
+ * operand as they stand (its keys in the order that the first product left them),
+ * and V comes transposed out of LDS (ds_read_b64_tr_b16).
+ *
+ * Few rows (up to 16 for a key head: decoding) are bound by the pages' bytes: a
+ * workgroup's waves take 32 keys in turn each, K straight into registers, V
+ * through LDS of the wave's own, with no barrier before the end. 61 sequences of
+ * 500 to 32,000 tokens, 504 MB: 93 us, 5.4 TB/s, and 6 for the join; one of
+ * 130,002 tokens, 133 MB: 27 us (4 of them until the first keys are there: length,
+ * page and key hang on each other) and 6.
+ * Many rows (128 for a key head) are bound by the matrix cores, whose clock falls
+ * to 1.9 GHz under it: 8192 rows over themselves with 16 heads of 128 take 482 -
+ * 499 us, 1100 - 1140 TFLOP/s of products, which a library product of 8192^3 fp16
+ * reaches (1159); 3 terms and heads of 256, 2049 rows: 215 us, 950 TFLOP/s.
  */
-#include "kq_device.h"
 #include <math.h>
 
+#include "kq_device.h"
 #include "kq_dma.h"
 #include "kq_launch.h"
 #include "kq_paged.h"
@@ -15,15 +43,21 @@ typedef float f4 __attribute__((ext_vector_type(4)));
 typedef float f16v __attribute__((ext_vector_type(16)));
 typedef short s4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
-typedef __attribute__((address_space(3))) char lds_char;
 
 constexpr int kThreads = 256;
 constexpr uint32_t kTile = 64;       /* keys of a tile */
 constexpr uint32_t kFew = 16;        /* rows of an item whose waves share out its keys */
 constexpr uint32_t kMany = 128;      /* rows of an item whose waves share out its rows */
-constexpr uint32_t kLeast = 2;       /* tiles of a part */
-constexpr uint32_t kShort = 8;       /* tiles of a part of few rows that are worth a second round */
-constexpr uint32_t kParts = 1024;    /* of few rows; of many half of them */
+/* Parts that a call's items are cut into. Of few rows 1024, three to four rounds
+ * of the device's waves that follow each other: 61 sequences 102 us, with 512
+ * parts 116, with 2048 111. But parts of fewer than 8 tiles are not worth a
+ * second round: one sequence of 130,002 tokens takes 34 us in parts of 8 tiles
+ * (512), 38 in parts of 4. Of many rows 512, whose partial results are 64 KB or
+ * more each: 509 rows over 65,509 keys 464 us, 2049 rows of 256-wide heads 215;
+ * with 1024 parts 475 and 231, with 256 505 and 224. */
+constexpr uint32_t kParts = 1024;
+constexpr uint32_t kShort = 8;       /* tiles */
+constexpr uint32_t kLeast = 2;       /* tiles */
 constexpr uint32_t kSlots = (4u * kParts + 2u) / 3u;
 constexpr uint32_t kByLane = 64;     /* sequences that each wave plans by itself */
 constexpr float kSlack = 8.0f;       /* by which a row's largest exponent may pass its stand-in */
@@ -35,10 +69,10 @@ struct Args {
     kq_launch_seqs q;
     uint32_t group;     /* query heads of a key head */
     uint32_t slot_rows; /* rows that a slot of the partial results holds */
-    uint32_t slots;
+    uint32_t slots;     /* partial results that there is room for */
     float factor_high, factor_low; /* scale log2(e), 1 .. 2 and its exponent */
     int factor_exponent;
-    struct Item *items; /* of each workgroup, for the join */
+    struct Item *items; /* of the slots, for the join */
     float *partial;     /* slots of [slot_rows][width] sums, then tops, then totals */
     uint32_t *plan;     /* tiles a part of few rows, parts, tiles a part of many rows, slots; with
                            more sequences than kByLane their first parts, then first slots */
@@ -581,14 +615,17 @@ template <int D>
 constexpr uint32_t many_bytes() {
     return 512u * D; /* 2 x 64 rows of K and V */
 }
-/* workgroups a CU that registers allow */
+/* Waves a SIMD that registers are given for. Heads of 128 in fp16 need 148: three
+ * (61 sequences 109 us; four, at 128 with 24 of them in memory, 136). */
 template <bool BF, int D>
 constexpr int few_side() {
     return D == 256 ? 2 : D == 128 ? 3 : 4;
 }
 
 /* Up to 16 rows: a wave takes every W-th 32 keys, S' = K Q' and O' = V' P' of
- * 16 x 16 x 32 products, and the waves' results are joined in LDS. */
+ * 16 x 16 x 32 products, and the waves' results are joined in LDS. One set of
+ * registers and one buffer a wave: three workgroups a CU hide the loads better
+ * than a second set would (two workgroups then: 115 us for the 61 sequences). */
 template <bool BF, int D, int W>
 __device__ __forceinline__ void few_rows(const Args &g, const Part &p, char *lds, bool &badin,
                                          bool &bad, bool &badseq) {
@@ -786,7 +823,9 @@ __device__ __forceinline__ void few_rows(const Args &g, const Part &p, char *lds
  * two buffers of 64 keys. S' = K Q' and O' = V' P' of products of M x M: 32 (4
  * waves) moves half the bytes out of LDS that 16 (8 waves) does, and 16 holds a
  * head of 256 in the registers of two waves a SIMD, one of which multiplies
- * while the other has exponentials to form. */
+ * while the other forms exponentials (2049 rows of bf16 heads: 282 us, with 32
+ * and one wave 429). Heads of 64 leave room for three (19 ragged sequences 47,
+ * with two 54). */
 template <int D>
 struct Many {
     static constexpr int M = D == 256 ? 16 : 32;
