@@ -516,29 +516,35 @@ __device__ __forceinline__ e8<BF> join8(s4 a, s4 b) {
 
 /* ------------------------------------------------------------ the results */
 
-/* A piece of four values of a row, all keys in: the sink, the division and the
- * gate, and where it goes */
-__device__ __forceinline__ void put(const Args &g, uint32_t begin, uint32_t head,
-                                    uint32_t row, uint32_t d, uint32_t width, f4 o, float top,
-                                    float total, bool &badin, bool &bad) {
-    const uint32_t h = head * g.group + row % g.group;
-    const size_t token = begin + row / g.group;
-    if (g.a.sinks != nullptr)
-        total += __builtin_amdgcn_exp2f((float)((double)g.a.sinks[h] * 1.4426950408889634 - top));
+/* What a row's sums are divided by, all keys in and the sink, whose exponent has
+ * its factor in 48 bits as the queries have */
+__device__ __forceinline__ float inverse_of_row(const Args &g, uint32_t h, float top, float total,
+                                                bool &bad) {
+    if (g.a.sinks != nullptr) {
+        const float sink = g.a.sinks[h];
+        total += __builtin_amdgcn_exp2f(
+            fmaf(sink, 0x1.715476p+0f, fmaf(sink, 0x1.4ae0cp-26f, -top)));
+    }
     bad |= !(total > 0.0f); /* of a row's keys one at least has a weight of its slack */
-    o *= 1.0f / total;
-    const size_t at = (size_t)h * width + d;
+    return 1.0f / total;
+}
+
+/* Four values of a row, at d of head h: its gate, and where they go */
+__device__ __forceinline__ void put(const Args &g, uint32_t token, uint32_t h, uint32_t d, f4 o,
+                                    float inverse, bool &badin, bool &bad) {
+    const size_t at = (size_t)h * g.c.width + d;
+    o *= inverse;
     if (g.a.gated) {
-        const float4 e = *(const float4 *)(g.a.gate + token * g.a.gs + at);
-        badin |= !kq_isfinite(e.x) || !kq_isfinite(e.y) || !kq_isfinite(e.z) || !kq_isfinite(e.w);
-        o[0] *= kq::sigmoid(e.x);
-        o[1] *= kq::sigmoid(e.y);
-        o[2] *= kq::sigmoid(e.z);
-        o[3] *= kq::sigmoid(e.w);
+        const f4 e = *(const f4 *)(g.a.gate + (size_t)token * g.a.gs + at);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            badin |= !kq_isfinite(e[i]);
+            o[i] *= kq::sigmoid(e[i]);
+        }
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) bad |= !kq_isfinite(o[i]);
-    *(f4 *)(g.a.y + token * g.a.ys + at) = o;
+    *(f4 *)(g.a.y + (size_t)token * g.a.ys + at) = o;
 }
 
 __device__ __forceinline__ float *slot_at(const Args &g, uint32_t slot) {
@@ -812,8 +818,10 @@ __device__ __forceinline__ void few_rows(const Args &g, const Part &p, char *lds
         }
         if (slot != nullptr)
             keep(g, slot, r, d, D, v, t, l);
-        else
-            put(g, p.seq.begin, p.head, p.row0 + r, d, D, v, t, l, badin, bad);
+        else {
+            const uint32_t row = p.row0 + r, h = p.head * g.group + row % g.group;
+            put(g, p.seq.begin + row / g.group, h, d, v, inverse_of_row(g, h, t, l, bad), badin, bad);
+        }
     }
 }
 
@@ -1000,6 +1008,7 @@ __device__ __forceinline__ void many_rows(const Args &g, const Part &p, char *ld
         if (t + 1u < p.t1) load(t + 1u, 1u - decltype(buffer)::value);
         if (t * kTile < see1 && t * kTile + kTile > see0) compute(t, buffer);
     };
+    /* two tiles a round, so that the buffers' places are constants (8192 rows: 4%) */
     uint32_t t = p.t0;
     for (; t + 1u < p.t1; t += 2u) {
         step(t, Buffer<0u>{});
@@ -1024,11 +1033,12 @@ __device__ __forceinline__ void many_rows(const Args &g, const Part &p, char *ld
         return;
     }
     if (!some) return;
+    const float inverse = inverse_of_row(g, h, top, total, bad);
 #pragma unroll
     for (uint32_t k = 0; k < BLOCKS * REGS / 4u; ++k) {
         const uint32_t b = k / (REGS / 4u), i = k % (REGS / 4u) * 4u;
-        put(g, p.seq.begin, p.head, row, T::column(k, lane), D,
-            f4{o[b][i], o[b][i + 1], o[b][i + 2], o[b][i + 3]}, top, total, badin, bad);
+        put(g, p.seq.begin + token, h, T::column(k, lane),
+            f4{o[b][i], o[b][i + 1], o[b][i + 2], o[b][i + 3]}, inverse, badin, bad);
     }
 }
 
@@ -1151,9 +1161,12 @@ __global__ __launch_bounds__(kThreads) void join_parts(Args g, uint32_t *status)
         }
 #pragma unroll
         for (uint32_t u = 0; u < kAtOnce; ++u)
-            if (group == 0u && have[u])
-                put(g, p.begin, p.head_few & 0xffffu, p.row0 + row[u], d[u], width, v[u].v, v[u].top, v[u].total,
-                    badin, bad);
+            if (group == 0u && have[u]) {
+                const uint32_t r = p.row0 + row[u];
+                const uint32_t h = (p.head_few & 0xffffu) * g.group + r % g.group;
+                put(g, p.begin + r / g.group, h, d[u], v[u].v,
+                    inverse_of_row(g, h, v[u].top, v[u].total, bad), badin, bad);
+            }
     }
     if (badin) kq_flag(status, KQ_DEV_INPUT);
     if (bad) kq_flag(status, KQ_DEV_NUMERIC);
