@@ -58,6 +58,7 @@ constexpr uint32_t kMany = 128;      /* rows of an item whose waves share out it
 constexpr uint32_t kParts = 1024;
 constexpr uint32_t kShort = 8;       /* tiles */
 constexpr uint32_t kLeast = 2;       /* tiles */
+constexpr uint32_t kSmall = 512;     /* tiles in all of items of many rows */
 constexpr uint32_t kSlots = (4u * kParts + 2u) / 3u;
 constexpr uint32_t kByLane = 64;     /* sequences that each wave plans by itself */
 constexpr float kSlack = 8.0f;       /* by which a row's largest exponent may pass its stand-in */
@@ -70,6 +71,7 @@ struct Args {
     uint32_t group;     /* query heads of a key head */
     uint32_t slot_rows; /* rows that a slot of the partial results holds */
     uint32_t slots;     /* partial results that there is room for */
+    uint32_t parts;     /* workgroups */
     float factor_high, factor_low; /* scale log2(e), 1 .. 2 and its exponent */
     int factor_exponent;
     struct Item *items; /* of the slots, for the join */
@@ -80,20 +82,25 @@ struct Args {
 
 /* ---------------------------------------------------------------- the plan */
 
+/* Tiles a part, of items of few and of many rows; many 0: all items have few. */
+struct Lengths {
+    uint32_t few, many;
+};
+
+__device__ __forceinline__ uint32_t block_of(uint32_t rows, bool small) {
+    return rows <= kFew || small ? kFew : kMany;
+}
+
 /* What a sequence asks for: its items (blocks of rows, for each key head) and
  * the tiles of keys that an item reads at most. */
 struct Need {
-    uint32_t blocks, tiles;
+    uint32_t blocks, tiles, block;
 };
 
-__device__ __forceinline__ uint32_t rows_of_block(const Args &g, uint32_t rows) {
-    return (uint64_t)rows * g.group <= kFew ? kFew : kMany;
-}
-
-__device__ __forceinline__ Need need_of(const Args &g, const kq::PagedSeq &s) {
-    Need n = {0u, 0u};
+__device__ __forceinline__ Need need_of(const Args &g, const kq::PagedSeq &s, bool small) {
+    const uint32_t rows = s.rows * g.group, block = block_of(rows, small);
+    Need n = {0u, 0u, block};
     if (!s.live || s.rows == 0u) return n;
-    const uint32_t rows = s.rows * g.group, block = rows_of_block(g, s.rows);
     n.blocks = (rows + block - 1u) / block;
     n.tiles = (s.past + s.rows + kTile - 1u) / kTile;
     if (g.a.window != 0u && g.a.causal != 0u) {
@@ -106,29 +113,35 @@ __device__ __forceinline__ Need need_of(const Args &g, const kq::PagedSeq &s) {
     return n;
 }
 
+/* all its items' tiles */
 __device__ __forceinline__ uint64_t cost_of(const Args &g, const Need &n) {
     return (uint64_t)n.blocks * g.c.heads * n.tiles;
 }
 
-/* Tiles a part: items are cut so that the device is full and its workgroups'
- * ends do not lie far apart. */
-struct Lengths {
-    uint32_t few, many;
-};
+/* Whether a call's items of many rows, of that cost in all, are better cut into
+ * items of few: a workgroup of many rows begins with 5 us of queries and first
+ * tiles and takes 2 us a tile when the device is not full, and its parts are
+ * joined. 97 rows of 24 heads over themselves (48 tiles) 10.6 us, 19.4 as items of
+ * many rows; 92 rows over 1321 keys (105) 17.9, 20.8; 794 rows of 10 sequences (736)
+ * 42, 36: items of few read their keys eight times. Heads of 256, whose workgroups
+ * have no room beside each other, are faster as they are (116 rows of 32 heads: 23
+ * us, 32). */
+__device__ __forceinline__ bool is_small(const Args &g, uint64_t cost_of_many) {
+    return g.c.width != 256u && cost_of_many != 0u && cost_of_many < kSmall;
+}
 
-__device__ __forceinline__ Lengths part_tiles(uint64_t cost) {
+__device__ __forceinline__ Lengths part_tiles(uint64_t cost, bool small) {
     const uint32_t fine = (uint32_t)((cost + kParts - 1u) / kParts);
     const uint32_t coarse = (uint32_t)((cost + kParts / 2u - 1u) / (kParts / 2u));
     Lengths l;
     l.few = coarse < kShort ? coarse : fine > kShort ? fine : kShort;
-    l.many = coarse;
     l.few = l.few < kLeast ? kLeast : l.few;
-    l.many = l.many < kLeast ? kLeast : l.many;
+    l.many = small ? 0u : coarse < kLeast ? kLeast : coarse;
     return l;
 }
 
-__device__ __forceinline__ uint32_t length_of(const Lengths &l, uint32_t block) {
-    return block == kFew ? l.few : l.many;
+__device__ __forceinline__ uint32_t length_of(const Lengths &l, const Need &n) {
+    return n.block == kFew ? l.few : l.many;
 }
 
 /* parts of so many tiles, the nearest number: an item a little longer than a
@@ -181,11 +194,11 @@ __device__ __forceinline__ void leave(const Args &g, const Part &p) {
     }
 }
 
-__device__ __forceinline__ Part part_of(const Args &g, const kq::PagedSeq &s, const Need &n,
-                                        uint32_t length, uint32_t u, uint32_t first_slot) {
-    Part p;
+__device__ __forceinline__ void part_of(Part &p, const Args &g, const kq::PagedSeq &s,
+                                        const Need &n, uint32_t length, uint32_t u,
+                                        uint32_t first_slot) {
     p.seq = s;
-    p.block = rows_of_block(g, s.rows);
+    p.block = n.block;
     /* Workgroups go to the XCDs in turn, so neighbours in number should have
      * work alike: heads, then blocks, whose last rows see the most keys and go
      * first, then parts, of which an item may have fewer than its sequence. (With
@@ -217,7 +230,6 @@ __device__ __forceinline__ Part part_of(const Args &g, const kq::PagedSeq &s, co
     p.slotted = parts_of(n.tiles, length) > 1u;
     p.live = p.part < p.parts &&
              (p.parts == 1u || p.slot + (p.parts - 1u) * p.step < g.slots);
-    return p;
 }
 
 
@@ -276,11 +288,25 @@ __device__ __forceinline__ Part find_part(const Args &g, uint32_t index, uint32_
             }
             return p;
         }
-        const Need n = need_of(g, s);
-        const Lengths length = part_tiles(lanes_add(cost_of(g, n)));
-        const uint32_t each = parts_of(n.tiles, length_of(length, rows_of_block(g, s.rows)));
-        const uint32_t mine = n.blocks * g.c.heads * each;
-        const uint32_t first = lanes_before(mine);
+        bool small = false;
+        if (g.slot_rows == kMany) {
+            const Need n = need_of(g, s, false);
+            small = is_small(g, lanes_add(n.block == kMany ? cost_of(g, n) : 0u));
+        }
+        Need n;
+        Lengths length;
+        uint32_t each, mine, through, total;
+        for (;;) {
+            n = need_of(g, s, small);
+            length = part_tiles(lanes_add(cost_of(g, n)), small);
+            each = parts_of(n.tiles, length_of(length, n));
+            mine = n.blocks * g.c.heads * each;
+            through = lanes_through(mine);
+            total = __builtin_amdgcn_readlane(through, 63);
+            if (!small || total <= g.parts) break;
+            small = false;
+        }
+        const uint32_t first = through - mine;
         const uint32_t held = each > 1u ? mine : 0u, slots = lanes_through(held);
         const uint32_t first_slot = slots - held;
         if (index == 0u && lane == 63u) g.plan[3] = slots; /* for the join */
@@ -293,16 +319,20 @@ __device__ __forceinline__ Part find_part(const Args &g, uint32_t index, uint32_
         w.past = __builtin_amdgcn_readlane(s.past, at);
         w.slot = __builtin_amdgcn_readlane(s.slot, at);
         w.live = true;
-        return part_of(g, w, need_of(g, w), length_of(length, rows_of_block(g, w.rows)),
-                       index - __builtin_amdgcn_readlane(first, at),
-                       __builtin_amdgcn_readlane(first_slot, at));
+        const Need need = need_of(g, w, small);
+        part_of(p, g, w, need, length_of(length, need),
+                index - __builtin_amdgcn_readlane(first, at),
+                __builtin_amdgcn_readlane(first_slot, at));
+        return p;
     } else {
         if (index >= g.plan[1]) return p;
         const uint32_t *first = g.plan + 4u, *slots = first + g.q.count + 1u;
         const uint32_t s = kq::wave_find(first, g.q.count, index);
         const kq::PagedSeq w = kq::paged_seq(g.q, g.c, s, bad);
-        return part_of(g, w, need_of(g, w), g.plan[rows_of_block(g, w.rows) == kFew ? 0 : 2],
-                       index - first[s], slots[s]);
+        const Lengths length = {g.plan[0], g.plan[2]};
+        const Need need = need_of(g, w, length.many == 0u);
+        part_of(p, g, w, need, length_of(length, need), index - first[s], slots[s]);
+        return p;
     }
 }
 
@@ -311,63 +341,77 @@ __global__ __launch_bounds__(1024) void plan_many(Args g, uint32_t *status) {
     __shared__ uint64_t sums[16];
     __shared__ uint32_t parts[16], slots[16];
     const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x / 64u;
-    uint64_t cost = 0u;
     bool bad = false;
-    for (uint32_t s = threadIdx.x; s < g.q.count; s += 1024u)
-        cost += cost_of(g, need_of(g, kq::paged_seq(g.q, g.c, s, bad)));
+    /* a value of every sequence, added up */
+    auto sum = [&](auto of) {
+        uint64_t v = 0u;
+        for (uint32_t s = threadIdx.x; s < g.q.count; s += 1024u)
+            v += of(kq::paged_seq(g.q, g.c, s, bad));
+        v = lanes_add(v);
+        if (lane == 0u) sums[wave] = v;
+        __syncthreads();
+        v = 0u;
+        for (int w = 0; w < 16; ++w) v += sums[w];
+        __syncthreads();
+        return v;
+    };
+    bool small = is_small(g, sum([&](const kq::PagedSeq &s) {
+                              const Need n = need_of(g, s, false);
+                              return n.block == kMany ? cost_of(g, n) : (uint64_t)0u;
+                          }));
     if (bad) kq_flag(status, KQ_DEV_SEQUENCE);
     if (__syncthreads_or(bad)) {
         if (threadIdx.x == 0u) g.plan[1] = g.plan[3] = 0u;
         return;
     }
-    cost = lanes_add(cost);
-    if (lane == 0u) sums[wave] = cost;
-    __syncthreads();
-    cost = 0u;
-    for (int w = 0; w < 16; ++w) cost += sums[w];
-    const Lengths length = part_tiles(cost);
     uint32_t *first = g.plan + 4u, *slot = first + g.q.count + 1u;
-    uint32_t parts_before = 0u, slots_before = 0u;
-    for (uint32_t base = 0u; base < g.q.count; base += 1024u) {
-        const uint32_t s = base + threadIdx.x;
-        uint32_t mine = 0u, held = 0u;
-        if (s < g.q.count) {
-            const kq::PagedSeq q = kq::paged_seq(g.q, g.c, s, bad);
-            const Need n = need_of(g, q);
-            const uint32_t each = parts_of(n.tiles, length_of(length, rows_of_block(g, q.rows)));
-            mine = n.blocks * g.c.heads * each;
-            held = each > 1u ? mine : 0u;
-        }
-        const uint32_t p = lanes_before(mine), h = lanes_before(held);
-        if (lane == 63u) {
-            parts[wave] = p + mine;
-            slots[wave] = h + held;
-        }
-        __syncthreads();
-        uint32_t pw = 0u, hw = 0u, pa = 0u, ha = 0u;
-        for (uint32_t w = 0; w < 16u; ++w) {
-            if (w < wave) {
-                pw += parts[w];
-                hw += slots[w];
+    for (;;) {
+        const Lengths length = part_tiles(
+            sum([&](const kq::PagedSeq &s) { return cost_of(g, need_of(g, s, small)); }), small);
+        uint32_t parts_before = 0u, slots_before = 0u;
+        for (uint32_t base = 0u; base < g.q.count; base += 1024u) {
+            const uint32_t s = base + threadIdx.x;
+            uint32_t mine = 0u, held = 0u;
+            if (s < g.q.count) {
+                const Need n = need_of(g, kq::paged_seq(g.q, g.c, s, bad), small);
+                const uint32_t each = parts_of(n.tiles, length_of(length, n));
+                mine = n.blocks * g.c.heads * each;
+                held = each > 1u ? mine : 0u;
             }
-            pa += parts[w];
-            ha += slots[w];
+            const uint32_t p = lanes_before(mine), h = lanes_before(held);
+            if (lane == 63u) {
+                parts[wave] = p + mine;
+                slots[wave] = h + held;
+            }
+            __syncthreads();
+            uint32_t pw = 0u, hw = 0u, pa = 0u, ha = 0u;
+            for (uint32_t w = 0; w < 16u; ++w) {
+                if (w < wave) {
+                    pw += parts[w];
+                    hw += slots[w];
+                }
+                pa += parts[w];
+                ha += slots[w];
+            }
+            if (s < g.q.count) {
+                first[s] = parts_before + pw + p;
+                slot[s] = slots_before + hw + h;
+            }
+            parts_before += pa;
+            slots_before += ha;
+            __syncthreads();
         }
-        if (s < g.q.count) {
-            first[s] = parts_before + pw + p;
-            slot[s] = slots_before + hw + h;
+        if (small && parts_before > g.parts) {
+            small = false;
+            continue;
         }
-        parts_before += pa;
-        slots_before += ha;
-        __syncthreads();
-    }
-    if (threadIdx.x == 0u) {
-        g.plan[0] = length.few;
-        g.plan[2] = length.many;
-        g.plan[3] = slots_before;
-        g.plan[1] = parts_before;
-        first[g.q.count] = parts_before;
-        slot[g.q.count] = slots_before;
+        if (threadIdx.x == 0u) {
+            g.plan[0] = length.few;
+            g.plan[1] = parts_before;
+            g.plan[2] = length.many;
+            g.plan[3] = slots_before;
+        }
+        return;
     }
 }
 
@@ -1064,11 +1108,11 @@ __global__ __launch_bounds__(Many<D>::THREADS, D == 64 ? 3 : 2) void attend(Args
     constexpr uint32_t BYTES = Many<D>::LDS > few_bytes<D, W>() ? Many<D>::LDS : few_bytes<D, W>();
     /* a row's pieces are found by flipping address bits below its size */
     __shared__ __attribute__((aligned(1024))) char lds[BYTES];
+    bool badin = false, bad = false, badseq = false;
     Part p = find_part<MANY>(g, blockIdx.x, status);
     leave(g, p);
     if (!p.live) return;
     p.pin();
-    bool badin = false, bad = false, badseq = false;
     if (p.block == kFew)
         few_rows<BF, D, W>(g, p, lds, badin, bad, badseq);
     else
@@ -1193,7 +1237,10 @@ Sizes sizes_of(const kq_launch_pattn &a, const kq_launch_paged &c, const kq_laun
      * have two parts or more have slots: of w tiles, at least 3/2 parts long,
      * which makes at most 4/3 of their length by a part's. */
     const uint64_t tiles = (((uint64_t)c.table_pages << c.page_shift) + kTile - 1u) / kTile;
-    const uint64_t most = z.items * ((tiles + kLeast / 2u) / kLeast + 1u);
+    /* where a call is small, items of many rows are kMany / kFew of few, if there
+     * are workgroups for them */
+    const uint64_t finest = z.slot_rows == kFew ? z.items : z.items * (kMany / kFew);
+    const uint64_t most = finest * ((tiles + kLeast / 2u) / kLeast + 1u);
     z.parts = most < kParts + z.items ? most : kParts + z.items;
     z.slots = most < kSlots ? most : kSlots;
     z.plan_bytes = ((4u + (q.count > kByLane ? 2u * (q.count + 1u) : 0u)) * 4u + 255u) / 256u * 256u;
@@ -1203,7 +1250,7 @@ Sizes sizes_of(const kq_launch_pattn &a, const kq_launch_paged &c, const kq_laun
 }
 
 template <bool MANY>
-hipError_t launch(const Args &g, uint32_t parts, uint32_t *status, hipStream_t s) {
+hipError_t launch(const Args &g, uint32_t *status, hipStream_t s) {
     if (MANY) {
         hipLaunchKernelGGL(plan_many, dim3(1), dim3(1024), 0, s, g, status);
         const hipError_t e = hipGetLastError();
@@ -1211,10 +1258,10 @@ hipError_t launch(const Args &g, uint32_t parts, uint32_t *status, hipStream_t s
     }
 #define KQ_ATTEND(BF, D)                                                                     \
     if (g.slot_rows == kFew)                                                                 \
-        hipLaunchKernelGGL(HIP_KERNEL_NAME(attend_few<BF, D, MANY>), dim3(parts), dim3(kThreads), \
+        hipLaunchKernelGGL(HIP_KERNEL_NAME(attend_few<BF, D, MANY>), dim3(g.parts), dim3(kThreads), \
                            0, s, g, status);                                                 \
     else                                                                                     \
-        hipLaunchKernelGGL(HIP_KERNEL_NAME(attend<BF, D, MANY>), dim3(parts),                \
+        hipLaunchKernelGGL(HIP_KERNEL_NAME(attend<BF, D, MANY>), dim3(g.parts),                \
                            dim3(Many<D>::THREADS), 0, s, g, status)
     switch (g.c.width * 2u + (g.c.bf16 ? 1u : 0u)) {
     case 128u: KQ_ATTEND(false, 64); break;
@@ -1252,6 +1299,7 @@ extern "C" hipError_t kq_launch_pattn_run(const kq_launch_pattn *a, const kq_lau
     g.group = a->query_heads / c->heads;
     g.slot_rows = z.slot_rows;
     g.slots = (uint32_t)z.slots;
+    g.parts = (uint32_t)z.parts;
     int exponent = 0;
     const double factor = 2.0 * frexp((double)a->scale * 1.4426950408889634, &exponent);
     g.factor_high = (float)factor;
@@ -1260,6 +1308,6 @@ extern "C" hipError_t kq_launch_pattn_run(const kq_launch_pattn *a, const kq_lau
     g.plan = (uint32_t *)scratch;
     g.items = (Item *)((char *)scratch + z.plan_bytes);
     g.partial = (float *)((char *)scratch + z.plan_bytes + z.item_bytes);
-    return q->count > kByLane ? launch<true>(g, (uint32_t)z.parts, status, s)
-                              : launch<false>(g, (uint32_t)z.parts, status, s);
+    return q->count > kByLane ? launch<true>(g, status, s)
+                              : launch<false>(g, status, s);
 }

@@ -521,6 +521,72 @@ def test_more_sequences_than_a_round_of_the_plan(ctx):  # noqa: F811
     a.check(a.got(ctx))
 
 
+# calls large enough for items of many rows, which share out rows in place of keys
+LARGE = [([130, 65, 257], [900, 33, 0]), ([300], [1700]), ([700, 1, 90, 0, 1], [0, 800, 64, 3, 40]),
+         ([129], [3000])]
+
+
+@pytest.mark.parametrize("type_", TYPES)
+@pytest.mark.parametrize("shape", [(8, 4, 64, 16), (8, 4, 128, 64), (7, 5, 128, 128),
+                                   (4, 17, 64, 32), (6, 3, 256, 64)], ids=str)
+@pytest.mark.parametrize("rows,past", LARGE, ids=str)
+def test_many_rows(ctx, type_, shape, rows, past):  # noqa: F811
+    say("many rows", type_, shape, rows, past)
+    heads, group, width, page = shape
+    n = len(rows)
+    slots = np.random.default_rng(n).permutation(n + 1)[:n].tolist()
+    a = Attention(sum(rows), type_, heads, group, width, page, past, rows, slots, n + 1, lead=1,
+                  gap=2, pad=4)
+    a.check(a.got(ctx, pad=4))
+
+
+@pytest.mark.parametrize("mode", [dict(window=1), dict(window=100), dict(causal=False),
+                                  dict(causal=False, window=70), dict(sinks=True, gate=True),
+                                  dict(scale=-0.2)], ids=str)
+@pytest.mark.parametrize("type_,width", [("f16", 64), ("bf16", 128), ("f16", 256)])
+def test_many_rows_forms(ctx, mode, type_, width):  # noqa: F811
+    say("many rows, forms", mode, type_, width)
+    a = Attention(5, type_, 32, 2, width, 16, [400, 64, 1000], [200, 301, 128], **mode)
+    a.check(a.got(ctx))
+
+
+@pytest.mark.parametrize("where", ["query", "value"])
+def test_many_rows_non_finite(ctx, where):  # noqa: F811
+    say("many rows, non-finite", where)
+    a = Attention(2, "f16", 8, 4, 128, 16, [1500], [300])
+    if where == "query":
+        a.q[211, 77] = np.nan
+    else:
+        a.k.values[a.k.table[0, 70], 3, 3, 9] = NAN
+    assert attending(ctx, a) == "NUMERIC_DOMAIN"
+
+
+def test_many_rows_nothing_outside_the_window(ctx):  # noqa: F811
+    """Pages that a window has left behind do not exist any more."""
+    say("many rows, pages gone")
+    for width, rows in ((64, 400), (128, 300), (256, 260), (128, 1), (128, 9)):
+        a = Attention(2, "bf16", 32, 2, width, 16, [3000], [rows], window=200)
+        gone = (3000 + 1 - 200) // 16
+        for p in a.k.table[0, :gone]:
+            a.k.keys[p] = a.k.values[p] = NAN
+        clean = a.k.table.copy()
+        a.k.table[0, :gone] = 0xFFFFFFFF
+        got = a.got(ctx)
+        a.k.table = clean
+        for p in a.k.table[0, :gone]:
+            a.k.keys[p] = a.k.values[p] = 0
+        # places of the first page that is left, before the window
+        a.check(got)
+
+
+def test_small_items_of_many_heads(ctx):  # noqa: F811
+    """Items of few rows for a small call would be more than its workgroups."""
+    say("many heads")
+    for count, rows in ((7, 32), (70, 7)):
+        a = Attention(5, "f16", 64, 4, 64, 16, [0] * count, [rows] * count)
+        a.check(a.got(ctx))
+
+
 def test_slots_may_be_shared(ctx):  # noqa: F811
     # several rows' worth of queries over one sequence's pages: read, not written
     say("shared")
