@@ -232,7 +232,6 @@ __device__ __forceinline__ void part_of(Part &p, const Args &g, const kq::PagedS
              (p.parts == 1u || p.slot + (p.parts - 1u) * p.step < g.slots);
 }
 
-
 /* x of the lane that CTRL (a DPP control) names, 0 where there is none or ROWS
  * leaves the row of 16 lanes out */
 template <int CTRL, int ROWS>
@@ -823,6 +822,11 @@ __device__ __forceinline__ void few_rows(const Args &g, const Part &p, char *lds
             if (next + 32u * W < end) pages(next + 32u * W);
         }
         weights(key, s, pw);
+        /* V is there: loads return in order, and only the next K's come behind it */
+        if (next < end)
+            wait_vm<2 * STEPS>();
+        else
+            wait_vm<0>();
         gather(pw);
         if (next < end) {
             wait_lgkm0(); /* V is read */
