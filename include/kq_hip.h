@@ -829,7 +829,8 @@ typedef struct kq_hip_rotary {
  *   LINEAR  divided by factor
  *   BANDS   those that turn at least `fast` times in the original context as
  *           they are, at most `slow` times divided by factor, and between
- *           both, along the index i of the plain frequencies, a straight line
+ *           both, along the index i of the plain frequencies (whole indices
+ *           outwards of those that turn so often, from 0 on), a straight line
  *           from one to the other. magnitude: 0.1 ln(factor) + 1. */
 typedef enum kq_hip_rotary_scaling_kind {
     KQ_HIP_ROTARY_SCALING_NONE = 0,

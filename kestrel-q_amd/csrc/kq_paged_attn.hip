@@ -529,7 +529,7 @@ __device__ __forceinline__ void split_query(const Args &g, const Raw<STEPS> &r, 
     const float top = kq::lanes_max<LANES>(__uint_as_float(most < 0x7f800000u ? most : 0u));
     /* the largest value's exponent, 0 for a row of zeros */
     int e = (int)(__float_as_uint(top) >> 23) - 127;
-    e = top == 0.0f ? 0 : e < -100 ? -100 : e;
+    e = top == 0.0f ? 0 : e < -114 ? -114 : e; /* the factor's scale stays finite */
     /* the factor as two numbers: its own rounding would be the same for all keys */
     const float high = __builtin_ldexpf(g.factor_high, TOP - e);
     const float low = __builtin_ldexpf(g.factor_low, TOP - e);

@@ -302,7 +302,7 @@ __global__ __launch_bounds__(kThreads) void append_rows(kq_launch_paged c, kq_la
             x.put(
                 h, u, turns, n, some,
                 [&](uint32_t t) {
-                    return pool + page_of[t] * c.heads * head_values +
+                    return pool + (size_t)page_of[t] * c.heads * head_values +
                            (size_t)(pos_of[t] & mask) * c.width;
                 },
                 badin, bad);

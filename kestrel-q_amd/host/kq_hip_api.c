@@ -84,8 +84,8 @@ static kq_status device_flags(uint32_t flags, kq_diagnostic *diag) {
         return kq_fail(diag, KQ_STATUS_INVALID_ARGUMENT, "an expert id is out of range");
     if (flags & KQ_DEV_SEQUENCE)
         return kq_fail(diag, KQ_STATUS_INVALID_ARGUMENT,
-                       "a sequence's rows decrease or pass the tokens, or its slot is out of "
-                       "range or taken twice");
+                       "a sequence's rows decrease or pass the tokens, its slot is out of range "
+                       "or taken twice, or its tokens pass its pages");
     if (flags & KQ_DEV_INPUT)
         return kq_fail(diag, KQ_STATUS_NUMERIC_DOMAIN, "non-finite input on the device path");
     if (flags & KQ_DEV_MALFORMED)

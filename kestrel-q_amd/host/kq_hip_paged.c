@@ -80,7 +80,8 @@ kq_status kq_hip_rotary_frequencies(const kq_hip_rotary_scaling *v, uint32_t dim
         const double per = (double)dims / (2.0 * log(v->base));
         low = floor(per * log(v->original_context / (turn * v->fast)));
         high = ceil(per * log(v->original_context / (turn * v->slow)));
-        if (low < 0.0) low = 0.0;
+        if (high <= 0.0) low = -1.0; /* none turns more than `slow` times */
+        else if (low < 0.0) low = 0.0;
         if (high > (double)dims - 1.0) high = (double)dims - 1.0;
         if (high - low < 0.001) high = low + 0.001;
     }

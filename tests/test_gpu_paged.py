@@ -615,6 +615,28 @@ def test_sizes_of_queries(ctx, type_, rows, past, size):  # noqa: F811
     a.check(a.got(ctx), rel=2e-6 * grow, big=3e-5 * grow)
 
 
+@pytest.mark.parametrize("type_", TYPES)
+@pytest.mark.parametrize("rows,past", [([1], [200]), ([300], [900])], ids=str)
+def test_tiny_queries_and_a_huge_scale(ctx, type_, rows, past):  # noqa: F811
+    # near the ends of binary32 both; queries below 2^-114 keep their bits too
+    say("tiny queries", type_, rows, past)
+    a = Attention(8, type_, 8, 2, 64, 32, past, rows)
+    a.q *= np.float32(1e-36)
+    a.scale = np.float32(1e36 * 64 ** -0.5)
+    a.check(a.got(ctx))
+
+
+@pytest.mark.parametrize("rows,past", [([1], [60]), ([1], [3000]), ([300], [900])], ids=str)
+def test_sinks_of_any_size(ctx, rows, past):  # noqa: F811
+    """-inf: no sink; a large one takes all the weight."""
+    say("sinks", rows, past)
+    a = Attention(8, "f16", 2, 4, 64, 32, past, rows, sinks=True)
+    a.sinks[:] = [-np.inf, -80.0, 0.0, 3.0, 12.0, 30.0, -3e38, 5.0]
+    a.check(a.got(ctx))
+    a.sinks[:] = 3e38
+    assert not a.got(ctx)[a.mine].any()
+
+
 def test_growing_scores(ctx):  # noqa: F811
     """Keys whose scores grow along the sequence: each tile moves the maximum, by
     little (within the slack) and by much. Scores up to 100: errors 12 times."""

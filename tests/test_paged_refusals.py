@@ -212,6 +212,10 @@ def test_frequencies():
         step = base ** (2.0 / dims)
         assert np.allclose(f[turns > 32 * step], plain[turns > 32 * step], rtol=1e-14, atol=0)
         assert np.allclose(f[turns < 1 / step], plain[turns < 1 / step] / 8, rtol=1e-14, atol=0)
+    # an original context in which nothing, or everything, turns often enough
+    plain = F(64, 1e4)[0]
+    assert np.array_equal(F(64, 1e4, "bands", 8.0, 6.0)[0], plain / 8)
+    assert np.array_equal(F(64, 1e4, "bands", 8.0, 1e9)[0], plain)
     f, _ = F(128, 1e6, "bands", 8.0, 32768.0)
     # a straight line between the borders
     low = math.floor(128 * math.log(32768 / (32 * 2 * math.pi)) / (2 * math.log(1e6)))
