@@ -533,7 +533,9 @@ __device__ __forceinline__ void split_query(const Args &g, const Raw<STEPS> &r, 
     /* the factor as two numbers: its own rounding would be the same for all keys */
     const float high = __builtin_ldexpf(g.factor_high, TOP - e);
     const float low = __builtin_ldexpf(g.factor_low, TOP - e);
-    q.unscale = __builtin_ldexpf(1.0f, e + g.factor_exponent - TOP);
+    /* at least 2^-126, where scores are 0 to any precision: a masked -inf times 0 is none */
+    const int back = e + g.factor_exponent - TOP;
+    q.unscale = __builtin_ldexpf(1.0f, back < -126 ? -126 : back);
 #pragma unroll
     for (int s = 0; s < STEPS; ++s) {
         float x[8];

@@ -626,6 +626,19 @@ def test_tiny_queries_and_a_huge_scale(ctx, type_, rows, past):  # noqa: F811
     a.check(a.got(ctx))
 
 
+@pytest.mark.parametrize("type_", TYPES)
+@pytest.mark.parametrize("rows,past", [([1], [200]), ([300], [900])], ids=str)
+@pytest.mark.parametrize("scale", [0.0, 1e-30])
+def test_scores_of_nothing(ctx, type_, rows, past, scale):  # noqa: F811
+    """Scores far below binary32's range, and a scale of 0: all keys that a row sees
+    weigh the same, and those that its mask leaves out nothing."""
+    say("scores of nothing", type_, rows, past, scale)
+    a = Attention(9, type_, 8, 2, 64, 32, past, rows, window=150)
+    a.q *= np.float32(1e-30)
+    a.scale = np.float32(scale)
+    a.check(a.got(ctx))
+
+
 @pytest.mark.parametrize("rows,past", [([1], [60]), ([1], [3000]), ([300], [900])], ids=str)
 def test_sinks_of_any_size(ctx, rows, past):  # noqa: F811
     """-inf: no sink; a large one takes all the weight."""
