@@ -59,6 +59,15 @@ constexpr uint32_t kParts = 1024;
 constexpr uint32_t kShort = 8;       /* tiles */
 constexpr uint32_t kLeast = 2;       /* tiles */
 constexpr uint32_t kSmall = 512;     /* tiles in all of items of many rows */
+/* Items of few rows are a workgroup's each, of as many waves as a CU holds, where
+ * there are CUs for all of them and the table's lines are short: 6 tiles of 128,
+ * 196 KB of keys and values, which those waves bring in at once. There is nothing
+ * to join then. 8 sequences of 30 to 318 keys 7.0 - 9.9 us, in parts of two tiles
+ * and a join 7.7 - 10.8; heads of 64 of 30 to 700 keys 5.9 - 9.8, 7.8 - 9.9. Behind
+ * that a CU alone is slow, 47 GB/s: 2000 keys 23.7, 11.2. And 512 items, two to a
+ * CU one after the other, 15.3, 13.9. */
+constexpr uint32_t kWholeItems = 256;
+constexpr uint32_t kWhole = 768; /* tiles times width */
 constexpr uint32_t kSlots = (4u * kParts + 2u) / 3u;
 constexpr uint32_t kByLane = 64;     /* sequences that each wave plans by itself */
 constexpr float kSlack = 8.0f;       /* by which a row's largest exponent may pass its stand-in */
@@ -271,7 +280,7 @@ __device__ __forceinline__ uint64_t lanes_add(uint64_t v) {
  * has done so. Offsets, slots and lengths that break the rules leave no part at
  * all: where they hold, the rows of all sequences are at most the call's tokens,
  * which the host's sizes go by. */
-template <bool MANY>
+template <bool MANY, bool WHOLE = false>
 __device__ __forceinline__ Part find_part(const Args &g, uint32_t index, uint32_t *status) {
     Part p;
     p.live = p.slotted = false;
@@ -297,7 +306,10 @@ __device__ __forceinline__ Part find_part(const Args &g, uint32_t index, uint32_
         uint32_t each, mine, through, total;
         for (;;) {
             n = need_of(g, s, small);
-            length = part_tiles(lanes_add(cost_of(g, n)), small);
+            if (WHOLE)
+                length = Lengths{1u << 24, 0u};
+            else
+                length = part_tiles(lanes_add(cost_of(g, n)), small);
             each = parts_of(n.tiles, length_of(length, n));
             mine = n.blocks * g.c.heads * each;
             through = lanes_through(mine);
@@ -1108,6 +1120,22 @@ __global__ __launch_bounds__(kThreads, (few_side<BF, D>())) void attend_few(Args
     if (bad) kq_flag(status, KQ_DEV_NUMERIC);
 }
 
+/* calls of few rows that need no join: an item is a workgroup's */
+template <bool BF, int D>
+__global__ __launch_bounds__((256 * few_side<BF, D>()), (few_side<BF, D>())) void attend_whole(
+    Args g, uint32_t *status) {
+    constexpr int W = 4 * few_side<BF, D>();
+    __shared__ __attribute__((aligned(16))) char lds[few_bytes<D, W>()];
+    Part p = find_part<false, true>(g, blockIdx.x, status);
+    if (!p.live) return;
+    p.pin();
+    bool badin = false, bad = false, badseq = false;
+    few_rows<BF, D, W>(g, p, lds, badin, bad, badseq);
+    if (badseq) kq_flag(status, KQ_DEV_SEQUENCE);
+    if (badin) kq_flag(status, KQ_DEV_INPUT);
+    if (bad) kq_flag(status, KQ_DEV_NUMERIC);
+}
+
 template <bool BF, int D, bool MANY>
 __global__ __launch_bounds__(Many<D>::THREADS, D == 64 ? 3 : 2) void attend(Args g, uint32_t *status) {
     constexpr int W = Many<D>::W;
@@ -1227,6 +1255,7 @@ __global__ __launch_bounds__(kThreads) void join_parts(Args g, uint32_t *status)
 struct Sizes {
     uint64_t items, parts, slots;
     uint32_t slot_rows;
+    bool whole;
     uint64_t plan_bytes, item_bytes, bytes;
 };
 
@@ -1243,12 +1272,21 @@ Sizes sizes_of(const kq_launch_pattn &a, const kq_launch_paged &c, const kq_laun
      * have two parts or more have slots: of w tiles, at least 3/2 parts long,
      * which makes at most 4/3 of their length by a part's. */
     const uint64_t tiles = (((uint64_t)c.table_pages << c.page_shift) + kTile - 1u) / kTile;
+    uint64_t sees = tiles; /* that an item reads at most */
+    if (a.window != 0u && a.causal != 0u) {
+        const uint64_t keys = (uint64_t)a.window + z.slot_rows;
+        sees = (keys + kTile - 1u) / kTile + 1u < tiles ? (keys + kTile - 1u) / kTile + 1u : tiles;
+    }
+    z.whole = z.slot_rows == kFew && q.count <= kByLane && z.items <= kWholeItems &&
+              sees * c.width <= (uint64_t)kWhole;
     /* where a call is small, items of many rows are kMany / kFew of few, if there
      * are workgroups for them */
     const uint64_t finest = z.slot_rows == kFew ? z.items : z.items * (kMany / kFew);
     const uint64_t most = finest * ((tiles + kLeast / 2u) / kLeast + 1u);
     z.parts = most < kParts + z.items ? most : kParts + z.items;
     z.slots = most < kSlots ? most : kSlots;
+    if (z.whole) z.parts = z.items;
+    if (z.whole || sees < kLeast * 3u / 2u) z.slots = 0u; /* nothing has two parts */
     z.plan_bytes = ((4u + (q.count > kByLane ? 2u * (q.count + 1u) : 0u)) * 4u + 255u) / 256u * 256u;
     z.item_bytes = (z.slots * sizeof(Item) + 255u) / 256u * 256u;
     z.bytes = z.plan_bytes + z.item_bytes + z.slots * z.slot_rows * (c.width + 2u) * 4u;
@@ -1256,14 +1294,17 @@ Sizes sizes_of(const kq_launch_pattn &a, const kq_launch_paged &c, const kq_laun
 }
 
 template <bool MANY>
-hipError_t launch(const Args &g, uint32_t *status, hipStream_t s) {
+hipError_t launch(const Args &g, bool whole, uint32_t *status, hipStream_t s) {
     if (MANY) {
         hipLaunchKernelGGL(plan_many, dim3(1), dim3(1024), 0, s, g, status);
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess) return e;
     }
 #define KQ_ATTEND(BF, D)                                                                     \
-    if (g.slot_rows == kFew)                                                                 \
+    if (whole)                                                                               \
+        hipLaunchKernelGGL(HIP_KERNEL_NAME(attend_whole<BF, D>), dim3(g.parts),                \
+                           dim3(256 * few_side<BF, D>()), 0, s, g, status);                   \
+    else if (g.slot_rows == kFew)                                                                 \
         hipLaunchKernelGGL(HIP_KERNEL_NAME(attend_few<BF, D, MANY>), dim3(g.parts), dim3(kThreads), \
                            0, s, g, status);                                                 \
     else                                                                                     \
@@ -1280,7 +1321,7 @@ hipError_t launch(const Args &g, uint32_t *status, hipStream_t s) {
     }
 #undef KQ_ATTEND
     const hipError_t e = hipGetLastError();
-    if (e != hipSuccess) return e;
+    if (e != hipSuccess || g.slots == 0u) return e; /* nothing to join */
     /* where rows are many, a part's share is shared out again: kAtOnce pieces a thread */
     hipLaunchKernelGGL(join_parts, dim3(g.slots, g.slot_rows == kFew ? 1u : g.c.width / 64u),
                        dim3(kThreads), 0, s, g, status);
@@ -1314,6 +1355,6 @@ extern "C" hipError_t kq_launch_pattn_run(const kq_launch_pattn *a, const kq_lau
     g.plan = (uint32_t *)scratch;
     g.items = (Item *)((char *)scratch + z.plan_bytes);
     g.partial = (float *)((char *)scratch + z.plan_bytes + z.item_bytes);
-    return q->count > kByLane ? launch<true>(g, status, s)
-                              : launch<false>(g, status, s);
+    return q->count > kByLane ? launch<true>(g, z.whole, status, s)
+                              : launch<false>(g, z.whole, status, s);
 }

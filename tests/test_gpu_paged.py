@@ -587,6 +587,46 @@ def test_small_items_of_many_heads(ctx):  # noqa: F811
         a.check(a.got(ctx))
 
 
+@pytest.mark.parametrize("type_", TYPES)
+@pytest.mark.parametrize("width,tiles", [(64, 12), (128, 6), (256, 3)])
+@pytest.mark.parametrize("over", [0, 1])
+def test_short_lines(ctx, type_, width, tiles, over):  # noqa: F811
+    """Lines of the table at the size where a workgroup takes an item whole, and past
+    it; sequences of every length that fits, with the window and the sink besides."""
+    say("short lines", type_, width, tiles, over)
+    keys = (tiles + over) * 64
+    past = [0, 1, 31, 32, 63, 64, 127, keys - 65, keys - 33, keys - 3]
+    a = Attention(12, type_, 2, 8, width, 32, past, [1] * 10, line=keys // 32, sinks=True)
+    a.check(a.got(ctx))
+    a = Attention(13, type_, 2, 4, width, 64, [keys - 3], [3], line=keys // 64, window=130)
+    a.check(a.got(ctx))
+    a = Attention(14, type_, 4, 2, width, 16, past[-4:], [2, 0, 1, 3], line=keys // 16,
+                  causal=False, gate=True, lead=1, gap=1)
+    a.check(a.got(ctx))
+
+
+@pytest.mark.parametrize("type_,width", [("f16", 128), ("bf16", 64)])
+@pytest.mark.parametrize("rows", [1, 60])
+@pytest.mark.parametrize("line", [8, 12])
+def test_lines_of_two_and_three_tiles(ctx, type_, width, rows, line):  # noqa: F811
+    # no item has two parts in lines of two tiles; long lines behind a window of two
+    say("two and three tiles", type_, width, rows, line)
+    past = [line * 16 - rows, 3, 0, 65]
+    a = Attention(15, type_, 2, 4, width, 16, past, [rows] * 4, line=line)
+    a.check(a.got(ctx))
+    a = Attention(16, type_, 80, 1, width, 16, past, [1] * 4, line=line)  # 320 items
+    a.check(a.got(ctx))
+    a = Attention(17, type_, 2, 4, width, 16, [5000, 20, 700], [1, 1, 1], window=60)
+    a.check(a.got(ctx))
+
+
+def test_bad_slot_in_a_short_line(ctx):  # noqa: F811
+    say("bad slot, short lines")
+    a = Attention(18, "f16", 2, 4, 128, 32, [5, 90], [1, 1], line=4)
+    a.k.slots = [0, 2]
+    assert attending(ctx, a) == "INVALID_ARGUMENT"
+
+
 def test_slots_may_be_shared(ctx):  # noqa: F811
     # several rows' worth of queries over one sequence's pages: read, not written
     say("shared")
