@@ -68,6 +68,11 @@ constexpr uint32_t kSmall = 512;     /* tiles in all of items of many rows */
  * CU one after the other, 15.3, 13.9. */
 constexpr uint32_t kWholeItems = 256;
 constexpr uint32_t kWhole = 768; /* tiles times width */
+/* Calls of many rows over short lines have items of one part too: 7 tiles of 128
+ * (97 rows of 24 heads over themselves 8.1 us, 9.8 with parts and a join; 1000 rows
+ * of 9 sequences 22.6, 31.3; 500 of one, 9 tiles, would take 23.4, 22.7, and in bf16
+ * 30.6, 24.8), 14 of 64, of which 12 measured 19.5, 22.5. */
+constexpr uint32_t kWholeMany = 896;
 constexpr uint32_t kSlots = (4u * kParts + 2u) / 3u;
 constexpr uint32_t kByLane = 64;     /* sequences that each wave plans by itself */
 constexpr float kSlack = 8.0f;       /* by which a row's largest exponent may pass its stand-in */
@@ -81,6 +86,7 @@ struct Args {
     uint32_t slot_rows; /* rows that a slot of the partial results holds */
     uint32_t slots;     /* partial results that there is room for */
     uint32_t parts;     /* workgroups */
+    bool whole;         /* each item is one part */
     float factor_high, factor_low; /* scale log2(e), 1 .. 2 and its exponent */
     int factor_exponent;
     struct Item *items; /* of the slots, for the join */
@@ -130,7 +136,7 @@ __device__ __forceinline__ uint64_t cost_of(const Args &g, const Need &n) {
 /* Whether a call's items of many rows, of that cost in all, are better cut into
  * items of few: a workgroup of many rows begins with 5 us of queries and first
  * tiles and takes 2 us a tile when the device is not full, and its parts are
- * joined. 97 rows of 24 heads over themselves (48 tiles) 10.6 us, 19.4 as items of
+ * joined. 97 rows of 24 heads over themselves (48 tiles) 8.1 us, 19.4 as items of
  * many rows; 92 rows over 1321 keys (105) 17.9, 20.8; 794 rows of 10 sequences (736)
  * 42, 36: items of few read their keys eight times. Heads of 256, whose workgroups
  * have no room beside each other, are faster as they are (116 rows of 32 heads: 23
@@ -139,7 +145,8 @@ __device__ __forceinline__ bool is_small(const Args &g, uint64_t cost_of_many) {
     return g.c.width != 256u && cost_of_many != 0u && cost_of_many < kSmall;
 }
 
-__device__ __forceinline__ Lengths part_tiles(uint64_t cost, bool small) {
+__device__ __forceinline__ Lengths part_tiles(const Args &g, uint64_t cost, bool small) {
+    if (g.whole) return Lengths{1u << 24, small ? 0u : 1u << 24};
     const uint32_t fine = (uint32_t)((cost + kParts - 1u) / kParts);
     const uint32_t coarse = (uint32_t)((cost + kParts / 2u - 1u) / (kParts / 2u));
     Lengths l;
@@ -280,7 +287,7 @@ __device__ __forceinline__ uint64_t lanes_add(uint64_t v) {
  * has done so. Offsets, slots and lengths that break the rules leave no part at
  * all: where they hold, the rows of all sequences are at most the call's tokens,
  * which the host's sizes go by. */
-template <bool MANY, bool WHOLE = false>
+template <bool MANY>
 __device__ __forceinline__ Part find_part(const Args &g, uint32_t index, uint32_t *status) {
     Part p;
     p.live = p.slotted = false;
@@ -306,10 +313,7 @@ __device__ __forceinline__ Part find_part(const Args &g, uint32_t index, uint32_
         uint32_t each, mine, through, total;
         for (;;) {
             n = need_of(g, s, small);
-            if (WHOLE)
-                length = Lengths{1u << 24, 0u};
-            else
-                length = part_tiles(lanes_add(cost_of(g, n)), small);
+            length = part_tiles(g, lanes_add(cost_of(g, n)), small);
             each = parts_of(n.tiles, length_of(length, n));
             mine = n.blocks * g.c.heads * each;
             through = lanes_through(mine);
@@ -378,7 +382,7 @@ __global__ __launch_bounds__(1024) void plan_many(Args g, uint32_t *status) {
     uint32_t *first = g.plan + 4u, *slot = first + g.q.count + 1u;
     for (;;) {
         const Lengths length = part_tiles(
-            sum([&](const kq::PagedSeq &s) { return cost_of(g, need_of(g, s, small)); }), small);
+            g, sum([&](const kq::PagedSeq &s) { return cost_of(g, need_of(g, s, small)); }), small);
         uint32_t parts_before = 0u, slots_before = 0u;
         for (uint32_t base = 0u; base < g.q.count; base += 1024u) {
             const uint32_t s = base + threadIdx.x;
@@ -1126,7 +1130,7 @@ __global__ __launch_bounds__((256 * few_side<BF, D>()), (few_side<BF, D>())) voi
     Args g, uint32_t *status) {
     constexpr int W = 4 * few_side<BF, D>();
     __shared__ __attribute__((aligned(16))) char lds[few_bytes<D, W>()];
-    Part p = find_part<false, true>(g, blockIdx.x, status);
+    Part p = find_part<false>(g, blockIdx.x, status);
     if (!p.live) return;
     p.pin();
     bool badin = false, bad = false, badseq = false;
@@ -1255,7 +1259,7 @@ __global__ __launch_bounds__(kThreads) void join_parts(Args g, uint32_t *status)
 struct Sizes {
     uint64_t items, parts, slots;
     uint32_t slot_rows;
-    bool whole;
+    bool whole, wide; /* each item is one part; and a workgroup's of many waves */
     uint64_t plan_bytes, item_bytes, bytes;
 };
 
@@ -1277,16 +1281,16 @@ Sizes sizes_of(const kq_launch_pattn &a, const kq_launch_paged &c, const kq_laun
         const uint64_t keys = (uint64_t)a.window + z.slot_rows;
         sees = (keys + kTile - 1u) / kTile + 1u < tiles ? (keys + kTile - 1u) / kTile + 1u : tiles;
     }
-    z.whole = z.slot_rows == kFew && q.count <= kByLane && z.items <= kWholeItems &&
-              sees * c.width <= (uint64_t)kWhole;
+    z.wide = z.slot_rows == kFew && q.count <= kByLane && z.items <= kWholeItems &&
+             sees * c.width <= (uint64_t)kWhole;
+    z.whole = z.wide || sees < kLeast * 3u / 2u ||
+              (z.slot_rows == kMany && sees * c.width <= (uint64_t)kWholeMany);
     /* where a call is small, items of many rows are kMany / kFew of few, if there
      * are workgroups for them */
     const uint64_t finest = z.slot_rows == kFew ? z.items : z.items * (kMany / kFew);
-    const uint64_t most = finest * ((tiles + kLeast / 2u) / kLeast + 1u);
+    const uint64_t most = finest * (z.whole ? 1u : (tiles + kLeast / 2u) / kLeast + 1u);
     z.parts = most < kParts + z.items ? most : kParts + z.items;
-    z.slots = most < kSlots ? most : kSlots;
-    if (z.whole) z.parts = z.items;
-    if (z.whole || sees < kLeast * 3u / 2u) z.slots = 0u; /* nothing has two parts */
+    z.slots = z.whole ? 0u : most < kSlots ? most : kSlots;
     z.plan_bytes = ((4u + (q.count > kByLane ? 2u * (q.count + 1u) : 0u)) * 4u + 255u) / 256u * 256u;
     z.item_bytes = (z.slots * sizeof(Item) + 255u) / 256u * 256u;
     z.bytes = z.plan_bytes + z.item_bytes + z.slots * z.slot_rows * (c.width + 2u) * 4u;
@@ -1294,14 +1298,14 @@ Sizes sizes_of(const kq_launch_pattn &a, const kq_launch_paged &c, const kq_laun
 }
 
 template <bool MANY>
-hipError_t launch(const Args &g, bool whole, uint32_t *status, hipStream_t s) {
+hipError_t launch(const Args &g, bool wide, uint32_t *status, hipStream_t s) {
     if (MANY) {
         hipLaunchKernelGGL(plan_many, dim3(1), dim3(1024), 0, s, g, status);
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess) return e;
     }
 #define KQ_ATTEND(BF, D)                                                                     \
-    if (whole)                                                                               \
+    if (wide)                                                                                \
         hipLaunchKernelGGL(HIP_KERNEL_NAME(attend_whole<BF, D>), dim3(g.parts),                \
                            dim3(256 * few_side<BF, D>()), 0, s, g, status);                   \
     else if (g.slot_rows == kFew)                                                                 \
@@ -1347,6 +1351,7 @@ extern "C" hipError_t kq_launch_pattn_run(const kq_launch_pattn *a, const kq_lau
     g.slot_rows = z.slot_rows;
     g.slots = (uint32_t)z.slots;
     g.parts = (uint32_t)z.parts;
+    g.whole = z.whole;
     int exponent = 0;
     const double factor = 2.0 * frexp((double)a->scale * 1.4426950408889634, &exponent);
     g.factor_high = (float)factor;
@@ -1355,6 +1360,6 @@ extern "C" hipError_t kq_launch_pattn_run(const kq_launch_pattn *a, const kq_lau
     g.plan = (uint32_t *)scratch;
     g.items = (Item *)((char *)scratch + z.plan_bytes);
     g.partial = (float *)((char *)scratch + z.plan_bytes + z.item_bytes);
-    return q->count > kByLane ? launch<true>(g, z.whole, status, s)
-                              : launch<false>(g, z.whole, status, s);
+    return q->count > kByLane ? launch<true>(g, z.wide, status, s)
+                              : launch<false>(g, z.wide, status, s);
 }

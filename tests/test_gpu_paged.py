@@ -620,6 +620,22 @@ def test_lines_of_two_and_three_tiles(ctx, type_, width, rows, line):  # noqa: F
     a.check(a.got(ctx))
 
 
+@pytest.mark.parametrize("type_", TYPES)
+@pytest.mark.parametrize("width,tiles", [(64, 14), (128, 7), (256, 3)])
+@pytest.mark.parametrize("over", [0, 1])
+def test_short_lines_of_many_rows(ctx, type_, width, tiles, over):  # noqa: F811
+    say("short lines, many rows", type_, width, tiles, over)
+    keys = (tiles + over) * 64
+    for seed, heads, rows in ((19, 1, [20, 1, 0, 65, 129]), (20, 24, [190, 60, 5, 128, 190])):
+        past = [keys - rows[0], 3, 0, 64, keys - 190]
+        a = Attention(seed, type_, heads, 3, width, 64, past, rows, line=keys // 64)
+        a.check(a.got(ctx))
+    a = Attention(21, type_, 2, 5, width, 32, [1000], [70], window=40, gate=True)
+    a.check(a.got(ctx))
+    a = Attention(22, type_, 2, 2, width, 32, [3] * 70, [7] * 70, line=keys // 32, causal=False)
+    a.check(a.got(ctx))
+
+
 def test_bad_slot_in_a_short_line(ctx):  # noqa: F811
     say("bad slot, short lines")
     a = Attention(18, "f16", 2, 4, 128, 32, [5, 90], [1, 1], line=4)
