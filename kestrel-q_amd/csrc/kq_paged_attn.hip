@@ -133,16 +133,24 @@ __device__ __forceinline__ uint64_t cost_of(const Args &g, const Need &n) {
     return (uint64_t)n.blocks * g.c.heads * n.tiles;
 }
 
-/* Whether a call's items of many rows, of that cost in all, are better cut into
- * items of few: a workgroup of many rows begins with 5 us of queries and first
- * tiles and takes 2 us a tile when the device is not full, and its parts are
+/* the tiles of its items of many rows, as many as their rows see on the average */
+__device__ __forceinline__ uint64_t seen_by_many(const Args &g, const kq::PagedSeq &s,
+                                                 const Need &n) {
+    if (n.block != kMany) return 0u;
+    const uint32_t mean = (s.past + s.rows / 2u + kTile - 1u) / kTile;
+    return (uint64_t)n.blocks * g.c.heads * (g.a.causal && mean < n.tiles ? mean : n.tiles);
+}
+
+/* Whether a call's items of many rows, that see so many tiles in all, are better
+ * cut into items of few: a workgroup of many rows begins with 5 us of queries and
+ * first tiles and takes 2 us a tile when the device is not full, and its parts are
  * joined. 97 rows of 24 heads over themselves (48 tiles) 8.1 us, 19.4 as items of
  * many rows; 92 rows over 1321 keys (105) 17.9, 20.8; 794 rows of 10 sequences (736)
  * 42, 36: items of few read their keys eight times. Heads of 256, whose workgroups
  * have no room beside each other, are faster as they are (116 rows of 32 heads: 23
  * us, 32). */
-__device__ __forceinline__ bool is_small(const Args &g, uint64_t cost_of_many) {
-    return g.c.width != 256u && cost_of_many != 0u && cost_of_many < kSmall;
+__device__ __forceinline__ bool is_small(const Args &g, uint64_t seen) {
+    return g.c.width != 256u && seen != 0u && seen < kSmall;
 }
 
 __device__ __forceinline__ Lengths part_tiles(const Args &g, uint64_t cost, bool small) {
@@ -305,8 +313,7 @@ __device__ __forceinline__ Part find_part(const Args &g, uint32_t index, uint32_
         }
         bool small = false;
         if (g.slot_rows == kMany) {
-            const Need n = need_of(g, s, false);
-            small = is_small(g, lanes_add(n.block == kMany ? cost_of(g, n) : 0u));
+            small = is_small(g, lanes_add(seen_by_many(g, s, need_of(g, s, false))));
         }
         Need n;
         Lengths length;
@@ -371,8 +378,7 @@ __global__ __launch_bounds__(1024) void plan_many(Args g, uint32_t *status) {
         return v;
     };
     bool small = is_small(g, sum([&](const kq::PagedSeq &s) {
-                              const Need n = need_of(g, s, false);
-                              return n.block == kMany ? cost_of(g, n) : (uint64_t)0u;
+                              return seen_by_many(g, s, need_of(g, s, false));
                           }));
     if (bad) kq_flag(status, KQ_DEV_SEQUENCE);
     if (__syncthreads_or(bad)) {
