@@ -48,6 +48,7 @@ constexpr int kThreads = 256;
 constexpr uint32_t kTile = 64;       /* keys of a tile */
 constexpr uint32_t kFew = 16;        /* rows of an item whose waves share out its keys */
 constexpr uint32_t kMany = 128;      /* rows of an item whose waves share out its rows */
+constexpr uint32_t kMid = 64;        /* the same, where the device is not full */
 /* Parts that a call's items are cut into. Of few rows 1024, three to four rounds
  * of the device's waves that follow each other: 61 sequences 102 us, with 512
  * parts 116, with 2048 111. But parts of fewer than 8 tiles are not worth a
@@ -59,6 +60,9 @@ constexpr uint32_t kParts = 1024;
 constexpr uint32_t kShort = 8;       /* tiles */
 constexpr uint32_t kLeast = 2;       /* tiles */
 constexpr uint32_t kSmall = 512;     /* tiles in all of items of many rows */
+constexpr uint32_t kMiddle = 2560;
+constexpr uint32_t kFill = 448;
+constexpr uint32_t kEven = 700;
 /* Items of few rows are a workgroup's each, of as many waves as a CU holds, where
  * there are CUs for all of them and the table's lines are short: 6 tiles of 128,
  * 196 KB of keys and values, which those waves bring in at once. There is nothing
@@ -73,6 +77,7 @@ constexpr uint32_t kWhole = 768; /* tiles times width */
  * of 9 sequences 22.6, 31.3; 500 of one, 9 tiles, would take 23.4, 22.7, and in bf16
  * 30.6, 24.8), 14 of 64, of which 12 measured 19.5, 22.5. */
 constexpr uint32_t kWholeMany = 896;
+constexpr uint32_t kPlan = 5;        /* words of the plan before the sequences' */
 constexpr uint32_t kSlots = (4u * kParts + 2u) / 3u;
 constexpr uint32_t kByLane = 64;     /* sequences that each wave plans by itself */
 constexpr float kSlack = 8.0f;       /* by which a row's largest exponent may pass its stand-in */
@@ -97,13 +102,13 @@ struct Args {
 
 /* ---------------------------------------------------------------- the plan */
 
-/* Tiles a part, of items of few and of many rows; many 0: all items have few. */
+/* Tiles a part, of items of few and of more rows. */
 struct Lengths {
     uint32_t few, many;
 };
 
-__device__ __forceinline__ uint32_t block_of(uint32_t rows, bool small) {
-    return rows <= kFew || small ? kFew : kMany;
+__device__ __forceinline__ uint32_t block_of(uint32_t rows, uint32_t most) {
+    return rows <= kFew ? kFew : most;
 }
 
 /* What a sequence asks for: its items (blocks of rows, for each key head) and
@@ -112,8 +117,8 @@ struct Need {
     uint32_t blocks, tiles, block;
 };
 
-__device__ __forceinline__ Need need_of(const Args &g, const kq::PagedSeq &s, bool small) {
-    const uint32_t rows = s.rows * g.group, block = block_of(rows, small);
+__device__ __forceinline__ Need need_of(const Args &g, const kq::PagedSeq &s, uint32_t most) {
+    const uint32_t rows = s.rows * g.group, block = block_of(rows, most);
     Need n = {0u, 0u, block};
     if (!s.live || s.rows == 0u) return n;
     n.blocks = (rows + block - 1u) / block;
@@ -149,18 +154,33 @@ __device__ __forceinline__ uint64_t seen_by_many(const Args &g, const kq::PagedS
  * 42, 36: items of few read their keys eight times. Heads of 256, whose workgroups
  * have no room beside each other, are faster as they are (116 rows of 32 heads: 23
  * us, 32). */
-__device__ __forceinline__ bool is_small(const Args &g, uint64_t seen) {
-    return g.c.width != 256u && seen != 0u && seen < kSmall;
+__device__ __forceinline__ uint32_t rows_of_items(const Args &g, uint64_t seen) {
+    return g.c.width == 256u || seen >= kMiddle ? kMany : seen < kSmall ? kFew : kMid;
+}
+/* Whether a plan of items of `most` rows with so many parts holds; otherwise `most`
+ * becomes what is planned next. */
+__device__ __forceinline__ bool plan_holds(const Args &g, uint32_t &most, bool &last,
+                                           uint32_t parts, uint64_t seen, uint64_t cost) {
+    if (most == kMany) {
+        const bool uneven = parts < kEven && seen * 4u <= cost * 3u;
+        if (last || g.c.width == 256u || !(parts < kFill || uneven)) return true;
+        most = kMid;
+    } else {
+        if (parts <= g.parts) return true;
+        most = g.c.width == 256u || most == kMid ? kMany : kMid;
+    }
+    last = true;
+    return false;
 }
 
-__device__ __forceinline__ Lengths part_tiles(const Args &g, uint64_t cost, bool small) {
-    if (g.whole) return Lengths{1u << 24, small ? 0u : 1u << 24};
+__device__ __forceinline__ Lengths part_tiles(const Args &g, uint64_t cost) {
+    if (g.whole) return Lengths{1u << 24, 1u << 24};
     const uint32_t fine = (uint32_t)((cost + kParts - 1u) / kParts);
     const uint32_t coarse = (uint32_t)((cost + kParts / 2u - 1u) / (kParts / 2u));
     Lengths l;
     l.few = coarse < kShort ? coarse : fine > kShort ? fine : kShort;
     l.few = l.few < kLeast ? kLeast : l.few;
-    l.many = small ? 0u : coarse < kLeast ? kLeast : coarse;
+    l.many = coarse < kLeast ? kLeast : coarse;
     return l;
 }
 
@@ -180,7 +200,7 @@ __device__ __forceinline__ uint32_t parts_of(uint32_t tiles, uint32_t length) {
 struct Part {
     kq::PagedSeq seq;
     uint32_t row0, rows;  /* of the sequence's rows x group */
-    uint32_t block;       /* kFew or kMany */
+    uint32_t block;       /* kFew, kMid or kMany */
     uint32_t head;
     uint32_t part, parts; /* this one, and how many the item really has */
     uint32_t t0, t1;      /* its tiles */
@@ -203,7 +223,7 @@ struct Part {
  * where its item's partial results lie. The part's workgroup leaves it, by slot;
  * plan[3] says how many slots there are. */
 struct __attribute__((aligned(16))) Item {
-    uint32_t begin, row0, rows, head_few; /* rows 0: nothing to join; few: the upper half */
+    uint32_t begin, row0, rows, head_kind; /* rows 0: nothing to join; kind: the upper half */
     uint32_t part, parts, slot, step;
 };
 
@@ -211,7 +231,8 @@ __device__ __forceinline__ void leave(const Args &g, const Part &p) {
     if (threadIdx.x != 0u || !p.slotted) return;
     const uint32_t at = p.slot + p.part * p.step;
     if (at < g.slots) {
-        Item t = {p.seq.begin, p.row0, p.rows, p.head | (p.block == kFew ? 1u << 16 : 0u),
+        const uint32_t kind = p.block == kFew ? 1u : p.block == kMid || g.c.width == 256u ? 2u : 0u;
+        Item t = {p.seq.begin, p.row0, p.rows, p.head | kind << 16,
                   p.part, p.parts, p.slot, p.step};
         if (!p.live || p.parts == 1u) t.rows = 0u;
         g.items[at] = t;
@@ -311,22 +332,25 @@ __device__ __forceinline__ Part find_part(const Args &g, uint32_t index, uint32_
             }
             return p;
         }
-        bool small = false;
+        uint32_t most = kFew;
+        uint64_t seen = 0u;
         if (g.slot_rows == kMany) {
-            small = is_small(g, lanes_add(seen_by_many(g, s, need_of(g, s, false))));
+            seen = lanes_add(seen_by_many(g, s, need_of(g, s, kMany)));
+            most = rows_of_items(g, seen);
         }
         Need n;
         Lengths length;
         uint32_t each, mine, through, total;
+        bool last = false;
         for (;;) {
-            n = need_of(g, s, small);
-            length = part_tiles(g, lanes_add(cost_of(g, n)), small);
+            n = need_of(g, s, most);
+            const uint64_t cost = lanes_add(cost_of(g, n));
+            length = part_tiles(g, cost);
             each = parts_of(n.tiles, length_of(length, n));
             mine = n.blocks * g.c.heads * each;
             through = lanes_through(mine);
             total = __builtin_amdgcn_readlane(through, 63);
-            if (!small || total <= g.parts) break;
-            small = false;
+            if (plan_holds(g, most, last, total, seen, cost)) break;
         }
         const uint32_t first = through - mine;
         const uint32_t held = each > 1u ? mine : 0u, slots = lanes_through(held);
@@ -341,18 +365,18 @@ __device__ __forceinline__ Part find_part(const Args &g, uint32_t index, uint32_
         w.past = __builtin_amdgcn_readlane(s.past, at);
         w.slot = __builtin_amdgcn_readlane(s.slot, at);
         w.live = true;
-        const Need need = need_of(g, w, small);
+        const Need need = need_of(g, w, most);
         part_of(p, g, w, need, length_of(length, need),
                 index - __builtin_amdgcn_readlane(first, at),
                 __builtin_amdgcn_readlane(first_slot, at));
         return p;
     } else {
         if (index >= g.plan[1]) return p;
-        const uint32_t *first = g.plan + 4u, *slots = first + g.q.count + 1u;
+        const uint32_t *first = g.plan + kPlan, *slots = first + g.q.count + 1u;
         const uint32_t s = kq::wave_find(first, g.q.count, index);
         const kq::PagedSeq w = kq::paged_seq(g.q, g.c, s, bad);
         const Lengths length = {g.plan[0], g.plan[2]};
-        const Need need = need_of(g, w, length.many == 0u);
+        const Need need = need_of(g, w, g.plan[4]);
         part_of(p, g, w, need, length_of(length, need), index - first[s], slots[s]);
         return p;
     }
@@ -377,24 +401,27 @@ __global__ __launch_bounds__(1024) void plan_many(Args g, uint32_t *status) {
         __syncthreads();
         return v;
     };
-    bool small = is_small(g, sum([&](const kq::PagedSeq &s) {
-                              return seen_by_many(g, s, need_of(g, s, false));
-                          }));
+    const uint64_t seen = sum([&](const kq::PagedSeq &s) {
+        return seen_by_many(g, s, need_of(g, s, kMany));
+    });
+    uint32_t most = g.slot_rows == kFew ? kFew : rows_of_items(g, seen);
+    bool last = false;
     if (bad) kq_flag(status, KQ_DEV_SEQUENCE);
     if (__syncthreads_or(bad)) {
         if (threadIdx.x == 0u) g.plan[1] = g.plan[3] = 0u;
         return;
     }
-    uint32_t *first = g.plan + 4u, *slot = first + g.q.count + 1u;
+    uint32_t *first = g.plan + kPlan, *slot = first + g.q.count + 1u;
     for (;;) {
-        const Lengths length = part_tiles(
-            g, sum([&](const kq::PagedSeq &s) { return cost_of(g, need_of(g, s, small)); }), small);
+        const uint64_t cost =
+            sum([&](const kq::PagedSeq &s) { return cost_of(g, need_of(g, s, most)); });
+        const Lengths length = part_tiles(g, cost);
         uint32_t parts_before = 0u, slots_before = 0u;
         for (uint32_t base = 0u; base < g.q.count; base += 1024u) {
             const uint32_t s = base + threadIdx.x;
             uint32_t mine = 0u, held = 0u;
             if (s < g.q.count) {
-                const Need n = need_of(g, kq::paged_seq(g.q, g.c, s, bad), small);
+                const Need n = need_of(g, kq::paged_seq(g.q, g.c, s, bad), most);
                 const uint32_t each = parts_of(n.tiles, length_of(length, n));
                 mine = n.blocks * g.c.heads * each;
                 held = each > 1u ? mine : 0u;
@@ -422,15 +449,13 @@ __global__ __launch_bounds__(1024) void plan_many(Args g, uint32_t *status) {
             slots_before += ha;
             __syncthreads();
         }
-        if (small && parts_before > g.parts) {
-            small = false;
-            continue;
-        }
+        if (!plan_holds(g, most, last, parts_before, seen, cost)) continue;
         if (threadIdx.x == 0u) {
             g.plan[0] = length.few;
             g.plan[1] = parts_before;
             g.plan[2] = length.many;
             g.plan[3] = slots_before;
+            g.plan[4] = most;
         }
         return;
     }
@@ -906,10 +931,10 @@ __device__ __forceinline__ void few_rows(const Args &g, const Part &p, char *lds
  * while the other forms exponentials (2049 rows of bf16 heads: 282 us, with 32
  * and one wave 429). Heads of 64 leave room for three (19 ragged sequences 47,
  * with two 54). */
-template <int D>
+template <int D, bool MID = false>
 struct Many {
-    static constexpr int M = D == 256 ? 16 : 32;
-    static constexpr int W = kMany / M, THREADS = 64 * W;
+    static constexpr int M = MID || D == 256 ? 16 : 32;
+    static constexpr int W = (MID ? kMid : kMany) / M, THREADS = 64 * W;
     static constexpr int KEYS = 64 / W;         /* that a wave brings in */
     static constexpr int REGS = M * M / 64;     /* values of a block that a lane holds */
     static constexpr int STEPS = D * M / 512;   /* products along a head */
@@ -939,10 +964,10 @@ struct Buffer {
     static constexpr uint32_t value = I;
 };
 
-template <bool BF, int D>
+template <bool BF, int D, bool MID>
 __device__ __forceinline__ void many_rows(const Args &g, const Part &p, char *lds, bool &badin,
                                           bool &bad, bool &badseq) {
-    typedef Many<D> T;
+    typedef Many<D, MID> T;
     typedef typename T::acc acc;
     constexpr int M = T::M, REGS = T::REGS, STEPS = T::STEPS, BLOCKS = T::BLOCKS;
     constexpr int TERMS = Type<BF>::TERMS, SETS = kTile / M, LANES = M == 32 ? 32 : 48;
@@ -1146,6 +1171,10 @@ __global__ __launch_bounds__((256 * few_side<BF, D>()), (few_side<BF, D>())) voi
     if (bad) kq_flag(status, KQ_DEV_NUMERIC);
 }
 
+__device__ __forceinline__ uint32_t in_turn(uint32_t u) {
+    return u < 256u && gridDim.x >= 256u ? (u & 7u) | (248u - (u & ~7u)) : u;
+}
+
 template <bool BF, int D, bool MANY>
 __global__ __launch_bounds__(Many<D>::THREADS, D == 64 ? 3 : 2) void attend(Args g, uint32_t *status) {
     constexpr int W = Many<D>::W;
@@ -1153,14 +1182,16 @@ __global__ __launch_bounds__(Many<D>::THREADS, D == 64 ? 3 : 2) void attend(Args
     /* a row's pieces are found by flipping address bits below its size */
     __shared__ __attribute__((aligned(1024))) char lds[BYTES];
     bool badin = false, bad = false, badseq = false;
-    Part p = find_part<MANY>(g, blockIdx.x, status);
+    Part p = find_part<MANY>(g, in_turn(blockIdx.x), status);
     leave(g, p);
     if (!p.live) return;
     p.pin();
     if (p.block == kFew)
         few_rows<BF, D, W>(g, p, lds, badin, bad, badseq);
+    else if (D != 256 && p.block == kMid)
+        many_rows<BF, D, D != 256>(g, p, lds, badin, bad, badseq);
     else
-        many_rows<BF, D>(g, p, lds, badin, bad, badseq);
+        many_rows<BF, D, false>(g, p, lds, badin, bad, badseq);
     if (badseq) kq_flag(status, KQ_DEV_SEQUENCE);
     if (badin) kq_flag(status, KQ_DEV_INPUT);
     if (bad) kq_flag(status, KQ_DEV_NUMERIC);
@@ -1196,8 +1227,8 @@ __global__ __launch_bounds__(kThreads) void join_parts(Args g, uint32_t *status)
     if (blockIdx.x >= g.plan[3] || p.rows == 0u) return;
     bool badin = false, bad = false;
     /* pieces of four values, in the slots' order: by rows, or by waves and lanes */
-    const uint32_t width = g.c.width, tall = width == 256u ? Many<256>::M : Many<128>::M;
-    const bool by_rows = p.head_few >> 16 != 0u;
+    const uint32_t width = g.c.width, tall = p.head_kind >> 16 == 2u ? Many<256>::M : Many<128>::M;
+    const bool by_rows = p.head_kind >> 16 == 1u;
     const uint32_t pieces =
         (by_rows ? p.rows : (p.rows + tall - 1u) / tall * tall) * (width / 4u);
     const uint32_t share = p.part * gridDim.y + blockIdx.y, shares = p.parts * gridDim.y;
@@ -1251,7 +1282,7 @@ __global__ __launch_bounds__(kThreads) void join_parts(Args g, uint32_t *status)
         for (uint32_t u = 0; u < kAtOnce; ++u)
             if (group == 0u && have[u]) {
                 const uint32_t r = p.row0 + row[u];
-                const uint32_t h = (p.head_few & 0xffffu) * g.group + r % g.group;
+                const uint32_t h = (p.head_kind & 0xffffu) * g.group + r % g.group;
                 put(g, p.begin + r / g.group, h, d[u], v[u].v,
                     inverse_of_row(g, h, v[u].top, v[u].total, bad), badin, bad);
             }
@@ -1297,7 +1328,7 @@ Sizes sizes_of(const kq_launch_pattn &a, const kq_launch_paged &c, const kq_laun
     const uint64_t most = finest * (z.whole ? 1u : (tiles + kLeast / 2u) / kLeast + 1u);
     z.parts = most < kParts + z.items ? most : kParts + z.items;
     z.slots = z.whole ? 0u : most < kSlots ? most : kSlots;
-    z.plan_bytes = ((4u + (q.count > kByLane ? 2u * (q.count + 1u) : 0u)) * 4u + 255u) / 256u * 256u;
+    z.plan_bytes = ((kPlan + (q.count > kByLane ? 2u * (q.count + 1u) : 0u)) * 4u + 255u) / 256u * 256u;
     z.item_bytes = (z.slots * sizeof(Item) + 255u) / 256u * 256u;
     z.bytes = z.plan_bytes + z.item_bytes + z.slots * z.slot_rows * (c.width + 2u) * 4u;
     return z;
