@@ -60,6 +60,7 @@ constexpr uint32_t kParts = 1024;
 constexpr uint32_t kShort = 8;       /* tiles */
 constexpr uint32_t kLeast = 2;       /* tiles */
 constexpr uint32_t kSmall = 512;     /* tiles in all of items of many rows */
+constexpr uint32_t kSmallWide = 48;
 constexpr uint32_t kMiddle = 2560;
 constexpr uint32_t kFill = 448;
 constexpr uint32_t kEven = 700;
@@ -155,7 +156,8 @@ __device__ __forceinline__ uint64_t seen_by_many(const Args &g, const kq::PagedS
  * have no room beside each other, are faster as they are (116 rows of 32 heads: 23
  * us, 32). */
 __device__ __forceinline__ uint32_t rows_of_items(const Args &g, uint64_t seen) {
-    return g.c.width == 256u || seen >= kMiddle ? kMany : seen < kSmall ? kFew : kMid;
+    if (g.c.width == 256u) return seen < kSmallWide ? kFew : kMany;
+    return seen >= kMiddle ? kMany : seen < kSmall ? kFew : kMid;
 }
 /* Whether a plan of items of `most` rows with so many parts holds; otherwise `most`
  * becomes what is planned next. */

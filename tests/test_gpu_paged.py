@@ -636,6 +636,31 @@ def test_short_lines_of_many_rows(ctx, type_, width, tiles, over):  # noqa: F811
     a.check(a.got(ctx))
 
 
+@pytest.mark.parametrize("type_", TYPES)
+@pytest.mark.parametrize("width", [64, 128, 256])
+@pytest.mark.parametrize("mode", [{}, dict(window=300), dict(causal=False, gate=True)], ids=str)
+def test_middle_calls(ctx, type_, width, mode):  # noqa: F811
+    """Calls that do not fill the device: items of 64 rows (heads of 256: of 128)."""
+    say("middle", type_, width, mode)
+    for seed, heads, group, past, rows in ((23, 4, 4, [2000], [301]), (24, 4, 3, [0], [917]),
+                                           (25, 2, 5, [0, 900, 70, 3], [333, 1, 250, 407])):
+        a = Attention(seed, type_, heads, group, width, 64, past, rows, line=64, **mode)
+        a.check(a.got(ctx))
+
+
+def test_middle_calls_of_many_sequences(ctx):  # noqa: F811
+    say("middle, many sequences")
+    a = Attention(26, "f16", 4, 4, 64, 32, [400 - 5 * i for i in range(70)], [30] * 70)
+    a.check(a.got(ctx))
+
+
+@pytest.mark.parametrize("type_,width", [("f16", 128), ("bf16", 64)])
+def test_uneven_calls(ctx, type_, width):  # noqa: F811
+    say("uneven", type_, width)
+    a = Attention(27, type_, 4, 8, width, 128, [0], [1500])
+    a.check(a.got(ctx))
+
+
 def test_bad_slot_in_a_short_line(ctx):  # noqa: F811
     say("bad slot, short lines")
     a = Attention(18, "f16", 2, 4, 128, 32, [5, 90], [1, 1], line=4)
