@@ -26,8 +26,8 @@
  * 130,002 tokens, 133 MB: 27 us (4 of them until the first keys are there: length,
  * page and key hang on each other) and 6.
  * Many rows (128 for a key head) are bound by the matrix cores, whose clock falls
- * to 1.9 GHz under it: 8192 rows over themselves with 16 heads of 128 take 482 -
- * 499 us, 1100 - 1140 TFLOP/s of products, which a library product of 8192^3 fp16
+ * to 1.9 GHz under it: 8192 rows over themselves with 16 heads of 128 take 464 -
+ * 479 us, 1145 - 1185 TFLOP/s of products, which a library product of 8192^3 fp16
  * reaches (1159); 3 terms and heads of 256, 2049 rows: 215 us, 950 TFLOP/s.
  */
 #include <math.h>
@@ -48,21 +48,21 @@ constexpr int kThreads = 256;
 constexpr uint32_t kTile = 64;       /* keys of a tile */
 constexpr uint32_t kFew = 16;        /* rows of an item whose waves share out its keys */
 constexpr uint32_t kMany = 128;      /* rows of an item whose waves share out its rows */
-constexpr uint32_t kMid = 64;        /* the same, where the device is not full */
+constexpr uint32_t kMid = 64;        /* the same, where 128 would not fill the device */
 /* Parts that a call's items are cut into. Of few rows 1024, three to four rounds
  * of the device's waves that follow each other: 61 sequences 102 us, with 512
  * parts 116, with 2048 111. But parts of fewer than 8 tiles are not worth a
  * second round: one sequence of 130,002 tokens takes 34 us in parts of 8 tiles
  * (512), 38 in parts of 4. Of many rows 512, whose partial results are 64 KB or
- * more each: 509 rows over 65,509 keys 464 us, 2049 rows of 256-wide heads 215;
+ * more each (32 KB of 64 rows): 509 rows over 65,509 keys 464 us, 2049 rows of 256-wide heads 215;
  * with 1024 parts 475 and 231, with 256 505 and 224. */
 constexpr uint32_t kParts = 1024;
 constexpr uint32_t kShort = 8;       /* tiles */
 constexpr uint32_t kLeast = 2;       /* tiles */
-constexpr uint32_t kSmall = 512;     /* tiles in all of items of many rows */
+constexpr uint32_t kSmall = 512;     /* tiles in all of items of many rows (rows_of_items) */
 constexpr uint32_t kSmallWide = 48;
 constexpr uint32_t kMiddle = 2560;
-constexpr uint32_t kFill = 448;
+constexpr uint32_t kFill = 448;      /* parts (plan_holds) */
 constexpr uint32_t kEven = 700;
 /* Items of few rows are a workgroup's each, of as many waves as a CU holds, where
  * there are CUs for all of them and the table's lines are short: 6 tiles of 128,
@@ -147,20 +147,31 @@ __device__ __forceinline__ uint64_t seen_by_many(const Args &g, const kq::PagedS
     return (uint64_t)n.blocks * g.c.heads * (g.a.causal && mean < n.tiles ? mean : n.tiles);
 }
 
-/* Whether a call's items of many rows, that see so many tiles in all, are better
- * cut into items of few: a workgroup of many rows begins with 5 us of queries and
- * first tiles and takes 2 us a tile when the device is not full, and its parts are
- * joined. 97 rows of 24 heads over themselves (48 tiles) 8.1 us, 19.4 as items of
- * many rows; 92 rows over 1321 keys (105) 17.9, 20.8; 794 rows of 10 sequences (736)
- * 42, 36: items of few read their keys eight times. Heads of 256, whose workgroups
- * have no room beside each other, are faster as they are (116 rows of 32 heads: 23
- * us, 32). */
+/* Rows of the items of a call whose items of 128 rows would see so many tiles in all.
+ * A workgroup of 128 rows begins with 3 us of queries (64 KB, at what a CU alone reads)
+ * and takes 2 us a tile where it has its CU to itself. So small calls have items of
+ * 16 rows, which read their keys eight times: 97 rows of 24 heads over themselves (48
+ * tiles) 8.1 us, 19.4 in items of 128; 500 of 16 heads (256) 17.4, 22.8; but 300 over
+ * 1300 keys (684) 37, 27. Those in the middle have items of 64, which begin sooner and
+ * are joined from fewer parts: 300 rows over 1300 keys 24.5, 27; 1200 rows of 8
+ * sequences (1364) 30, 39; 500 over 2500 (2304) 37, 39; but they read LDS twice as
+ * often for a product: 2003 ragged rows of heads of 64 (3300) 53, 49. Heads of 256,
+ * whose workgroups have no room beside each other, have no such form, and items of 16
+ * rows up to 48 tiles (116 rows of 32 heads, 32 tiles, 13.2, 18.7; 250 of 16, 64 tiles,
+ * 29.7, 27). */
 __device__ __forceinline__ uint32_t rows_of_items(const Args &g, uint64_t seen) {
     if (g.c.width == 256u) return seen < kSmallWide ? kFew : kMany;
     return seen >= kMiddle ? kMany : seen < kSmall ? kFew : kMid;
 }
+
 /* Whether a plan of items of `most` rows with so many parts holds; otherwise `most`
- * becomes what is planned next. */
+ * becomes what is planned next. Items of 64 rows also take the place of items of 128
+ * that are planned fewer parts than the 512 workgroups that have room at once (3000
+ * rows over themselves, 376 parts: 83 us, 105), or fewer than 700 that are uneven, as
+ * the rows see three quarters or less of the most (2500 rows, 628 parts: 66, 87; 4096,
+ * 512: 148, 155, bf16 186, 208; 2048, 512: 54, 63). With even parts items of 128 are
+ * faster: 300 rows over 10,300 keys 67, 88; 509 over 65,509 474, 509. A plan of smaller
+ * items that has more parts than the call has workgroups falls back to larger ones. */
 __device__ __forceinline__ bool plan_holds(const Args &g, uint32_t &most, bool &last,
                                            uint32_t parts, uint64_t seen, uint64_t cost) {
     if (most == kMany) {
@@ -932,7 +943,7 @@ __device__ __forceinline__ void few_rows(const Args &g, const Part &p, char *lds
  * head of 256 in the registers of two waves a SIMD, one of which multiplies
  * while the other forms exponentials (2049 rows of bf16 heads: 282 us, with 32
  * and one wave 429). Heads of 64 leave room for three (19 ragged sequences 47,
- * with two 54). */
+ * with two 54). MID: up to 64 rows, four waves of 16. */
 template <int D, bool MID = false>
 struct Many {
     static constexpr int M = MID || D == 256 ? 16 : 32;
@@ -1173,6 +1184,11 @@ __global__ __launch_bounds__((256 * few_side<BF, D>()), (few_side<BF, D>())) voi
     if (bad) kq_flag(status, KQ_DEV_NUMERIC);
 }
 
+/* The first 256 workgroups, which begin on a CU each, in reverse: items come longest
+ * first, so that the longest of the next 256 lie beside the shortest of these. 8192 rows
+ * over themselves 478 us, 496 without; 4096 rows of bf16 174, 184; only 1500 rows of 8
+ * key heads over 500 more keys are slower, 62, 59. By eights, which leaves a head's
+ * workgroups on their XCD. */
 __device__ __forceinline__ uint32_t in_turn(uint32_t u) {
     return u < 256u && gridDim.x >= 256u ? (u & 7u) | (248u - (u & ~7u)) : u;
 }
