@@ -108,8 +108,12 @@ struct Lengths {
     uint32_t few, many;
 };
 
-__device__ __forceinline__ uint32_t block_of(uint32_t rows, uint32_t most) {
-    return rows <= kFew ? kFew : most;
+/* Rows of a sequence's items. 17 to 32 rows are one wave of an item of 128, two of one
+ * of 64: 4 rows of each of 61 sequences, 32 for a key head, 112 us, 125; of 64 rows, two
+ * waves or four, 135 and 132. */
+__device__ __forceinline__ uint32_t block_of(const Args &g, uint32_t rows, uint32_t most) {
+    if (rows <= kFew) return kFew;
+    return most == kMany && rows <= kMid / 2u && g.c.width != 256u ? kMid : most;
 }
 
 /* What a sequence asks for: its items (blocks of rows, for each key head) and
@@ -119,7 +123,7 @@ struct Need {
 };
 
 __device__ __forceinline__ Need need_of(const Args &g, const kq::PagedSeq &s, uint32_t most) {
-    const uint32_t rows = s.rows * g.group, block = block_of(rows, most);
+    const uint32_t rows = s.rows * g.group, block = block_of(g, rows, most);
     Need n = {0u, 0u, block};
     if (!s.live || s.rows == 0u) return n;
     n.blocks = (rows + block - 1u) / block;
@@ -142,7 +146,7 @@ __device__ __forceinline__ uint64_t cost_of(const Args &g, const Need &n) {
 /* the tiles of its items of many rows, as many as their rows see on the average */
 __device__ __forceinline__ uint64_t seen_by_many(const Args &g, const kq::PagedSeq &s,
                                                  const Need &n) {
-    if (n.block != kMany) return 0u;
+    if (n.block == kFew) return 0u;
     const uint32_t mean = (s.past + s.rows / 2u + kTile - 1u) / kTile;
     return (uint64_t)n.blocks * g.c.heads * (g.a.causal && mean < n.tiles ? mean : n.tiles);
 }

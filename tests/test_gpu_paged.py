@@ -648,6 +648,17 @@ def test_middle_calls(ctx, type_, width, mode):  # noqa: F811
         a.check(a.got(ctx))
 
 
+@pytest.mark.parametrize("type_", TYPES)
+@pytest.mark.parametrize("width", [64, 128, 256])
+def test_rows_of_two_waves(ctx, type_, width):  # noqa: F811
+    """17 to 32 rows for a key head, beside sequences of one and of many rows."""
+    say("two waves", type_, width)
+    for seed, rows, past in ((28, [4, 3, 1, 4], [9000, 70, 5000, 8200]), (29, [4], [30000]),
+                             (30, [3, 500, 4, 1], [4000, 3000, 64, 63])):
+        a = Attention(seed, type_, 2, 8, width, 64, past, rows, line=512)
+        a.check(a.got(ctx))
+
+
 def test_middle_calls_of_many_sequences(ctx):  # noqa: F811
     say("middle, many sequences")
     a = Attention(26, "f16", 4, 4, 64, 32, [400 - 5 * i for i in range(70)], [30] * 70)
