@@ -1351,8 +1351,13 @@ Sizes sizes_of(const kq_launch_pattn &a, const kq_launch_paged &c, const kq_laun
     z.parts = most < kParts + z.items ? most : kParts + z.items;
     z.slots = z.whole ? 0u : most < kSlots ? most : kSlots;
     z.plan_bytes = ((kPlan + (q.count > kByLane ? 2u * (q.count + 1u) : 0u)) * 4u + 255u) / 256u * 256u;
-    z.item_bytes = (z.slots * sizeof(Item) + 255u) / 256u * 256u;
-    z.bytes = z.plan_bytes + z.item_bytes + z.slots * z.slot_rows * (c.width + 2u) * 4u;
+    /* a call that joins nothing asks for what one of single rows would: scratch of the
+     * largest call is enough for all */
+    const uint64_t few = c.heads * q.count * ((tiles + kLeast / 2u) / kLeast + 1u);
+    const uint64_t held = !z.whole ? z.slots : sees < kLeast * 3u / 2u ? 0u : few < kSlots ? few : kSlots;
+    z.item_bytes = (held * sizeof(Item) + 255u) / 256u * 256u;
+    z.bytes = z.plan_bytes + z.item_bytes +
+              held * (z.whole ? kFew : z.slot_rows) * (c.width + 2u) * 4u;
     return z;
 }
 

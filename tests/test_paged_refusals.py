@@ -188,6 +188,23 @@ def test_scratch_bytes():
     assert f(A(256, 1.0), big, seqs(262144, 65535, 65535)) < 400 << 20
 
 
+@pytest.mark.parametrize("window", [0, 40, 500])
+@pytest.mark.parametrize("group", [1, 8, 16, 17])
+def test_scratch_of_the_largest_call_is_enough(group, window):
+    f = kq_hip.paged_attention_scratch_bytes
+    for heads in (1, 8):
+        a = kq_hip.paged_attention(heads * group, 1.0, True, window)
+        for width in (64, 128, 256):
+            for line in (1, 8, 12, 20, 28, 40, 400):
+                c = kq_hip.paged_cache(kq_hip.TYPE_F16, heads, width, 16, 9, line, 0, 0, 0, 0)
+                largest = 0
+                for n in (1, 2, 16, 33, 64, 65, 300):
+                    one = f(a, c, kq_hip.sequences(n, n, n))
+                    few, many = (f(a, c, kq_hip.sequences(t, n, n, 64)) for t in (n, 50 * n))
+                    assert 0 < one <= many and few <= many and largest <= many
+                    largest = many
+
+
 def test_frequencies():
     """Against the formulas; powers and products of binary64 in another order are
     a few 2^-53 apart, each times its exponent's size (log of 1e7 is 16)."""
