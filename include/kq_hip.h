@@ -943,8 +943,10 @@ typedef struct kq_hip_paged_attention {
 } kq_hip_paged_attention;
 
 /* Device scratch of a call with these sizes (only counts are looked at, and
- * whether offsets is NULL); 0 for arguments that the call refuses. Calls that
- * may run at the same time need scratch of their own. */
+ * whether offsets is NULL); 0 for arguments that the call refuses. What a call
+ * with offsets asks for is enough for all with as many sequences and tokens or
+ * fewer, offsets NULL among them. Calls that may run at the same time need
+ * scratch of their own. */
 uint64_t kq_hip_paged_attention_scratch_bytes(const kq_hip_paged_attention *attention,
                                               const kq_hip_paged_cache *cache,
                                               const kq_hip_sequences *sequences);
