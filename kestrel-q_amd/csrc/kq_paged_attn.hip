@@ -6,7 +6,7 @@
  * weights, both binary32:
  *   s_t = scale log2(e) q . k_t,  w_t = 2^(s_t - M),  l = sum w_t,
  *   y = (sum w_t v_t) / (l + 2^(sink log2(e) - M))
- * M follows a row's largest s only when that has passed it by 2^kSlack, so that
+ * M follows a row's largest s only when that has passed it by SLACK, so that
  * the sums are rarely scaled; what they are held by cancels in the end. Partial
  * sums (of waves, of parts of a long context) are added by their M.
  *
@@ -14,8 +14,9 @@
  * The queries and the weights, which are binary32, are two fp16 (three bf16)
  * numbers each, whose products add up in one accumulator: twice (three times) the
  * matrix work buys results off by 2-9 x 10^-7 of their 2-norm, as those of
- * binary32 products are, where one fp16 term would leave 2 x 10^-4. S' = K Q' and
- * O' = V' P': a lane has one row's scores, whose weights are the next product's
+ * binary32 products are, where one fp16 term would leave 2 x 10^-4. Weights too small
+ * for fp16's exponents are multiplied at a scale of their own (kRest). S' = K Q'
+ * and O' = V' P': a lane has one row's scores, whose weights are the next product's
  * operand as they stand (its keys in the order that the first product left them),
  * and V comes transposed out of LDS (ds_read_b64_tr_b16).
  *
@@ -81,7 +82,6 @@ constexpr uint32_t kWholeMany = 896;
 constexpr uint32_t kPlan = 5;        /* words of the plan before the sequences' */
 constexpr uint32_t kSlots = (4u * kParts + 2u) / 3u;
 constexpr uint32_t kByLane = 64;     /* sequences that each wave plans by itself */
-constexpr float kSlack = 8.0f;       /* by which a row's largest exponent may pass its stand-in */
 constexpr float kLowest = -0x1.fffffep127f;
 
 struct Args {
@@ -488,16 +488,17 @@ struct Type {
     typedef _Float16 e;
     static constexpr int TERMS = 2;
     /* fp16's own range is short: a row's largest query is brought to 2^12 .. 2^14, and
-     * weights are held times 2^7, at most 2^15 with the slack */
+     * the largest of its weights so far to 2^13, 2^15 with what its exponent may pass its
+     * stand-in by, the slack */
     static constexpr int TOP = 12;
-    static constexpr float LIFT = 7.0f;
+    static constexpr float LIFT = 13.0f, SLACK = 2.0f;
 };
 template <>
 struct Type<true> {
     typedef __bf16 e;
     static constexpr int TERMS = 3;
     static constexpr int TOP = 0;
-    static constexpr float LIFT = 0.0f;
+    static constexpr float LIFT = 0.0f, SLACK = 8.0f;
 };
 
 template <bool BF>
@@ -551,6 +552,57 @@ __device__ __forceinline__ void split(const float (&x)[8], e8<BF> (&t)[Type<BF>:
     for (int k = 0; k < Type<BF>::TERMS; ++k) t[k] = __builtin_bit_cast(e8<BF>, p[k]);
 }
 
+/* fp16 ends at 2^-24, so that two terms hold 22 bits of a weight of 2^-2 or more: 2^-15
+ * of a row's largest, 10 nats. Behind a key that leads by more, smaller ones can be the
+ * whole sum (its own value may be next to nothing). Where a wave has any, what their two
+ * terms leave, at most 2^-25, is multiplied as well, times 2^40 and with the sums times
+ * 2^40 for as long: powers of two, which change no bit, and the sums of 2^24 keys, below
+ * 2^55, have room. That holds 22 bits down to 2^-55 of the largest, 38 nats. bf16 has
+ * binary32's exponents and needs none of it. 61 sequences decoding take 107 us where
+ * all waves have such weights, 104 where none has. */
+constexpr float kHeld = 0x1p-2f, kHeldLog2 = -2.0f;
+constexpr float kRest = 0x1p40f;
+/* Of many rows it is left out where it could not be told from the sums' own roundings:
+ * of a tile's 64 keys it is at most 2^-25 8 times the 2-norm of all their values, by
+ * Cauchy and Schwarz, and where the square of a row's sums is 2^4 times that of the values,
+ * below 2^-24 of the sums, to which the tile is added in eight or more roundings. So
+ * scores that are merely wide cost a look at the values: 8192 rows with scores 4 nats
+ * wide 582 us, with all rests 865, without small weights 478. Squares below fp16's normal
+ * numbers may be taken for 0: kNoSquare stands for more of them than a lane has. */
+constexpr float kRestMatters = 0x1p4f;
+constexpr float kNoSquare = 0x1p-20f;
+
+__device__ __forceinline__ void rest_of(float (&w)[8]) {
+    e8<false> t[2];
+    split<false>(w, t);
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        w[i] = w[i] < kHeld ? (w[i] - (float)t[0][i] - (float)t[1][i]) * kRest : 0.0f;
+}
+
+/* sums and the squares of fp16 values */
+__device__ __forceinline__ f4 squares(f4 sums, u4 v) {
+    typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const h2 x = __builtin_bit_cast(h2, (uint32_t)v[i]);
+        sums[i] = __builtin_amdgcn_fdot2(x, x, sums[i], false);
+    }
+    return sums;
+}
+
+/* x as a value that is not known: what comes of it is formed again, not held */
+template <typename T>
+__device__ __forceinline__ T again(T x) {
+    asm volatile("" : "+v"(x));
+    return x;
+}
+/* the lane's number, likewise */
+__device__ __forceinline__ uint32_t lane_again() {
+    const uint32_t all = again(~0u);
+    return __builtin_amdgcn_mbcnt_hi(all, __builtin_amdgcn_mbcnt_lo(all, 0u));
+}
+
 /* A row's queries, as operands: the exponent's factor put in to 48 bits, and
  * the row's largest value brought to 2^TOP .. 2^(TOP + 2) by a power of two. */
 template <bool BF, int STEPS>
@@ -589,7 +641,7 @@ __device__ __forceinline__ void split_query(const Args &g, const Raw<STEPS> &r, 
                 const uint32_t b = __float_as_uint((&r.v[s][i].x)[c]) & 0x7fffffffu;
                 most = b > most ? b : most;
             }
-    badin |= most >= 0x7f800000u;
+    badin |= __any(most >= 0x7f800000u);
     const float top = kq::lanes_max<LANES>(__uint_as_float(most < 0x7f800000u ? most : 0u));
     /* the largest value's exponent, 0 for a row of zeros */
     int e = (int)(__float_as_uint(top) >> 23) - 127;
@@ -821,8 +873,8 @@ __device__ __forceinline__ void few_rows(const Args &g, const Part &p, char *lds
                 for (int m = 0; m < TERMS; ++m) s[b] = mma(k[b][t], q.x[t][m], s[b]);
         }
     };
-    auto weights = [&](uint32_t at, const f4 (&s)[2], e8<BF> (&pw)[TERMS]) {
-        float w[8];
+    /* whether any is too small for its terms */
+    auto weights = [&](uint32_t at, const f4 (&s)[2], float (&w)[8]) {
         float peak = kLowest;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
@@ -831,7 +883,7 @@ __device__ __forceinline__ void few_rows(const Args &g, const Part &p, char *lds
             peak = fmaxf(peak, w[i]);
         }
         peak = kq::lanes_max<48>(peak) - Type<BF>::LIFT;
-        if (__any(peak > top + kSlack)) {
+        if (__any(peak > top + Type<BF>::SLACK)) {
             const float next = fmaxf(top, peak);
             const float f = __builtin_amdgcn_exp2f(top - next);
             top = next;
@@ -840,18 +892,20 @@ __device__ __forceinline__ void few_rows(const Args &g, const Part &p, char *lds
             for (int b = 0; b < BLOCKS; ++b) o[b] *= f;
         }
         float sum = 0.0f;
+        bool small = false;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             w[i] = __builtin_amdgcn_exp2f(w[i] - top);
             sum += w[i];
+            small |= !BF && w[i] > 0.0f && w[i] < kHeld;
         }
         total += sum;
-        split<BF>(w, pw);
+        return !BF && __any(small);
     };
-    auto gather = [&](const e8<BF> (&pw)[TERMS]) {
+    auto gather = [&](const e8<BF> (&pw)[TERMS], uint32_t lane) {
+        const uint32_t n = lane & 15u, r = lane / 4u; /* 4 a quarter, and n / 4 */
 #pragma unroll
         for (uint32_t b = 0; b < BLOCKS; ++b) {
-            const uint32_t r = 4u * quarter + n / 4u;
             const uint32_t a = mine_at + r * (2u * D) +
                                few_piece<D>(r, 2u * b + (n % 4u) / 2u) * 16u + (n & 1u) * 8u;
             const e8<BF> v = join8<BF>(transposed(a), transposed(a + 32u * D));
@@ -880,6 +934,7 @@ __device__ __forceinline__ void few_rows(const Args &g, const Part &p, char *lds
     while (key < end) {
         const uint32_t next = key + 32u * W;
         f4 s[2];
+        float w[8];
         e8<BF> pw[TERMS];
         scores(s);
         if (next < end) {
@@ -887,13 +942,31 @@ __device__ __forceinline__ void few_rows(const Args &g, const Part &p, char *lds
             load_k(next);
             if (next + 32u * W < end) pages(next + 32u * W);
         }
-        weights(key, s, pw);
+        const bool small = weights(key, s, w);
         /* V is there: loads return in order, and only the next K's come behind it */
-        if (next < end)
-            wait_vm<2 * STEPS>();
-        else
-            wait_vm<0>();
-        gather(pw);
+        auto wait = [&]() {
+            if (next < end)
+                wait_vm<2 * STEPS>();
+            else
+                wait_vm<0>();
+        };
+        if constexpr (!BF)
+            if (small) {
+                float x[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) x[i] = again(w[i]);
+                rest_of(x);
+                split<BF>(x, pw);
+                wait();
+#pragma unroll
+                for (int b = 0; b < BLOCKS; ++b) o[b] *= kRest;
+                gather(pw, lane_again());
+#pragma unroll
+                for (int b = 0; b < BLOCKS; ++b) o[b] *= 1.0f / kRest;
+            }
+        split<BF>(w, pw);
+        wait();
+        gather(pw, lane);
         if (next < end) {
             wait_lgkm0(); /* V is read */
             load_v(next);
@@ -906,16 +979,18 @@ __device__ __forceinline__ void few_rows(const Args &g, const Part &p, char *lds
     float *tops = (float *)lds, *totals = tops + W * 16, *sums = totals + W * 16;
     constexpr uint32_t kRow = D + 4u; /* rows 16 bytes apart in the banks */
     __syncthreads();
-    if (quarter == 0u) {
-        tops[wave * 16u + n] = top;
-        totals[wave * 16u + n] = total;
+    const uint32_t l = lane_again(), at = wave * 16u + l % 16u;
+    if (l < 16u) {
+        tops[at] = top;
+        totals[at] = total;
     }
 #pragma unroll
     for (uint32_t b = 0; b < BLOCKS; ++b)
-        *(f4 *)(sums + (wave * 16u + n) * kRow + 16u * b + 4u * quarter) = o[b];
+        *(f4 *)(sums + at * kRow + 16u * b + 4u * (l / 16u)) = o[b];
     __syncthreads();
     float *slot = p.parts > 1u ? slot_at(g, p.slot + p.part * p.step) : nullptr;
-    for (uint32_t i = threadIdx.x; i < p.rows * (D / 4u); i += 64u * W) {
+    const uint32_t group = again(g.group); /* its reciprocal is not held either */
+    for (uint32_t i = 64u * wave + l; i < p.rows * (D / 4u); i += 64u * W) {
         const uint32_t r = i / (D / 4u), d = i % (D / 4u) * 4u;
         float t = tops[r];
 #pragma unroll
@@ -933,8 +1008,8 @@ __device__ __forceinline__ void few_rows(const Args &g, const Part &p, char *lds
         if (slot != nullptr)
             keep(g, slot, r, d, D, v, t, l);
         else {
-            const uint32_t row = p.row0 + r, h = p.head * g.group + row % g.group;
-            put(g, p.seq.begin + row / g.group, h, d, v, inverse_of_row(g, h, t, l, bad), badin, bad);
+            const uint32_t row = p.row0 + r, h = p.head * g.group + row % group;
+            put(g, p.seq.begin + row / group, h, d, v, inverse_of_row(g, h, t, l, bad), badin, bad);
         }
     }
 }
@@ -1071,20 +1146,26 @@ __device__ __forceinline__ void many_rows(const Args &g, const Part &p, char *ld
 #pragma unroll
                 for (uint32_t b = 0; b < SETS; ++b) s[b] = mma(k[b], q.x[st][m], s[b]);
         }
+        float lowest = INFINITY; /* of the keys that the row sees */
         if (at + kTile > all1 || at < all0) {
 #pragma unroll
             for (uint32_t b = 0; b < SETS; ++b)
 #pragma unroll
                 for (uint32_t i = 0; i < REGS; ++i) {
                     const uint32_t key = at + M * b + 256u / M * (i / 4u) + 4u * part + i % 4u;
-                    s[b][i] = key < last && key >= from ? s[b][i] : -INFINITY;
+                    const bool seen = key < last && key >= from;
+                    if (!BF) lowest = fminf(lowest, seen ? s[b][i] : INFINITY);
+                    s[b][i] = seen ? s[b][i] : -INFINITY;
                 }
+        } else if (!BF) {
+#pragma unroll
+            for (int i = 0; i < SETS * REGS; ++i) lowest = fminf(lowest, s[i / REGS][i % REGS]);
         }
         float peak = s[0][0];
 #pragma unroll
         for (int i = 1; i < SETS * REGS; ++i) peak = fmaxf(peak, s[i / REGS][i % REGS]);
         peak = fmaxf(kq::lanes_max<LANES>(peak) * q.unscale, kLowest) - Type<BF>::LIFT;
-        if (__any(peak > top + kSlack)) {
+        if (__any(peak > top + Type<BF>::SLACK)) {
             const float next = fmaxf(top, peak);
             const float f = __builtin_amdgcn_exp2f(top - next);
             top = next;
@@ -1092,18 +1173,16 @@ __device__ __forceinline__ void many_rows(const Args &g, const Part &p, char *ld
 #pragma unroll
             for (int b = 0; b < BLOCKS; ++b) o[b] *= f;
         }
-        float sum = 0.0f;
         constexpr uint32_t CHUNK = 512u / M; /* keys of a product */
-#pragma unroll
-        for (uint32_t c = 0; c < kTile / CHUNK; ++c) {
-            float w[8];
+        /* M 32: half of a block; M 16: four values of each of two */
+        auto weights = [&](uint32_t c, float (&w)[8], float top) {
 #pragma unroll
             for (uint32_t i = 0; i < 8u; ++i) {
-                /* M 32: half of a block; M 16: four values of each of two */
                 const uint32_t x = 8u * c + i;
                 w[i] = __builtin_amdgcn_exp2f(fmaf(s[x / REGS][x % REGS], q.unscale, -top));
-                sum += w[i];
             }
+        };
+        auto gather = [&](uint32_t c, const float (&w)[8], uint32_t v_at) {
             e8<BF> pw[TERMS];
             split<BF>(w, pw);
 #pragma unroll
@@ -1113,6 +1192,47 @@ __device__ __forceinline__ void many_rows(const Args &g, const Part &p, char *ld
 #pragma unroll
                 for (int m = 0; m < TERMS; ++m) o[b] = mma(v, pw[m], o[b]);
             }
+        };
+        if constexpr (!BF) {
+            const bool small = fmaf(lowest, q.unscale, -top) < kHeldLog2;
+            bool rest = __any(small);
+            if (rest) {
+                f4 vv = f4{kNoSquare, 0.0f, 0.0f, 0.0f}, oo = f4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+                for (uint32_t i = 0; i < D / 8u; ++i)
+                    vv = squares(vv, *(__attribute__((address_space(3))) u4 *)(uintptr_t)(
+                                         again(base) + kTile * T::ROW + BUF + 1024u * i +
+                                         16u * lane));
+#pragma unroll
+                for (int b = 0; b < BLOCKS; ++b)
+#pragma unroll
+                    for (int i = 0; i < REGS; ++i) oo[i % 4] = fmaf(o[b][i], o[b][i], oo[i % 4]);
+                const float mine = kq::lanes_sum<LANES>(oo[0] + oo[1] + (oo[2] + oo[3]));
+                const float tile = kq::lanes_sum<63>(vv[0] + vv[1] + (vv[2] + vv[3]));
+                rest = __any(small && !(mine >= kRestMatters * tile));
+            }
+            if (rest) {
+#pragma unroll
+                for (int b = 0; b < BLOCKS; ++b) o[b] *= kRest;
+#pragma unroll
+                for (uint32_t c = 0; c < kTile / CHUNK; ++c) {
+                    float w[8];
+                    weights(c, w, again(top));
+                    rest_of(w);
+                    gather(c, w, again(v_at));
+                }
+#pragma unroll
+                for (int b = 0; b < BLOCKS; ++b) o[b] *= 1.0f / kRest;
+            }
+        }
+        float sum = 0.0f;
+#pragma unroll
+        for (uint32_t c = 0; c < kTile / CHUNK; ++c) {
+            float w[8];
+            weights(c, w, top);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) sum += w[i];
+            gather(c, w, v_at);
         }
         total += sum;
     };

@@ -1,0 +1,66 @@
+"""Rotary positions and attention over a paged cache where their arithmetic and
+their launches end, on the device, against the definitions in binary64
+(tests/paged64.py)."""
+import numpy as np
+import pytest
+
+import paged64
+from test_gpu_gdn import ctx, near, say  # noqa: F401
+from test_gpu_paged import TYPES, Attention
+
+pytestmark = pytest.mark.gpu
+
+
+# ------------------------------------------- weights far below a row's largest
+
+# where a workgroup takes an item, where items have parts, and items of 64 and 128 rows
+FORMS = [(1, [1], [200]), (1, [1], [3000]), (4, [3, 1, 40], [90, 700, 300]), (8, [300], [900]),
+         (8, [700, 1, 300], [0, 64, 1500])]
+
+
+def leading_key(ctx, type_, width, heads, rows, past, ahead, at, value):  # noqa: F811
+    """One key leads the others by `ahead` (nats) and its value is next to nothing, so
+    that the others' small weights are what counts. Every weight of a row stands beside
+    one number of its own, the leading key's score of up to `ahead`, whose query is held
+    to 2^-23, rounded with its factor (2^-24) and summed of two terms (2^-24 each): at
+    most 1.25 2^-22 of `ahead`, 1.5 2^-22 allowed beside the 2e-6 of scores of the order
+    of 1 (15 times that for an element)."""
+    a = Attention(ahead, type_, heads, 4, width, 64, past, rows)
+    q = a.q.reshape(a.total, a.hq, width)
+    q *= np.float32(0.5)
+    g = np.random.default_rng(ahead)
+    q[:, :, 0] = g.uniform(3.5, 4.0, (a.total, a.hq))
+    lead = np.zeros(width, np.float32)
+    lead[0] = ahead * width ** 0.5 / 4.0
+    for s in a.k.slots:
+        ids = a.k.table[s][a.k.table[s] < a.k.pages]
+        a.k.keys[ids, :, :, 0] = 0
+        a.k.keys[ids[0], :, at] = paged64.to_bits(lead, a.k.bf16)
+        a.k.values[ids[0], :, at] = paged64.to_bits(
+            g.normal(size=(heads, width)).astype(np.float32) * np.float32(value), a.k.bf16)
+    bar = 2e-6 + ahead * 1.5 * 2.0 ** -22
+    got, want = (x.reshape(a.total, a.hq, width) for x in (a.got(ctx).astype(np.float64), a.want()))
+    size = np.linalg.norm(want, axis=2, keepdims=True)
+    assert not got[size[..., 0] == 0].any()  # rows that see the leading key alone
+    size[size == 0] = 1.0
+    near(got / size, want / size, bar, 15 * bar)
+
+
+@pytest.mark.parametrize("type_", TYPES)
+@pytest.mark.parametrize("width", [64, 128, 256])
+@pytest.mark.parametrize("heads,rows,past", FORMS, ids=str)
+@pytest.mark.parametrize("ahead", [6, 12, 18, 24, 36])
+@pytest.mark.parametrize("at", [0, 60])
+def test_a_leading_key_without_a_value(ctx, type_, width, heads, rows, past, ahead, at):  # noqa: F811
+    say("leading key", type_, width, heads, rows, past, ahead, at)
+    leading_key(ctx, type_, width, heads, rows, past, ahead, at, 0.0)
+
+
+@pytest.mark.parametrize("width", [64, 128, 256])
+@pytest.mark.parametrize("heads,rows,past", FORMS[2:], ids=str)
+@pytest.mark.parametrize("ahead", [12, 16])
+@pytest.mark.parametrize("value", [1e-1, 1e-2, 1e-3, 1e-5])
+def test_a_leading_key_of_a_small_value(ctx, width, heads, rows, past, ahead, value):  # noqa: F811
+    # on both sides of where the small weights' last bits are looked at
+    say("leading key", width, heads, rows, past, ahead, value)
+    leading_key(ctx, "f16", width, heads, rows, past, ahead, 0, value)
