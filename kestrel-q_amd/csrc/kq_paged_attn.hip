@@ -79,6 +79,9 @@ constexpr uint32_t kWhole = 768; /* tiles times width */
  * of 9 sequences 22.6, 31.3; 500 of one, 9 tiles, would take 23.4, 22.7, and in bf16
  * 30.6, 24.8), 14 of 64, of which 12 measured 19.5, 22.5. */
 constexpr uint32_t kWholeMany = 896;
+/* Workgroups of a launch, which has fewer than 2^32 threads, up to 512 a workgroup: 65,535
+ * sequences of 256 key heads have 16.8 million */
+constexpr uint32_t kLaunch = 1u << 22;
 constexpr uint32_t kPlan = 5;        /* words of the plan before the sequences' */
 constexpr uint32_t kSlots = (4u * kParts + 2u) / 3u;
 constexpr uint32_t kByLane = 64;     /* sequences that each wave plans by itself */
@@ -92,6 +95,7 @@ struct Args {
     uint32_t slot_rows; /* rows that a slot of the partial results holds */
     uint32_t slots;     /* partial results that there is room for */
     uint32_t parts;     /* workgroups */
+    uint32_t first;     /* of this launch */
     bool whole;         /* each item is one part */
     float factor_high, factor_low; /* scale log2(e), 1 .. 2 and its exponent */
     int factor_exponent;
@@ -1281,7 +1285,7 @@ template <bool BF, int D, bool MANY>
 __global__ __launch_bounds__(kThreads, (few_side<BF, D>())) void attend_few(Args g,
                                                                             uint32_t *status) {
     __shared__ __attribute__((aligned(16))) char lds[few_bytes<D, 4>()];
-    Part p = find_part<MANY>(g, blockIdx.x, status);
+    Part p = find_part<MANY>(g, g.first + blockIdx.x, status);
     leave(g, p);
     if (!p.live) return;
     p.pin();
@@ -1324,7 +1328,7 @@ __global__ __launch_bounds__(Many<D>::THREADS, D == 64 ? 3 : 2) void attend(Args
     /* a row's pieces are found by flipping address bits below its size */
     __shared__ __attribute__((aligned(1024))) char lds[BYTES];
     bool badin = false, bad = false, badseq = false;
-    Part p = find_part<MANY>(g, in_turn(blockIdx.x), status);
+    Part p = find_part<MANY>(g, g.first + in_turn(blockIdx.x), status);
     leave(g, p);
     if (!p.live) return;
     p.pin();
@@ -1482,21 +1486,16 @@ Sizes sizes_of(const kq_launch_pattn &a, const kq_launch_paged &c, const kq_laun
 }
 
 template <bool MANY>
-hipError_t launch(const Args &g, bool wide, uint32_t *status, hipStream_t s) {
-    if (MANY) {
-        hipLaunchKernelGGL(plan_many, dim3(1), dim3(1024), 0, s, g, status);
-        const hipError_t e = hipGetLastError();
-        if (e != hipSuccess) return e;
-    }
-#define KQ_ATTEND(BF, D)                                                                     \
-    if (wide)                                                                                \
-        hipLaunchKernelGGL(HIP_KERNEL_NAME(attend_whole<BF, D>), dim3(g.parts),                \
-                           dim3(256 * few_side<BF, D>()), 0, s, g, status);                   \
-    else if (g.slot_rows == kFew)                                                                 \
-        hipLaunchKernelGGL(HIP_KERNEL_NAME(attend_few<BF, D, MANY>), dim3(g.parts), dim3(kThreads), \
-                           0, s, g, status);                                                 \
-    else                                                                                     \
-        hipLaunchKernelGGL(HIP_KERNEL_NAME(attend<BF, D, MANY>), dim3(g.parts),                \
+hipError_t launch_parts(const Args &g, uint32_t parts, bool wide, uint32_t *status, hipStream_t s) {
+#define KQ_ATTEND(BF, D)                                                                       \
+    if (wide)                                                                                  \
+        hipLaunchKernelGGL(HIP_KERNEL_NAME(attend_whole<BF, D>), dim3(parts),                  \
+                           dim3(256 * few_side<BF, D>()), 0, s, g, status);                    \
+    else if (g.slot_rows == kFew)                                                              \
+        hipLaunchKernelGGL(HIP_KERNEL_NAME(attend_few<BF, D, MANY>), dim3(parts),              \
+                           dim3(kThreads), 0, s, g, status);                                   \
+    else                                                                                       \
+        hipLaunchKernelGGL(HIP_KERNEL_NAME(attend<BF, D, MANY>), dim3(parts),                  \
                            dim3(Many<D>::THREADS), 0, s, g, status)
     switch (g.c.width * 2u + (g.c.bf16 ? 1u : 0u)) {
     case 128u: KQ_ATTEND(false, 64); break;
@@ -1508,7 +1507,19 @@ hipError_t launch(const Args &g, bool wide, uint32_t *status, hipStream_t s) {
     default: return hipErrorInvalidValue;
     }
 #undef KQ_ATTEND
-    const hipError_t e = hipGetLastError();
+    return hipGetLastError();
+}
+
+template <bool MANY>
+hipError_t launch(Args &g, bool wide, uint32_t *status, hipStream_t s) {
+    hipError_t e = hipSuccess;
+    if (MANY) {
+        hipLaunchKernelGGL(plan_many, dim3(1), dim3(1024), 0, s, g, status);
+        e = hipGetLastError();
+    }
+    for (g.first = 0u; e == hipSuccess && g.first < g.parts; g.first += kLaunch)
+        e = launch_parts<MANY>(g, g.parts - g.first < kLaunch ? g.parts - g.first : kLaunch, wide,
+                               status, s);
     if (e != hipSuccess || g.slots == 0u) return e; /* nothing to join */
     /* where rows are many, a part's share is shared out again: kAtOnce pieces a thread */
     hipLaunchKernelGGL(join_parts, dim3(g.slots, g.slot_rows == kFew ? 1u : g.c.width / 64u),
@@ -1535,6 +1546,7 @@ extern "C" hipError_t kq_launch_pattn_run(const kq_launch_pattn *a, const kq_lau
     g.slot_rows = z.slot_rows;
     g.slots = (uint32_t)z.slots;
     g.parts = (uint32_t)z.parts;
+    g.first = 0u;
     g.whole = z.whole;
     int exponent = 0;
     const double factor = 2.0 * frexp((double)a->scale * 1.4426950408889634, &exponent);

@@ -4,9 +4,10 @@ their launches end, on the device, against the definitions in binary64
 import numpy as np
 import pytest
 
+import kq_hip
 import paged64
-from test_gpu_gdn import ctx, near, say  # noqa: F401
-from test_gpu_paged import TYPES, Attention
+from test_gpu_gdn import Call, Gen, ctx, near, say  # noqa: F401
+from test_gpu_paged import SENTINEL, TYPES, Attention, Cache, u32
 
 pytestmark = pytest.mark.gpu
 
@@ -39,7 +40,8 @@ def leading_key(ctx, type_, width, heads, rows, past, ahead, at, value):  # noqa
         a.k.values[ids[0], :, at] = paged64.to_bits(
             g.normal(size=(heads, width)).astype(np.float32) * np.float32(value), a.k.bf16)
     bar = 2e-6 + ahead * 1.5 * 2.0 ** -22
-    got, want = (x.reshape(a.total, a.hq, width) for x in (a.got(ctx).astype(np.float64), a.want()))
+    got = a.got(ctx).astype(np.float64).reshape(a.total, a.hq, width)
+    want = a.want().reshape(a.total, a.hq, width)
     size = np.linalg.norm(want, axis=2, keepdims=True)
     assert not got[size[..., 0] == 0].any()  # rows that see the leading key alone
     size[size == 0] = 1.0
@@ -64,3 +66,37 @@ def test_a_leading_key_of_a_small_value(ctx, width, heads, rows, past, ahead, va
     # on both sides of where the small weights' last bits are looked at
     say("leading key", width, heads, rows, past, ahead, value)
     leading_key(ctx, "f16", width, heads, rows, past, ahead, 0, value)
+
+
+# ------------------------------------------------------------- the largest calls
+
+
+def test_more_workgroups_than_a_launch(ctx):  # noqa: F811
+    """As many sequences as a call may have, of as many key heads: 16.8 million items of
+    a workgroup each, more than 2^32 threads. The rows repeat, and so do their results."""
+    say("65535 sequences of 256 heads")
+    n, heads, width, again = 65535, 256, 64, 60
+    past = [0, 3, 64, 130, 255]
+    k = Cache(4, "f16", heads, width, 64, past, [1] * 5, line=4)
+    slots = np.arange(n) % 5
+    few = Gen(9).normal(again, heads * width)
+    with Call(ctx) as c:
+        seqs = kq_hip.sequences(n, n, 5, None, u32(c, slots))
+        at = kq_hip.paged_attention(heads, width ** -0.5)
+        cache = k.describe(c)
+        q = c.up(few[np.arange(n) % again])
+        out = np.full((n, heads * width), SENTINEL)
+        y = c.up(out)
+        size = kq_hip.paged_attention_scratch_bytes(at, cache, seqs)
+        say("launching")
+        ctx.paged_attention(at, cache, seqs, q, heads * width, None, 0, y, heads * width,
+                            c.scratch(size), size)
+        say("done")
+        got = c.down(y, out)
+    fk, fv = k.floats()
+    want = paged64.attention(few.reshape(again, heads, width), fk, fv, k.table, k.lengths,
+                             [(i, i + 1) for i in range(again)], slots[:again], None, width ** -0.5,
+                             out=np.zeros((again, heads, width)))
+    near(got[:again], want.reshape(again, -1))
+    for i in range(again, n, again):
+        assert np.array_equal(got[i:i + again], got[:min(again, n - i)])
