@@ -6,8 +6,9 @@
  *
  * a = position x frequency. The angle's quarter turns are formed in binary64
  * (a position of 2^20 has 2^-33 of a turn left then, where binary32 would
- * have 2^-4), their fraction, at most 1/2, is rounded once to binary32, and
- * sine and cosine of the eighth turn are their series, 2^-27 off.
+ * have 2^-4), and their fraction, pi/4 at most in radians, goes on as two
+ * binary32 numbers: one alone would be 2^-25 off. Sine and cosine are their
+ * series, below 2^-27 off and rounded once.
  *
  * Bound by memory: 3 operations a value of 8 bytes moved. A workgroup forms
  * the cosines and sines of its tokens once, in LDS, for all heads; a thread
@@ -32,17 +33,19 @@ struct Turn {
 __device__ __forceinline__ Turn turn_of(uint32_t position, double frequency, float m) {
     const double quarters = (double)position * (frequency * 0.63661977236758134308);
     const double whole = rint(quarters);
-    const float r = (float)((quarters - whole) * 1.57079632679489661923); /* -pi/4 .. pi/4 */
-    const float z = r * r;
+    const double x = (quarters - whole) * 1.57079632679489661923; /* -pi/4 .. pi/4 */
+    const float r = (float)x, d = (float)(x - (double)r);
+    const float z = r * r, e = fmaf(r, r, -z); /* r^2 = z + e */
     /* the series of sine and cosine; the next terms are below 2^-29 */
     float s = fmaf(z, 2.755731922e-6f, -1.984126984e-4f);
     s = fmaf(z, s, 8.333333333e-3f);
     s = fmaf(z, s, -1.666666667e-1f);
-    s = fmaf(z * r, s, r);
+    const float h = fmaf(z, -0.5f, 1.0f); /* its rounding is put back */
+    s = r + fmaf(z * r, s, h * d);
     float c = fmaf(z, -2.755731922e-7f, 2.480158730e-5f);
     c = fmaf(z, c, -1.388888889e-3f);
     c = fmaf(z, c, 4.166666667e-2f);
-    c = fmaf(z * z, c, fmaf(z, -0.5f, 1.0f));
+    c = h + fmaf(z * z, c, fmaf(-r, d, fmaf(e, -0.5f, fmaf(z, -0.5f, 1.0f - h))));
     /* whole quarters modulo 4: of up to 2^32 positions and any frequency */
     const int n = (int)(whole - 4.0 * floor(whole * 0.25));
     Turn t;

@@ -100,3 +100,27 @@ def test_more_workgroups_than_a_launch(ctx):  # noqa: F811
     near(got[:again], want.reshape(again, -1))
     for i in range(again, n, again):
         assert np.array_equal(got[i:i + again], got[:min(again, n - i)])
+
+
+# ------------------------------------------------------------------- the rotation
+
+
+@pytest.mark.parametrize("rows,first", [(700, 1 << 23), (4096, 0), (4096, (1 << 24) - 4096)])
+def test_angles(ctx, rows, first):  # noqa: F811
+    """Sines and cosines of angles up to 2^24, seen by a vector of length 1: rounded once,
+    2^-25 below 1, of an angle held to 2^-27 and by series 2^-27 off."""
+    say("angles", rows, first)
+    half = 512
+    freq = np.exp(-np.sort(Gen(rows).uniform(0.0, 7.0, half).astype(np.float64)))
+    at = first + np.arange(rows, dtype=np.uint32)
+    x = np.zeros((rows, 2 * half), np.float32)
+    x[:, :half] = 1.0
+    with Call(ctx) as c:
+        y = c.up(np.zeros_like(x))
+        ctx.rotary(kq_hip.rotary(2 * half, c.up(freq)), 1, 2 * half, rows, u32(c, at), c.up(x),
+                   2 * half, y, 2 * half)
+        got = c.down(y, x)
+    angle = at.astype(np.longdouble)[:, None] * freq.astype(np.longdouble)
+    off = np.abs(got - np.concatenate([np.cos(angle), np.sin(angle)], 1)).max()
+    say("   off", float(off) * 2.0 ** 25, "times 2^-25")
+    assert off <= 2.0 ** -25 + 2.0 ** -27 + 2.0 ** -27
