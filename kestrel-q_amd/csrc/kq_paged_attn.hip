@@ -23,13 +23,14 @@
  * Few rows (up to 16 for a key head: decoding) are bound by the pages' bytes: a
  * workgroup's waves take 32 keys in turn each, K straight into registers, V
  * through LDS of the wave's own, with no barrier before the end. 61 sequences of
- * 500 to 32,000 tokens, 504 MB: 93 us, 5.4 TB/s, and 6 for the join; one of
- * 130,002 tokens, 133 MB: 27 us (4 of them until the first keys are there: length,
+ * 500 to 32,000 tokens, 504 MB: 94 us, 5.4 TB/s, and 6 for the join; one of
+ * 130,002 tokens, 133 MB: 28 us (4 of them until the first keys are there: length,
  * page and key hang on each other) and 6.
  * Many rows (128 for a key head) are bound by the matrix cores, whose clock falls
- * to 1.9 GHz under it: 8192 rows over themselves with 16 heads of 128 take 464 -
- * 479 us, 1145 - 1185 TFLOP/s of products, which a library product of 8192^3 fp16
- * reaches (1159); 3 terms and heads of 256, 2049 rows: 215 us, 950 TFLOP/s.
+ * to 1.9 GHz under it: 8192 rows over themselves with 16 heads of 128 take 473 -
+ * 508 us on different cards, 1082 - 1163 TFLOP/s of products, where a library
+ * product of 8192^3 fp16 reached 1159 on one; 3 terms and heads of 256, 2049 rows:
+ * 216 - 221 us, 925 - 945 TFLOP/s.
  */
 #include <math.h>
 
@@ -55,8 +56,8 @@ constexpr uint32_t kMid = 64;        /* the same, where 128 would not fill the d
  * parts 116, with 2048 111. But parts of fewer than 8 tiles are not worth a
  * second round: one sequence of 130,002 tokens takes 34 us in parts of 8 tiles
  * (512), 38 in parts of 4. Of many rows 512, whose partial results are 64 KB or
- * more each (32 KB of 64 rows): 509 rows over 65,509 keys 464 us, 2049 rows of 256-wide heads 215;
- * with 1024 parts 475 and 231, with 256 505 and 224. */
+ * more each (32 KB of 64 rows): 509 rows over 65,509 keys 464 us, 2049 rows of
+ * 256-wide heads 215; with 1024 parts 475 and 231, with 256 505 and 224. */
 constexpr uint32_t kParts = 1024;
 constexpr uint32_t kShort = 8;       /* tiles */
 constexpr uint32_t kLeast = 2;       /* tiles */
@@ -113,8 +114,10 @@ struct Lengths {
 };
 
 /* Rows of a sequence's items. 17 to 32 rows are one wave of an item of 128, two of one
- * of 64: 4 rows of each of 61 sequences, 32 for a key head, 112 us, 125; of 64 rows, two
- * waves or four, 135 and 132. */
+ * of 64: 4 rows of each of 61 sequences of 500 to 32,000 tokens, 32 for a key head, 116 us
+ * (bf16 120), 128 (139) in items of 128. 33 to 64 rows keep items of 128: 488 rows spread
+ * unevenly over sequences of up to 16,000 tokens 133 us (155), 138 (157) in items of 64; where
+ * all have so many items of 64 would be faster: 8 rows of each 119 (120), now 128 (157). */
 __device__ __forceinline__ uint32_t block_of(const Args &g, uint32_t rows, uint32_t most) {
     if (rows <= kFew) return kFew;
     return most == kMany && rows <= kMid / 2u && g.c.width != 256u ? kMid : most;
@@ -136,8 +139,8 @@ __device__ __forceinline__ Need need_of(const Args &g, const kq::PagedSeq &s, ui
         /* keys from the first token's window to the last token of a block */
         const uint32_t span = (rows < block ? rows - 1u : block - 1u) / g.group + 1u;
         const uint64_t keys = (uint64_t)g.a.window + span;
-        const uint64_t most = (keys + kTile - 1u) / kTile + 1u;
-        if (most < n.tiles) n.tiles = (uint32_t)most;
+        const uint64_t seen = (keys + kTile - 1u) / kTile + 1u;
+        if (seen < n.tiles) n.tiles = (uint32_t)seen;
     }
     return n;
 }
@@ -162,8 +165,11 @@ __device__ __forceinline__ uint64_t seen_by_many(const Args &g, const kq::PagedS
  * tiles) 8.1 us, 19.4 in items of 128; 500 of 16 heads (256) 17.4, 22.8; but 300 over
  * 1300 keys (684) 37, 27. Those in the middle have items of 64, which begin sooner and
  * are joined from fewer parts: 300 rows over 1300 keys 24.5, 27; 1200 rows of 8
- * sequences (1364) 30, 39; 500 over 2500 (2304) 37, 39; but they read LDS twice as
- * often for a product: 2003 ragged rows of heads of 64 (3300) 53, 49. Heads of 256,
+ * sequences (1364) 30, 39; but they read LDS twice as often for a product: 2003 ragged
+ * rows of heads of 64 (3300) 53, 49. Where one sequence's rows stand behind many keys
+ * the sides cross later than kMiddle: 500 rows of 2 key heads over 1500 keys more (1792)
+ * 35, 38, over 2000 (2304) 39.5, 40.7, over 2500 (2752) 43, 44, over 5500 (5760) 63, 66
+ * (bf16 73, 80). Heads of 256,
  * whose workgroups have no room beside each other, have no such form, and items of 16
  * rows up to 48 tiles (116 rows of 32 heads, 32 tiles, 13.2, 18.7; 250 of 16, 64 tiles,
  * 29.7, 27). */
@@ -209,8 +215,9 @@ __device__ __forceinline__ uint32_t length_of(const Lengths &l, const Need &n) {
     return n.block == kFew ? l.few : l.many;
 }
 
-/* parts of so many tiles, the nearest number: an item a little longer than a
- * part stays whole. Of `length` and 1.5 times that, and at least 2, tiles. */
+/* parts of so many tiles, the nearest number: an item a little longer than a part
+ * stays whole, up to 1.5 times `length`; several parts have 0.75 to 1.25 times
+ * `length` on the average, to whole tiles (3 tiles by 2: one of 2, one of 1). */
 __device__ __forceinline__ uint32_t parts_of(uint32_t tiles, uint32_t length) {
     if (tiles == 0u) return 0u;
     const uint32_t n = (tiles + length / 2u) / length;
@@ -627,7 +634,8 @@ __device__ __forceinline__ void fetch_query(Raw<STEPS> &r, bool some, At at) {
     for (int s = 0; s < STEPS; ++s)
 #pragma unroll
         for (int i = 0; i < 2; ++i)
-            r.v[s][i] = some ? *(const float4 *)(at(s) + 4 * i) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            r.v[s][i] =
+                some ? *(const float4 *)(at(s) + 4 * i) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 }
 
 /* LANES: the lanes that share a row */
@@ -786,9 +794,9 @@ template <int D>
 constexpr uint32_t many_bytes() {
     return 512u * D; /* 2 x 64 rows of K and V */
 }
-/* Waves a SIMD that registers are given for. Heads of 128 in fp16 need 148: three
+/* Waves a SIMD that registers are given for. Heads of 128 in fp16 need 150: three
  * (61 sequences 109 us; four, at 128 with 24 of them in memory, 136). */
-template <bool BF, int D>
+template <int D>
 constexpr int few_side() {
     return D == 256 ? 2 : D == 128 ? 3 : 4;
 }
@@ -801,7 +809,8 @@ template <bool BF, int D, int W>
 __device__ __forceinline__ void few_rows(const Args &g, const Part &p, char *lds, bool &badin,
                                          bool &bad, bool &badseq) {
     constexpr int STEPS = D / 32, BLOCKS = D / 16, TERMS = Type<BF>::TERMS;
-    const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64u);
+    const uint32_t lane = threadIdx.x & 63u;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64u);
     const uint32_t n = lane & 15u, quarter = lane >> 4;
     const bool some = n < p.rows;
     const uint32_t row = p.row0 + n, token = some ? row / g.group : 0u;
@@ -862,8 +871,8 @@ __device__ __forceinline__ void few_rows(const Args &g, const Part &p, char *lds
                                          : kOut;
                 __builtin_amdgcn_raw_ptr_buffer_load_lds(
                     values,
-                    (__attribute__((address_space(3))) void *)(mine + b * (32u * D) + j * 1024u), 16,
-                    off, 0, 0, 0);
+                    (__attribute__((address_space(3))) void *)(mine + b * (32u * D) + j * 1024u),
+                    16, off, 0, 0, 0);
             }
         }
     };
@@ -1067,7 +1076,8 @@ __device__ __forceinline__ void many_rows(const Args &g, const Part &p, char *ld
     typedef typename T::acc acc;
     constexpr int M = T::M, REGS = T::REGS, STEPS = T::STEPS, BLOCKS = T::BLOCKS;
     constexpr int TERMS = Type<BF>::TERMS, SETS = kTile / M, LANES = M == 32 ? 32 : 48;
-    const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64u);
+    const uint32_t lane = threadIdx.x & 63u;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64u);
     const uint32_t n = lane % M, part = lane / M;
     const uint32_t r0 = wave * M;
     const bool some = r0 + n < p.rows;
@@ -1282,7 +1292,7 @@ __device__ __forceinline__ void many_rows(const Args &g, const Part &p, char *ld
 
 /* calls whose items all have few rows, as where every sequence decodes */
 template <bool BF, int D, bool MANY>
-__global__ __launch_bounds__(kThreads, (few_side<BF, D>())) void attend_few(Args g,
+__global__ __launch_bounds__(kThreads, (few_side<D>())) void attend_few(Args g,
                                                                             uint32_t *status) {
     __shared__ __attribute__((aligned(16))) char lds[few_bytes<D, 4>()];
     Part p = find_part<MANY>(g, g.first + blockIdx.x, status);
@@ -1298,9 +1308,9 @@ __global__ __launch_bounds__(kThreads, (few_side<BF, D>())) void attend_few(Args
 
 /* calls of few rows that need no join: an item is a workgroup's */
 template <bool BF, int D>
-__global__ __launch_bounds__((256 * few_side<BF, D>()), (few_side<BF, D>())) void attend_whole(
+__global__ __launch_bounds__((256 * few_side<D>()), (few_side<D>())) void attend_whole(
     Args g, uint32_t *status) {
-    constexpr int W = 4 * few_side<BF, D>();
+    constexpr int W = 4 * few_side<D>();
     __shared__ __attribute__((aligned(16))) char lds[few_bytes<D, W>()];
     Part p = find_part<false>(g, blockIdx.x, status);
     if (!p.live) return;
@@ -1314,15 +1324,17 @@ __global__ __launch_bounds__((256 * few_side<BF, D>()), (few_side<BF, D>())) voi
 
 /* The first 256 workgroups, which begin on a CU each, in reverse: items come longest
  * first, so that the longest of the next 256 lie beside the shortest of these. 8192 rows
- * over themselves 478 us, 496 without; 4096 rows of bf16 174, 184; only 1500 rows of 8
- * key heads over 500 more keys are slower, 62, 59. By eights, which leaves a head's
- * workgroups on their XCD. */
+ * over themselves 496 us, 515 without (bf16 643, 668); 4096 151, 155 (177, 186). Where all
+ * items are long there is nothing to even out, and it costs: 2000 rows of 8 key heads over
+ * 4000 more keys 188, 181 (bf16 246, 231), 4096 rows of heads of 64 94, 89. By eights,
+ * which leaves a head's workgroups on their XCD. */
 __device__ __forceinline__ uint32_t in_turn(uint32_t u) {
     return u < 256u && gridDim.x >= 256u ? (u & 7u) | (248u - (u & ~7u)) : u;
 }
 
 template <bool BF, int D, bool MANY>
-__global__ __launch_bounds__(Many<D>::THREADS, D == 64 ? 3 : 2) void attend(Args g, uint32_t *status) {
+__global__ __launch_bounds__(Many<D>::THREADS, D == 64 ? 3 : 2) void attend(Args g,
+                                                                            uint32_t *status) {
     constexpr int W = Many<D>::W;
     constexpr uint32_t BYTES = Many<D>::LDS > few_bytes<D, W>() ? Many<D>::LDS : few_bytes<D, W>();
     /* a row's pieces are found by flipping address bits below its size */
@@ -1356,7 +1368,8 @@ struct Sum {
     }
     __device__ __forceinline__ void add(const Sum &o) {
         const float next = fmaxf(top, o.top);
-        const float f = __builtin_amdgcn_exp2f(top - next), e = __builtin_amdgcn_exp2f(o.top - next);
+        const float f = __builtin_amdgcn_exp2f(top - next);
+        const float e = __builtin_amdgcn_exp2f(o.top - next);
         top = next;
         total = fmaf(total, f, o.total * e);
 #pragma unroll
@@ -1398,7 +1411,8 @@ __global__ __launch_bounds__(kThreads) void join_parts(Args g, uint32_t *status)
             if (!by_rows) {
                 const uint32_t lane = i[u] % 64u, piece = i[u] / 64u % (tall * width / 256u);
                 row[u] = i[u] / (tall * width / 4u) * tall + lane % tall;
-                d[u] = tall == 16u ? Many<256>::column(piece, lane) : Many<128>::column(piece, lane);
+                d[u] = tall == 16u ? Many<256>::column(piece, lane)
+                                   : Many<128>::column(piece, lane);
             }
             have[u] = i[u] < b && row[u] < p.rows;
             v[u].clear();
@@ -1474,11 +1488,13 @@ Sizes sizes_of(const kq_launch_pattn &a, const kq_launch_paged &c, const kq_laun
     const uint64_t most = finest * (z.whole ? 1u : (tiles + kLeast / 2u) / kLeast + 1u);
     z.parts = most < kParts + z.items ? most : kParts + z.items;
     z.slots = z.whole ? 0u : most < kSlots ? most : kSlots;
-    z.plan_bytes = ((kPlan + (q.count > kByLane ? 2u * (q.count + 1u) : 0u)) * 4u + 255u) / 256u * 256u;
+    const uint64_t firsts = q.count > kByLane ? 2u * (q.count + 1u) : 0u;
+    z.plan_bytes = ((kPlan + firsts) * 4u + 255u) / 256u * 256u;
     /* a call that joins nothing asks for what one of single rows would: scratch of the
      * largest call is enough for all */
     const uint64_t few = c.heads * q.count * ((tiles + kLeast / 2u) / kLeast + 1u);
-    const uint64_t held = !z.whole ? z.slots : sees < kLeast * 3u / 2u ? 0u : few < kSlots ? few : kSlots;
+    const uint64_t held =
+        !z.whole ? z.slots : sees < kLeast * 3u / 2u ? 0u : few < kSlots ? few : kSlots;
     z.item_bytes = (held * sizeof(Item) + 255u) / 256u * 256u;
     z.bytes = z.plan_bytes + z.item_bytes +
               held * (z.whole ? kFew : z.slot_rows) * (c.width + 2u) * 4u;
@@ -1490,7 +1506,7 @@ hipError_t launch_parts(const Args &g, uint32_t parts, bool wide, uint32_t *stat
 #define KQ_ATTEND(BF, D)                                                                       \
     if (wide)                                                                                  \
         hipLaunchKernelGGL(HIP_KERNEL_NAME(attend_whole<BF, D>), dim3(parts),                  \
-                           dim3(256 * few_side<BF, D>()), 0, s, g, status);                    \
+                           dim3(256 * few_side<D>()), 0, s, g, status);                    \
     else if (g.slot_rows == kFew)                                                              \
         hipLaunchKernelGGL(HIP_KERNEL_NAME(attend_few<BF, D, MANY>), dim3(parts),              \
                            dim3(kThreads), 0, s, g, status);                                   \

@@ -156,7 +156,8 @@ template <int V, int TOK>
 struct Values {
     Vec<V> a[TOK], b[TOK];
 
-    __device__ __forceinline__ void load(const Heads &h, const Unit<V> &u, uint32_t t0, uint32_t n) {
+    __device__ __forceinline__ void load(const Heads &h, const Unit<V> &u, uint32_t t0,
+                                         uint32_t n) {
         const float *p = h.rows + (size_t)t0 * h.stride + u.head * h.width;
 #pragma unroll
         for (uint32_t t = 0; t < TOK; ++t) {
@@ -347,6 +348,12 @@ Shape shape_of(uint64_t tokens, uint64_t units) {
     return s;
 }
 
+/* Whether the turned part is made of units of four values, of which a thread takes
+ * one, in HALVES one of each half. Others go value by value: 8191 rows of 24 heads
+ * of 128 with 58 turned 58.5 us (in pairs 54.5), with 64 47.5 (38.8); 4099 rows of 48
+ * heads into pages with 58 turned 60.4 (60.8), with 128 41.5. */
+bool whole_vectors(const kq_launch_rotary &r) { return r.dims % (r.pairs ? 4u : 8u) == 0u; }
+
 }  // namespace
 
 extern "C" hipError_t kq_launch_rotary_rows(const kq_launch_rotary *r, uint32_t heads,
@@ -354,7 +361,7 @@ extern "C" hipError_t kq_launch_rotary_rows(const kq_launch_rotary *r, uint32_t 
                                             const uint32_t *positions, const float *x, uint64_t xs,
                                             float *y, uint64_t ys, uint32_t *status,
                                             hipStream_t s) {
-    const bool v4 = r->dims % (r->pairs ? 4u : 8u) == 0u && width % 4u == 0u && xs % 4u == 0u && ys % 4u == 0u &&
+    const bool v4 = whole_vectors(*r) && width % 4u == 0u && xs % 4u == 0u && ys % 4u == 0u &&
                     (((uintptr_t)x | (uintptr_t)y) & 15u) == 0u;
     const Heads h = {x, xs, heads, width, r->dims, r->pairs};
     const Shape g = shape_of(tokens, (uint64_t)heads * width / (v4 ? 4u : 1u));
@@ -381,12 +388,12 @@ namespace {
 template <typename T>
 hipError_t append(const kq_launch_paged &c, const kq_launch_seqs &q, const kq_launch_append &a,
                   const kq_launch_rotary &r, uint32_t *status, hipStream_t s) {
-    const bool v4 = r.dims % (r.pairs ? 4u : 8u) == 0u;
+    const bool v4 = whole_vectors(r);
     const Shape g =
         shape_of(q.tokens, (uint64_t)(2u * c.heads + a.query_heads) * c.width / (v4 ? 4u : 1u));
 #define KQ_APPEND(V, TOK)                                                                         \
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(append_rows<T, V, TOK>), g.grid, dim3(kThreads), 0, s, c, q, \
-                       a, r, status)
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(append_rows<T, V, TOK>), g.grid, dim3(kThreads), 0, s, c,  \
+                       q, a, r, status)
     if (g.one) {
         if (v4)
             KQ_APPEND(4, 1);
