@@ -929,7 +929,8 @@ kq_status kq_hip_cache_append_f32(kq_hip_context *context, const kq_hip_paged_ca
  * but that with an F16 cache a query is held to 2^-23 of itself, at best to
  * 2^-37 of its head's largest in the row, and a weight to 2^-23 of itself, at
  * best to 2^-78 of its row's largest (below 2^-55 of it, 38 nats, it loses
- * bits). With a BF16 cache both are held to 2^-24.
+ * bits), or to less than what the row's sums are rounded by. With a BF16 cache
+ * both are held to 2^-24.
  * Offsets as in kq_hip_sequences; a slot may be named more than once here.
  * Rows that belong to no sequence keep what the output held. Strides count
  * floats between rows, up to 2^22; queries, gate, output, cache and scratch
