@@ -695,8 +695,12 @@ __device__ __forceinline__ float inverse_of_row(const Args &g, uint32_t h, float
                                                 bool &bad) {
     if (g.a.sinks != nullptr) {
         const float sink = g.a.sinks[h];
-        total += __builtin_amdgcn_exp2f(
-            fmaf(sink, 0x1.715476p+0f, fmaf(sink, 0x1.4ae0cp-26f, -top)));
+        const float e = fmaf(sink, 0x1.715476p+0f, fmaf(sink, 0x1.4ae0cp-26f, -top));
+        if (e > 64.0f) { /* by the sink's weight, in halves: it may be beyond the range */
+            const float half = __builtin_amdgcn_exp2f(-0.5f * e);
+            return half * (half / fmaf(total * half, half, 1.0f));
+        }
+        total += __builtin_amdgcn_exp2f(e);
     }
     bad |= !(total > 0.0f); /* of a row's keys one at least has a weight of its slack */
     return 1.0f / total;
@@ -1293,7 +1297,7 @@ __device__ __forceinline__ void many_rows(const Args &g, const Part &p, char *ld
 /* calls whose items all have few rows, as where every sequence decodes */
 template <bool BF, int D, bool MANY>
 __global__ __launch_bounds__(kThreads, (few_side<D>())) void attend_few(Args g,
-                                                                            uint32_t *status) {
+                                                                        uint32_t *status) {
     __shared__ __attribute__((aligned(16))) char lds[few_bytes<D, 4>()];
     Part p = find_part<MANY>(g, g.first + blockIdx.x, status);
     leave(g, p);
@@ -1506,7 +1510,7 @@ hipError_t launch_parts(const Args &g, uint32_t parts, bool wide, uint32_t *stat
 #define KQ_ATTEND(BF, D)                                                                       \
     if (wide)                                                                                  \
         hipLaunchKernelGGL(HIP_KERNEL_NAME(attend_whole<BF, D>), dim3(parts),                  \
-                           dim3(256 * few_side<D>()), 0, s, g, status);                    \
+                           dim3(256 * few_side<D>()), 0, s, g, status);                        \
     else if (g.slot_rows == kFew)                                                              \
         hipLaunchKernelGGL(HIP_KERNEL_NAME(attend_few<BF, D, MANY>), dim3(parts),              \
                            dim3(kThreads), 0, s, g, status);                                   \

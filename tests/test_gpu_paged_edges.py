@@ -68,6 +68,24 @@ def test_a_leading_key_of_a_small_value(ctx, width, heads, rows, past, ahead, va
     leading_key(ctx, "f16", width, heads, rows, past, ahead, 0, value)
 
 
+@pytest.mark.parametrize("type_", TYPES)
+@pytest.mark.parametrize("width", [64, 128, 256])
+@pytest.mark.parametrize("heads,rows,past", FORMS[:4], ids=str)
+@pytest.mark.parametrize("ahead", [60, 76, 80, 84, 86])
+def test_sinks_far_above_the_scores(ctx, type_, width, heads, rows, past, ahead):  # noqa: F811
+    """A sink's weight against weights that are held times up to 2^15: outputs are normal
+    numbers still. What a row is multiplied by is held to 2^-150 where it is not, that is
+    2^-135 e^ahead of itself, as the largest scores are above 0; the sink's own exponent
+    has a relative error of 2^-24 beside the 2e-6 of the scores, and the outputs a last
+    half step, 2^-150."""
+    say("sinks ahead", type_, width, heads, rows, past, ahead)
+    a = Attention(ahead, type_, heads, 4, width, 64, [max(p, 60) for p in past], rows, sinks=True)
+    a.sinks[:] = ahead
+    bar = 2e-6 + ahead * 2.0 ** -23 + 2.0 ** -135 * np.exp(ahead)
+    got, want = a.got(ctx).astype(np.float64), a.want()
+    assert np.linalg.norm(got - want) <= bar * np.linalg.norm(want) + 2.0 ** -150 * want.size ** 0.5
+
+
 # ------------------------------------------------------------- the largest calls
 
 
