@@ -28,7 +28,7 @@
  * page and key hang on each other) and 6.
  * Many rows (128 for a key head) are bound by the matrix cores, whose clock falls
  * to 1.9 GHz under it: 8192 rows over themselves with 16 heads of 128 take 473 -
- * 508 us on different cards, 1082 - 1163 TFLOP/s of products, where a library
+ * 514 us on different cards, 1070 - 1163 TFLOP/s of products, where a library
  * product of 8192^3 fp16 reached 1159 on one; 3 terms and heads of 256, 2049 rows:
  * 216 - 221 us, 925 - 945 TFLOP/s.
  */
